@@ -7,8 +7,9 @@ reference's Rust interface:
 - ``gpu``: DType, EyebrowseError, Device, Tensor, Recorder (crates/eyebrowse-gpu);
 - ``kernels``: attn_prefill, attn_decode, kv_write, rmsnorm, rope (crates/eyebrowse-kernels),
   linear_f16w (the projections around attention), plus chunked / windowed attention, the
-  fused decode step and IEEE-half and OCP FP8 E4M3 caches;
-- ``nn``: Linear, Rope, KvCache, Attention (crates/eyebrowse-nn).
+  fused decode step and IEEE-half and OCP FP8 E4M3 caches; and a quantised model's operators:
+  4-bit projections (linear_q4), block-scaled 8-bit caches (kv_write_i8, attn_*_i8), sampling;
+- ``nn``: Linear, LinearQ4, Rope, KvCache, Attention (crates/eyebrowse-nn).
 """
 from ._lib import LIB_PATH, lib
 from .gpu import (DType, Device, DeviceUnavailable, EyebrowseError, Graph, LoadError,
@@ -30,8 +31,14 @@ from .kernels import (argmax, argmax_workspace_floats, attn_decode, attn_decode_
                       attn_decode_noalloc_max_floats, launch_linear_f16w, launch_rmsnorm, launch_rope, linear_f16w,
                       linear_f16w_multi, linear_workspace_floats, rmsnorm, rope,
                       LANE_OPS_ROWS, launch_selftest_lane_ops, attn_prefill_pv16,
-                      launch_attn_prefill_pv16, launch_attn_prefill_pv16_ws)
-from .nn import Attention, KvCache, Linear, Rope
+                      launch_attn_prefill_pv16, launch_attn_prefill_pv16_ws,
+                      linear_q4, linear_q4_multi, linear_q4_workspace_floats, launch_linear_q4,
+                      kv_write_i8, kv_read_i8, attn_decode_i8, attn_decode_step_i8,
+                      attn_prefill_chunk_i8, attn_i8_workspace_floats, launch_kv_write_i8,
+                      launch_kv_read_i8, launch_attn_decode_i8, launch_attn_prefill_chunk_i8,
+                      sample, sample_workspace_floats, launch_sample)
+from ._lib import CacheI8
+from .nn import Attention, KvCache, Linear, LinearQ4, Rope
 
 __all__ = [
     "LIB_PATH", "lib", "DType", "Device", "DeviceUnavailable", "EyebrowseError", "Graph",
@@ -51,5 +58,10 @@ __all__ = [
     "launch_rope", "launch_attn_prologue", "launch_attn_decode_step_noalloc",
     "attn_decode_noalloc_max_floats", "rmsnorm", "rope", "Attention", "KvCache", "Linear", "Rope",
     "LANE_OPS_ROWS", "launch_selftest_lane_ops", "attn_prefill_pv16", "launch_attn_prefill_pv16",
-    "launch_attn_prefill_pv16_ws",
+    "launch_attn_prefill_pv16_ws", "LinearQ4", "CacheI8",
+    "linear_q4", "linear_q4_multi", "linear_q4_workspace_floats", "launch_linear_q4",
+    "kv_write_i8", "kv_read_i8", "attn_decode_i8", "attn_decode_step_i8",
+    "attn_prefill_chunk_i8", "attn_i8_workspace_floats", "launch_kv_write_i8",
+    "launch_kv_read_i8", "launch_attn_decode_i8", "launch_attn_prefill_chunk_i8", "sample",
+    "sample_workspace_floats", "launch_sample",
 ]

@@ -39,6 +39,34 @@ class AttentionDesc(ctypes.Structure):
     ]
 
 
+class Q4Weight(ctypes.Structure):
+    """eb_q4_weight."""
+    _fields_ = [
+        ("w", c_vp),
+        ("scales", c_vp),
+        ("zeros", c_vp),
+        ("in_f", c_size),
+        ("out_f", c_size),
+        ("group", c_size),
+    ]
+
+
+class CacheI8(ctypes.Structure):
+    """eb_cache_i8."""
+    _fields_ = [
+        ("k", c_vp),
+        ("k_exp", c_vp),
+        ("v", c_vp),
+        ("v_exp", c_vp),
+        ("code_numel", c_size),
+        ("exp_numel", c_size),
+        ("max_seq", c_size),
+        ("hkv", c_size),
+        ("hd", c_size),
+        ("block", c_size),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/eyebrowse_hip.h declares.
 SIGNATURES = {
     "eb_last_error": (ctypes.c_char_p, []),
@@ -202,6 +230,43 @@ SIGNATURES = {
     "eb_kv_cache_max_seq": (c_size, [c_vp]),
     "eb_attention_new": (c_st, [ctypes.POINTER(AttentionDesc), ctypes.POINTER(c_vp)]),
     "eb_attention_release": (None, [c_vp]),
+    "eb_linear_q4": (c_st, [c_vp, c_vp, ctypes.POINTER(Q4Weight), c_vp, c_size]),
+    "eb_linear_q4_multi": (c_st, [c_vp, c_vp, c_size, ctypes.POINTER(Q4Weight),
+                                  ctypes.POINTER(c_vp), c_size]),
+    "eb_linear_q4_workspace_floats": (c_size, [c_size, c_size]),
+    "eb_launch_linear_q4": (c_st, [c_vp, c_vp, c_size, c_vp, c_size, c_vp, c_size, c_vp, c_size,
+                                   c_vp, c_size, c_size, c_size, c_size, c_size, c_vp, c_size]),
+    "eb_attention_new_q4": (c_st, [ctypes.POINTER(AttentionDesc), ctypes.POINTER(Q4Weight),
+                                   ctypes.POINTER(c_vp)]),
+    "eb_kv_cache_new_i8": (c_st, [c_vp, ctypes.POINTER(c_size), c_size, c_size, c_size, c_size,
+                                  ctypes.POINTER(c_vp)]),
+    "eb_kv_cache_k_scale": (c_vp, [c_vp, c_size]),
+    "eb_kv_cache_v_scale": (c_vp, [c_vp, c_size]),
+    "eb_kv_cache_block": (c_size, [c_vp]),
+    "eb_kv_write_i8": (c_st, [c_vp, c_vp, c_size, c_vp, c_vp, c_size, c_size]),
+    "eb_kv_read_i8": (c_st, [c_vp, c_vp, c_size, c_vp, c_vp, c_size, c_size]),
+    "eb_attn_decode_i8": (c_st, [c_vp, c_vp, c_vp, c_size, c_vp, c_size, c_size, c_float,
+                                 c_size]),
+    "eb_attn_decode_step_i8": (c_st, [c_vp, c_vp, c_vp, c_vp, c_vp, c_size, c_vp, c_size, c_size,
+                                      c_float, c_size]),
+    "eb_attn_prefill_chunk_i8": (c_st, [c_vp, c_vp, c_vp, c_size, c_vp, c_size, c_size, c_size,
+                                        c_float, c_size]),
+    "eb_launch_kv_write_i8": (c_st, [c_vp, ctypes.POINTER(CacheI8), c_vp, c_vp, c_size, c_size,
+                                     c_size]),
+    "eb_launch_kv_read_i8": (c_st, [c_vp, ctypes.POINTER(CacheI8), c_vp, c_vp, c_size, c_size,
+                                    c_size]),
+    "eb_attn_i8_workspace_floats": (c_size, [c_size, c_size, c_size, c_size, c_size, c_size,
+                                             c_size, c_int]),
+    "eb_launch_attn_decode_i8": (c_st, [c_vp, c_vp, c_size, c_vp, c_vp, c_size,
+                                        ctypes.POINTER(CacheI8), c_vp, c_size, c_size, c_size,
+                                        c_float, c_size, c_vp, c_size, c_int]),
+    "eb_launch_attn_prefill_chunk_i8": (c_st, [c_vp, c_vp, c_size, ctypes.POINTER(CacheI8), c_vp,
+                                               c_size, c_size, c_size, c_size, c_float, c_size,
+                                               c_vp, c_size, c_int]),
+    "eb_sample": (c_st, [c_vp, c_vp, c_vp, c_vp, c_size, c_size, c_vp, c_vp, c_vp, c_vp]),
+    "eb_sample_workspace_floats": (c_size, [c_size, c_size]),
+    "eb_launch_sample": (c_st, [c_vp, c_vp, c_size, c_vp, c_vp, c_size, c_size, c_vp, c_vp, c_vp,
+                                c_vp, c_vp, c_size]),
     "eb_attention_forward": (c_st, [c_vp, c_vp, c_vp, c_vp, c_vp, c_size, c_size, c_size,
                                     ctypes.POINTER(c_vp)]),
     "eb_attention_forward_qkv": (c_st, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_size,

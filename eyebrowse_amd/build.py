@@ -45,6 +45,11 @@ SOURCES = [
     "eb_linear.hip",
     "eb_argmax.hip",
     "eb_noalloc.hip",
+    "eb_quant.cpp",
+    "eb_cache_i8.hip",
+    "eb_decode_i8.hip",
+    "eb_linear_q4.hip",
+    "eb_sample.hip",
 ]
 
 
@@ -55,6 +60,8 @@ SOURCES = [
 SOURCE_FLAGS = {
     "eb_decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "eb_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "eb_decode_i8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "eb_linear_q4.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

@@ -102,6 +102,12 @@ __device__ __forceinline__ float class_reduce(float x) {
 // 2^x on the hardware transcendental unit (v_exp_f32); exp2(-inf) = 0.
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// The bits of |x|, which order as the magnitudes do (NaN above infinity above all else). A float
+// parameter, not an expression: the compiler's bit cast of a vector's element x[i] reads x[0].
+__device__ __forceinline__ unsigned magnitude_bits(float x) {
+    return __builtin_bit_cast(unsigned, x) & 0x7FFFFFFFu;
+}
+
 // ---- OCP FP8 E4M3 ("e4m3fn": sign, 4 exponent bits with bias 7, 3 fraction bits, no
 // infinities, S.1111.111 NaN, largest finite 448) -------------------------------------
 

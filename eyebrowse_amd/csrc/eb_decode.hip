@@ -1630,6 +1630,23 @@ eb_status launch_attn_decode_any(hipStream_t st, const float *q, const void *kc,
     return check_launch("attn_decode");
 }
 
+eb_status launch_decode_merge(hipStream_t st, const float *part_acc, const float *part_ml, float *o, size_t h,
+                              size_t hkv, size_t hd, int nsplit) {
+#define EB_MERGE_HD(D)                                                                           \
+    case D: {                                                                                    \
+        constexpr int DS = merge_dims_per_block(D);                                              \
+        const dim3 grid((unsigned)h, (unsigned)((D + DS - 1) / DS));                             \
+        decode_merge_kernel<D><<<grid, kThreads, 0, st>>>(part_acc, part_ml, o, (int)h, (int)hkv, nsplit); \
+        break;                                                                                   \
+    }
+    switch (hd) {
+        EB_HEAD_DIMS(EB_MERGE_HD)
+        default: return fail(EB_UNSUPPORTED_CONFIG, "attn_decode merge: head_dim %zu", hd);
+    }
+#undef EB_MERGE_HD
+    return check_launch("attn_decode (merge)");
+}
+
 eb_status launch_attn_decode(hipStream_t st, const float *q, const float *kc, const float *vc,
                              float *kc_w, float *vc_w, const float *knew, const float *vnew,
                              float *o, size_t h, size_t hkv, size_t pos, size_t hd,

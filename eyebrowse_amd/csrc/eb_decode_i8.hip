@@ -1,0 +1,619 @@
+// Attention of a few query rows over the block-scaled 8-bit cache (eb_cache_i8.h) for gfx950:
+// a single token, with its cache append folded in, or a short run of rows (a draft to verify, a
+// short next chunk). Split keys, then the log-sum-exp merge of the decode path.
+//
+//   o[c] = sum_j 2^(s_cj - m) v_j / sum_j 2^(s_cj - m),   s_cj = scale log2(e) q_c . k_j
+//
+// over the keys j that column c sees. A column is one query head of one row; the up to 16 columns
+// of a workgroup share a KV head, so that every key row is read once for all of them.
+//
+// Grid (hkv * nsub) x nsplit, 4 waves. A tile is 16 keys at an aligned position, hence inside one
+// block of the cache: its two scales are the same for the whole tile. Lane (n, g) is lane
+// n + 16 g.
+//  - Scores S[key][column] = K q^T on v_mfma_f32_16x16x32_f16. A: lane (n, g) holds 16 dims of
+//    key n per 64-dim piece, straight from one 16-byte load, converted to f16 (exact: whole
+//    numbers up to 128). B: column n's q as f16 high and low halves of q * scale * log2(e) scaled
+//    by a power of two (its largest |q| in [2^13, 2^14)). Lane (n, g) then holds the scores of
+//    keys 4g .. 4g + 3 for column n; the tile's K scale and the column's power of two come back
+//    in one multiply.
+//  - Online softmax with a reference m per column that moves only when a score exceeds it by
+//    more than kSlack.
+//  - O[column][dim] += P V on v_mfma_f32_16x16x32_f16: the 32 contracted indices are the 16 keys
+//    twice, with the weights' high halves and their remainders, against the same V. A: lane
+//    (n, g)'s own score registers. B: lane (n, g) loads HD/16 dims of keys 4g .. 4g + 3.
+//    No lane exchange and no LDS between the products.
+//  - The weights carry the tile's V scale: p * 2^(ev - u + 7), u a whole number per column (the
+//    unit of its accumulators) that moves, with a rescale, when a term would exceed it by more
+//    than the slack. So a block of large values beside blocks of small ones costs neither range
+//    nor the small ones' precision where the large ones have no weight.
+// The products sum in f32; the f16 pairs keep 22 bits of q and of the weights.
+//
+// Fused append (one row): the split with the fewest tiles owns the token's block. It normalises
+// and rotates the new K and V rows, writes their codes (and the block's earlier codes again where
+// the exponent grew), and then takes the block's tiles itself, from the cache; no other split
+// reads that block. With more than 16 columns several workgroups would read it, and the append is
+// a launch of its own.
+#include "eb_cache_i8.h"
+
+#include <algorithm>
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * 64;
+constexpr int kTile = 16;    // keys per tile
+constexpr int kCols = 16;    // columns per workgroup
+constexpr float kSlack = 8.0f;  // log2 units a score may exceed its reference by
+constexpr float kNoUnit = -100000.0f;  // u before the first tile
+
+template <int HD>
+struct Shape {
+    static constexpr int NC = HD / 32;   // 32-dim chunks of a key row
+    static constexpr int KL = HD / 64;   // 16-byte K loads per lane and tile
+    static constexpr int DV = HD / 16;   // V dims per lane and row
+    static constexpr int VW = DV / 4;    // words per lane and V row
+    static constexpr int QS = HD + 4;    // floats per LDS row (bank spread)
+    // LDS (floats): q [kCols][QS], later the waves' accumulators [kWaves][ncol][QS]; then the new
+    // rows [2][HD]; column exponents [kCols]; m and l [kCols][kWaves] each.
+    static constexpr size_t lds_floats(int ncol) {
+        const int a = kCols * QS, b = kWaves * ncol * QS;
+        return (size_t)(a > b ? a : b) + 2 * HD + kCols + 2 * kCols * kWaves;
+    }
+};
+
+struct Args {
+    const float *q;  // [rows, h, hd]
+    eb::CacheI8 c;
+    const float *knew, *vnew;  // [hkv, hd] (null: no append)
+    float *o;                  // [rows, h, hd]
+    float *part_acc, *part_ml;
+    int h, g, rows, ncols;  // ncols: columns of a KV head, rows * g
+    int pos0;               // position of row 0
+    int window;             // 0: none
+    int tile0, tiles;       // the tiles dealt to the splits: tile0 .. tile0 + tiles - 1
+    int owner, tail0, tails;  // the append's split and its block's tiles
+    int nsplit, block_log2;
+    float scale_log2;
+    bool prologue;
+    const float *qn_w, *kn_w, *vn_w;
+    float eps;
+    const float *rcos, *rsin;
+};
+
+// Two codes as packed f16, exact: their bytes (the sign bit flipped, so 0..255) become the low
+// bits of 1024 + byte, from which 1152 is subtracted. sel picks the bytes of w (0..3).
+__device__ __forceinline__ unsigned codes_f16(unsigned flipped, bool high) {
+    const unsigned b = __builtin_amdgcn_perm(0x64646464u, flipped, high ? 0x04030402u : 0x04010400u);
+    const f16x2 off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+    return __builtin_bit_cast(unsigned, __builtin_bit_cast(f16x2, b) + off);
+}
+
+__device__ __forceinline__ unsigned pk_f16(float a, float b) {  // (rounded toward zero)
+    return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(a, b));
+}
+__device__ __forceinline__ float f16_lo(unsigned w) {
+    return (float)__builtin_bit_cast(_Float16, (unsigned short)(w & 0xFFFFu));
+}
+__device__ __forceinline__ float f16_hi(unsigned w) {
+    return (float)__builtin_bit_cast(_Float16, (unsigned short)(w >> 16));
+}
+
+// First dim of lane group g's 8 dims in 32-dim chunk c: a 16-byte load holds 16 dims, the first 8
+// in chunk 2C, the rest in chunk 2C + 1.
+__device__ __forceinline__ int chunk_dim(int c, int g) { return 64 * (c / 2) + 16 * g + 8 * (c % 2); }
+
+// hd: the rows' head dim, at most HD; what a lane reads past it (the next head's codes, or zeros
+// past the cache) meets q's zeros in the scores and is not stored from the output.
+template <int HD>
+__global__ __launch_bounds__(kThreads, 2) void decode_i8_kernel(Args a, int hd) {
+    using S = Shape<HD>;
+    constexpr int NC = S::NC, KL = S::KL, DV = S::DV, VW = S::VW, QS = S::QS;
+    extern __shared__ float smem[];
+    const int tid = threadIdx.x;
+    const int lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 15;
+    const int g4 = lane >> 4;
+    const int hkv = (int)a.c.hkv;
+    const int kvh = blockIdx.x % hkv;
+    const int col0 = (int)(blockIdx.x / hkv) * kCols;
+    const int ncol = min(kCols, a.ncols - col0);
+    const int split = blockIdx.y;
+    const bool owner = a.knew != nullptr && split == a.owner;
+    const int lds_rows = max(kCols, kWaves * ncol);
+    float *s_q = smem;
+    float *s_new = smem + lds_rows * QS;
+    int *s_qe = reinterpret_cast<int *>(s_new + 2 * HD);
+    float *s_m = reinterpret_cast<float *>(s_qe + kCols);
+    float *s_l = s_m + kCols * kWaves;
+
+    // ---- tile loads ------------------------------------------------------------------------
+    const int row_bytes = hkv * hd;
+    const int end = a.pos0 + a.rows;  // keys held
+    const int kvo = n * row_bytes + 16 * g4;
+    const int vvo = 4 * g4 * row_bytes + DV * n;
+    const uint8_t *kbase = a.c.k + (size_t)kvh * hd, *vbase = a.c.v + (size_t)kvh * hd;
+    struct Tile {
+        unsigned k[KL][4], v[4][VW];
+        unsigned ek, ev;
+    };
+    // Tile t of the cache; one at or past the last key reads zeros and touches no memory.
+    auto load_tile = [&](int t, Tile &x) {
+        const int r0 = t * kTile;
+        const int left = min(end - r0, kTile);
+        const int nbytes = left > 0 ? (left - 1) * row_bytes + hd : 0;
+        const size_t off = left > 0 ? (size_t)r0 * row_bytes : 0;
+        const __amdgpu_buffer_rsrc_t kres = eb::make_rsrc(kbase + off, nbytes);
+        const __amdgpu_buffer_rsrc_t vres = eb::make_rsrc(vbase + off, nbytes);
+#pragma unroll
+        for (int c = 0; c < KL; ++c) {
+            const u32x4 w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(kres, kvo, 64 * c, 0));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x.k[c][i] = w[i];
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int vo = vvo + r * row_bytes;
+            if constexpr (VW == 4) {
+                const u32x4 w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(vres, vo, 0, 0));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x.v[r][i] = w[i];
+            } else if constexpr (VW == 2) {
+                const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(vres, vo, 0, 0));
+                x.v[r][0] = w[0];
+                x.v[r][1] = w[1];
+            } else {
+                x.v[r][0] = __builtin_amdgcn_raw_buffer_load_b32(vres, vo, 0, 0);
+            }
+        }
+        const size_t b = left > 0 ? (size_t)(r0 >> a.block_log2) * hkv + kvh : 0;
+        x.ek = a.c.ks[b];
+        x.ev = a.c.vs[b];
+    };
+    // Local tile i of this wave (all waves and splits together walk one stretch of the cache).
+    auto tile_of = [&](int i) {
+        const int t = (i * kWaves + wave) * a.nsplit + split;
+        return t < a.tiles ? a.tile0 + t : INT_MAX / kTile;
+    };
+
+    // ---- q, its first loads, then the first two tiles' ---------------------------------------
+    for (int i = tid; i < kCols * (HD / 4); i += kThreads) {
+        const int c = i / (HD / 4), d = 4 * (i % (HD / 4));
+        const int cc = col0 + min(c, ncol - 1);
+        const size_t at = ((size_t)(cc / a.g) * a.h + kvh * a.g + cc % a.g) * hd + d;
+        const f32x4 x = d < hd ? *reinterpret_cast<const f32x4 *>(a.q + at) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        *reinterpret_cast<f32x4 *>(s_q + c * QS + d) = x;
+    }
+    if (owner)
+        for (int i = tid; i < 2 * (HD / 4); i += kThreads) {
+            const int d = 4 * (i % (HD / 4));
+            const float *src = (i < HD / 4 ? a.knew : a.vnew) + (size_t)kvh * hd + d;
+            *reinterpret_cast<f32x4 *>(s_new + (i / (HD / 4)) * HD + d) =
+                d < hd ? *reinterpret_cast<const f32x4 *>(src) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+    Tile ta, tb;
+    load_tile(tile_of(0), ta);
+    load_tile(tile_of(1), tb);
+    __syncthreads();
+
+    // Row jobs: the columns' q, then the new K and V rows. A lane owns the dim pairs (p, p + hd/2),
+    // so that RMSNorm and RoPE never read another lane's dims.
+    {
+        constexpr int NP = (HD / 2 + 63) / 64;
+        const int half = hd / 2;
+        const size_t trow = (size_t)a.pos0 * half;
+        const int njobs = owner ? ncol + 2 : ncol;
+        for (int job = wave; job < njobs; job += kWaves) {
+            float *x = job < ncol ? s_q + job * QS : s_new + (job - ncol) * HD;
+            const float *w = !a.prologue ? nullptr : job < ncol ? a.qn_w : job == ncol ? a.kn_w : a.vn_w;
+            const bool rope = a.prologue && a.rcos && job <= ncol;
+            float x1[NP], x2[NP];
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const int p = lane + 64 * i;
+                x1[i] = p < half ? x[p] : 0.0f;
+                x2[i] = p < half ? x[p + half] : 0.0f;
+            }
+            if (w) {  // x * (1 / sqrt(mean x^2 + eps)) * w
+                float ss = 0.0f;
+#pragma unroll
+                for (int i = 0; i < NP; ++i) ss += x1[i] * x1[i] + x2[i] * x2[i];
+                ss = eb::class_reduce<1, false>(ss);
+                const float inv = 1.0f / sqrtf(ss / (float)hd + a.eps);
+#pragma unroll
+                for (int i = 0; i < NP; ++i) {
+                    const int p = lane + 64 * i;
+                    if (p < half) {
+                        x1[i] = x1[i] * inv * w[p];
+                        x2[i] = x2[i] * inv * w[p + half];
+                    }
+                }
+            }
+            if (rope) {  // pairs (p, p + hd/2), without fused multiply-adds as the row pass
+#pragma unroll
+                for (int i = 0; i < NP; ++i) {
+                    const int p = lane + 64 * i;
+                    if (p < half) {
+                        const float cs = a.rcos[trow + p], sn = a.rsin[trow + p];
+                        const float y1 = __fsub_rn(__fmul_rn(x1[i], cs), __fmul_rn(x2[i], sn));
+                        const float y2 = __fadd_rn(__fmul_rn(x2[i], cs), __fmul_rn(x1[i], sn));
+                        x1[i] = y1;
+                        x2[i] = y2;
+                    }
+                }
+            }
+            int ex = 0;
+            if (job < ncol) {  // q * scale * log2(e), then the column's power of two
+                float top = 0.0f;
+#pragma unroll
+                for (int i = 0; i < NP; ++i) {
+                    x1[i] *= a.scale_log2;
+                    x2[i] *= a.scale_log2;
+                    top = fmaxf(top, fmaxf(fabsf(x1[i]), fabsf(x2[i])));
+                }
+                top = eb::class_reduce<1, true>(top);
+                if (top > 0.0f && top <= 3.0e38f) {
+                    frexpf(top, &ex);
+                    ex = 14 - ex;
+                }
+                if (lane == 0) s_qe[job] = -ex;
+            }
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const int p = lane + 64 * i;
+                if (p < half) {
+                    x[p] = ldexpf(x1[i], ex);
+                    x[p + half] = ldexpf(x2[i], ex);
+                }
+            }
+        }
+    }
+    __syncthreads();
+
+    // ---- the append ---------------------------------------------------------------------------
+    if (owner && wave < 2) {  // wave 0: K, wave 1: V
+        uint8_t *codes = (wave ? a.c.v : a.c.k) + (size_t)kvh * hd;
+        uint8_t *exps = wave ? a.c.vs : a.c.ks;
+        const float *x = s_new + wave * HD;
+        const int b = a.pos0 >> a.block_log2, first = b << a.block_log2, lead = a.pos0 - first;
+        const unsigned old_e = lead ? exps[(size_t)b * hkv + kvh] : 0u;
+        const int d = 4 * lane;
+        f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (d < hd) y = *reinterpret_cast<const f32x4 *>(x + d);
+        unsigned top = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned u = eb::magnitude_bits(y[i]);
+            top = u > top ? u : top;
+        }
+#pragma unroll
+        for (int m = 32; m > 0; m >>= 1) {
+            const unsigned o = __shfl_xor(top, m);
+            top = o > top ? o : top;
+        }
+        unsigned e = eb::i8_exponent(top);
+        if (lead) e = eb::i8_join(old_e, e);
+        if (d < hd) {
+            unsigned w = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w |= eb::i8_code(y[i], e) << (8 * i);
+            *reinterpret_cast<unsigned *>(codes + (size_t)a.pos0 * row_bytes + d) = w;
+        }
+        if (lead && e != old_e && e != eb::kNanExponent) {
+            const int per_row = hd / 4;
+            for (int i = lane; i < lead * per_row; i += 64) {
+                unsigned *p = reinterpret_cast<unsigned *>(codes + (size_t)(first + i / per_row) * row_bytes +
+                                                           4 * (i % per_row));
+                *p = eb::i8_recode(*p, old_e, e);
+            }
+        }
+        if (lane == 0) exps[(size_t)b * hkv + kvh] = (uint8_t)e;
+    }
+    // The block's tiles are loaded below, after a barrier that completes these stores.
+
+    // ---- operands and state -------------------------------------------------------------------
+    const int own = min(n, ncol - 1);  // this lane's column (the last one, repeated, past ncol)
+    f16x8 qh[NC], ql[NC];
+    const int qe = s_qe[own];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const float *src = s_q + own * QS + chunk_dim(c, g4);
+        const f32x4 v0 = *reinterpret_cast<const f32x4 *>(src);
+        const f32x4 v1 = *reinterpret_cast<const f32x4 *>(src + 4);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float v = j < 4 ? v0[j % 4] : v1[j % 4];
+            const _Float16 hi = (_Float16)v;
+            qh[c][j] = hi;
+            ql[c][j] = (_Float16)(v - (float)hi);
+        }
+    }
+    const int my_pos = a.pos0 + (col0 + own) / a.g;  // the column's last key
+    const int my_first = a.window > 0 ? my_pos - a.window + 1 : 0;  // and its first
+    // Tiles wholly inside every column's keys need no mask.
+    const int safe_lo = a.window > 0 ? end - a.window : 0, safe_hi = a.pos0;
+    f32x4 acc[DV];
+#pragma unroll
+    for (int e = 0; e < DV; ++e) acc[e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f, u = kNoUnit;  // per lane: of its own column
+
+    auto consume = [&](int t, const Tile &x) {
+        const int k0 = t * kTile;
+        if (k0 >= end) return;  // (uniform)
+        f32x4 s1 = {0.0f, 0.0f, 0.0f, 0.0f}, s2 = s1;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const unsigned w0 = x.k[c / 2][2 * (c % 2)] ^ 0x80808080u;
+            const unsigned w1 = x.k[c / 2][2 * (c % 2) + 1] ^ 0x80808080u;
+            const f16x8 kk = __builtin_bit_cast(f16x8, u32x4{codes_f16(w0, false), codes_f16(w0, true),
+                                                             codes_f16(w1, false), codes_f16(w1, true)});
+            s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, qh[c], s1, 0, 0, 0);
+            s2 = __builtin_amdgcn_mfma_f32_16x16x32_f16(kk, ql[c], s2, 0, 0, 0);
+        }
+        const float cs = eb::i8_scale(x.ek, qe);
+        float sc[4], w[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sc[r] = (s1[r] + s2[r]) * cs;
+        const bool edge = k0 < safe_lo || k0 + kTile - 1 > safe_hi;  // (uniform)
+        if (edge) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int key = k0 + 4 * g4 + r;
+                if (key > my_pos || key < my_first) sc[r] = -INFINITY;
+            }
+        }
+        // A score above m + slack moves m; a term above 2^(u + slack) in V's units moves u (but
+        // weights below 2^-126 are nothing, whatever their V's scale).
+        const float ev = (float)((int)x.ev - 127);
+        const float top = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
+        const float over = top - m;
+        if (__builtin_amdgcn_ballot_w64(over > fminf(kSlack, fmaxf(u + kSlack - ev, -126.0f)) ||
+                                        (m == -INFINITY && top > -INFINITY)) != 0) {
+            float t1 = fmaxf(top, eb::lane_xor16(top));
+            t1 = fmaxf(t1, eb::lane_xor32(t1));  // the column's largest score in the tile
+            const float mn = m == -INFINITY || t1 > m + kSlack ? t1 : m;
+            const float d = mn == m ? 0.0f : mn - m;  // (infinite at the column's first keys)
+            const float ub = d < 1.0e6f ? u - floorf(d) : kNoUnit;
+            const float x1 = ceilf(t1 - mn);
+            const float un = x1 > -126.0f && x1 + ev > ub + kSlack ? x1 + ev : ub;
+            const float f = d < 1.0e6f ? eb::fast_exp2((u - un) - d) : 0.0f;
+            l *= d < 1.0e6f ? eb::fast_exp2(-d) : 0.0f;
+            m = mn;
+            u = un;
+            // the accumulators' columns are 4 g4 + r: their factors from those columns' lanes
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float fr = __shfl(f, 4 * g4 + r);
+#pragma unroll
+                for (int e = 0; e < DV; ++e) acc[e][r] *= fr;
+            }
+        }
+        const float mref = m == -INFINITY ? 0.0f : m;
+        const float vs = x.ev == eb::kNanExponent ? __builtin_nanf("") : ldexpf(1.0f, (int)fminf(ev - u + 7.0f, 126.0f));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float p = eb::fast_exp2(sc[r] - mref);
+            l += p;
+            w[r] = p * vs;
+        }
+        if (edge) {  // (a NaN scale does not reach keys that the column does not see)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (sc[r] == -INFINITY) w[r] = 0.0f;
+        }
+        const unsigned h01 = pk_f16(w[0], w[1]), h23 = pk_f16(w[2], w[3]);
+        const unsigned l01 = pk_f16(w[0] - f16_lo(h01), w[1] - f16_hi(h01));
+        const unsigned l23 = pk_f16(w[2] - f16_lo(h23), w[3] - f16_hi(h23));
+        const f16x8 pp = __builtin_bit_cast(f16x8, u32x4{h01, h23, l01, l23});
+        unsigned vx[4][VW];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int i = 0; i < VW; ++i) vx[r][i] = x.v[r][i] ^ 0x80808080u;
+#pragma unroll
+        for (int e = 0; e < DV; e += 2) {
+            // bytes e, e + 1 of rows 0, 1 (and 2, 3) as [r0.e, r1.e, r0.e+1, r1.e+1]
+            const unsigned k = (unsigned)(e % 4);
+            const unsigned sel = k | (4u + k) << 8 | (k + 1u) << 16 | (5u + k) << 24;
+            const unsigned b01 = __builtin_amdgcn_perm(vx[1][e / 4], vx[0][e / 4], sel);
+            const unsigned b23 = __builtin_amdgcn_perm(vx[3][e / 4], vx[2][e / 4], sel);
+            const unsigned c0 = codes_f16(b01, false), c1 = codes_f16(b23, false);
+            const unsigned d0 = codes_f16(b01, true), d1 = codes_f16(b23, true);
+            acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pp, __builtin_bit_cast(f16x8, u32x4{c0, c1, c0, c1}),
+                                                            acc[e], 0, 0, 0);
+            acc[e + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                pp, __builtin_bit_cast(f16x8, u32x4{d0, d1, d0, d1}), acc[e + 1], 0, 0, 0);
+        }
+    };
+
+    // ---- the tiles, in pairs, each buffer refilled once consumed --------------------------------
+    const int mine = a.tiles > split ? (a.tiles - split + a.nsplit - 1) / a.nsplit : 0;
+    const int steps = (mine + kWaves - 1) / kWaves;
+    for (int i = 0; i < steps; i += 2) {
+        consume(tile_of(i), ta);
+        load_tile(tile_of(i + 2), ta);
+        if (i + 1 < steps) consume(tile_of(i + 1), tb);
+        load_tile(tile_of(i + 3), tb);
+    }
+    if (owner) {  // (uniform over the workgroup)
+        __threadfence_block();
+        __syncthreads();
+        for (int t = wave; t < a.tails; t += kWaves) {
+            load_tile(a.tail0 + t, ta);
+            consume(a.tail0 + t, ta);
+        }
+    }
+
+    // ---- the waves' states meet in LDS ----------------------------------------------------------
+    l += eb::lane_xor16(l);
+    l += eb::lane_xor32(l);
+    __syncthreads();  // (q's rows are read no more)
+    float *s_acc = smem + wave * ncol * QS;
+    if (g4 == 0 && n < ncol) {
+        s_m[n * kWaves + wave] = m;
+        s_l[n * kWaves + wave] = l;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int c = 4 * g4 + r;
+        const float back = ldexpf(1.0f, (int)fmaxf(__shfl(u, c) - 7.0f, -1000.0f));
+        if (c < ncol) {
+#pragma unroll
+            for (int e = 0; e < DV; e += 4)
+                *reinterpret_cast<f32x4 *>(s_acc + c * QS + DV * n + e) =
+                    f32x4{acc[e][r] * back, acc[e + 1][r] * back, acc[e + 2][r] * back, acc[e + 3][r] * back};
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < ncol * hd; i += kThreads) {
+        const int c = i / hd, d = i % hd;
+        const f32x4 m4 = *reinterpret_cast<const f32x4 *>(s_m + c * kWaves);
+        const f32x4 l4 = *reinterpret_cast<const f32x4 *>(s_l + c * kWaves);
+        const float M = fmaxf(fmaxf(m4.x, m4.y), fmaxf(m4.z, m4.w));
+        const float mref = M == -INFINITY ? 0.0f : M;
+        float A = 0.0f, L = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float f = eb::fast_exp2(m4[w] - mref);
+            A += f * smem[(w * ncol + c) * QS + d];
+            L += f * l4[w];
+        }
+        const int cc = col0 + c;
+        const size_t at = (size_t)(cc / a.g) * a.h + kvh * a.g + cc % a.g;
+        if (a.nsplit == 1) {
+            a.o[at * hd + d] = A / L;
+        } else {
+            const size_t slot = (size_t)split * a.rows * a.h + at;
+            a.part_acc[slot * hd + d] = A;
+            if (d == 0) {
+                a.part_ml[slot * 2 + 0] = M;
+                a.part_ml[slot * 2 + 1] = L;
+            }
+        }
+    }
+}
+
+struct Plan {
+    int nsub, nsplit, tile0, tiles, tail0, tails;
+    bool fused;
+};
+
+// Splits: enough workgroups for two on every CU, each wave with at least one tile; fewer than
+// kMinSplitKeys keys stay in one workgroup (a second launch costs more than the split saves).
+constexpr size_t kMinSplitKeys = 128;
+constexpr int kWgsPerCu = 2;
+constexpr size_t kMaxSplits = 256;
+Plan plan_of(size_t h, size_t hkv, size_t pos0, size_t rows, size_t block, size_t window, bool append,
+             int cu_count) {
+    Plan p{};
+    const size_t cols = rows * (h / hkv);
+    p.nsub = (int)((cols + kCols - 1) / kCols);
+    p.fused = append && p.nsub == 1;
+    const size_t end = pos0 + rows;
+    const size_t first = window > 0 && pos0 + 1 > window ? pos0 + 1 - window : 0;
+    size_t stop = (end + kTile - 1) / kTile;
+    p.tile0 = (int)(first / kTile);
+    if (p.fused) {
+        const size_t b0 = std::max(pos0 / block * block / kTile, (size_t)p.tile0);
+        p.tail0 = (int)b0;
+        p.tails = (int)(stop - b0);
+        stop = b0;
+    }
+    p.tiles = (int)(stop - p.tile0);
+    size_t nsplit = std::max<size_t>(1, (size_t)cu_count * kWgsPerCu / (hkv * p.nsub));
+    nsplit = std::min(nsplit, std::max<size_t>(1, (size_t)p.tiles / kWaves));
+    nsplit = std::min(nsplit, kMaxSplits);
+    if (end - first < kMinSplitKeys) nsplit = 1;
+    p.nsplit = (int)nsplit;
+    return p;
+}
+
+template <int HD>
+hipError_t launch(hipStream_t st, const Args &a, const Plan &p, size_t hd) {
+    const size_t lds = Shape<HD>::lds_floats(std::min(kCols, a.ncols)) * sizeof(float);
+    static_assert(Shape<HD>::lds_floats(kCols) * sizeof(float) <= 80 * 1024, "two workgroups per CU");
+    if (lds > 64 * 1024) {
+        static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&decode_i8_kernel<HD>),
+                                                        hipFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);
+        if (e != hipSuccess) return e;
+    }
+    decode_i8_kernel<HD><<<dim3((unsigned)(a.c.hkv * p.nsub), (unsigned)p.nsplit), kThreads, lds, st>>>(a, (int)hd);
+    return hipSuccess;
+}
+
+}  // namespace
+
+namespace eb {
+
+// Workspace (floats): part_acc [nsplit * rows * h * hd], part_ml [nsplit * rows * h * 2]; a
+// window only lowers the splits.
+size_t decode_i8_workspace_floats(size_t h, size_t hkv, size_t pos0, size_t rows, size_t hd, size_t block,
+                                  int cu_count) {
+    size_t n = 0;
+    for (int append = 0; append < 2; ++append) {
+        const Plan p = plan_of(h, hkv, pos0, rows, block, 0, append && rows == 1, cu_count);
+        if (p.nsplit > 1) n = std::max(n, (size_t)p.nsplit * rows * h * (hd + 2));
+    }
+    return n;
+}
+
+eb_status launch_attn_decode_i8(hipStream_t st, const float *q, const CacheI8 &c, const float *knew,
+                                const float *vnew, float *o, size_t h, size_t pos0, size_t rows, float scale,
+                                size_t window, float *ws, size_t ws_floats, int cu_count,
+                                const DecodePrologue *pro) {
+    const Plan p = plan_of(h, c.hkv, pos0, rows, c.block, window, knew != nullptr, cu_count);
+    if (knew && !p.fused) {
+        if (pro) return fail(EB_OTHER, "attn_decode_i8: more than %d heads per KV head need the row pass", kCols);
+        const eb_status s = launch_kv_write_i8(st, c, knew, vnew, pos0, 1);
+        if (s != EB_OK) return s;
+    }
+    const size_t need = p.nsplit > 1 ? (size_t)p.nsplit * rows * h * (c.hd + 2) : 0;
+    if (need > 0 && (!ws || ws_floats < need))
+        return fail(EB_SHAPE_MISMATCH, "attn_decode_i8: workspace holds %zu floats, needs %zu", ws_floats, need);
+    Args a{};
+    a.q = q;
+    a.c = c;
+    a.knew = p.fused ? knew : nullptr;
+    a.vnew = p.fused ? vnew : nullptr;
+    a.o = o;
+    a.part_acc = ws;
+    a.part_ml = ws ? ws + (size_t)p.nsplit * rows * h * c.hd : nullptr;
+    a.h = (int)h;
+    a.g = (int)(h / c.hkv);
+    a.rows = (int)rows;
+    a.ncols = (int)(rows * (h / c.hkv));
+    a.pos0 = (int)pos0;
+    a.window = (int)std::min<size_t>(window, INT_MAX);
+    a.tile0 = p.tile0;
+    a.tiles = p.tiles;
+    a.owner = p.tiles % p.nsplit;  // (the first split that has one tile less, if any)
+    a.tail0 = p.tail0;
+    a.tails = p.tails;
+    a.nsplit = p.nsplit;
+    while ((size_t)1 << a.block_log2 < c.block) ++a.block_log2;
+    a.scale_log2 = scale * kLog2e;
+    if (pro) {
+        a.prologue = true;
+        a.qn_w = pro->q_norm;
+        a.kn_w = pro->k_norm;
+        a.vn_w = pro->v_norm;
+        a.eps = pro->eps;
+        a.rcos = pro->rope_cos;
+        a.rsin = pro->rope_sin;
+    }
+    const hipError_t e = c.hd <= 64    ? launch<64>(st, a, p, c.hd)
+                         : c.hd <= 128 ? launch<128>(st, a, p, c.hd)
+                                       : launch<256>(st, a, p, c.hd);
+    if (e != hipSuccess) return hip_fail(e, "attn_decode_i8 launch set-up");
+    eb_status s = check_launch("attn_decode_i8");
+    if (s != EB_OK || p.nsplit == 1) return s;
+    return launch_decode_merge(st, a.part_acc, a.part_ml, o, rows * h, c.hkv, c.hd, p.nsplit);
+}
+
+}  // namespace eb

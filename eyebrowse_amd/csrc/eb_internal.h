@@ -7,6 +7,8 @@
 #include <cstdarg>
 #include <cstddef>
 #include <cstdint>
+#include <initializer_list>
+#include <mutex>
 
 #include "eyebrowse_hip.h"
 
@@ -32,6 +34,8 @@ eb_status check_launch(const char *kernel);
 // Shared argument checks. Each returns EB_OK or records why the shape is refused.
 eb_status check_ptr(const void *p, const char *name);
 eb_status check_numel(size_t have, size_t need, const char *name);
+// (the product of dims, refused when it wraps)
+eb_status check_numel(size_t have, std::initializer_list<size_t> dims, const char *name);
 eb_status check_heads(size_t h, size_t hkv);
 // Head dims the attention kernels serve: 4, every multiple of 8 up to 128 and every multiple
 // of 16 up to 256. Decode is instantiated for each (X-macro below); prefill runs the next
@@ -43,8 +47,21 @@ bool attn_head_dim_supported(size_t hd);
 // Largest element count a 32-bit-indexed kernel may address.
 constexpr size_t kMaxIndex = (size_t)1 << 31;
 
+// One layer of a block-scaled 8-bit cache (eb_cache_i8.h) in device memory.
+struct CacheI8 {
+    uint8_t *k, *ks, *v, *vs;  // codes [max_seq, hkv, hd], exponents [ceil(max_seq / block), hkv]
+    size_t max_seq, hkv, hd, block;
+};
+
 // The device that owns a tensor.
 eb_device *tensor_device(const eb_tensor *t);
+
+// Entry points outside eb_runtime.cpp: the recorder may record (its device becomes current and goes
+// to *dev), an operand of a type on that device, and the device's workspace, grown to hold
+// `floats` and handed out with its mutex held in *lk until the launch is enqueued.
+eb_status recorder_ready(eb_recorder *rec, eb_device **dev);
+eb_status check_tensor(const eb_tensor *t, eb_dtype dt, const char *name, eb_device *dev);
+eb_status device_workspace(eb_device *dev, size_t floats, float **out, std::unique_lock<std::mutex> &lk);
 
 // Compute units of the current device (cached per ordinal).
 int current_cu_count();
@@ -152,6 +169,30 @@ eb_status launch_attn_prefill_chunk_cache(hipStream_t st, const float *q, const 
                                           size_t pos0, size_t rows, size_t hd, float scale,
                                           size_t window, CacheElem ce, float *ws = nullptr,
                                           size_t ws_floats = 0);
+// ---- the block-scaled 8-bit cache (arguments checked by the caller; count, rows > 0) ---------
+// K and V rows k / v [count, hkv, hd] to rows dst.., and rows start.. as f32.
+eb_status launch_kv_write_i8(hipStream_t st, const CacheI8 &c, const float *k, const float *v, size_t dst,
+                             size_t count);
+eb_status launch_kv_read_i8(hipStream_t st, const CacheI8 &c, float *k, float *v, size_t start, size_t count);
+eb_status launch_fill_u8(hipStream_t st, uint8_t *p, uint8_t value, size_t n);
+// Few query rows, q [rows, h, hd] at positions pos0.., over the cache; with knew / vnew (one row)
+// they are appended at pos0 first, after the optional prologue (then at most 16 heads per KV head).
+// A workspace of decode_i8_workspace_floats serves any window.
+size_t decode_i8_workspace_floats(size_t h, size_t hkv, size_t pos0, size_t rows, size_t hd, size_t block,
+                                  int cu_count);
+eb_status launch_attn_decode_i8(hipStream_t st, const float *q, const CacheI8 &c, const float *knew,
+                                const float *vnew, float *o, size_t h, size_t pos0, size_t rows, float scale,
+                                size_t window, float *ws, size_t ws_floats, int cu_count,
+                                const DecodePrologue *pro = nullptr);
+constexpr size_t kDecodeI8Cols = 16;  // columns (rows x heads of a KV head) that share a workgroup
+// Causal attention of many rows; the workspace (16-byte aligned) is needed in full.
+size_t prefill_i8_workspace_floats(size_t h, size_t hkv, size_t hd, size_t pos0, size_t rows, size_t window);
+eb_status launch_attn_prefill_i8(hipStream_t st, const float *q, const CacheI8 &c, float *o, size_t h, size_t pos0,
+                                 size_t rows, float scale, size_t window, float *ws, size_t ws_floats);
+// The decode path's merge of split partials: part_acc [nsplit, h, hd], part_ml [nsplit, h, 2].
+eb_status launch_decode_merge(hipStream_t st, const float *part_acc, const float *part_ml, float *o, size_t h,
+                              size_t hkv, size_t hd, int nsplit);
+
 // Attention::decode after the projections as one fused step: RMSNorm (null gains: none)
 // and RoPE (null tables: none) of q and the new K row, RMSNorm of the new V row, the
 // cache-row write and the attention. Handle-level, used by eb_attention_forward_qkv.
@@ -187,6 +228,28 @@ size_t linear_usable_workspace_floats(const float *x, const uint16_t *const *w,
 eb_status launch_linear_f16w_multi(hipStream_t st, const float *x, const uint16_t *const *w,
                                    float *const *y, const size_t *out_f, int nseg, size_t m,
                                    size_t in_f, float *ws, size_t ws_floats);
+// linear_q4: nseg (1..kLinearMaxSegs) weight/output pairs that share x, in_f and group, with zero
+// points all or none; linear_q4_workspace_floats(m, in_f) floats, 16-byte aligned.
+struct Q4Weight {
+    const uint32_t *w;       // [out_f, in_f / 8]
+    const uint16_t *scales;  // [out_f, in_f / group]
+    const uint8_t *zeros;    // the same, or null
+    size_t in_f, out_f, group;
+};
+size_t linear_q4_workspace_floats(size_t m, size_t in_f);
+eb_status launch_linear_q4(hipStream_t st, const float *x, const Q4Weight *w, float *const *y, int nseg, size_t m,
+                           float *ws);
+// Sampling (arguments checked by the caller; rows, vocab > 0): a workspace of
+// sample_workspace_floats, 16-byte aligned.
+struct SampleArgs {
+    const float *logits, *u, *temperature;  // temperature .. min_p may be null
+    const uint32_t *top_k;
+    const float *top_p, *min_p;
+    uint32_t *out;
+    size_t rows, vocab;
+};
+size_t sample_workspace_floats(size_t rows, size_t vocab);
+eb_status launch_sample(hipStream_t st, const SampleArgs &a, float *ws);
 // argmax (sampling.rs:6-53 semantics): out[0] = winning index of x[0..n); workspace of
 // argmax_workspace_floats(n) floats, 8-byte aligned.
 size_t argmax_workspace_floats(size_t n);

@@ -9,24 +9,8 @@
 #include <memory>
 #include <vector>
 
+#include "eb_handles.h"
 #include "eb_internal.h"
-
-struct eb_rope_tables {
-    eb_tensor *cos = nullptr;
-    eb_tensor *sin = nullptr;
-    size_t head_dim = 0;
-    size_t max_seq = 0;
-};
-
-struct eb_kv_cache {
-    std::vector<eb_tensor *> k, v;
-    size_t max_seq = 0;
-    size_t n_kv_heads = 0;
-};
-
-struct eb_attention {
-    eb_attention_desc d{};
-};
 
 using eb::fail;
 
@@ -38,20 +22,7 @@ using eb::fail;
 
 namespace {
 
-// Owns a tensor for the duration of a forward; released (back to the pool) on scope exit.
-struct Owned {
-    eb_tensor *t = nullptr;
-    Owned() = default;
-    explicit Owned(eb_tensor *x) : t(x) {}
-    Owned(const Owned &) = delete;
-    Owned &operator=(const Owned &) = delete;
-    ~Owned() { eb_tensor_release(t); }
-    eb_tensor *release() {
-        eb_tensor *x = t;
-        t = nullptr;
-        return x;
-    }
-};
+using eb::Owned;
 
 eb_device *tensor_device_of(const eb_tensor *t) { return eb::tensor_device(t); }
 
@@ -155,6 +126,8 @@ void eb_kv_cache_release(eb_kv_cache *kv) {
     if (!kv) return;
     for (eb_tensor *t : kv->k) eb_tensor_release(t);
     for (eb_tensor *t : kv->v) eb_tensor_release(t);
+    for (eb_tensor *t : kv->k_scale) eb_tensor_release(t);
+    for (eb_tensor *t : kv->v_scale) eb_tensor_release(t);
     delete kv;
 }
 
@@ -240,6 +213,8 @@ extern "C" eb_status eb_attention_forward_qkv(const eb_attention *attn, eb_recor
         eb_tensor_numel(v) != rows * Hkv * hd)
         return fail(EB_SHAPE_MISMATCH, "attention_forward: q/k/v are not [rows, heads*head_dim]");
 
+    if (kv->block)
+        return eb::attention_forward_i8(d, rec, q, k, v, rope, kv, layer, rows, base_pos, out);
     const eb::CacheElem ce = eb_tensor_dtype(kc) == EB_F16    ? eb::CacheElem::F16
                              : eb_tensor_dtype(kc) == EB_F8E4M3 ? eb::CacheElem::E4M3
                                                                 : eb::CacheElem::F32;
@@ -312,7 +287,8 @@ extern "C" eb_status eb_attention_forward(const eb_attention *attn, eb_recorder 
     if (!attn || !rec || !x || !out) return fail(EB_OTHER, "attention_forward: null argument");
     *out = nullptr;
     const eb_attention_desc &d = attn->d;
-    if (!d.q_proj) return fail(EB_SHAPE_MISMATCH, "attention_forward: no projection weights");
+    if (!d.q_proj && !attn->q4)
+        return fail(EB_SHAPE_MISMATCH, "attention_forward: no projection weights");
     const size_t qd = d.n_heads * d.head_dim, kd = d.n_kv_heads * d.head_dim;
     if (eb_tensor_dtype(x) != EB_F32 || eb_tensor_numel(x) != rows * d.hidden)
         return fail(EB_SHAPE_MISMATCH, "attention_forward: x is not [rows, hidden] f32");
@@ -328,7 +304,10 @@ extern "C" eb_status eb_attention_forward(const eb_attention *attn, eb_recorder 
     const eb_tensor *w[3] = {d.q_proj, d.k_proj, d.v_proj};
     eb_tensor *c[3] = {q.t, k.t, v.t};
     const size_t of[3] = {qd, kd, kd};
-    EB_TRY(eb_linear_f16w_multi(rec, x, 3, w, c, of, rows, d.hidden));
+    if (attn->q4)
+        EB_TRY(eb_linear_q4_multi(rec, x, 3, attn->proj, c, rows));
+    else
+        EB_TRY(eb_linear_f16w_multi(rec, x, 3, w, c, of, rows, d.hidden));
     eb_tensor *ot = nullptr;
     EB_TRY(eb_attention_forward_qkv(attn, rec, q.t, k.t, v.t, rope, kv, layer, rows, base_pos,
                                     &ot));
@@ -337,7 +316,10 @@ extern "C" eb_status eb_attention_forward(const eb_attention *attn, eb_recorder 
     eb_tensor *yt = nullptr;
     EB_TRY(eb_tensor_empty(dev, ys, 2, EB_F32, &yt));
     Owned y(yt);
-    EB_TRY(eb_linear_f16w(rec, o.t, d.o_proj, y.t, rows, qd, d.hidden));
+    if (attn->q4)
+        EB_TRY(eb_linear_q4(rec, o.t, &attn->proj[3], y.t, rows));
+    else
+        EB_TRY(eb_linear_f16w(rec, o.t, d.o_proj, y.t, rows, qd, d.hidden));
     *out = y.release();
     return eb::ok();
 }

@@ -47,6 +47,7 @@
 //
 // FLOPs per launch: 2*H*HD*T*(T+1) algorithmic (QK^T and PV over the causal pairs); the
 // kernel issues MFMA work for whole 32x32 tiles, i.e. slightly more on the diagonal.
+#include "eb_cache_i8.h"
 #include "eb_common.h"
 #include "eb_internal.h"
 
@@ -212,13 +213,17 @@ __device__ __forceinline__ int hv_chunk(int p, int c) { return C::KC + c * C::HD
 // T read as zero. Every element is assigned on every call (clamped addresses, selected
 // values): conditionally written register arrays end up in scratch memory.
 // EB: bytes per k/v element: 4 (f32), 2 (IEEE half) or 1 (OCP FP8 E4M3), converted to f32
-// here (exactly).
+// here (exactly); kCodes: the codes of a block-scaled cache with their exponents ks, vs, one for
+// 2^lb rows and a KV head (code * 2^(e - 127), exact in f32 too).
+constexpr int kCodes = -1;
 template <class C, int EB, bool NT = false>
 __device__ __forceinline__ void prefill_load_step(const void *__restrict__ k,
                                                   const void *__restrict__ v,
                                                   f32x4 (&rk)[C::NLD], f32x4 (&rv)[C::NLD],
                                                   int kb, int T, int Hkv, int kvh, int tid,
-                                                  int hdr) {
+                                                  int hdr, const uint8_t *__restrict__ ks = nullptr,
+                                                  const uint8_t *__restrict__ vs = nullptr,
+                                                  int lb = 0) {
     constexpr int HD = C::HD_;
 #pragma unroll
     for (int r = 0; r < C::NLD; ++r) {
@@ -240,6 +245,16 @@ __device__ __forceinline__ void prefill_load_step(const void *__restrict__ k,
                 *reinterpret_cast<const unsigned *>(static_cast<const uint8_t *>(k) + off));
             vx = eb::f8x4_to_f32(
                 *reinterpret_cast<const unsigned *>(static_cast<const uint8_t *>(v) + off));
+        } else if constexpr (EB == kCodes) {
+            const size_t b = (size_t)(min(key, T - 1) >> lb) * Hkv + kvh;
+            const float fk = eb::i8_scale(ks[b], 0), fv = eb::i8_scale(vs[b], 0);
+            const unsigned wk = *reinterpret_cast<const unsigned *>(static_cast<const uint8_t *>(k) + off);
+            const unsigned wv = *reinterpret_cast<const unsigned *>(static_cast<const uint8_t *>(v) + off);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                kx[i] = eb::i8_f32(wk, i) * fk;
+                vx[i] = eb::i8_f32(wv, i) * fv;
+            }
         } else {
             const f32x4 *kp = reinterpret_cast<const f32x4 *>(static_cast<const float *>(k) + off);
             const f32x4 *vp = reinterpret_cast<const f32x4 *>(static_cast<const float *>(v) + off);
@@ -517,11 +532,12 @@ __global__ __launch_bounds__(PresplitCfg<HD>::THREADS) void preconvert_kernel(
 // per key instead of once per workgroup that reads the key.
 
 // V16: records of the scores-accurate mode (V rows rounded to f16 as they are). Caches of
-// EB = 2 or 1 bytes an element get half images.
+// EB = 2 or 1 bytes an element, or of codes, get half images.
 template <int HD, int EB, bool NT, bool V16 = false>
 __global__ __launch_bounds__(PresplitCfg<HD>::THREADS) void presplit_kernel(
     const void *__restrict__ k, const void *__restrict__ v, float *__restrict__ ps, int nkeys,
-    int Hkv, int tlo, int nt, int hdr) {
+    int Hkv, int tlo, int nt, int hdr, const uint8_t *__restrict__ ks = nullptr,
+    const uint8_t *__restrict__ vs = nullptr, int lb = 0) {
     using C = PresplitCfg<HD>;
     static_assert(C::SPV, "pre-split needs the split V path");
     static_assert(C::BUF == PrefillCfg<HD, 4, 1, 1>::BUF &&
@@ -536,7 +552,8 @@ __global__ __launch_bounds__(PresplitCfg<HD>::THREADS) void presplit_kernel(
     // (The tile image is the record. Its padding past the exponents, and with V16 its V^T lo
     // halves and V exponents, are left as they are: nothing reads them.)
     f32x4 rk[C::NLD], rv[C::NLD];
-    prefill_load_step<C, EB, NT>(k, v, rk, rv, (tlo + t) * kTile, nkeys, Hkv, kvh, tid, hdr);
+    prefill_load_step<C, EB, NT>(k, v, rk, rv, (tlo + t) * kTile, nkeys, Hkv, kvh, tid, hdr, ks, vs,
+                                 lb);
     prefill_store_step<C, false, V16, HALF>(smem, rk, rv, 0, tid);
     __syncthreads();
     f32x4 *rec = reinterpret_cast<f32x4 *>(ps + ((size_t)kvh * nt + t) * IMGX);
@@ -1542,6 +1559,10 @@ struct PrefillRange {
     float *ws;   // workspace (null: no pre-split pass, no key chunks)
     size_t ws_floats;
     int hdr;     // the rows' head dim (at most the instantiation's; the rest reads as zeros)
+    // The exponents of a block-scaled cache (null: none) of 2^lb rows a block; its rows always
+    // become records, and its ce is F16, whose half images they are.
+    const uint8_t *ks = nullptr, *vs = nullptr;
+    int lb = 0;
 };
 
 // The instantiation a head dim runs on: the next power of two (4 .. 256). Head dims 48, 80,
@@ -1591,7 +1612,7 @@ size_t presplit_floats(size_t hd, size_t h, size_t hkv, const PrefillRange &r) {
     if (hd < 32 || r.rows <= 0 || r.nkeys <= 0) return 0;
     const int qb_rows = kTile * prefill_shape(hd, (int)h, (int)(h / hkv), r.rows).wph;
     const int nqb = (r.rows + qb_rows - 1) / qb_rows;
-    if (nqb < (hd > 128 ? kPresplitMinBlocks256 : kPresplitMinBlocks)) return 0;
+    if (!r.ks && nqb < (hd > 128 ? kPresplitMinBlocks256 : kPresplitMinBlocks)) return 0;
     const size_t rec = hd == 32    ? PrefillCfg<32, 4, 1, 1>::PS_FLOATS
                        : hd == 64  ? PrefillCfg<64, 4, 1, 1>::PS_FLOATS
                        : hd == 128 ? PrefillCfg<128, 4, 1, 1>::PS_FLOATS
@@ -1742,6 +1763,9 @@ eb_status launch_prefill_t(hipStream_t st, const float *q, const void *k, const 
             else if (PV1)
                 presplit_kernel<HD, 4, false, true><<<grid, PresplitCfg<HD>::THREADS, 0, st>>>(
                     k, v, ps, r.nkeys, Hkv, presplit_tlo(r), nt, r.hdr);
+            else if (r.ks)
+                presplit_kernel<HD, kCodes, false><<<grid, PresplitCfg<HD>::THREADS, 0, st>>>(
+                    k, v, ps, r.nkeys, Hkv, presplit_tlo(r), nt, r.hdr, r.ks, r.vs, r.lb);
             else if (r.ce == eb::CacheElem::F16)
                 presplit_kernel<HD, 2, false><<<grid, PresplitCfg<HD>::THREADS, 0, st>>>(
                     k, v, ps, r.nkeys, Hkv, presplit_tlo(r), nt, r.hdr);
@@ -1958,6 +1982,29 @@ size_t prefill_workspace_floats(size_t h, size_t hkv, size_t hd, size_t rows, si
     return workspace_floats(padded_hd(hd), (int)h, (int)hkv,
                             PrefillRange{(int)rows, (int)nkeys, (int)qbase, (int)window, CacheElem::F32,
                                          nullptr, 0, (int)hd});
+}
+
+static PrefillRange i8_range(size_t pos0, size_t rows, size_t hd, size_t window, const uint8_t *ks,
+                             const uint8_t *vs, size_t block, float *ws, size_t ws_floats) {
+    PrefillRange r{(int)rows, (int)(pos0 + rows), (int)pos0, (int)std::min<size_t>(window, pos0 + rows),
+                   CacheElem::F16, ws, ws_floats, (int)hd, ks, vs, 0};
+    while ((size_t)1 << r.lb < block) ++r.lb;
+    return r;
+}
+
+size_t prefill_i8_workspace_floats(size_t h, size_t hkv, size_t hd, size_t pos0, size_t rows, size_t window) {
+    const uint8_t some = 0;  // (any exponents: only whether there are some counts here)
+    return workspace_floats(padded_hd(hd), (int)h, (int)hkv,
+                            i8_range(pos0, rows, hd, window, &some, &some, 1, nullptr, 0));
+}
+
+eb_status launch_attn_prefill_i8(hipStream_t st, const float *q, const CacheI8 &c, float *o, size_t h, size_t pos0,
+                                 size_t rows, float scale, size_t window, float *ws, size_t ws_floats) {
+    if (ws_floats < prefill_i8_workspace_floats(h, c.hkv, c.hd, pos0, rows, window) || !ws ||
+        (reinterpret_cast<uintptr_t>(ws) & 15))
+        return fail(EB_SHAPE_MISMATCH, "attn_prefill_chunk_i8: workspace too small or not 16-byte aligned");
+    return launch_prefill_range(st, q, c.k, c.v, o, h, c.hkv, c.hd, scale,
+                                i8_range(pos0, rows, c.hd, window, c.ks, c.vs, c.block, ws, ws_floats));
 }
 
 eb_status launch_attn_prefill(hipStream_t st, const float *q, const float *k, const float *v,

@@ -258,7 +258,7 @@ size_t eb_dtype_size(eb_dtype dt) {
     switch (dt) {
         case EB_F32: case EB_U32: case EB_I32: return 4;
         case EB_F16: return 2;
-        case EB_F8E4M3: return 1;
+        case EB_F8E4M3: case EB_I8: case EB_U8: return 1;
     }
     return 0;
 }
@@ -1033,6 +1033,24 @@ static eb_status device_workspace_up_to(eb_device *dev, size_t want, size_t leas
 static eb_status device_workspace(eb_device *dev, size_t floats, float **out, WsLock &lk) {
     size_t got;
     return device_workspace_up_to(dev, floats, floats, out, &got, lk);
+}
+
+eb_status eb::device_workspace(eb_device *dev, size_t floats, float **out, WsLock &lk) {
+    return ::device_workspace(dev, floats, out, lk);
+}
+
+eb_status eb::recorder_ready(eb_recorder *rec, eb_device **dev) {
+    EB_TRY(rec_ready(rec));
+    *dev = rec->dev;
+    return EB_OK;
+}
+
+eb_status eb::check_tensor(const eb_tensor *t, eb_dtype dt, const char *name, eb_device *dev) {
+    static const char *const names[] = {"f32", "f16", "u32", "i32", "f8e4m3", "i8", "u8"};
+    if (!t) return fail(EB_SHAPE_MISMATCH, "%s is null", name);
+    if (t->dtype != dt) return fail(EB_SHAPE_MISMATCH, "%s must be %s", name, names[dt]);
+    if (t->dev != dev) return fail(EB_OTHER, "%s lives on another device", name);
+    return EB_OK;
 }
 
 // Room for floats that is the running capture's own: its graph keeps it, so that the capture

@@ -17,12 +17,15 @@ from ._lib import c_size, c_vp, lib
 
 class DType(enum.IntEnum):
     """crates/eyebrowse-core/src/lib.rs:8-25; F8E4M3 (OCP FP8 E4M3 KV caches, one byte per
-    element) has no counterpart in the reference."""
+    element), I8 (codes of block-scaled KV caches) and U8 (their exponents, 4-bit weights' zero
+    points) have no counterpart in the reference."""
     F32 = 0
     F16 = 1
     U32 = 2
     I32 = 3
     F8E4M3 = 4
+    I8 = 5
+    U8 = 6
 
     def size(self) -> int:
         return int(lib().eb_dtype_size(int(self)))
@@ -155,6 +158,19 @@ class Tensor:
                                        a.ctypes.data_as(ctypes.POINTER(ctypes.c_uint32)), a.size,
                                        ctypes.byref(out)))
         return cls(out.value, dev)
+
+    @classmethod
+    def from_array(cls, dev: Device, data) -> "Tensor":
+        """A tensor of the array's shape and bytes: float32, float16, uint32, int32, int8 or
+        uint8 elements (no counterpart in the reference)."""
+        a = np.ascontiguousarray(data)
+        types = {"float32": DType.F32, "float16": DType.F16, "uint32": DType.U32,
+                 "int32": DType.I32, "int8": DType.I8, "uint8": DType.U8}
+        if a.dtype.name not in types:
+            raise ShapeMismatch(f"from_array: no tensor type for {a.dtype}")
+        t = cls.empty(dev, a.shape, types[a.dtype.name])
+        t.write(a)
+        return t
 
     @classmethod
     def from_f16_packed(cls, dev: Device, logical_shape, data) -> "Tensor":

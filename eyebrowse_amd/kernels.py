@@ -4,7 +4,9 @@ caller-owned device memory.
 """
 from __future__ import annotations
 
-from ._lib import c_size, c_vp, lib
+import ctypes
+
+from ._lib import CacheI8, Q4Weight, c_size, c_vp, lib
 from .gpu import Recorder, Tensor, check
 
 
@@ -114,6 +116,132 @@ def linear_f16w_multi(rec: Recorder, a: Tensor, ws, cs, out_fs, m: int, in_f: in
 
 def linear_workspace_floats(m: int, in_f: int) -> int:
     return int(lib().eb_linear_workspace_floats(m, in_f))
+
+
+def linear_q4(rec: Recorder, a: Tensor, w, c: Tensor, m: int) -> None:
+    """c [m, out_f] = a [m, in_f] . W^T for a LinearQ4 w (no counterpart in the reference)."""
+    check(lib().eb_linear_q4(rec.handle, a.handle, ctypes.byref(w.desc), c.handle, m))
+
+
+def linear_q4_multi(rec: Recorder, a: Tensor, ws, cs, m: int) -> None:
+    """Up to three 4-bit projections of the same a in one launch: cs[i] = a . ws[i]^T."""
+    n = len(ws)
+    assert len(cs) == n
+    warr = (Q4Weight * max(n, 1))(*[w.desc for w in ws])
+    carr = (c_vp * max(n, 1))(*[t.handle for t in cs])
+    check(lib().eb_linear_q4_multi(rec.handle, a.handle, n, warr, carr, m))
+
+
+def linear_q4_workspace_floats(m: int, in_f: int) -> int:
+    return int(lib().eb_linear_q4_workspace_floats(m, in_f))
+
+
+def launch_linear_q4(stream: int, a_ptr: int, a_numel: int, w_ptr: int, w_words: int,
+                     scales_ptr: int, scales_numel: int, zeros_ptr: int, zeros_numel: int,
+                     c_ptr: int, c_numel: int, m: int, in_f: int, out_f: int, group: int,
+                     ws_ptr: int = 0, ws_floats: int = 0) -> None:
+    """linear_q4 on caller memory (zeros_ptr 0: zero point 8)."""
+    check(lib().eb_launch_linear_q4(c_vp(stream), a_ptr, a_numel, w_ptr, w_words, scales_ptr,
+                                    scales_numel, zeros_ptr or None, zeros_numel, c_ptr, c_numel,
+                                    m, in_f, out_f, group, ws_ptr or None, ws_floats))
+
+
+def kv_write_i8(rec: Recorder, kv, layer: int, k: Tensor, v: Tensor, count: int,
+                dst_start: int) -> None:
+    """K and V rows k, v [count, hkv, hd] to rows dst_start.. of a block-scaled KvCache's layer,
+    in one launch (no counterpart in the reference)."""
+    check(lib().eb_kv_write_i8(rec.handle, kv.handle, layer, k.handle, v.handle, count,
+                               dst_start))
+
+
+def kv_read_i8(rec: Recorder, kv, layer: int, k: Tensor, v: Tensor, count: int,
+               src_start: int) -> None:
+    """Rows src_start.. of a block-scaled KvCache's layer as f32 k, v [count, hkv, hd]."""
+    check(lib().eb_kv_read_i8(rec.handle, kv.handle, layer, k.handle, v.handle, count,
+                              src_start))
+
+
+def attn_decode_i8(rec: Recorder, q: Tensor, kv, layer: int, o: Tensor, h: int, pos: int,
+                   scale: float, window: int = 0) -> None:
+    """attn_decode_window over a block-scaled KvCache's layer."""
+    check(lib().eb_attn_decode_i8(rec.handle, q.handle, kv.handle, layer, o.handle, h, pos, scale,
+                                  window))
+
+
+def attn_decode_step_i8(rec: Recorder, q: Tensor, knew: Tensor, vnew: Tensor, kv, layer: int,
+                        o: Tensor, h: int, pos: int, scale: float, window: int = 0) -> None:
+    """kv_write_i8 of one row at pos, then attn_decode_i8, in one call."""
+    check(lib().eb_attn_decode_step_i8(rec.handle, q.handle, knew.handle, vnew.handle, kv.handle,
+                                       layer, o.handle, h, pos, scale, window))
+
+
+def attn_prefill_chunk_i8(rec: Recorder, q: Tensor, kv, layer: int, o: Tensor, h: int, pos0: int,
+                          rows: int, scale: float, window: int = 0) -> None:
+    """attn_prefill_chunk over a block-scaled KvCache's layer, which holds the rows already."""
+    check(lib().eb_attn_prefill_chunk_i8(rec.handle, q.handle, kv.handle, layer, o.handle, h,
+                                         pos0, rows, scale, window))
+
+
+def attn_i8_workspace_floats(h: int, hkv: int, hd: int, pos0: int, rows: int, block: int,
+                             window: int = 0, cu_count: int = 256) -> int:
+    return int(lib().eb_attn_i8_workspace_floats(h, hkv, hd, pos0, rows, block, window, cu_count))
+
+
+def launch_kv_write_i8(stream: int, cache: CacheI8, k_ptr: int, v_ptr: int, numel: int, count: int,
+                       dst_start: int) -> None:
+    check(lib().eb_launch_kv_write_i8(c_vp(stream), ctypes.byref(cache), k_ptr, v_ptr, numel, count,
+                                      dst_start))
+
+
+def launch_kv_read_i8(stream: int, cache: CacheI8, k_ptr: int, v_ptr: int, numel: int, count: int,
+                      src_start: int) -> None:
+    check(lib().eb_launch_kv_read_i8(c_vp(stream), ctypes.byref(cache), k_ptr, v_ptr, numel, count,
+                                     src_start))
+
+
+def launch_attn_decode_i8(stream: int, q_ptr: int, q_numel: int, knew_ptr: int, vnew_ptr: int,
+                          new_numel: int, cache: CacheI8, o_ptr: int, o_numel: int, h: int, pos: int,
+                          scale: float, window: int = 0, ws_ptr: int = 0, ws_floats: int = 0,
+                          cu_count: int = 256) -> None:
+    """attn_decode_step_i8 on caller memory (knew_ptr and vnew_ptr 0: attention alone)."""
+    check(lib().eb_launch_attn_decode_i8(c_vp(stream), q_ptr, q_numel, knew_ptr or None,
+                                         vnew_ptr or None, new_numel, ctypes.byref(cache), o_ptr,
+                                         o_numel, h, pos, scale, window, ws_ptr or None, ws_floats,
+                                         cu_count))
+
+
+def launch_attn_prefill_chunk_i8(stream: int, q_ptr: int, q_numel: int, cache: CacheI8, o_ptr: int,
+                                 o_numel: int, h: int, pos0: int, rows: int, scale: float,
+                                 window: int = 0, ws_ptr: int = 0, ws_floats: int = 0,
+                                 cu_count: int = 256) -> None:
+    check(lib().eb_launch_attn_prefill_chunk_i8(c_vp(stream), q_ptr, q_numel, ctypes.byref(cache),
+                                                o_ptr, o_numel, h, pos0, rows, scale, window,
+                                                ws_ptr or None, ws_floats, cu_count))
+
+
+def sample(rec: Recorder, logits: Tensor, u: Tensor, out_idx: Tensor, rows: int, vocab: int, *,
+           temperature: Tensor = None, top_k: Tensor = None, top_p: Tensor = None,
+           min_p: Tensor = None) -> None:
+    """The token each row of logits [rows, vocab] gives for its random number u[r] in [0, 1), kept
+    by its temperature, top-k, top-p and min-p ([rows] tensors, top_k U32; None: 1, off, off,
+    off). No counterpart in the reference, whose sampling is argmax."""
+    h = lambda t: t.handle if t is not None else None  # noqa: E731
+    check(lib().eb_sample(rec.handle, logits.handle, u.handle, out_idx.handle, rows, vocab,
+                          h(temperature), h(top_k), h(top_p), h(min_p)))
+
+
+def sample_workspace_floats(rows: int, vocab: int) -> int:
+    return int(lib().eb_sample_workspace_floats(rows, vocab))
+
+
+def launch_sample(stream: int, logits_ptr: int, logits_numel: int, u_ptr: int, out_ptr: int,
+                  rows: int, vocab: int, temperature_ptr: int = 0, top_k_ptr: int = 0,
+                  top_p_ptr: int = 0, min_p_ptr: int = 0, ws_ptr: int = 0,
+                  ws_floats: int = 0) -> None:
+    """sample on caller memory (a parameter's pointer 0: as None above)."""
+    check(lib().eb_launch_sample(c_vp(stream), logits_ptr, logits_numel, u_ptr, out_ptr, rows, vocab,
+                                 temperature_ptr or None, top_k_ptr or None, top_p_ptr or None,
+                                 min_p_ptr or None, ws_ptr or None, ws_floats))
 
 
 def argmax(rec: Recorder, logits: Tensor, out_idx: Tensor, vocab: int) -> None:

@@ -10,9 +10,11 @@ import ctypes
 from dataclasses import dataclass
 from typing import Optional
 
-from ._lib import AttentionDesc, c_size, c_vp, lib
-from .gpu import DType, Device, Recorder, Tensor, check
-from .kernels import linear_f16w
+import numpy as np
+
+from ._lib import AttentionDesc, Q4Weight, c_size, c_vp, lib
+from .gpu import DType, Device, Recorder, Tensor, UnsupportedConfig, check
+from .kernels import linear_f16w, linear_q4
 
 
 class _Borrowed(Tensor):
@@ -85,6 +87,53 @@ class Linear:
         return out
 
 
+class LinearQ4:
+    """A bias-free projection with 4-bit codes and group scales (no counterpart in the reference):
+    W[o, k] = (code[o, k] - zero[o, k // group]) * scale[o, k // group]. w: U32 [out_f, in_f / 8],
+    eight codes per word along k, lowest bits first; scales: F16 [out_f, in_f / group]; zeros: U8 of
+    that shape, or None (8 everywhere). group is 32, 64 or 128 and divides in_f."""
+
+    def __init__(self, w: Tensor, scales: Tensor, zeros: Optional[Tensor], in_f: int, out_f: int,
+                 group: int):
+        self.w, self.scales, self.zeros = w, scales, zeros
+        self.in_f, self.out_f, self.group = in_f, out_f, group
+
+    @property
+    def desc(self) -> Q4Weight:
+        return Q4Weight(self.w.handle, self.scales.handle,
+                        self.zeros.handle if self.zeros is not None else None, self.in_f,
+                        self.out_f, self.group)
+
+    @classmethod
+    def from_f32(cls, dev: Device, weight, group: int = 128, symmetric: bool = True) -> "LinearQ4":
+        """Round weight [out_f, in_f] to the nearest codes. Symmetric: scale = largest |w| of the
+        group / 7, zero point 8; else scale = (largest - smallest) / 15 over the group and 0."""
+        w = np.asarray(weight, np.float32)
+        out_f, in_f = w.shape
+        if group not in (32, 64, 128) or in_f % group:
+            raise UnsupportedConfig(f"LinearQ4: group {group} for in_f {in_f}")
+        x = w.reshape(out_f, in_f // group, group)
+        if symmetric:
+            s = (np.abs(x).max(-1) / 7).astype(np.float16)
+            z = np.full(s.shape, 8, np.uint8)
+        else:
+            lo, hi = np.minimum(x.min(-1), 0), np.maximum(x.max(-1), 0)
+            s = ((hi - lo) / 15).astype(np.float16)
+        d = np.where(s > 0, s, 1).astype(np.float32)  # (a group of zeros: scale 0, any code)
+        if not symmetric:
+            z = np.clip(np.rint(-lo / d), 0, 15).astype(np.uint8)
+        c = np.clip(np.rint(x / d[..., None]) + z[..., None], 0, 15).astype(np.uint32)
+        c = c.reshape(out_f, in_f // 8, 8)
+        words = np.bitwise_or.reduce(c << (4 * np.arange(8, dtype=np.uint32)), axis=-1)
+        return cls(Tensor.from_array(dev, words.astype(np.uint32)), Tensor.from_array(dev, s),
+                   None if symmetric else Tensor.from_array(dev, z), in_f, out_f, group)
+
+    def forward(self, rec: Recorder, x: Tensor, rows: int) -> Tensor:
+        out = Tensor.empty(rec.dev, (rows, self.out_f))
+        linear_q4(rec, x, self, out, rows)
+        return out
+
+
 class KvCache:
     """KvCache (crates/eyebrowse-nn/src/kv_cache.rs:9-50): per-layer K/V tensors
     [max_seq, n_kv_heads, head_dims[l]]."""
@@ -116,6 +165,31 @@ class KvCache:
                                                     n_kv_heads, int(dtype), ctypes.byref(out)))
         return cls(out.value, dev, len(head_dims), max_seq, n_kv_heads, DType(dtype))
 
+    @classmethod
+    def new_i8(cls, dev: Device, n_layers: int, max_seq: int, n_kv_heads: int, head_dim: int,
+               block: int = 64) -> "KvCache":
+        """A block-scaled 8-bit cache (no counterpart in the reference): int8 codes and one
+        power-of-two scale for each block of `block` rows and KV head; see new_i8_per_layer."""
+        return cls.new_i8_per_layer(dev, [head_dim] * n_layers, max_seq, n_kv_heads, block)
+
+    @classmethod
+    def new_i8_per_layer(cls, dev: Device, head_dims, max_seq: int, n_kv_heads: int,
+                         block: int = 64) -> "KvCache":
+        """k[l], v[l]: I8 codes [max_seq, n_kv_heads, head_dims[l]]; k_scale[l], v_scale[l]: U8
+        exponents e [ceil(max_seq / block), n_kv_heads]: a code stands for code * 2^(e - 127).
+        block: a power of two from 16 to 256; head dims: multiples of 16 from 32 to 256."""
+        arr = (c_size * max(1, len(head_dims)))(*head_dims)
+        out = c_vp()
+        check(lib().eb_kv_cache_new_i8(dev.handle, arr, len(head_dims), max_seq, n_kv_heads, block,
+                                       ctypes.byref(out)))
+        kv = cls(out.value, dev, len(head_dims), max_seq, n_kv_heads, DType.I8)
+        kv.block = block
+        kv.k_scale = [_Borrowed(lib().eb_kv_cache_k_scale(kv._h, l), dev, kv)
+                      for l in range(len(head_dims))]
+        kv.v_scale = [_Borrowed(lib().eb_kv_cache_v_scale(kv._h, l), dev, kv)
+                      for l in range(len(head_dims))]
+        return kv
+
     @property
     def handle(self):
         return self._h
@@ -131,7 +205,8 @@ class KvCache:
 class Attention:
     """Attention (crates/eyebrowse-nn/src/attention.rs:10-23): head counts, scale, optional
     per-head q/k/v RMSNorm weights ([head_dim] f32 tensors) and, optionally, the four
-    packed-f16 projections (all or none) with the model width `hidden`."""
+    packed-f16 projections (all or none) with the model width `hidden`; or, with `hidden`, the four
+    as 4-bit LinearQ4 in q4."""
     n_heads: int
     n_kv_heads: int
     head_dim: int
@@ -146,6 +221,7 @@ class Attention:
     v_proj: Optional[Tensor] = None
     o_proj: Optional[Tensor] = None  # [hidden, n_heads*head_dim]
     hidden: int = 0
+    q4: Optional[tuple] = None  # (q, k, v, o) LinearQ4; q, k and v share group and zero points
 
     def __post_init__(self):
         h = lambda t: t.handle if t is not None else None  # noqa: E731
@@ -154,7 +230,12 @@ class Attention:
                           h(self.q_proj), h(self.k_proj), h(self.v_proj), h(self.o_proj),
                           self.hidden)
         out = c_vp()
-        check(lib().eb_attention_new(ctypes.byref(d), ctypes.byref(out)))
+        if self.q4 is not None:
+            q, k, v, o = self.q4
+            proj = (Q4Weight * 4)(q.desc, k.desc, v.desc, o.desc)
+            check(lib().eb_attention_new_q4(ctypes.byref(d), proj, ctypes.byref(out)))
+        else:
+            check(lib().eb_attention_new(ctypes.byref(d), ctypes.byref(out)))
         self._h = out
 
     def forward_qkv(self, rec: Recorder, q: Tensor, k: Tensor, v: Tensor, rope: Rope,

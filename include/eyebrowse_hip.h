@@ -41,8 +41,12 @@ typedef enum eb_status {
 } eb_status;
 
 /* EB_F32 .. EB_I32 mirror DType (crates/eyebrowse-core/src/lib.rs:8-25). EB_F8E4M3 (OCP FP8
- * E4M3, one byte per element, for KV caches) has no counterpart in the reference. */
-typedef enum eb_dtype { EB_F32 = 0, EB_F16 = 1, EB_U32 = 2, EB_I32 = 3, EB_F8E4M3 = 4 } eb_dtype;
+ * E4M3, one byte per element, for KV caches), EB_I8 (the codes of block-scaled KV caches) and
+ * EB_U8 (their exponents, and the zero points of 4-bit weights) have no counterpart in the
+ * reference. */
+typedef enum eb_dtype {
+    EB_F32 = 0, EB_F16 = 1, EB_U32 = 2, EB_I32 = 3, EB_F8E4M3 = 4, EB_I8 = 5, EB_U8 = 6
+} eb_dtype;
 
 typedef struct eb_device eb_device;
 typedef struct eb_tensor eb_tensor;
@@ -563,6 +567,136 @@ eb_status eb_attention_forward_qkv(const eb_attention *attn, eb_recorder *rec,
 eb_status eb_attention_forward(const eb_attention *attn, eb_recorder *rec, const eb_tensor *x,
                                const eb_rope_tables *rope, eb_kv_cache *kv, size_t layer,
                                size_t rows, size_t base_pos, eb_tensor **out);
+
+/* ---- projections with 4-bit weights (no counterpart in the reference) ----------------
+ * c [m, out_f] = a [m, in_f] . W^T with W[o, k] = (code[o, k] - zero[o, k / group]) *
+ * scale[o, k / group]. Codes 0..15 are packed eight per u32 word along k, lowest bits first:
+ * w is an EB_U32 tensor [out_f, in_f / 8]. scales is EB_F16 [out_f, in_f / group]; zeros is
+ * EB_U8 of that shape, or NULL: 8 everywhere (symmetric codes). group is 32, 64 or 128 and
+ * divides in_f; out_f is any size. a and c are f32. Every code less its zero point is exact
+ * in f16; the products run on the matrix cores against a's rows split into two halves (about
+ * f32 accuracy, as linear_f16w's many-row form), are summed in f32 within a group, and the
+ * groups' sums are scaled and added in f32. The order of a sum depends on the shape alone. */
+typedef struct eb_q4_weight {
+    const eb_tensor *w;
+    const eb_tensor *scales;
+    const eb_tensor *zeros; /* may be NULL */
+    size_t in_f, out_f, group;
+} eb_q4_weight;
+eb_status eb_linear_q4(eb_recorder *rec, const eb_tensor *a, const eb_q4_weight *w, eb_tensor *c,
+                       size_t m);
+/* n (1..3) projections of the same a in one launch, e.g. a layer's q/k/v; the weights share
+ * in_f and group, and have zero points all or none. */
+eb_status eb_linear_q4_multi(eb_recorder *rec, const eb_tensor *a, size_t n,
+                             const eb_q4_weight *w, eb_tensor *const *c, size_t m);
+/* On caller memory. The workspace (16-byte aligned, no initialisation) holds the split rows;
+ * launches that share one must not overlap. */
+size_t eb_linear_q4_workspace_floats(size_t m, size_t in_f);
+eb_status eb_launch_linear_q4(void *stream, const float *a, size_t a_numel, const uint32_t *w,
+                              size_t w_words, const uint16_t *scales, size_t scales_numel,
+                              const uint8_t *zeros, size_t zeros_numel, float *c, size_t c_numel,
+                              size_t m, size_t in_f, size_t out_f, size_t group,
+                              float *workspace, size_t workspace_floats);
+/* eb_attention_new with 4-bit projections: proj[0..3] are q, k, v and o, of the shapes the
+ * descriptor asks for; the descriptor's own projections are NULL, its hidden is set. */
+eb_status eb_attention_new_q4(const eb_attention_desc *desc, const eb_q4_weight proj[4],
+                              eb_attention **out);
+
+/* ---- block-scaled 8-bit KV caches (no counterpart in the reference) -------------------
+ * K and V are int8 codes [max_seq, hkv, hd] (EB_I8) and one exponent byte e for each block of
+ * `block` consecutive rows and KV head (EB_U8, [ceil(max_seq / block), hkv]); a code stands
+ * for code * 2^(e - 127). A quarter of an f32 cache's bytes, like E4M3, with a step of 1/127 to
+ * 2/127 of the block's largest value: about 1e-2 rel-L2 on N(0,1) rows, whatever their scale,
+ * against E4M3's 3e-2 and its range of +-448.
+ * block is a power of two from 16 to 256; head dims are the multiples of 16 from 32 to 256.
+ * Writing rows dst.. : a block's exponent becomes the least with every new |x| <= 127 *
+ * 2^(e - 127) (e >= 1), and at least the old one where rows before dst share the block; the
+ * codes of those rows are rounded again (to nearest even) where the exponent grew. New codes
+ * are the nearest whole numbers to x * 2^(127 - e), ties to even. Rows behind the last one
+ * written keep their bytes, and stand for nothing until they are written. A value that is not
+ * finite makes e = 255: the block (of its head, K or V) reads as NaN until it is written from
+ * its first row on. Attention computes in f32 on the values the codes stand for. */
+eb_status eb_kv_cache_new_i8(eb_device *dev, const size_t *head_dims, size_t n_layers,
+                             size_t max_seq, size_t n_kv_heads, size_t block,
+                             eb_kv_cache **out);
+eb_tensor *eb_kv_cache_k_scale(eb_kv_cache *kv, size_t layer); /* NULL for other caches */
+eb_tensor *eb_kv_cache_v_scale(eb_kv_cache *kv, size_t layer);
+size_t eb_kv_cache_block(const eb_kv_cache *kv); /* 0 for other caches */
+/* k, v [count, hkv, hd] f32 to rows dst.. of the layer's K and V, in one launch. */
+eb_status eb_kv_write_i8(eb_recorder *rec, eb_kv_cache *kv, size_t layer, const eb_tensor *k,
+                         const eb_tensor *v, size_t count, size_t dst_start);
+/* Rows start.. of the layer's K and V as f32 k, v [count, hkv, hd]. */
+eb_status eb_kv_read_i8(eb_recorder *rec, const eb_kv_cache *kv, size_t layer, eb_tensor *k,
+                        eb_tensor *v, size_t count, size_t src_start);
+/* eb_attn_decode_window and eb_attn_decode_step_window over the layer: q, o [h, hd]. The step
+ * writes knew / vnew [hkv, hd] to row pos as eb_kv_write_i8 does, then attends. */
+eb_status eb_attn_decode_i8(eb_recorder *rec, const eb_tensor *q, const eb_kv_cache *kv,
+                            size_t layer, eb_tensor *o, size_t h, size_t pos, float scale,
+                            size_t window);
+eb_status eb_attn_decode_step_i8(eb_recorder *rec, const eb_tensor *q, const eb_tensor *knew,
+                                 const eb_tensor *vnew, eb_kv_cache *kv, size_t layer,
+                                 eb_tensor *o, size_t h, size_t pos, float scale,
+                                 size_t window);
+/* eb_attn_prefill_chunk over the layer: q, o [rows, h, hd] at positions pos0.., whose K and V
+ * rows the cache holds already. */
+eb_status eb_attn_prefill_chunk_i8(eb_recorder *rec, const eb_tensor *q, const eb_kv_cache *kv,
+                                   size_t layer, eb_tensor *o, size_t h, size_t pos0,
+                                   size_t rows, float scale, size_t window);
+/* On caller memory: the codes 16-byte aligned, as q, o, k, v and the workspace are. The workspace
+ * holds eb_attn_i8_workspace_floats floats for this many rows at pos0 (1 for a token) with this
+ * window; it needs no initialisation, and launches that share one must not overlap. */
+typedef struct eb_cache_i8 {
+    int8_t *k;
+    uint8_t *k_exp;
+    int8_t *v;
+    uint8_t *v_exp;
+    size_t code_numel; /* elements of k, and of v */
+    size_t exp_numel;  /* bytes of k_exp, and of v_exp */
+    size_t max_seq, hkv, hd, block;
+} eb_cache_i8;
+eb_status eb_launch_kv_write_i8(void *stream, const eb_cache_i8 *cache, const float *k,
+                                const float *v, size_t numel, size_t count, size_t dst_start);
+eb_status eb_launch_kv_read_i8(void *stream, const eb_cache_i8 *cache, float *k, float *v,
+                               size_t numel, size_t count, size_t src_start);
+size_t eb_attn_i8_workspace_floats(size_t h, size_t hkv, size_t hd, size_t pos0, size_t rows,
+                                   size_t block, size_t window, int cu_count);
+/* knew and vnew NULL: attention alone. */
+eb_status eb_launch_attn_decode_i8(void *stream, const float *q, size_t q_numel,
+                                   const float *knew, const float *vnew, size_t new_numel,
+                                   const eb_cache_i8 *cache, float *o, size_t o_numel, size_t h,
+                                   size_t pos, float scale, size_t window, float *workspace,
+                                   size_t workspace_floats, int cu_count);
+eb_status eb_launch_attn_prefill_chunk_i8(void *stream, const float *q, size_t q_numel,
+                                          const eb_cache_i8 *cache, float *o, size_t o_numel,
+                                          size_t h, size_t pos0, size_t rows, float scale,
+                                          size_t window, float *workspace,
+                                          size_t workspace_floats, int cu_count);
+
+/* ---- sampling (no counterpart in the reference, whose sampling is argmax) --------------
+ * out_idx[r] (EB_U32, [rows]) = the token that row r of logits [rows, vocab] (f32) gives for
+ * the random number u[r] in [0, 1). Each token's weight is exp((x - max x) / temperature[r]).
+ * Kept are the top_k[r] largest; of those the fewest largest whose weights reach top_p[r] of
+ * their sum; of those the ones of at least min_p[r] times the largest weight. Equal logits
+ * rank by index, the lower first. The token is the first index, in the vocabulary's order, at
+ * which the kept weights' running sum exceeds u[r] times their total (u >= 1: the last kept;
+ * u < 0 or NaN: the first).
+ * temperature, top_p, min_p are f32 [rows], top_k u32 [rows], all in device memory, so that a
+ * captured graph reads the current ones; each may be NULL: temperature 1, the others off.
+ * A temperature that is not above 0 takes the largest logit (the lowest index of equals).
+ * top_k 0 or at least vocab, a top_p that is not below 1 and a min_p that is not above 0 are
+ * off; a top_p of 0 or below, or a min_p above 1, keeps the first of the largest logits (all
+ * of the equal largest, for min_p = 1). NaN logits are never taken; +inf outweighs all else; a
+ * row of only -inf and NaN gives 0.
+ * The choice is exact up to the f64 rounding of the weights, which are summed as whole numbers
+ * (units of 2^-k, k >= 38), so it does not depend on any order of summation. */
+eb_status eb_sample(eb_recorder *rec, const eb_tensor *logits, const eb_tensor *u,
+                    eb_tensor *out_idx, size_t rows, size_t vocab, const eb_tensor *temperature,
+                    const eb_tensor *top_k, const eb_tensor *top_p, const eb_tensor *min_p);
+size_t eb_sample_workspace_floats(size_t rows, size_t vocab);
+eb_status eb_launch_sample(void *stream, const float *logits, size_t logits_numel,
+                           const float *u, uint32_t *out_idx, size_t rows, size_t vocab,
+                           const float *temperature, const uint32_t *top_k, const float *top_p,
+                           const float *min_p, float *workspace, size_t workspace_floats);
 
 /* ---- self-check (no counterpart in the reference) ----------------------------------
  * One wave applies the lane exchanges that every wave reduction in the kernels is built

@@ -1,0 +1,167 @@
+"""4-bit projections on the GPU against their definition in 64 bits, within the bound of the
+kernels' arithmetic (tests/_quant.py)."""
+import numpy as np
+import pytest
+
+import eyebrowse_amd as eb
+from tests._gpu import note
+from tests._quant import linear_q4_bound, pack_q4
+
+pytestmark = pytest.mark.gpu
+
+
+def weight(rng, out_f, in_f, group, zeros):
+    codes = rng.integers(0, 16, (out_f, in_f))
+    scales = (np.exp(rng.standard_normal((out_f, in_f // group))) * 0.02).astype(np.float16)
+    scales *= rng.choice(np.array([-1, 1], np.float16), scales.shape)
+    z = rng.integers(0, 16, scales.shape).astype(np.uint8) if zeros else None
+    return codes, scales, z
+
+
+def device_weight(dev, codes, scales, z, group):
+    return eb.LinearQ4(eb.Tensor.from_array(dev, pack_q4(codes)), eb.Tensor.from_array(dev, scales),
+                       None if z is None else eb.Tensor.from_array(dev, z), codes.shape[1], codes.shape[0], group)
+
+
+def run(dev, a, w):
+    out = eb.Tensor.empty(dev, (len(a), w.out_f))
+    out.write(np.full((len(a), w.out_f), np.nan, np.float32))
+    rec = eb.Recorder(dev)
+    eb.linear_q4(rec, eb.Tensor.from_array(dev, a), w, out, len(a))
+    rec.submit()
+    return out.to_f32().reshape(len(a), w.out_f)
+
+
+def close(got, want, bound, what):
+    assert np.isfinite(got).all(), f"{what}: non-finite output"
+    err = np.abs(got - want)
+    worst = float((err / np.maximum(bound, 1e-300)).max())
+    assert (err <= bound).all(), f"{what}: {worst:.3f} of the bound"
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("m", [1, 2, 3, 8, 9, 31, 33, 64, 65, 130])
+def test_rows(dev, m, group, zeros):
+    note(f"q4 {m} rows group {group} zeros {zeros}")
+    rng = np.random.default_rng(m)
+    for in_f, out_f in ((128, 1), (384, 129), (640, 48), (group, 7), (3 * group, 130), (2048, 300)):
+        codes, scales, z = weight(rng, out_f, in_f, group, zeros)
+        a = (rng.standard_normal((m, in_f)) * np.exp(2 * rng.standard_normal((m, 1)))).astype(np.float32)
+        want, bound = linear_q4_bound(a, codes, scales, z, group)
+        close(run(dev, a, device_weight(dev, codes, scales, z, group)), want, bound, f"{in_f} to {out_f}")
+
+
+@pytest.mark.parametrize("m,in_f,out_f", [(1, 1024, 20000), (4, 4096, 5000), (8, 4736, 257), (8, 6144, 100), (1, 16384, 64),
+                                          (300, 1152, 777), (1, 40960, 33), (2, 1024, 9000)])
+def test_large(dev, m, in_f, out_f):
+    note(f"q4 {m} rows {in_f} to {out_f}")
+    rng = np.random.default_rng(in_f)
+    codes, scales, z = weight(rng, out_f, in_f, 64, True)
+    a = rng.standard_normal((m, in_f)).astype(np.float32)
+    want, bound = linear_q4_bound(a, codes, scales, z, 64)
+    close(run(dev, a, device_weight(dev, codes, scales, z, 64)), want, bound, "large")
+
+
+@pytest.mark.parametrize("m", [1, 20, 100])
+def test_extreme_rows(dev, m):
+    """Rows of zeros, of tiny and of huge values beside ordinary ones; a zero point above 15."""
+    rng = np.random.default_rng(7)
+    codes, scales, z = weight(rng, 40, 256, 64, True)
+    z[:] = rng.integers(0, 256, z.shape)
+    a = rng.standard_normal((m, 256)).astype(np.float32)
+    for i, f in enumerate((1e-38, 1e30, 0.0)):
+        a[i * m // 3] *= np.float32(f)
+    want, bound = linear_q4_bound(a, codes, scales, z, 64)
+    # (below f32's normal range a result may lose bits: one step of 2^-149, with its sums')
+    close(run(dev, a, device_weight(dev, codes, scales, z, 64)), want, bound + 1e-42, "extreme")
+
+
+@pytest.mark.parametrize("m", [2, 70])
+def test_a_row_that_is_not_finite_stays_alone(dev, m):
+    rng = np.random.default_rng(9)
+    codes, scales, z = weight(rng, 50, 256, 32, False)
+    a = rng.standard_normal((m, 256)).astype(np.float32)
+    a[1, 17] = np.inf
+    got = run(dev, a, device_weight(dev, codes, scales, z, 32))
+    assert not np.isfinite(got[1]).any()
+    a[1] = 0
+    want, bound = linear_q4_bound(a, codes, scales, z, 32)
+    got[1] = 0
+    close(got, want, bound, "the other rows")
+
+
+@pytest.mark.parametrize("m", [1, 5, 40, 200])
+def test_multi_is_the_single_calls(dev, m):
+    rng = np.random.default_rng(m)
+    a = rng.standard_normal((m, 512)).astype(np.float32)
+    ws = [device_weight(dev, *weight(rng, n, 512, 64, True), 64) for n in (256, 100, 33)]
+    at = eb.Tensor.from_array(dev, a)
+    outs = [eb.Tensor.empty(dev, (m, w.out_f)) for w in ws]
+    rec = eb.Recorder(dev)
+    eb.linear_q4_multi(rec, at, ws, outs, m)
+    rec.submit()
+    for w, o in zip(ws, outs):
+        want = run(dev, a, w)
+        # (the grid, and with it how waves share a contraction, may differ: f32 sums, not bits)
+        np.testing.assert_allclose(o.to_f32().reshape(m, -1), want, rtol=0, atol=1e-4 * np.abs(want).max())
+
+
+def test_from_f32_and_forward(dev):
+    rng = np.random.default_rng(1)
+    w = rng.standard_normal((96, 256)).astype(np.float32)
+    w[3, :64] = 0
+    x = rng.standard_normal((3, 256)).astype(np.float32)
+    for group in (32, 64, 128):
+        for symmetric in (True, False):
+            p = eb.LinearQ4.from_f32(dev, w, group, symmetric)
+            rec = eb.Recorder(dev)
+            y = p.forward(rec, eb.Tensor.from_array(dev, x), 3)
+            rec.submit()
+            got = y.to_f32().reshape(3, 96)
+            # a code is off by half a step (and a clipped end by one): the group's range / 14 or / 15
+            span = np.ptp(np.concatenate((w, np.zeros((96, 1), np.float32)), 1), axis=1).max() if not symmetric else 2 * np.abs(w).max()
+            assert np.abs(got - x @ w.T).max() <= span / 14 * np.abs(x).sum(1).max()
+
+
+def test_graph_replays(dev):
+    rng = np.random.default_rng(2)
+    codes, scales, z = weight(rng, 70, 512, 128, True)
+    w = device_weight(dev, codes, scales, z, 128)
+    for m in (1, 50):
+        at, out = eb.Tensor.empty(dev, (m, 512)), eb.Tensor.empty(dev, (m, 70))
+        at.write(np.zeros((m, 512), np.float32))
+
+        def step():
+            rec = eb.Recorder(dev)
+            eb.linear_q4(rec, at, w, out, m)
+            rec.submit()
+
+        step()
+        dev.begin_capture()
+        step()
+        graph = dev.end_capture()
+        for _ in range(3):
+            a = rng.standard_normal((m, 512)).astype(np.float32)
+            at.write(a)
+            graph.launch()
+            dev.synchronize()
+            want, bound = linear_q4_bound(a, codes, scales, z, 128)
+            close(out.to_f32().reshape(m, 70), want, bound, "replay")
+            assert run(dev, a, w).tobytes() == out.to_f32().tobytes()
+
+
+def test_raw_launch(dev):
+    rng = np.random.default_rng(3)
+    codes, scales, z = weight(rng, 65, 256, 64, True)
+    w = device_weight(dev, codes, scales, z, 64)
+    for m in (1, 17):
+        a = rng.standard_normal((m, 256)).astype(np.float32)
+        at, out = eb.Tensor.from_array(dev, a), eb.Tensor.empty(dev, (m, 65))
+        floats = eb.linear_q4_workspace_floats(m, 256)
+        ws = eb.Tensor.empty(dev, (max(floats, 1),))
+        eb.launch_linear_q4(dev.stream, at.data_ptr, a.size, w.w.data_ptr, w.w.numel(), w.scales.data_ptr,
+                            w.scales.numel(), w.zeros.data_ptr, w.zeros.numel(), out.data_ptr, m * 65, m, 256, 65, 64,
+                            ws.data_ptr, floats)
+        dev.synchronize()
+        assert out.to_f32().tobytes() == run(dev, a, w).tobytes()
