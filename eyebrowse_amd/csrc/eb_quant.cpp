@@ -522,6 +522,9 @@ static eb_status sample_checked(hipStream_t st, const Room &src, const eb::Sampl
     EB_TRY(eb::check_numel(numel, {a.rows, a.vocab}, "logits"));
     if (a.rows == 0) return eb::ok();
     if (a.vocab == 0) return fail(EB_SHAPE_MISMATCH, "sample: vocab must be > 0");
+    if (a.vocab > ((size_t)1 << 24) || a.rows > 65535)
+        return fail(EB_UNSUPPORTED_CONFIG, "sample: [%zu, %zu] logits (at most 65535 rows of a vocab of 2^24)", a.rows,
+                    a.vocab);
     EB_TRY(eb::check_ptr(a.logits, "logits"));
     EB_TRY(eb::check_ptr(a.u, "u"));
     EB_TRY(eb::check_ptr(a.out, "out_idx"));

@@ -4,24 +4,63 @@
 // A token's weight is w = 2^((x - max) log2(e) / T), computed in f64 and rounded once to a whole
 // number of 2^-F units (F = 62 - ceil(log2 vocab), so that a row's sum fits 64 bits). Sums of
 // whole numbers do not depend on their order: histograms may be filled by atomics, and the choice
-// is the same on every run. Ranks go by the logit's bits made monotonic (equal logits by index).
+// is the same on every run. Ranks go by the logit's bits made monotonic (equal logits by index): a
+// token's rank key is those bits over the complement of its index.
+//
+// What top-k and top-p keep is the tokens down to a cut in that order. A sort would find it; here
+// a histogram does. Over slices of 4096 tokens, so that one row fills many CUs:
+//  1. max: the slice's largest rank key;
+//  2. histogram: tokens by their distance below the largest logit, in steps of 1/64 (of the
+//     temperature where it is above 1), with each step's count and weight;
+//  3. collect: every slice finds from the histogram the steps that can hold the cut, lists its
+//     tokens of those steps, and sums the kept weights of the steps above them;
+//  4. choose: one workgroup per row sorts the listed tokens (some hundreds), walks them to the
+//     exact cut, adds what is kept of them to their slices' sums, and finds the token in its slice.
+// Steps 2 and 3 do nothing for rows that need only the best token. A row whose steps list more
+// than kListed tokens (many equal logits; logits of enormous range) is solved by the choosing
+// workgroup alone, by radix selection over the row. A vocabulary of one slice is step 4 alone,
+// over all of its tokens.
 #include "eb_common.h"
 #include "eb_internal.h"
 
+#include <algorithm>
 #include <cstdint>
 
 namespace {
 
 typedef unsigned long long u64;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 1024;  // of the choosing workgroup
 constexpr int kWaves = kThreads / 64;
-constexpr int kTile = 4096;   // tokens whose kept weights are summed together
-constexpr int kDigits = 256;  // of a radix pass
+constexpr int kTile = 4096;     // tokens of a slice
+constexpr int kSliceThreads = 512;
+constexpr int kPer = kTile / kSliceThreads;  // tokens per thread of a slice
+constexpr int kDigits = 256;    // of a radix pass
+constexpr int kBins = 2048;     // steps of the histogram
+constexpr float kBinsPerUnit = 64.0f;
+constexpr int kListed = 4096;   // most listed tokens of a row
+
+// Per row, written by step 3.
+struct Cut {
+    u64 before_cut;   // weight of the steps above the first that can hold the cut
+    u64 before_topk;  // and above the one that holds top-k's last token
+    unsigned above;   // tokens above that one
+    int topk_bin;     // that one (kBins: no top-k)
+};
 
 struct Args {
     eb::SampleArgs s;
     int frac;  // F
+    int tiles;
+    // workspace
+    u64 *best;         // [rows, tiles] rank keys
+    u64 *tile_sum;     // [rows, tiles]
+    u64 *hist_w;       // [rows, kBins]
+    unsigned *hist_c;  // [rows, kBins]
+    u64 *listed;       // [rows, kListed]
+    unsigned *count;   // [rows]
+    Cut *cut;          // [rows]
 };
 
 // The logit's bits in an order that follows its value; 0 for NaN. -0 counts as +0.
@@ -34,6 +73,9 @@ __device__ __forceinline__ unsigned key_of(float x) {
 __device__ __forceinline__ float value_of(unsigned key) {
     return __builtin_bit_cast(float, (key & 0x80000000u) ? key & 0x7FFFFFFFu : ~key);
 }
+__device__ __forceinline__ u64 rank_of(float x, unsigned i) { return (u64)key_of(x) << 32 | (u64)(unsigned)~i; }
+__device__ __forceinline__ unsigned index_of(u64 rank) { return ~(unsigned)rank; }
+constexpr u64 kLeastRank = 1ull << 32;  // at most every rank but NaN's
 
 // 2^y for y <= 0: 2^n times the Taylor sum of e^(f ln 2) for y = n + f, |f| <= 1/2 (the first term
 // left out is below 2e-16).
@@ -57,18 +99,47 @@ __device__ __forceinline__ double exp2_f64(double y) {
     return ldexp(p, (int)n);
 }
 
+// A row's parameters.
 struct Row {
     double rate;    // log2(e) / T
-    float top;      // the largest logit
     double min_p;   // 0: off
+    float top;      // the largest logit
+    float per_bin;  // steps per unit of distance
+    float top_p;
+    unsigned top_k;
+    bool none, best, use_k, use_p;  // no candidate; only the best token; which cuts
     int frac;
+
+    __device__ __forceinline__ Row(const Args &a, size_t r, unsigned best_key) {
+        const float temp = a.s.temperature ? a.s.temperature[r] : 1.0f;
+        const float mp = a.s.min_p ? a.s.min_p[r] : 0.0f;
+        top_p = a.s.top_p ? a.s.top_p[r] : 1.0f;
+        top_k = a.s.top_k ? a.s.top_k[r] : 0u;
+        none = best_key <= key_of(-INFINITY);  // (only -inf and NaN)
+        best = !(temp > 0.0f) || mp > 1.0f || top_k == 1 || top_p <= 0.0f;
+        use_k = top_k > 0 && top_k < (unsigned)a.s.vocab;
+        use_p = top_p < 1.0f;
+        rate = 1.4426950408889634073599 / (double)temp;
+        min_p = mp > 0.0f ? (double)mp : 0.0;
+        top = value_of(best_key);
+        per_bin = kBinsPerUnit / fmaxf(temp, 1.0f);
+        frac = a.frac;
+    }
     __device__ __forceinline__ double weight(float x) const {
         if (x == top) return 1.0;  // (top is finite or +inf)
         if (x == -INFINITY) return 0.0;
         return exp2_f64(((double)x - (double)top) * rate);
     }
     __device__ __forceinline__ u64 units(double w) const { return (u64)(ldexp(w, frac) + 0.5); }
+    __device__ __forceinline__ u64 units_kept(double w) const { return w >= min_p ? units(w) : 0; }
+    // The step a logit falls in; it rises as the logit falls.
+    __device__ __forceinline__ int bin(float x) const {
+        if (x == top) return 0;
+        return (int)fminf((top - x) * per_bin, (float)(kBins - 1));
+    }
 };
+
+// ---- workgroup reductions ---------------------------------------------------------------------
 
 template <class T>
 __device__ __forceinline__ T wave_total(T x) {
@@ -76,81 +147,281 @@ __device__ __forceinline__ T wave_total(T x) {
     for (int m = 32; m > 0; m >>= 1) x += __shfl_xor(x, m);
     return x;
 }
+__device__ __forceinline__ u64 wave_best(u64 k) {
+#pragma unroll
+    for (int m = 32; m > 0; m >>= 1) {
+        const u64 o = __shfl_xor(k, m);
+        k = o > k ? o : k;
+    }
+    return k;
+}
+// (each starts with a barrier, so that s_waves may be in use before)
+template <int THREADS, class T>
+__device__ __forceinline__ T block_total(T x, T *s_waves) {
+    x = wave_total(x);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) s_waves[threadIdx.x >> 6] = x;
+    __syncthreads();
+    T t = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) t += s_waves[w];
+    return t;
+}
+template <int THREADS>
+__device__ __forceinline__ u64 block_best(u64 k, u64 *s_waves) {
+    k = wave_best(k);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) s_waves[threadIdx.x >> 6] = k;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) k = s_waves[w] > k ? s_waves[w] : k;
+    return k;
+}
+// Inclusive sums over the threads.
+template <int THREADS, class T>
+__device__ __forceinline__ T block_scan(T x, T *s_waves) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const T o = __shfl_up(x, d);
+        if (lane >= d) x += o;
+    }
+    __syncthreads();
+    if (lane == 63) s_waves[wave] = x;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) x += s_waves[w];
+    return x;
+}
+
+// ---- steps 1 to 3: one workgroup per slice -----------------------------------------------------
+
+// The tokens of this thread in slice t: four at a time, NaN past the vocabulary.
+struct Slice {
+    float x[kPer];
+    int base;
+    __device__ __forceinline__ int at(int j) const { return base + j / 4 * kSliceThreads * 4 + j % 4; }
+    __device__ __forceinline__ Slice(const float *row, int n, int t) {
+        base = t * kTile + 4 * (int)threadIdx.x;
+        if ((n & 3) == 0 && (reinterpret_cast<uintptr_t>(row) & 15) == 0) {
+#pragma unroll
+            for (int j = 0; j < kPer; j += 4) {
+                const f32x4 nan = {__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+                const f32x4 v = at(j) < n ? *reinterpret_cast<const f32x4 *>(row + at(j)) : nan;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) x[j + c] = v[c];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) x[j] = at(j) < n ? row[at(j)] : __builtin_nanf("");
+        }
+    }
+};
+
+// Step 1, and the clearing of the row's histogram and list.
+__global__ __launch_bounds__(kSliceThreads) void sample_max_kernel(Args a) {
+    __shared__ u64 s_waves[kSliceThreads / 64];
+    const int t = blockIdx.x, tid = threadIdx.x;
+    const size_t r = blockIdx.y;
+    const Slice s(a.s.logits + r * a.s.vocab, (int)a.s.vocab, t);
+    for (int i = t * kSliceThreads + tid; i < kBins; i += a.tiles * kSliceThreads) {
+        a.hist_w[r * kBins + i] = 0;
+        a.hist_c[r * kBins + i] = 0;
+    }
+    if (t == 0 && tid == 0) a.count[r] = 0;
+    u64 k = 0;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        const u64 o = rank_of(s.x[j], (unsigned)s.at(j));
+        k = o > k ? o : k;
+    }
+    k = block_best<kSliceThreads>(k, s_waves);
+    if (tid == 0) a.best[r * a.tiles + t] = k;
+}
+
+// The row's largest rank key, from step 1's.
+template <int THREADS>
+__device__ __forceinline__ u64 row_best(const Args &a, size_t r, u64 *s_waves) {
+    u64 k = 0;
+    for (int i = threadIdx.x; i < a.tiles; i += THREADS) {
+        const u64 o = a.best[r * a.tiles + i];
+        k = o > k ? o : k;
+    }
+    return block_best<THREADS>(k, s_waves);
+}
+
+// Step 2: a histogram in LDS, its filled steps added to the row's.
+__global__ __launch_bounds__(kSliceThreads) void sample_histogram_kernel(Args a) {
+    __shared__ u64 s_w[kBins];
+    __shared__ unsigned s_c[kBins];
+    __shared__ u64 s_waves[kSliceThreads / 64];
+    const int tid = threadIdx.x;
+    const size_t r = blockIdx.y;
+    const Slice s(a.s.logits + r * a.s.vocab, (int)a.s.vocab, blockIdx.x);
+    const Row row(a, r, (unsigned)(row_best<kSliceThreads>(a, r, s_waves) >> 32));
+    if (row.none || row.best || !(row.use_k || row.use_p)) return;  // (uniform)
+    for (int i = tid; i < kBins; i += kSliceThreads) {
+        s_w[i] = 0;
+        s_c[i] = 0;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        if (s.x[j] != s.x[j]) continue;
+        const int b = row.bin(s.x[j]);
+        atomicAdd(&s_c[b], 1u);
+        if (row.use_p) {
+            const u64 w = row.units(row.weight(s.x[j]));
+            if (w) atomicAdd(&s_w[b], w);
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < kBins; i += kSliceThreads) {
+        if (s_c[i]) atomicAdd(&a.hist_c[r * kBins + i], s_c[i]);
+        if (s_w[i]) atomicAdd(&a.hist_w[r * kBins + i], s_w[i]);
+    }
+}
+
+// Step 3. Top-k's last token lies in the first step by which top_k tokens are counted. The weight
+// that top-k keeps lies between that of the steps above and that with the step's own; so the
+// cut of top-p lies between the steps that reach top_p of the one and of the other.
+__global__ __launch_bounds__(kSliceThreads) void sample_collect_kernel(Args a) {
+    constexpr int PB = kBins / kSliceThreads;  // steps per thread
+    __shared__ u64 s_waves[kSliceThreads / 64];
+    __shared__ unsigned s_waves32[kSliceThreads / 64];
+    __shared__ int s_topk, s_lo, s_hi;
+    __shared__ u64 s_before_topk, s_at_topk, s_before_cut;
+    __shared__ unsigned s_above, s_here, s_from;
+    const int tid = threadIdx.x;
+    const size_t r = blockIdx.y;
+    const Slice s(a.s.logits + r * a.s.vocab, (int)a.s.vocab, blockIdx.x);
+    const Row row(a, r, (unsigned)(row_best<kSliceThreads>(a, r, s_waves) >> 32));
+    if (row.none || row.best) return;  // (uniform)
+    // Steps below lo are kept; steps lo to hi, and topk, are listed (kBins: none).
+    int lo = kBins, hi = kBins, topk = kBins;
+    if (row.use_k || row.use_p) {
+        unsigned c[PB], csum = 0;
+        u64 w[PB], wsum = 0;
+#pragma unroll
+        for (int i = 0; i < PB; ++i) {
+            c[i] = a.hist_c[r * kBins + tid * PB + i];
+            w[i] = row.use_p ? a.hist_w[r * kBins + tid * PB + i] : 0;
+            csum += c[i];
+            wsum += w[i];
+        }
+        const unsigned cend = block_scan<kSliceThreads>(csum, s_waves32);
+        const u64 wend = block_scan<kSliceThreads>(wsum, s_waves);
+        if (tid == kSliceThreads - 1) {
+            s_topk = s_lo = s_hi = kBins;
+            s_here = 0;
+            s_before_topk = wend;
+            s_at_topk = s_before_cut = 0;
+            s_above = cend;
+        }
+        __syncthreads();
+        if (row.use_k && cend >= row.top_k && cend - csum < row.top_k) {  // (at most one thread)
+            unsigned above = cend - csum;
+            u64 before = wend - wsum;
+            bool found = false;
+#pragma unroll
+            for (int i = 0; i < PB; ++i) {
+                if (!found && above + c[i] >= row.top_k) {
+                    found = true;
+                    s_topk = tid * PB + i;
+                    s_above = above;
+                    s_before_topk = before;
+                    s_at_topk = w[i];
+                }
+                above += c[i];
+                before += w[i];
+            }
+        }
+        __syncthreads();
+        topk = s_topk;
+        lo = hi = topk;
+        if (row.use_p) {
+            const double least = (double)row.top_p * (double)s_before_topk;
+            const double most = (double)row.top_p * (double)(s_before_topk + s_at_topk);
+            u64 before = wend - wsum;
+#pragma unroll
+            for (int i = 0; i < PB; ++i) {
+                const u64 end = before + w[i];
+                const int b = tid * PB + i;
+                if ((double)end >= least && ((double)before < least || b == 0)) {  // (one step)
+                    s_lo = b;
+                    s_before_cut = before;
+                }
+                if ((double)end >= most && ((double)before < most || b == 0)) s_hi = b;
+                before = end;
+            }
+            __syncthreads();
+            lo = min(s_lo, topk);
+            hi = min(s_hi, topk);
+        }
+        if (blockIdx.x == 0 && tid == 0)
+            a.cut[r] = Cut{row.use_p ? s_before_cut : s_before_topk, s_before_topk, s_above, topk};
+    }
+    u64 sum = 0;
+    unsigned mine = 0;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        if (s.x[j] != s.x[j]) continue;
+        const int b = row.bin(s.x[j]);
+        if (b < lo)
+            sum += row.units_kept(row.weight(s.x[j]));
+        else if (b <= hi || b == topk)
+            ++mine;
+    }
+    if (lo < kBins) {
+        // This slice's part of the list (in any order: it is sorted).
+        unsigned at = mine ? atomicAdd(&s_here, mine) : 0;
+        __syncthreads();
+        if (tid == 0) s_from = s_here ? atomicAdd(&a.count[r], s_here) : 0;
+        __syncthreads();
+        at += s_from;
+        if (mine) {
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) {
+                if (s.x[j] != s.x[j]) continue;
+                const int b = row.bin(s.x[j]);
+                if (b >= lo && (b <= hi || b == topk)) {
+                    if (at < kListed) a.listed[r * kListed + at] = rank_of(s.x[j], (unsigned)s.at(j));
+                    ++at;
+                }
+            }
+        }
+    }
+    sum = block_total<kSliceThreads>(sum, s_waves);
+    if (tid == 0) a.tile_sum[r * a.tiles + blockIdx.x] = sum;
+}
+
+// ---- step 4: one workgroup per row --------------------------------------------------------------
 
 struct Shared {
     u64 wsum[kDigits];
     unsigned csum[kDigits];
-    u64 red[kWaves];
+    u64 waves[kWaves];
+    unsigned waves32[kWaves];
     unsigned digit;
-    u64 above_w;
-    unsigned above_c;
+    u64 above_w, cut, left;
+    unsigned above_c, in_last;
+    int tile, last;
 };
 
-__device__ __forceinline__ u64 block_total(u64 x, Shared &s) {
-    x = wave_total(x);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) s.red[threadIdx.x >> 6] = x;
-    __syncthreads();
-    u64 t = 0;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) t += s.red[w];
-    return t;
-}
-
-// One workgroup per row.
-__global__ __launch_bounds__(kThreads) void sample_row_kernel(Args a) {
-    __shared__ Shared s;
-    extern __shared__ u64 s_tiles[];  // [tiles] kept weight above the cut, then [tiles] u32 equal keys
-    const size_t r = blockIdx.x;
-    const int n = (int)a.s.vocab;
-    const int tid = threadIdx.x;
-    const float *x = a.s.logits + r * a.s.vocab;
-    const int tiles = (n + kTile - 1) / kTile;
-    unsigned *s_eq = reinterpret_cast<unsigned *>(s_tiles + tiles);
-
-    // ---- the row's largest logit ----
-    unsigned best = 0;
-    for (int i = tid; i < n; i += kThreads) {
-        const unsigned k = key_of(x[i]);
-        best = k > best ? k : best;
-    }
-#pragma unroll
-    for (int m = 32; m > 0; m >>= 1) {
-        const unsigned o = __shfl_xor(best, m);
-        best = o > best ? o : best;
-    }
-    if ((tid & 63) == 0) s.red[tid >> 6] = best;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) best = (unsigned)s.red[w] > best ? (unsigned)s.red[w] : best;
-    __syncthreads();
-    if (best <= key_of(-INFINITY)) {  // (only -inf and NaN)
-        if (tid == 0) a.s.out[r] = 0;
-        return;
-    }
-    const float temp = a.s.temperature ? a.s.temperature[r] : 1.0f;
-    const float min_p = a.s.min_p ? a.s.min_p[r] : 0.0f;
-    const float top_p = a.s.top_p ? a.s.top_p[r] : 1.0f;
-    const bool greedy = !(temp > 0.0f) || min_p > 1.0f;
-    unsigned top_k = a.s.top_k ? a.s.top_k[r] : 0u;
-    if (greedy) top_k = 1;
-    const bool use_k = top_k > 0 && top_k < (unsigned)n;
-    const bool use_p = top_p < 1.0f && !greedy;
-    Row row;
-    row.rate = 1.4426950408889634073599 / (temp > 0.0f ? (double)temp : 1.0);
-    row.top = value_of(best);
-    row.min_p = min_p > 0.0f && !greedy ? (double)min_p : 0.0;
-    row.frac = a.frac;
-
-    // The cut: tokens with a larger key are in, and the first `equal` of those with this key.
+// A row by itself: its cut by radix selection (returned as the least rank that is kept), and the
+// tiles' kept weights in s_tiles.
+__device__ __noinline__ u64 solve_row(const Args &a, const Row &row, const float *x, u64 *s_tiles, unsigned *s_eq,
+                                      Shared &s) {
+    const int n = (int)a.s.vocab, tiles = a.tiles, tid = threadIdx.x;
+    // Tokens with a larger key are in, and the first `equal` of those with this key.
     unsigned cut = 1, equal = 0xFFFFFFFFu;
 
-    // Radix selection, highest digit first: digit(sums, above) names the digit that the cut has.
+    // Highest digit first; pick(weight, count) says whether the cut lies no lower.
     auto radix = [&](bool weights, auto &&pick) {
         unsigned prefix = 0;
         u64 above_w = 0;
         unsigned above_c = 0;
         for (int shift = 24; shift >= 0; shift -= 8) {
+            __syncthreads();
             if (tid < kDigits) {
                 s.wsum[tid] = 0;
                 s.csum[tid] = 0;
@@ -162,10 +433,8 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(Args a) {
                 if (k == 0 || (shift < 24 && (k >> (shift + 8)) != prefix)) continue;
                 const unsigned d = (k >> shift) & 255u;
                 atomicAdd(&s.csum[d], 1u);
-                if (weights && k >= cut) {
-                    // (of the keys at top-k's cut only the first `equal` are in: taken off below)
-                    atomicAdd(&s.wsum[d], row.units(row.weight(v)));
-                }
+                // (of the tokens at top-k's cut only the first are in: `spare` below)
+                if (weights && k >= cut) atomicAdd(&s.wsum[d], row.units(row.weight(v)));
             }
             __syncthreads();
             if (tid == 0) {
@@ -187,29 +456,30 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(Args a) {
         return prefix;
     };
 
-    if (use_k) {
+    if (row.use_k) {
+        const unsigned top_k = row.top_k;
         const unsigned c = radix(false, [&](u64, unsigned count) { return count >= top_k; });
-        cut = c == 0 ? 1 : c;
-        equal = c == 0 ? 0xFFFFFFFFu : top_k - s.above_c;  // (fewer than k tokens: all are in)
-        __syncthreads();
+        if (c) {  // (0: fewer than top_k tokens, all are in)
+            cut = c;
+            equal = top_k - s.above_c;
+        }
     }
-    if (use_p) {
+    if (row.use_p) {
         // The total of what top-k keeps: keys above the cut, and `equal` times the cut's weight.
-        u64 part = 0;
-        unsigned same = 0;
+        u64 part = 0, same = 0;
         for (int i = tid; i < n; i += kThreads) {
             const float v = x[i];
             const unsigned k = key_of(v);
             if (k > cut) part += row.units(row.weight(v));
             if (k == cut) ++same;
         }
-        const u64 above = block_total(part, s);
-        const u64 eq = block_total(same, s);
+        const u64 above = block_total<kThreads>(part, s.waves);
+        const u64 eq = block_total<kThreads>(same, s.waves);
         const u64 in = eq < equal ? eq : equal;
         const u64 cut_w = eq ? row.units(row.weight(value_of(cut))) : 0;
         const u64 total = above + in * cut_w;
         const u64 spare = (eq - in) * cut_w;  // weight of the cut's tokens that are out
-        const double target = (double)top_p * (double)total;
+        const double target = (double)row.top_p * (double)total;
         const unsigned c = radix(true, [&](u64 w, unsigned count) {
             // (the digit that holds the cut's key counts its tokens that are out too; there the
             // target, at most the total, is reached whether they count or not)
@@ -224,15 +494,12 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(Args a) {
             const double j = __builtin_ceil((target - (double)before) / (double)w);
             keep = j < 1.0 ? 1u : j < 4.0e9 ? (unsigned)j : 0xFFFFFFFFu;
         }
-        if (key == cut)
-            equal = keep < equal ? keep : equal;
-        else
-            equal = keep;
+        equal = key == cut && equal < keep ? equal : keep;
         cut = key;
-        __syncthreads();
     }
 
-    // ---- the kept weights, tile by tile ----
+    // The kept weights above the cut, and the tokens at it, tile by tile.
+    __syncthreads();
     for (int t = tid; t < tiles; t += kThreads) {
         s_tiles[t] = 0;
         s_eq[t] = 0;
@@ -245,13 +512,9 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(Args a) {
         for (int j = 0; j < kTile / kThreads; ++j) {
             const int i = t * kTile + j * kThreads + tid;
             if (i >= n) continue;
-            const float v = x[i];
-            const unsigned k = key_of(v);
+            const unsigned k = key_of(x[i]);
             if (k == cut) ++same;
-            if (k > cut) {
-                const double w = row.weight(v);
-                if (w >= row.min_p) part += row.units(w);
-            }
+            if (k > cut) part += row.units_kept(row.weight(x[i]));
         }
         part = wave_total(part);
         same = wave_total(same);
@@ -261,107 +524,259 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(Args a) {
         }
     }
     __syncthreads();
-    const double cw = row.weight(value_of(cut));
-    const u64 cut_w = cw >= row.min_p ? row.units(cw) : 0;
-    __shared__ int s_tile;
-    __shared__ u64 s_left;       // weight still to pass inside the tile
-    __shared__ unsigned s_room;  // equal keys still in at its start
-    if (tid == 0) {
-        u64 total = 0;
+    if (tid == 0) {  // the first `equal` of the cut's tokens, in the tiles' order
+        const u64 cut_w = row.units_kept(row.weight(value_of(cut)));
         unsigned room = equal;
-        for (int t = 0; t < tiles; ++t) {
+        s.last = -1;
+        s.cut = (u64)cut << 32;
+        for (int t = 0; t < tiles && room; ++t) {
             const unsigned in = s_eq[t] < room ? s_eq[t] : room;
-            total += s_tiles[t] + (u64)in * cut_w;
+            if (in) {
+                s.last = t;
+                s.in_last = in;
+            }
+            s_tiles[t] += (u64)in * cut_w;
             room -= in;
         }
-        const float u = a.s.u[r];
-        const double at = u > 0.0f ? (double)u * (double)total : 0.0;
-        u64 thr = at >= (double)total ? total - 1 : (u64)at;
-        if (thr >= total) thr = total - 1;
-        room = equal;
-        int t = 0;
-        u64 cum = 0;
-        for (; t < tiles; ++t) {
-            const unsigned in = s_eq[t] < room ? s_eq[t] : room;
-            const u64 w = s_tiles[t] + (u64)in * cut_w;
-            if (cum + w > thr) break;
-            cum += w;
-            room -= in;
+    }
+    __syncthreads();
+    if (s.last >= 0) {  // the rank of the in_last-th of them in its tile
+        const int base = s.last * kTile + 4 * tid;
+        unsigned same = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) same += base + j < n && key_of(x[base + j]) == cut;
+        unsigned before = block_scan<kThreads>(same, s.waves32) - same;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (base + j < n && key_of(x[base + j]) == cut && ++before == s.in_last)
+                s.cut = rank_of(x[base + j], (unsigned)(base + j));
+    }
+    __syncthreads();
+    return s.cut;
+}
+
+// ONE: the vocabulary is one slice, and its tokens are the list.
+template <bool ONE>
+__global__ __launch_bounds__(kThreads) void sample_choose_kernel(Args a) {
+    constexpr int PT = kListed / kThreads;  // listed tokens per thread
+    static_assert(kListed >= kTile && kTile == 4 * kThreads, "a slice's tokens fit the list, four a thread");
+    __shared__ Shared s;
+    __shared__ u64 s_list[kListed];
+    extern __shared__ u64 s_tiles[];  // [tiles], then [tiles] u32
+    unsigned *s_eq = reinterpret_cast<unsigned *>(s_tiles + a.tiles);
+    const size_t r = blockIdx.x;
+    const int n = (int)a.s.vocab, tiles = a.tiles, tid = threadIdx.x;
+    const float *x = a.s.logits + r * a.s.vocab;
+
+    u64 best = 0;
+    if constexpr (ONE) {
+        for (int i = tid; i < kListed; i += kThreads) {
+            const u64 k = i < n ? rank_of(x[i], (unsigned)i) : 0;
+            s_list[i] = k;
+            best = k > best ? k : best;
         }
-        s_tile = t < tiles ? t : tiles - 1;
-        s_left = thr - cum;
-        s_room = room;
+        best = block_best<kThreads>(best, s.waves);
+    } else {
+        best = row_best<kThreads>(a, r, s.waves);
+    }
+    const Row row(a, r, (unsigned)(best >> 32));
+    if (row.none || row.best) {  // (uniform)
+        if (tid == 0) a.s.out[r] = row.none ? 0u : index_of(best);
+        return;
+    }
+    const bool cuts = row.use_k || row.use_p;
+    const unsigned listed = ONE ? (unsigned)n : cuts ? a.count[r] : 0u;
+    u64 cut = kLeastRank;
+    if (listed > kListed) {  // (uniform)
+        cut = solve_row(a, row, x, s_tiles, s_eq, s);
+    } else if (ONE && !cuts) {
+        u64 part = 0;
+        for (int i = tid; i < n; i += kThreads)
+            if (x[i] == x[i]) part += row.units_kept(row.weight(x[i]));
+        part = block_total<kThreads>(part, s.waves);
+        if (tid == 0) s_tiles[0] = part;
+    } else {
+        if constexpr (ONE) {
+            if (tid == 0) s_tiles[0] = 0;
+        } else {
+            for (int t = tid; t < tiles; t += kThreads) s_tiles[t] = a.tile_sum[r * tiles + t];
+            for (unsigned i = tid; i < kListed; i += kThreads) s_list[i] = i < listed ? a.listed[r * kListed + i] : 0;
+        }
+        __syncthreads();
+        if (listed > 0) {  // (0: every token is kept)
+            // Largest first (bitonic; zeros pad the list to a power of two).
+            int size = 1;
+            while (size < (int)listed) size *= 2;
+            for (int k = 2; k <= size; k *= 2)
+                for (int j = k / 2; j > 0; j /= 2) {
+                    for (int i = tid; i < size / 2; i += kThreads) {
+                        const int p = 2 * i - (i & (j - 1)), q = p + j;
+                        const u64 u = s_list[p], v = s_list[q];
+                        if ((u < v) == ((p & k) == 0)) {
+                            s_list[p] = v;
+                            s_list[q] = u;
+                        }
+                    }
+                    __syncthreads();
+                }
+            // Thread tid has places PT tid .. of the order.
+            const Cut c = ONE ? Cut{0, 0, 0, 0} : a.cut[r];
+            u64 rank[PT], w[PT];
+            bool in[PT], topk[PT];
+            unsigned here = 0;  // tokens of top-k's step
+#pragma unroll
+            for (int j = 0; j < PT; ++j) {
+                rank[j] = s_list[PT * tid + j];
+                const float v = value_of((unsigned)(rank[j] >> 32));
+                in[j] = rank[j] >= kLeastRank;
+                w[j] = in[j] ? row.units(row.weight(v)) : 0;
+                topk[j] = in[j] && (ONE || row.bin(v) == c.topk_bin);
+                here += topk[j];
+            }
+            // Top-k keeps the first top_k - above of its step; what it keeps weighs `total`.
+            unsigned place = block_scan<kThreads>(here, s.waves32) - here;
+            const unsigned keep_k = row.use_k ? row.top_k - c.above : 0xFFFFFFFFu;
+            u64 mine = 0;
+#pragma unroll
+            for (int j = 0; j < PT; ++j)
+                if (topk[j]) {
+                    in[j] = place++ < keep_k;
+                    if (in[j]) mine += w[j];
+                }
+            const u64 total = c.before_topk + block_total<kThreads>(mine, s.waves);
+            // Top-p keeps a token while the weight before it is below the target.
+            if (row.use_p) {
+                const double target = (double)row.top_p * (double)total;
+                mine = 0;
+#pragma unroll
+                for (int j = 0; j < PT; ++j) mine += in[j] ? w[j] : 0;
+                u64 before = c.before_cut + block_scan<kThreads>(mine, s.waves) - mine;
+#pragma unroll
+                for (int j = 0; j < PT; ++j) {
+                    const u64 after = before + (in[j] ? w[j] : 0);
+                    in[j] = in[j] && (rank[j] == best || (double)before < target);
+                    before = after;
+                }
+            }
+            // The cut is the last kept; the kept ones' weights join their slices' sums.
+            if (tid == 0) s.cut = ~0ull;
+            __syncthreads();
+            u64 least = ~0ull;
+#pragma unroll
+            for (int j = 0; j < PT; ++j) {
+                if (!in[j]) continue;
+                least = rank[j] < least ? rank[j] : least;
+                const u64 k = row.units_kept(row.weight(value_of((unsigned)(rank[j] >> 32))));
+                if (k) atomicAdd(&s_tiles[index_of(rank[j]) / kTile], k);
+            }
+            if (least != ~0ull) atomicMin(&s.cut, least);
+            __syncthreads();
+            cut = s.cut;
+        }
     }
     __syncthreads();
 
-    // ---- the tile in order: thread tid has tokens 4 tid .. 4 tid + 3 ----
-    const int base = s_tile * kTile + tid * 4;
-    float v[4];
-    unsigned same = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        v[j] = base + j < n ? x[base + j] : __builtin_nanf("");
-        same += key_of(v[j]) == cut;
+    // The slice that holds the token: thread tid has `per` tiles from per * tid on.
+    const int per = (tiles + kThreads - 1) / kThreads;
+    u64 mine = 0;
+    for (int t = per * tid; t < min(per * (tid + 1), tiles); ++t) mine += s_tiles[t];
+    const u64 end = block_scan<kThreads>(mine, s.waves);
+    const u64 total = block_total<kThreads>(mine, s.waves);
+    const float u = a.s.u[r];
+    const double place = u > 0.0f ? (double)u * (double)total : 0.0;
+    u64 thr = place >= (double)total ? total - 1 : (u64)place;
+    if (thr >= total) thr = total - 1;
+    if (thr < end && thr >= end - mine) {  // (one thread)
+        thr -= end - mine;
+        int t = per * tid;
+        while (thr >= s_tiles[t]) thr -= s_tiles[t++];
+        s.tile = t;
+        s.left = thr;
     }
-    const int lane = tid & 63, wave = tid >> 6;
-    auto exclusive = [&](u64 mine) {  // the sum over earlier threads
-        u64 inc = mine;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const u64 o = __shfl_up(inc, d);
-            if (lane >= d) inc += o;
-        }
-        __syncthreads();
-        if (lane == 63) s.red[wave] = inc;
-        __syncthreads();
-        u64 before = inc - mine;
-        for (int w = 0; w < wave; ++w) before += s.red[w];
-        return before;
-    };
-    unsigned rank = (unsigned)exclusive(same);
-    u64 w[4], mine = 0;
+    __syncthreads();
+    // And the token in it: thread tid has tokens 4 tid .. 4 tid + 3.
+    const int base = s.tile * kTile + tid * 4;
+    u64 w[4];
+    mine = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const unsigned k = key_of(v[j]);
-        w[j] = 0;
-        if (k == cut) {
-            if (rank < s_room) w[j] = cut_w;
-            ++rank;
-        } else if (k > cut) {
-            const double f = row.weight(v[j]);
-            if (f >= row.min_p) w[j] = row.units(f);
-        }
+        const float v = base + j < n ? x[base + j] : __builtin_nanf("");
+        w[j] = v == v && rank_of(v, (unsigned)(base + j)) >= cut ? row.units_kept(row.weight(v)) : 0;
         mine += w[j];
     }
-    u64 cum = exclusive(mine);
-    if (cum <= s_left && cum + mine > s_left) {
+    u64 cum = block_scan<kThreads>(mine, s.waves) - mine;
+    if (cum <= s.left && cum + mine > s.left) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            if (cum <= s_left && cum + w[j] > s_left) a.s.out[r] = (unsigned)(base + j);
+            if (cum <= s.left && cum + w[j] > s.left) a.s.out[r] = (unsigned)(base + j);
             cum += w[j];
         }
     }
 }
+
+struct Layout {
+    size_t best, tile_sum, hist_w, listed, cut, hist_c, count, floats;  // offsets in floats
+};
+Layout layout_of(size_t rows, size_t tiles) {
+    Layout l{};
+    size_t at = 0;
+    auto take = [&](size_t floats) {
+        const size_t here = at;
+        at += (floats + 3) / 4 * 4;
+        return here;
+    };
+    l.best = take(2 * rows * tiles);
+    l.tile_sum = take(2 * rows * tiles);
+    l.hist_w = take(2 * rows * kBins);
+    l.listed = take(2 * rows * kListed);
+    l.cut = take(sizeof(Cut) / 4 * rows);
+    l.hist_c = take(rows * kBins);
+    l.count = take(rows);
+    l.floats = at;
+    return l;
+}
+
+constexpr size_t kMaxVocab = (size_t)1 << 24;
 
 }  // namespace
 
 namespace eb {
 
 size_t sample_workspace_floats(size_t rows, size_t vocab) {
-    (void)rows;
-    (void)vocab;
-    return 0;
+    const size_t tiles = (vocab + kTile - 1) / kTile;
+    return tiles <= 1 ? 0 : layout_of(rows, tiles).floats;
 }
 
 eb_status launch_sample(hipStream_t st, const SampleArgs &s, float *ws) {
-    (void)ws;
-    if (s.vocab > ((size_t)1 << 24))
-        return fail(EB_UNSUPPORTED_CONFIG, "sample: vocab %zu (at most 2^24)", s.vocab);
-    Args a{s, 62};
+    Args a{};
+    a.s = s;
+    a.frac = 62;
     while (((size_t)1 << (62 - a.frac)) < s.vocab) --a.frac;
     const size_t tiles = (s.vocab + kTile - 1) / kTile;
+    a.tiles = (int)tiles;
     const size_t lds = tiles * 12 + 8;
-    sample_row_kernel<<<(unsigned)s.rows, kThreads, lds, st>>>(a);
+    if (tiles <= 1) {
+        sample_choose_kernel<true><<<(unsigned)s.rows, kThreads, lds, st>>>(a);
+        return check_launch("sample");
+    }
+    static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&sample_choose_kernel<false>),
+                                                    hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                    (int)(kMaxVocab / kTile * 12 + 8));
+    if (e != hipSuccess) return hip_fail(e, "sample launch set-up");
+    const Layout l = layout_of(s.rows, tiles);
+    a.best = reinterpret_cast<u64 *>(ws + l.best);
+    a.tile_sum = reinterpret_cast<u64 *>(ws + l.tile_sum);
+    a.hist_w = reinterpret_cast<u64 *>(ws + l.hist_w);
+    a.hist_c = reinterpret_cast<unsigned *>(ws + l.hist_c);
+    a.listed = reinterpret_cast<u64 *>(ws + l.listed);
+    a.count = reinterpret_cast<unsigned *>(ws + l.count);
+    a.cut = reinterpret_cast<Cut *>(ws + l.cut);
+    const dim3 grid((unsigned)tiles, (unsigned)s.rows);
+    sample_max_kernel<<<grid, kSliceThreads, 0, st>>>(a);
+    // (the parameters lie in device memory: which rows have a cut is known to the kernels alone)
+    if (s.top_k || s.top_p) sample_histogram_kernel<<<grid, kSliceThreads, 0, st>>>(a);
+    sample_collect_kernel<<<grid, kSliceThreads, 0, st>>>(a);
+    sample_choose_kernel<false><<<(unsigned)s.rows, kThreads, lds, st>>>(a);
     return check_launch("sample");
 }
 

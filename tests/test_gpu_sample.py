@@ -53,6 +53,14 @@ def test_largest_vocabulary_and_many_rows(dev):
     np.testing.assert_array_equal(run(dev, x, u, top_k=20, top_p=0.8), want(x, u, top_k=20, top_p=0.8))
 
 
+def test_a_very_long_row(dev):
+    rng = np.random.default_rng(10)
+    x = rng.standard_normal((1, 4300007)).astype(np.float32)
+    for u in (0.1, 0.93):
+        for c in (dict(top_k=30), dict(top_p=0.4)):
+            np.testing.assert_array_equal(run(dev, x, np.float32([u]), **c), want(x, np.float32([u]), **c))
+
+
 def test_each_row_has_its_own_parameters(dev):
     rng = np.random.default_rng(2)
     rows = 64
