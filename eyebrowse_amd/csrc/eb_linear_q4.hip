@@ -49,9 +49,12 @@ __device__ __forceinline__ int seg_of(const Segs &s, int u) {
 struct Zero {
     f16x2 low, high;  // -(1024 + z), -(64 + z), twice each
 };
-__device__ __forceinline__ Zero zero_of(unsigned z) {
-    const _Float16 a = (_Float16)(-1024.0f - (float)z), b = (_Float16)(-64.0f - (float)z);
-    return Zero{{a, a}, {b, b}};
+// From byte i of z4: 0xE400 + z is f16 -(1024 + z).
+__device__ __forceinline__ Zero zero_of(unsigned z4, int i) {
+    const f16x2 up = {(_Float16)960.0f, (_Float16)960.0f};
+    const unsigned sel = 0x04000400u | (unsigned)i * 0x00010001u;  // (z, 0xE4, z, 0xE4)
+    const f16x2 low = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0xE4E4E4E4u, z4, sel));
+    return Zero{low, low + up};
 }
 __device__ __forceinline__ f16x8 unpack(unsigned w, const Zero &z) {
     const f16x2 sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
@@ -92,29 +95,46 @@ __device__ __forceinline__ unsigned max_bits(unsigned top, f32x4 x) {
 // ------------------------------------------------------------------------ up to 8 rows --------
 // A wave takes tiles of 16 features: B of v_mfma_f32_16x16x32_f16 is 16 features' codes (lane
 // (n, g) = lane n + 16 g: feature n), A the x rows, hi halves in rows 0..7 and lo halves in rows
-// 8..15, so that one product serves both. A block is 128 of the contraction: group 128 takes it
-// as one group (lane (n, g): 16 bytes, k 32 g ..), 64 as two of 8 bytes, 32 as four words, so
-// that each product's 32 values lie in one group. The rows' halves stay in LDS; a workgroup
-// splits them once and then walks its tiles.
+// 8..15, so that one product serves both. A block is 128 of the contraction, 16 words of a
+// feature: lane (n, g) loads words 4g .. 4g + 3 in one 16-byte load. Each of the block's four
+// products takes one word of every lane, and these must lie in one group: at group 128 any
+// word does; at 64 lane groups 0, 1 hold the first group and 2, 3 the second, and two swaps of
+// wave halves bring each group's words together; at 32 a 4 x 4 transpose over lane groups and
+// words does (four swaps). The rows' halves stay in LDS; a workgroup splits them once and then
+// walks its tiles; kw waves share a tile's contraction.
 constexpr int kGemvWaves = 8;
 constexpr int kGemvThreads = kGemvWaves * 64;
 constexpr int kDepth = 4;  // blocks of weights in flight per wave
 
 template <int G>
 struct Block {
-    static constexpr int NG = 128 / G, W = 4 / NG;  // groups, words per lane and group
-    unsigned w[NG][W];
-    _Float16 s[NG];
-    unsigned z[NG];
+    static constexpr int NG = 128 / G;  // groups
+    unsigned w[4];
+    unsigned s[(NG + 1) / 2];  // scales, two halves a word
+    unsigned z;                // zero points, a byte each
 };
 
-// kw waves share a tile's contraction (1 or kGemvWaves), and sum through LDS.
-template <int G, bool ZERO>
-__global__ __launch_bounds__(kGemvThreads) void q4_gemv_kernel(const float *__restrict__ x, Segs segs, int m, int K,
-                                                               int kw) {
+// w[j] of lane group g for w[j'] of g', bit b of j and bit b of g exchanged (b = 1: wave halves,
+// b = 0: neighbouring 16-lane rows).
+__device__ __forceinline__ void swap_halves(unsigned &a, unsigned &b) {
+    const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    a = r[0];
+    b = r[1];
+}
+__device__ __forceinline__ void swap_rows(unsigned &a, unsigned &b) {
+    const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+    a = r[0];
+    b = r[1];
+}
+
+// VEC: a block's scales and zero points lie aligned in one load each (K % 128 == 0, aligned bases).
+template <int G, bool ZERO, bool VEC>
+__global__ __launch_bounds__(kGemvThreads, 4) void q4_gemv_kernel(const float *__restrict__ x, Segs segs, int m,
+                                                                  int K, int kw) {
     using B = Block<G>;
+    constexpr int NG = B::NG;
     extern __shared__ f16x8 lds[];  // [blocks * 16 chunks][2 m]: chunk c of row i: hi, then lo
-    __shared__ unsigned s_top[8];
+    __shared__ unsigned s_top[kGemvWaves][8];
     __shared__ float s_part[kGemvWaves][8][16];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -123,14 +143,14 @@ __global__ __launch_bounds__(kGemvThreads) void q4_gemv_kernel(const float *__re
     const int ngr = K / G;           // groups of a row
     const int nw = K / 8;            // words of a row
 
-    // This wave's walk: tiles t0, t0 + units, ..., of each `per` blocks from b0 on (those past the
-    // row's last are skipped, but walked: the waves of a shared tile meet at its end).
-    const int units = kw == 1 ? (int)gridDim.x * kGemvWaves : (int)gridDim.x;
-    const int t0 = kw == 1 ? (int)blockIdx.x * kGemvWaves + wave : (int)blockIdx.x;
+    // This wave's walk: tiles t0, t0 + units, ..., of each `per` blocks from b0 on. (Blocks past the
+    // row's last and tiles past the last are skipped, but walked: waves that share a tile meet at
+    // its end, in barriers of the workgroup.)
+    const int units = (int)gridDim.x * (kGemvWaves / kw);
+    const int t0 = (int)blockIdx.x * (kGemvWaves / kw) + wave / kw;
     const int per = (nb + kw - 1) / kw;
-    const int b0 = kw == 1 ? 0 : wave * per;
-    const int tiles = t0 < segs.total ? (segs.total - t0 + units - 1) / units : 0;
-    const int steps = tiles * per;
+    const int b0 = wave % kw * per;
+    const int steps = (segs.total + units - 1) / units * per;
 
     B ring[kDepth];
     int lt = t0, lb = 0;  // the next block to load
@@ -138,25 +158,33 @@ __global__ __launch_bounds__(kGemvThreads) void q4_gemv_kernel(const float *__re
         if (lt < segs.total && b0 + lb < nb) {
             const Seg &sg = segs.seg[seg_of(segs, lt)];
             const int o = min((lt - sg.first) * 16 + n, sg.n - 1);
-            const int k0 = (b0 + lb) * 128;
+            const int b = b0 + lb;
+            // (words past the row's end repeat its last ones, against zeros of x)
+            const int at = VEC ? 16 * b + 4 * g : min(16 * b + 4 * g, nw - 4);
+            const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(sg.w + (size_t)o * nw + at));
 #pragma unroll
-            for (int i = 0; i < B::NG; ++i) {
-                // (a group past the row's end repeats its last one, against zeros of x)
-                const int gr = min(k0 / G + i, ngr - 1);
-                const uint32_t *p = sg.w + (size_t)o * nw + gr * (G / 8) + g * B::W;
-                if constexpr (B::W == 4) {
-                    const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p));
+            for (int j = 0; j < 4; ++j) r.w[j] = v[j];
+            const size_t gr = (size_t)o * ngr + b * NG;
+            if constexpr (VEC && NG == 4) {
+                const u32x2 q = *reinterpret_cast<const u32x2 *>(sg.s + gr);
+                r.s[0] = q[0];
+                r.s[1] = q[1];
+                if constexpr (ZERO) r.z = *reinterpret_cast<const unsigned *>(sg.z + gr);
+            } else if constexpr (VEC && NG == 2) {
+                r.s[0] = *reinterpret_cast<const unsigned *>(sg.s + gr);
+                if constexpr (ZERO) r.z = *reinterpret_cast<const uint16_t *>(sg.z + gr);
+            } else {
+                unsigned z = 0;
+                unsigned sc[(NG + 1) / 2] = {};
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) r.w[i][j] = v[j];
-                } else if constexpr (B::W == 2) {
-                    const u32x2 v = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(p));
-                    r.w[i][0] = v[0];
-                    r.w[i][1] = v[1];
-                } else {
-                    r.w[i][0] = __builtin_nontemporal_load(p);
+                for (int i = 0; i < NG; ++i) {
+                    const size_t gi = (size_t)o * ngr + min(b * NG + i, ngr - 1);
+                    sc[i / 2] |= (unsigned)__builtin_bit_cast(uint16_t, sg.s[gi]) << (16 * (i % 2));
+                    if constexpr (ZERO) z |= (unsigned)sg.z[gi] << (8 * i);
                 }
-                r.s[i] = sg.s[(size_t)o * ngr + gr];
-                r.z[i] = ZERO ? sg.z[(size_t)o * ngr + gr] : 8u;
+#pragma unroll
+                for (int i = 0; i < (NG + 1) / 2; ++i) r.s[i] = sc[i];
+                r.z = z;
             }
         }
         if (++lb == per) {
@@ -166,30 +194,49 @@ __global__ __launch_bounds__(kGemvThreads) void q4_gemv_kernel(const float *__re
     };
 #pragma unroll
     for (int i = 0; i < kDepth; ++i) load(ring[i]);
+    __builtin_amdgcn_sched_barrier(0);
 
-    // The rows' exponents and halves.
-    if (tid < 8) s_top[tid] = 0;
-    __syncthreads();
-    for (int i = 0; i < m; ++i) {
-        unsigned top = 0;
-        for (int c = tid; c < K / 4; c += kGemvThreads)
-            top = max_bits(top, *reinterpret_cast<const f32x4 *>(x + (size_t)i * K + 4 * c));
+    // The rows' exponents and halves; a thread's first chunk of each row stays in registers.
+    f32x4 keep[8][2];
+    const f32x4 z4 = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (i >= m) break;
+        const f32x4 *p = reinterpret_cast<const f32x4 *>(x + (size_t)i * K);
+        keep[i][0] = tid < nw ? p[2 * tid] : z4;
+        keep[i][1] = tid < nw ? p[2 * tid + 1] : z4;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (i >= m) break;
+        const f32x4 *p = reinterpret_cast<const f32x4 *>(x + (size_t)i * K);
+        unsigned top = max_bits(max_bits(0u, keep[i][0]), keep[i][1]);
+        for (int c = tid + kGemvThreads; c < nw; c += kGemvThreads) top = max_bits(max_bits(top, p[2 * c]), p[2 * c + 1]);
 #pragma unroll
         for (int d = 32; d > 0; d >>= 1) {
             const unsigned o = __shfl_xor(top, d);
             top = o > top ? o : top;
         }
-        if (lane == 0) atomicMax(&s_top[i], top);
+        if (lane == 0) s_top[wave][i] = top;
     }
     __syncthreads();
-    for (int i = 0; i < m; ++i) {
-        const int e = row_exponent(s_top[i]);
+    auto exponent = [&](int i) {
+        unsigned top = 0;
+#pragma unroll
+        for (int w = 0; w < kGemvWaves; ++w) top = s_top[w][i] > top ? s_top[w][i] : top;
+        return row_exponent(top);
+    };
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (i >= m) break;
+        const f32x4 *p = reinterpret_cast<const f32x4 *>(x + (size_t)i * K);
+        const int e = exponent(i);
         for (int c = tid; c < nb * 16; c += kGemvThreads) {
             f16x8 hi = {}, lo = {};
-            if (c < K / 8) {
-                const f32x4 *p = reinterpret_cast<const f32x4 *>(x + (size_t)i * K + 8 * c);
-                split8(p[0], p[1], e, hi, lo);
-            }
+            if (c == tid)
+                split8(keep[i][0], keep[i][1], e, hi, lo);  // (zeros past the row's end)
+            else if (c < nw)
+                split8(p[2 * c], p[2 * c + 1], e, hi, lo);
             lds[c * 2 * m + i] = hi;
             lds[c * 2 * m + m + i] = lo;
         }
@@ -197,7 +244,10 @@ __global__ __launch_bounds__(kGemvThreads) void q4_gemv_kernel(const float *__re
     __syncthreads();
 
     const int row = (n < 8 ? 0 : m) + min(n & 7, m - 1);  // (rows past m: the last, not stored)
-    const f16x8 *xa = lds + row;
+    // The chunk of lane group g in product j: word 4 g' + j', bits of g and j exchanged.
+    const int gw = G == 128 ? 4 * g : G == 64 ? 4 * (g & 1) + (g & 2) : g;
+    auto word = [](int j) { return G == 128 ? j : G == 64 ? 4 * (j & 2) + (j & 1) : 4 * j; };
+    const f16x8 *xa = lds + gw * 2 * m + row;
     f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
     int ct = t0, cb = 0;
     auto finish = [&] {
@@ -205,44 +255,56 @@ __global__ __launch_bounds__(kGemvThreads) void q4_gemv_kernel(const float *__re
         float v[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[r] = acc[r] + eb::lane_xor32(acc[r]);
-        const Seg &sg = segs.seg[seg_of(segs, ct)];
-        const int o = (ct - sg.first) * 16 + n;
         if (kw == 1) {
-            if (g < 2 && o < sg.n)
+            if (ct < segs.total) {
+                const Seg &sg = segs.seg[seg_of(segs, ct)];
+                const int o = (ct - sg.first) * 16 + n;
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    if (4 * g + r < m)
-                        sg.y[(size_t)(4 * g + r) * sg.n + o] = ldexpf(v[r], row_exponent(s_top[4 * g + r]));
+                    if (g < 2 && o < sg.n && 4 * g + r < m)
+                        sg.y[(size_t)(4 * g + r) * sg.n + o] = ldexpf(v[r], exponent(4 * g + r));
+            }
         } else {
             if (g < 2)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) s_part[wave][4 * g + r][n] = v[r];
             __syncthreads();
-            const int i = tid >> 4, oo = (ct - sg.first) * 16 + (tid & 15);
-            if (i < m && oo < sg.n) {
-                float t = 0.0f;
+            // The first wave of each tile's waves adds their sums: lane (n, g) rows g and g + 4.
+            if (wave % kw == 0 && ct < segs.total) {
+                const Seg &sg = segs.seg[seg_of(segs, ct)];
+                const int o = (ct - sg.first) * 16 + n;
 #pragma unroll
-                for (int w = 0; w < kGemvWaves; ++w) t += s_part[w][i][tid & 15];
-                sg.y[(size_t)i * sg.n + oo] = ldexpf(t, row_exponent(s_top[i]));
+                for (int i = g; i < 8; i += 4)
+                    if (i < m && o < sg.n) {
+                        float t = 0.0f;
+                        for (int w = 0; w < kw; ++w) t += s_part[wave + w][i][n];
+                        sg.y[(size_t)i * sg.n + o] = ldexpf(t, exponent(i));
+                    }
             }
             __syncthreads();
         }
         acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         ct += units;
     };
-    auto consume = [&](const B &r) {
-        if (b0 + cb < nb) {
+    auto consume = [&](B &r) {
+        if (ct < segs.total && b0 + cb < nb) {
             const f16x8 *xb = xa + (size_t)(b0 + cb) * 16 * 2 * m;
+            if constexpr (G <= 64) {
+                swap_halves(r.w[0], r.w[2]);
+                swap_halves(r.w[1], r.w[3]);
+            }
+            if constexpr (G == 32) {
+                swap_rows(r.w[0], r.w[1]);
+                swap_rows(r.w[2], r.w[3]);
+            }
 #pragma unroll
-            for (int i = 0; i < B::NG; ++i) {
-                const Zero z = zero_of(r.z[i]);
+            for (int i = 0; i < NG; ++i) {
+                const Zero z = zero_of(ZERO ? r.z : 0x08080808u, i);
                 f32x4 t = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int j = 0; j < B::W; ++j) {
-                    const f16x8 a = xb[(i * (G / 8) + g * B::W + j) * 2 * m];
-                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, unpack(r.w[i][j], z), t, 0, 0, 0);
-                }
-                acc += t * (float)r.s[i];
+                for (int j = i * (4 / NG); j < (i + 1) * (4 / NG); ++j)
+                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(xb[word(j) * 2 * m], unpack(r.w[j], z), t, 0, 0, 0);
+                acc += t * (float)__builtin_bit_cast(_Float16, (unsigned short)(r.s[i / 2] >> (16 * (i % 2))));
             }
         }
         if (++cb == per) {
@@ -253,7 +315,7 @@ __global__ __launch_bounds__(kGemvThreads) void q4_gemv_kernel(const float *__re
     for (int s = 0; s < steps; s += kDepth) {
 #pragma unroll
         for (int i = 0; i < kDepth; ++i)
-            if (s + i < steps) {  // (the same in every wave that shares tiles)
+            if (s + i < steps) {  // (the same in every wave)
                 consume(ring[i]);
                 load(ring[i]);
             }
@@ -367,7 +429,7 @@ __global__ __launch_bounds__(kThreads, 1) void q4_gemm_kernel(const f16x8 *__res
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 const int o = min(n0 + 32 * b + n, sg.n - 1);
-                z[b] = zero_of(ZERO ? sg.z[(size_t)o * ngr + gr] : 8u);
+                z[b] = zero_of(ZERO ? sg.z[(size_t)o * ngr + gr] : 8u, 0);
                 sc[b] = (float)sg.s[(size_t)o * ngr + gr];
             }
 #pragma unroll
@@ -455,19 +517,29 @@ int number(Segs &s, int per) {
     return s.total = t;
 }
 
+// Waves that share a tile: the fewest that give every wave slot (two workgroups on a CU) a tile.
+template <int G, bool ZERO, bool VEC>
+hipError_t launch_gemv(hipStream_t st, const float *x, const Segs &s, int m, int K) {
+    static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&q4_gemv_kernel<G, ZERO, VEC>),
+                                                    hipFuncAttributeMaxDynamicSharedMemorySize, (int)kGemvLds);
+    if (e != hipSuccess) return e;
+    const int slots = 2 * eb::current_cu_count();
+    int kw = 1;
+    while (kw < kGemvWaves && s.total * kw < slots * kGemvWaves) kw *= 2;
+    const int tiles = kGemvWaves / kw;  // a workgroup's at a time
+    const int grid = std::min((s.total + tiles - 1) / tiles, slots);
+    q4_gemv_kernel<G, ZERO, VEC><<<grid, kGemvThreads, gemv_lds(m, K), st>>>(x, s, m, K, kw);
+    return hipSuccess;
+}
+
 template <int G, bool ZERO>
 hipError_t launch(hipStream_t st, const float *x, Segs s, int m, int K, float *ws) {
     if (gemv(m, K)) {
         number(s, 16);
-        static const hipError_t e =
-            hipFuncSetAttribute(reinterpret_cast<const void *>(&q4_gemv_kernel<G, ZERO>),
-                                hipFuncAttributeMaxDynamicSharedMemorySize, (int)kGemvLds);
-        if (e != hipSuccess) return e;
-        const int cus = eb::current_cu_count();
-        const bool shared = s.total < 2 * cus * kGemvWaves;
-        const int grid = shared ? std::min(s.total, 2 * cus) : 2 * cus;
-        q4_gemv_kernel<G, ZERO><<<grid, kGemvThreads, gemv_lds(m, K), st>>>(x, s, m, K, shared ? kGemvWaves : 1);
-        return hipSuccess;
+        bool vec = K % 128 == 0;
+        for (int i = 0; i < s.nseg; ++i)
+            vec = vec && ((reinterpret_cast<uintptr_t>(s.seg[i].s) | 2 * reinterpret_cast<uintptr_t>(s.seg[i].z)) & 7) == 0;
+        return vec ? launch_gemv<G, ZERO, true>(st, x, s, m, K) : launch_gemv<G, ZERO, false>(st, x, s, m, K);
     }
     const size_t mp = round_up(m, kRowPad), kp = round_up(K, 64);
     f16x8 *hi = reinterpret_cast<f16x8 *>(ws + mp), *lo = hi + mp * kp / 8;
