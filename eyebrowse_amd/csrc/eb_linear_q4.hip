@@ -328,35 +328,52 @@ __global__ __launch_bounds__(kGemvThreads, 4) void q4_gemv_kernel(const float *_
 // halves a plane on; rows past M and the contraction past K are zeros.
 constexpr int kThreads = 256;
 
-__global__ __launch_bounds__(kThreads) void q4_split_kernel(const float *__restrict__ x, float *__restrict__ ex,
-                                                            f16x8 *__restrict__ hi, f16x8 *__restrict__ lo, int M,
-                                                            int K, int KC) {
-    const int r = blockIdx.x * 8 + (threadIdx.x & 7), l = threadIdx.x >> 3;  // 8 rows, 32 lanes each
-    __shared__ unsigned s_top[8];
-    if (threadIdx.x < 8) s_top[threadIdx.x] = 0;
-    __syncthreads();
+// 8 rows a workgroup, 128 threads each; a thread's first kSplitKept chunks stay in registers
+// between the row's exponent and its halves (4096 of the contraction).
+constexpr int kSplitThreads = 1024, kSplitKept = 4;
+__global__ __launch_bounds__(kSplitThreads) void q4_split_kernel(const float *__restrict__ x, float *__restrict__ ex,
+                                                                 f16x8 *__restrict__ hi, f16x8 *__restrict__ lo, int M,
+                                                                 int K, int KC) {
+    __shared__ unsigned s_top[kSplitThreads / 64][8];
+    const int tid = threadIdx.x, i = tid & 7, l = tid >> 3;
+    constexpr int L = kSplitThreads / 8;
+    const int r = blockIdx.x * 8 + i, nw = K / 8;
+    const f32x4 *p = reinterpret_cast<const f32x4 *>(x + (size_t)min(r, M - 1) * K);
+    const int have = r < M ? nw : 0;  // chunks of the row
+    const f32x4 z4 = {0.0f, 0.0f, 0.0f, 0.0f};
+    f32x4 keep[kSplitKept][2];
+#pragma unroll
+    for (int j = 0; j < kSplitKept; ++j) {
+        const int c = l + j * L;
+        keep[j][0] = c < have ? p[2 * c] : z4;
+        keep[j][1] = c < have ? p[2 * c + 1] : z4;
+    }
     unsigned top = 0;
-    if (r < M)
-        for (int c = l; c < K / 4; c += 32) top = max_bits(top, *reinterpret_cast<const f32x4 *>(x + (size_t)r * K + 4 * c));
+#pragma unroll
+    for (int j = 0; j < kSplitKept; ++j) top = max_bits(max_bits(top, keep[j][0]), keep[j][1]);
+    for (int c = l + kSplitKept * L; c < have; c += L) top = max_bits(max_bits(top, p[2 * c]), p[2 * c + 1]);
 #pragma unroll
     for (int d = 32; d >= 8; d >>= 1) {
         const unsigned o = __shfl_xor(top, d);
         top = o > top ? o : top;
     }
-    if ((threadIdx.x & 63) < 8) atomicMax(&s_top[threadIdx.x & 7], top);
+    if ((tid & 63) < 8) s_top[tid >> 6][i] = top;
     __syncthreads();
-    const int e = row_exponent(s_top[threadIdx.x & 7]);
+#pragma unroll
+    for (int w = 0; w < kSplitThreads / 64; ++w) top = s_top[w][i] > top ? s_top[w][i] : top;
+    const int e = row_exponent(top);
     if (l == 0) ex[r] = (float)e;
-    for (int c = l; c < KC; c += 32) {
-        f16x8 h = {}, o = {};
-        if (r < M && c < K / 8) {
-            const f32x4 *p = reinterpret_cast<const f32x4 *>(x + (size_t)r * K + 8 * c);
-            split8(p[0], p[1], e, h, o);
-        }
+    auto put = [&](int c, f32x4 a, f32x4 b) {
+        f16x8 h, o;
+        split8(a, b, e, h, o);
         const size_t at = ((size_t)(r / 32) * KC + c) * 32 + r % 32;
         hi[at] = h;
         lo[at] = o;
-    }
+    };
+#pragma unroll
+    for (int j = 0; j < kSplitKept; ++j)
+        if (l + j * L < KC) put(l + j * L, keep[j][0], keep[j][1]);
+    for (int c = l + kSplitKept * L; c < KC; c += L) put(c, c < have ? p[2 * c] : z4, c < have ? p[2 * c + 1] : z4);
 }
 
 // Workgroup tile: 32 MB WM rows x 32 NB WN features, WM x WN waves of MB x NB blocks of 32 x 32
@@ -543,7 +560,7 @@ hipError_t launch(hipStream_t st, const float *x, Segs s, int m, int K, float *w
     }
     const size_t mp = round_up(m, kRowPad), kp = round_up(K, 64);
     f16x8 *hi = reinterpret_cast<f16x8 *>(ws + mp), *lo = hi + mp * kp / 8;
-    q4_split_kernel<<<(unsigned)(mp / 8), kThreads, 0, st>>>(x, ws, hi, lo, m, K, (int)(kp / 8));
+    q4_split_kernel<<<(unsigned)(mp / 8), kSplitThreads, 0, st>>>(x, ws, hi, lo, m, K, (int)(kp / 8));
     if (m <= 64) {
         number(s, 128);
         q4_gemm_kernel<G, ZERO, 1, 1, 1, 4>

@@ -2,24 +2,25 @@
 // that a given random number picks from what they keep.
 //
 // A token's weight is w = 2^((x - max) log2(e) / T), computed in f64 and rounded once to a whole
-// number of 2^-F units (F = 62 - ceil(log2 vocab), so that a row's sum fits 64 bits). Sums of
-// whole numbers do not depend on their order: histograms may be filled by atomics, and the choice
-// is the same on every run. Ranks go by the logit's bits made monotonic (equal logits by index): a
+// number of 2^-F units (F = 44, or less for a vocabulary above 2^18, so that a row's sum fits 62
+// bits). Sums of whole numbers do not depend on their order: histograms may be filled by atomics,
+// and the choice is the same on every run. Ranks go by the logit's bits made monotonic (equal logits by index): a
 // token's rank key is those bits over the complement of its index.
 //
 // What top-k and top-p keep is the tokens down to a cut in that order. A sort would find it; here
 // a histogram does. Over slices of 4096 tokens, so that one row fills many CUs:
 //  1. max: the slice's largest rank key;
-//  2. histogram: tokens by their distance below the largest logit, in steps of 1/64 (of the
+//  2. histogram: tokens by their distance below the largest logit, in steps of 1/32 (of the
 //     temperature where it is above 1), with each step's count and weight;
 //  3. collect: every slice finds from the histogram the steps that can hold the cut, lists its
 //     tokens of those steps, and sums the kept weights of the steps above them;
-//  4. choose: one workgroup per row sorts the listed tokens (some hundreds), walks them to the
-//     exact cut, adds what is kept of them to their slices' sums, and finds the token in its slice.
+//  4. choose: one workgroup per row sorts the listed tokens, walks them to the exact cut, adds
+//     what is kept of them to their slices' sums, and finds the token in its slice. Up to 256
+//     listed tokens (a language model's logits list a few, up to some hundred where the cut lies
+//     in the wide floor) are ranked by counting, a token per thread.
 // Steps 2 and 3 do nothing for rows that need only the best token. A row whose steps list more
 // than kListed tokens (many equal logits; logits of enormous range) is solved by the choosing
-// workgroup alone, by radix selection over the row. A vocabulary of one slice is step 4 alone,
-// over all of its tokens.
+// workgroup alone, by radix selection over the row.
 #include "eb_common.h"
 #include "eb_internal.h"
 
@@ -31,14 +32,14 @@ namespace {
 typedef unsigned long long u64;
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kThreads = 1024;  // of the choosing workgroup
+constexpr int kThreads = 512;   // of the choosing workgroup
 constexpr int kWaves = kThreads / 64;
 constexpr int kTile = 4096;     // tokens of a slice
 constexpr int kSliceThreads = 512;
 constexpr int kPer = kTile / kSliceThreads;  // tokens per thread of a slice
 constexpr int kDigits = 256;    // of a radix pass
-constexpr int kBins = 2048;     // steps of the histogram
-constexpr float kBinsPerUnit = 64.0f;
+constexpr int kBins = 1024;     // steps of the histogram
+constexpr float kBinsPerUnit = 32.0f;
 constexpr int kListed = 4096;   // most listed tokens of a row
 
 // Per row, written by step 3.
@@ -77,32 +78,45 @@ __device__ __forceinline__ u64 rank_of(float x, unsigned i) { return (u64)key_of
 __device__ __forceinline__ unsigned index_of(u64 rank) { return ~(unsigned)rank; }
 constexpr u64 kLeastRank = 1ull << 32;  // at most every rank but NaN's
 
-// 2^y for y <= 0: 2^n times the Taylor sum of e^(f ln 2) for y = n + f, |f| <= 1/2 (the first term
-// left out is below 2e-16).
-__device__ __forceinline__ double exp2_f64(double y) {
-    y = fmax(y, -2000.0);  // (0 from there on)
-    const double n = __builtin_rint(y);
-    const double f = (y - n) * 0.693147180559945309417232121458;
-    double p = 1.0 / 479001600;
-    p = __builtin_fma(p, f, 1.0 / 39916800);
-    p = __builtin_fma(p, f, 1.0 / 3628800);
-    p = __builtin_fma(p, f, 1.0 / 362880);
-    p = __builtin_fma(p, f, 1.0 / 40320);
-    p = __builtin_fma(p, f, 1.0 / 5040);
-    p = __builtin_fma(p, f, 1.0 / 720);
-    p = __builtin_fma(p, f, 1.0 / 120);
-    p = __builtin_fma(p, f, 1.0 / 24);
-    p = __builtin_fma(p, f, 1.0 / 6);
-    p = __builtin_fma(p, f, 0.5);
-    p = __builtin_fma(p, f, 1.0);
-    p = __builtin_fma(p, f, 1.0);
-    return ldexp(p, (int)n);
+// 2^(y + F) for y <= 0 and whole F (0 from y = -900 on): y = n + f, |f| <= 1/2, the Taylor sum of
+// e^(f ln 2) (the first term left out is below 2e-16), and n + F added to its exponent. Adding
+// 1.5 * 2^52 leaves n in the low bits of the sum.
+constexpr double kLn2 = 0.693147180559945309417232121458;
+constexpr double term(int k) { return k == 0 ? 1.0 : term(k - 1) * kLn2 / k; }
+template <int K>
+__device__ __forceinline__ double horner(double p, double f) {
+    constexpr double c = term(K);
+    p = __builtin_fma(p, f, c);
+    if constexpr (K > 0) return horner<K - 1>(p, f);
+    return p;
+}
+__device__ __forceinline__ double exp2_scaled(double y, int frac) {
+    y = fmax(y, -900.0);
+    const double t = y + 6755399441055744.0;
+    const double f = y - (t - 6755399441055744.0);
+    constexpr double last = term(12);
+    const double p = horner<11>(last, f);
+    const u64 bits = __builtin_bit_cast(u64, p) + ((u64)((unsigned)__builtin_bit_cast(u64, t) + (unsigned)frac) << 52);
+    return __builtin_bit_cast(double, bits);
 }
 
-// A row's parameters.
+// A row's parameters as given (loaded with a kernel's other first loads).
+struct Params {
+    float temperature, top_p, min_p;
+    unsigned top_k;
+    __device__ __forceinline__ Params(const Args &a, size_t r) {
+        temperature = a.s.temperature ? a.s.temperature[r] : 1.0f;
+        min_p = a.s.min_p ? a.s.min_p[r] : 0.0f;
+        top_p = a.s.top_p ? a.s.top_p[r] : 1.0f;
+        top_k = a.s.top_k ? a.s.top_k[r] : 0u;
+    }
+};
+
+// And as used.
 struct Row {
     double rate;    // log2(e) / T
-    double min_p;   // 0: off
+    double one;     // 2^F
+    double min_p;   // in the same units; 0: off
     float top;      // the largest logit
     float per_bin;  // steps per unit of distance
     float top_p;
@@ -110,27 +124,31 @@ struct Row {
     bool none, best, use_k, use_p;  // no candidate; only the best token; which cuts
     int frac;
 
-    __device__ __forceinline__ Row(const Args &a, size_t r, unsigned best_key) {
-        const float temp = a.s.temperature ? a.s.temperature[r] : 1.0f;
-        const float mp = a.s.min_p ? a.s.min_p[r] : 0.0f;
-        top_p = a.s.top_p ? a.s.top_p[r] : 1.0f;
-        top_k = a.s.top_k ? a.s.top_k[r] : 0u;
+    __device__ __forceinline__ Row(const Args &a, const Params &p, unsigned best_key) {
+        const float temp = p.temperature, mp = p.min_p;
+        top_p = p.top_p;
+        top_k = p.top_k;
         none = best_key <= key_of(-INFINITY);  // (only -inf and NaN)
         best = !(temp > 0.0f) || mp > 1.0f || top_k == 1 || top_p <= 0.0f;
         use_k = top_k > 0 && top_k < (unsigned)a.s.vocab;
         use_p = top_p < 1.0f;
         rate = 1.4426950408889634073599 / (double)temp;
-        min_p = mp > 0.0f ? (double)mp : 0.0;
+        frac = a.frac;
+        one = ldexp(1.0, frac);
+        min_p = mp > 0.0f ? (double)mp * one : 0.0;
         top = value_of(best_key);
         per_bin = kBinsPerUnit / fmaxf(temp, 1.0f);
-        frac = a.frac;
     }
+    // w in units of 2^-F, before its rounding.
     __device__ __forceinline__ double weight(float x) const {
-        if (x == top) return 1.0;  // (top is finite or +inf)
-        if (x == -INFINITY) return 0.0;
-        return exp2_f64(((double)x - (double)top) * rate);
+        const double w = exp2_scaled(((double)x - (double)top) * rate, frac);
+        // (top is finite or +inf; -inf has no weight, also where T is infinite)
+        return x == top ? one : x == -INFINITY ? 0.0 : w;
     }
-    __device__ __forceinline__ u64 units(double w) const { return (u64)(ldexp(w, frac) + 0.5); }
+    // Rounded: below 2^51, adding 2^52 leaves the whole number in the sum's low bits.
+    __device__ __forceinline__ u64 units(double w) const {
+        return __builtin_bit_cast(u64, w + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
+    }
     __device__ __forceinline__ u64 units_kept(double w) const { return w >= min_p ? units(w) : 0; }
     // The step a logit falls in; it rises as the logit falls.
     __device__ __forceinline__ int bin(float x) const {
@@ -193,6 +211,40 @@ __device__ __forceinline__ T block_scan(T x, T *s_waves) {
     return x;
 }
 
+// Two at once.
+template <int THREADS>
+__device__ __forceinline__ void block_scan2(unsigned &x, u64 &y, unsigned *s_x, u64 *s_y) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const unsigned o = __shfl_up(x, d);
+        const u64 q = __shfl_up(y, d);
+        if (lane >= d) {
+            x += o;
+            y += q;
+        }
+    }
+    __syncthreads();
+    if (lane == 63) {
+        s_x[wave] = x;
+        s_y[wave] = y;
+    }
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) {
+        x += s_x[w];
+        y += s_y[w];
+    }
+}
+__device__ __forceinline__ u64 wave_scan(u64 x) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const u64 o = __shfl_up(x, d);
+        if (lane >= d) x += o;
+    }
+    return x;
+}
+
 // ---- steps 1 to 3: one workgroup per slice -----------------------------------------------------
 
 // The tokens of this thread in slice t: four at a time, NaN past the vocabulary.
@@ -238,31 +290,30 @@ __global__ __launch_bounds__(kSliceThreads) void sample_max_kernel(Args a) {
     if (tid == 0) a.best[r * a.tiles + t] = k;
 }
 
-// The row's largest rank key, from step 1's.
-template <int THREADS>
-__device__ __forceinline__ u64 row_best(const Args &a, size_t r, u64 *s_waves) {
+// The row's largest rank key, from step 1's (every wave by itself: no barrier).
+__device__ __forceinline__ u64 row_best(const Args &a, size_t r) {
     u64 k = 0;
-    for (int i = threadIdx.x; i < a.tiles; i += THREADS) {
+    for (int i = threadIdx.x & 63; i < a.tiles; i += 64) {
         const u64 o = a.best[r * a.tiles + i];
         k = o > k ? o : k;
     }
-    return block_best<THREADS>(k, s_waves);
+    return wave_best(k);
 }
 
 // Step 2: a histogram in LDS, its filled steps added to the row's.
 __global__ __launch_bounds__(kSliceThreads) void sample_histogram_kernel(Args a) {
     __shared__ u64 s_w[kBins];
     __shared__ unsigned s_c[kBins];
-    __shared__ u64 s_waves[kSliceThreads / 64];
     const int tid = threadIdx.x;
     const size_t r = blockIdx.y;
     const Slice s(a.s.logits + r * a.s.vocab, (int)a.s.vocab, blockIdx.x);
-    const Row row(a, r, (unsigned)(row_best<kSliceThreads>(a, r, s_waves) >> 32));
-    if (row.none || row.best || !(row.use_k || row.use_p)) return;  // (uniform)
+    const Params params(a, r);
     for (int i = tid; i < kBins; i += kSliceThreads) {
         s_w[i] = 0;
         s_c[i] = 0;
     }
+    const Row row(a, params, (unsigned)(row_best(a, r) >> 32));
+    if (row.none || row.best || !(row.use_k || row.use_p)) return;  // (uniform)
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
@@ -294,22 +345,29 @@ __global__ __launch_bounds__(kSliceThreads) void sample_collect_kernel(Args a) {
     const int tid = threadIdx.x;
     const size_t r = blockIdx.y;
     const Slice s(a.s.logits + r * a.s.vocab, (int)a.s.vocab, blockIdx.x);
-    const Row row(a, r, (unsigned)(row_best<kSliceThreads>(a, r, s_waves) >> 32));
+    const Params params(a, r);
+    unsigned c[PB];
+    u64 w[PB];
+#pragma unroll
+    for (int i = 0; i < PB; ++i) {
+        c[i] = a.hist_c[r * kBins + tid * PB + i];
+        w[i] = a.hist_w[r * kBins + tid * PB + i];
+    }
+    const Row row(a, params, (unsigned)(row_best(a, r) >> 32));
     if (row.none || row.best) return;  // (uniform)
     // Steps below lo are kept; steps lo to hi, and topk, are listed (kBins: none).
     int lo = kBins, hi = kBins, topk = kBins;
     if (row.use_k || row.use_p) {
-        unsigned c[PB], csum = 0;
-        u64 w[PB], wsum = 0;
+        unsigned csum = 0;
+        u64 wsum = 0;
 #pragma unroll
         for (int i = 0; i < PB; ++i) {
-            c[i] = a.hist_c[r * kBins + tid * PB + i];
-            w[i] = row.use_p ? a.hist_w[r * kBins + tid * PB + i] : 0;
             csum += c[i];
             wsum += w[i];
         }
-        const unsigned cend = block_scan<kSliceThreads>(csum, s_waves32);
-        const u64 wend = block_scan<kSliceThreads>(wsum, s_waves);
+        unsigned cend = csum;
+        u64 wend = wsum;
+        block_scan2<kSliceThreads>(cend, wend, s_waves32, s_waves);
         if (tid == kSliceThreads - 1) {
             s_topk = s_lo = s_hi = kBins;
             s_here = 0;
@@ -395,6 +453,8 @@ __global__ __launch_bounds__(kSliceThreads) void sample_collect_kernel(Args a) {
 }
 
 // ---- step 4: one workgroup per row --------------------------------------------------------------
+
+constexpr int kTokens = kTile / kThreads;  // tokens per thread of the chosen slice
 
 struct Shared {
     u64 wsum[kDigits];
@@ -541,13 +601,11 @@ __device__ __noinline__ u64 solve_row(const Args &a, const Row &row, const float
     }
     __syncthreads();
     if (s.last >= 0) {  // the rank of the in_last-th of them in its tile
-        const int base = s.last * kTile + 4 * tid;
+        const int base = s.last * kTile + kTokens * tid;
         unsigned same = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) same += base + j < n && key_of(x[base + j]) == cut;
+        for (int j = 0; j < kTokens; ++j) same += base + j < n && key_of(x[base + j]) == cut;
         unsigned before = block_scan<kThreads>(same, s.waves32) - same;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < kTokens; ++j)
             if (base + j < n && key_of(x[base + j]) == cut && ++before == s.in_last)
                 s.cut = rank_of(x[base + j], (unsigned)(base + j));
     }
@@ -555,160 +613,193 @@ __device__ __noinline__ u64 solve_row(const Args &a, const Row &row, const float
     return s.cut;
 }
 
-// ONE: the vocabulary is one slice, and its tokens are the list.
-template <bool ONE>
+// The cut from a list of up to kThreads tokens, one per thread (`rank`: 0 for none), in LDS too;
+// the kept ones' weights join their slices' sums.
+__device__ __forceinline__ u64 cut_of_few(u64 rank, const u64 *s_list, u64 *s_sorted, unsigned listed, const Cut &c,
+                                          const Row &row, u64 best, u64 *s_tiles, Shared &s) {
+    const int tid = threadIdx.x;
+    // Its place, largest first, is the number of larger ones (ranks differ).
+    unsigned place = 0;
+    for (unsigned i = 0; i < listed; i += 4) {  // (past the list: zeros)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) place += s_list[i + j] > rank;
+    }
+    if (rank) s_sorted[place] = rank;
+    __syncthreads();
+    rank = (unsigned)tid < listed ? s_sorted[tid] : 0ull;
+    const float v = value_of((unsigned)(rank >> 32));
+    bool in = rank != 0;
+    const double f = in ? row.weight(v) : 0.0;
+    const u64 w = row.units(f);
+    // Top-k keeps the first top_k - above of its step (the last of the listed steps); what it keeps
+    // weighs `total`.
+    const bool topk = in && row.bin(v) == c.topk_bin;
+    const int others = __syncthreads_count(in && !topk);
+    if (topk) in = (unsigned)(tid - others) < row.top_k - c.above;
+    // Top-p keeps a token while the weight before it is below the target.
+    if (row.use_p) {
+        const u64 mine = in ? w : 0;
+        const u64 end = wave_scan(mine), of_topk = wave_total(topk ? mine : 0ull);
+        if ((tid & 63) == 63) s.waves[tid >> 6] = end;
+        if ((tid & 63) == 0) s.wsum[tid >> 6] = of_topk;
+        __syncthreads();
+        u64 before = c.before_cut + end - mine, total = c.before_topk;
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) {
+            if (i < tid >> 6) before += s.waves[i];
+            total += s.wsum[i];
+        }
+        in = in && (rank == best || (double)before < (double)row.top_p * (double)total);
+    }
+    if (in && w && f >= row.min_p) atomicAdd(&s_tiles[index_of(rank) / kTile], w);
+    const int kept = __syncthreads_count(in);  // (the first `kept` of the order, at least one)
+    return s_sorted[kept - 1];
+}
+
+// The same from a longer list, sorted in LDS, by the workgroup.
+__device__ __noinline__ u64 cut_of_list(u64 *s_list, u64 *s_w, unsigned listed, const Cut &c, const Row &row, u64 best,
+                                        u64 *s_tiles, Shared &s) {
+    const int tid = threadIdx.x;
+    int size = 1;
+    while (size < (int)listed) size *= 2;  // (zeros pad the list)
+    __syncthreads();
+    for (int k = 2; k <= size; k *= 2)
+        for (int j = k / 2; j > 0; j /= 2) {
+            for (int i = tid; i < size / 2; i += kThreads) {
+                const int p = 2 * i - (i & (j - 1)), q = p + j;
+                const u64 u = s_list[p], v = s_list[q];
+                if ((u < v) == ((p & k) == 0)) {
+                    s_list[p] = v;
+                    s_list[q] = u;
+                }
+            }
+            __syncthreads();
+        }
+    // Thread tid has places from .. to - 1 of the order.
+    const int pt = (size + kThreads - 1) / kThreads, from = min(pt * tid, (int)listed), to = min(from + pt, (int)listed);
+    auto value = [&](int i) { return value_of((unsigned)(s_list[i] >> 32)); };
+    unsigned here = 0;
+    for (int i = from; i < to; ++i) {
+        s_w[i] = row.units(row.weight(value(i)));
+        here += row.bin(value(i)) == c.topk_bin;
+    }
+    unsigned place = block_scan<kThreads>(here, s.waves32) - here;
+    const unsigned keep_k = row.use_k ? row.top_k - c.above : 0xFFFFFFFFu;
+    u64 mine = 0, all = 0;
+    int stop = to;  // this thread's first place that top-k does not keep
+    for (int i = from; i < to; ++i) {
+        const bool topk = row.bin(value(i)) == c.topk_bin;
+        if (topk && place++ >= keep_k) {
+            stop = i;
+            break;
+        }
+        if (topk) mine += s_w[i];
+        all += s_w[i];
+    }
+    const u64 total = c.before_topk + block_total<kThreads>(mine, s.waves);
+    if (row.use_p) {
+        const double target = (double)row.top_p * (double)total;
+        u64 before = c.before_cut + block_scan<kThreads>(all, s.waves) - all;
+        for (int i = from; i < stop; ++i) {
+            if (s_list[i] != best && !((double)before < target)) {
+                stop = i;
+                break;
+            }
+            before += s_w[i];
+        }
+    }
+    __syncthreads();
+    if (tid == 0) s.cut = ~0ull;
+    __syncthreads();
+    for (int i = from; i < stop; ++i)
+        if (s_w[i] && row.weight(value(i)) >= row.min_p) atomicAdd(&s_tiles[index_of(s_list[i]) / kTile], s_w[i]);
+    if (stop > from) atomicMin(&s.cut, s_list[stop - 1]);
+    __syncthreads();
+    return s.cut;
+}
+
 __global__ __launch_bounds__(kThreads) void sample_choose_kernel(Args a) {
-    constexpr int PT = kListed / kThreads;  // listed tokens per thread
-    static_assert(kListed >= kTile && kTile == 4 * kThreads, "a slice's tokens fit the list, four a thread");
     __shared__ Shared s;
-    __shared__ u64 s_list[kListed];
+    __shared__ u64 s_list[kListed], s_w[kListed];
     extern __shared__ u64 s_tiles[];  // [tiles], then [tiles] u32
     unsigned *s_eq = reinterpret_cast<unsigned *>(s_tiles + a.tiles);
     const size_t r = blockIdx.x;
-    const int n = (int)a.s.vocab, tiles = a.tiles, tid = threadIdx.x;
+    const int n = (int)a.s.vocab, tiles = a.tiles, tid = threadIdx.x, lane = tid & 63;
     const float *x = a.s.logits + r * a.s.vocab;
 
-    u64 best = 0;
-    if constexpr (ONE) {
-        for (int i = tid; i < kListed; i += kThreads) {
-            const u64 k = i < n ? rank_of(x[i], (unsigned)i) : 0;
-            s_list[i] = k;
-            best = k > best ? k : best;
-        }
-        best = block_best<kThreads>(best, s.waves);
-    } else {
-        best = row_best<kThreads>(a, r, s.waves);
-    }
-    const Row row(a, r, (unsigned)(best >> 32));
+    // (loads first; what a row does not need may be anything)
+    u64 rank = a.listed[r * kListed + tid];
+    const unsigned counted = a.count[r];
+    const Cut c = a.cut[r];
+    const float u = a.s.u[r];
+    const Params params(a, r);
+    for (int t = tid; t < tiles; t += kThreads) s_tiles[t] = a.tile_sum[r * tiles + t];
+    const u64 best = row_best(a, r);
+    const Row row(a, params, (unsigned)(best >> 32));
     if (row.none || row.best) {  // (uniform)
         if (tid == 0) a.s.out[r] = row.none ? 0u : index_of(best);
         return;
     }
-    const bool cuts = row.use_k || row.use_p;
-    const unsigned listed = ONE ? (unsigned)n : cuts ? a.count[r] : 0u;
+    const unsigned listed = row.use_k || row.use_p ? counted : 0u;  // (0: every token is kept)
     u64 cut = kLeastRank;
-    if (listed > kListed) {  // (uniform)
+    rank = (unsigned)tid < listed ? rank : 0ull;
+    s_list[tid] = rank;
+    __syncthreads();
+    if (listed > kListed) {  // (uniform, as below)
         cut = solve_row(a, row, x, s_tiles, s_eq, s);
-    } else if (ONE && !cuts) {
-        u64 part = 0;
-        for (int i = tid; i < n; i += kThreads)
-            if (x[i] == x[i]) part += row.units_kept(row.weight(x[i]));
-        part = block_total<kThreads>(part, s.waves);
-        if (tid == 0) s_tiles[0] = part;
-    } else {
-        if constexpr (ONE) {
-            if (tid == 0) s_tiles[0] = 0;
-        } else {
-            for (int t = tid; t < tiles; t += kThreads) s_tiles[t] = a.tile_sum[r * tiles + t];
-            for (unsigned i = tid; i < kListed; i += kThreads) s_list[i] = i < listed ? a.listed[r * kListed + i] : 0;
-        }
-        __syncthreads();
-        if (listed > 0) {  // (0: every token is kept)
-            // Largest first (bitonic; zeros pad the list to a power of two).
-            int size = 1;
-            while (size < (int)listed) size *= 2;
-            for (int k = 2; k <= size; k *= 2)
-                for (int j = k / 2; j > 0; j /= 2) {
-                    for (int i = tid; i < size / 2; i += kThreads) {
-                        const int p = 2 * i - (i & (j - 1)), q = p + j;
-                        const u64 u = s_list[p], v = s_list[q];
-                        if ((u < v) == ((p & k) == 0)) {
-                            s_list[p] = v;
-                            s_list[q] = u;
-                        }
-                    }
-                    __syncthreads();
-                }
-            // Thread tid has places PT tid .. of the order.
-            const Cut c = ONE ? Cut{0, 0, 0, 0} : a.cut[r];
-            u64 rank[PT], w[PT];
-            bool in[PT], topk[PT];
-            unsigned here = 0;  // tokens of top-k's step
-#pragma unroll
-            for (int j = 0; j < PT; ++j) {
-                rank[j] = s_list[PT * tid + j];
-                const float v = value_of((unsigned)(rank[j] >> 32));
-                in[j] = rank[j] >= kLeastRank;
-                w[j] = in[j] ? row.units(row.weight(v)) : 0;
-                topk[j] = in[j] && (ONE || row.bin(v) == c.topk_bin);
-                here += topk[j];
-            }
-            // Top-k keeps the first top_k - above of its step; what it keeps weighs `total`.
-            unsigned place = block_scan<kThreads>(here, s.waves32) - here;
-            const unsigned keep_k = row.use_k ? row.top_k - c.above : 0xFFFFFFFFu;
-            u64 mine = 0;
-#pragma unroll
-            for (int j = 0; j < PT; ++j)
-                if (topk[j]) {
-                    in[j] = place++ < keep_k;
-                    if (in[j]) mine += w[j];
-                }
-            const u64 total = c.before_topk + block_total<kThreads>(mine, s.waves);
-            // Top-p keeps a token while the weight before it is below the target.
-            if (row.use_p) {
-                const double target = (double)row.top_p * (double)total;
-                mine = 0;
-#pragma unroll
-                for (int j = 0; j < PT; ++j) mine += in[j] ? w[j] : 0;
-                u64 before = c.before_cut + block_scan<kThreads>(mine, s.waves) - mine;
-#pragma unroll
-                for (int j = 0; j < PT; ++j) {
-                    const u64 after = before + (in[j] ? w[j] : 0);
-                    in[j] = in[j] && (rank[j] == best || (double)before < target);
-                    before = after;
-                }
-            }
-            // The cut is the last kept; the kept ones' weights join their slices' sums.
-            if (tid == 0) s.cut = ~0ull;
-            __syncthreads();
-            u64 least = ~0ull;
-#pragma unroll
-            for (int j = 0; j < PT; ++j) {
-                if (!in[j]) continue;
-                least = rank[j] < least ? rank[j] : least;
-                const u64 k = row.units_kept(row.weight(value_of((unsigned)(rank[j] >> 32))));
-                if (k) atomicAdd(&s_tiles[index_of(rank[j]) / kTile], k);
-            }
-            if (least != ~0ull) atomicMin(&s.cut, least);
-            __syncthreads();
-            cut = s.cut;
-        }
+    } else if (listed > kThreads) {
+        for (unsigned i = tid + kThreads; i < kListed; i += kThreads) s_list[i] = i < listed ? a.listed[r * kListed + i] : 0;
+        cut = cut_of_list(s_list, s_w, listed, c, row, best, s_tiles, s);
+    } else if (listed > 0) {
+        cut = cut_of_few(rank, s_list, s_w, listed, c, row, best, s_tiles, s);
     }
-    __syncthreads();
+    if (listed > kThreads) __syncthreads();
 
-    // The slice that holds the token: thread tid has `per` tiles from per * tid on.
-    const int per = (tiles + kThreads - 1) / kThreads;
-    u64 mine = 0;
-    for (int t = per * tid; t < min(per * (tid + 1), tiles); ++t) mine += s_tiles[t];
-    const u64 end = block_scan<kThreads>(mine, s.waves);
-    const u64 total = block_total<kThreads>(mine, s.waves);
-    const float u = a.s.u[r];
-    const double place = u > 0.0f ? (double)u * (double)total : 0.0;
-    u64 thr = place >= (double)total ? total - 1 : (u64)place;
-    if (thr >= total) thr = total - 1;
-    if (thr < end && thr >= end - mine) {  // (one thread)
+    // The slice that holds the token, found by every wave: lane l has `per` tiles from per * l on.
+    int tile = 0;
+    u64 left = 0;
+    {
+        const int per = (tiles + 63) / 64;
+        u64 mine = 0;
+        for (int t = per * lane; t < min(per * (lane + 1), tiles); ++t) mine += s_tiles[t];
+        const u64 end = wave_scan(mine), total = __shfl(end, 63);
+        const double place = u > 0.0f ? (double)u * (double)total : 0.0;
+        u64 thr = place >= (double)total ? total - 1 : (u64)place;
+        if (thr >= total) thr = total - 1;
+        const bool here = thr < end && thr >= end - mine;  // (one lane)
         thr -= end - mine;
-        int t = per * tid;
-        while (thr >= s_tiles[t]) thr -= s_tiles[t++];
-        s.tile = t;
-        s.left = thr;
+        int t = per * lane;
+        while (here && thr >= s_tiles[t]) thr -= s_tiles[t++];
+        const int l = __ffsll((long long)__ballot(here)) - 1;
+        tile = __shfl(t, l);
+        left = __shfl(thr, l);
     }
-    __syncthreads();
-    // And the token in it: thread tid has tokens 4 tid .. 4 tid + 3.
-    const int base = s.tile * kTile + tid * 4;
-    u64 w[4];
-    mine = 0;
+    // And the token in it: thread tid has tokens kTokens * tid ...
+    const int base = tile * kTile + tid * kTokens;
+    float v[kTokens];
+    if ((n & 3) == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const float v = base + j < n ? x[base + j] : __builtin_nanf("");
-        w[j] = v == v && rank_of(v, (unsigned)(base + j)) >= cut ? row.units_kept(row.weight(v)) : 0;
+        for (int j = 0; j < kTokens; j += 4) {
+            const f32x4 q = *reinterpret_cast<const f32x4 *>(x + min(base + j, n - 4));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[j + i] = base + j < n ? q[i] : __builtin_nanf("");
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < kTokens; ++j) v[j] = base + j < n ? x[base + j] : __builtin_nanf("");
+    }
+    u64 w[kTokens], mine = 0;
+#pragma unroll
+    for (int j = 0; j < kTokens; ++j) {
+        w[j] = 0;
+        if (v[j] == v[j] && rank_of(v[j], (unsigned)(base + j)) >= cut) w[j] = row.units_kept(row.weight(v[j]));
         mine += w[j];
     }
     u64 cum = block_scan<kThreads>(mine, s.waves) - mine;
-    if (cum <= s.left && cum + mine > s.left) {
+    if (cum <= left && cum + mine > left) {  // (one thread)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (cum <= s.left && cum + w[j] > s.left) a.s.out[r] = (unsigned)(base + j);
+        for (int j = 0; j < kTokens; ++j) {
+            if (cum <= left && cum + w[j] > left) a.s.out[r] = (unsigned)(base + j);
             cum += w[j];
         }
     }
@@ -743,23 +834,18 @@ constexpr size_t kMaxVocab = (size_t)1 << 24;
 namespace eb {
 
 size_t sample_workspace_floats(size_t rows, size_t vocab) {
-    const size_t tiles = (vocab + kTile - 1) / kTile;
-    return tiles <= 1 ? 0 : layout_of(rows, tiles).floats;
+    return layout_of(rows, (vocab + kTile - 1) / kTile).floats;
 }
 
 eb_status launch_sample(hipStream_t st, const SampleArgs &s, float *ws) {
     Args a{};
     a.s = s;
-    a.frac = 62;
+    a.frac = 44;
     while (((size_t)1 << (62 - a.frac)) < s.vocab) --a.frac;
     const size_t tiles = (s.vocab + kTile - 1) / kTile;
     a.tiles = (int)tiles;
     const size_t lds = tiles * 12 + 8;
-    if (tiles <= 1) {
-        sample_choose_kernel<true><<<(unsigned)s.rows, kThreads, lds, st>>>(a);
-        return check_launch("sample");
-    }
-    static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&sample_choose_kernel<false>),
+    static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&sample_choose_kernel),
                                                     hipFuncAttributeMaxDynamicSharedMemorySize,
                                                     (int)(kMaxVocab / kTile * 12 + 8));
     if (e != hipSuccess) return hip_fail(e, "sample launch set-up");
@@ -776,7 +862,7 @@ eb_status launch_sample(hipStream_t st, const SampleArgs &s, float *ws) {
     // (the parameters lie in device memory: which rows have a cut is known to the kernels alone)
     if (s.top_k || s.top_p) sample_histogram_kernel<<<grid, kSliceThreads, 0, st>>>(a);
     sample_collect_kernel<<<grid, kSliceThreads, 0, st>>>(a);
-    sample_choose_kernel<false><<<(unsigned)s.rows, kThreads, lds, st>>>(a);
+    sample_choose_kernel<<<(unsigned)s.rows, kThreads, lds, st>>>(a);
     return check_launch("sample");
 }
 

@@ -106,7 +106,7 @@ def test_sample():
         return err(l.eb_launch_sample, None, x, xn, u, out, rows, vocab, None, None, None, None, None, 0)
 
     for over, status, word in ((dict(xn=299), 4, "logits"), (dict(x=None), 4, "null"), (dict(u=None), 4, "null"), (dict(out=None), 4, "null"),
-                               (dict(vocab=0), 4, "vocab"), (dict(vocab=(1 << 24) + 1, rows=1, xn=1 << 25), 3, "vocab"),
+                               (dict(vocab=0), 4, "vocab"), (dict(), 4, "workspace"), (dict(rows=65536, vocab=2, xn=1 << 17), 3, "rows"), (dict(vocab=(1 << 24) + 1, rows=1, xn=1 << 25), 3, "vocab"),
                                (dict(rows=1 << 40, vocab=1 << 40), 3, "overflows")):
         st, msg = call(**over)
         assert st == status and word in msg, (over, msg)
