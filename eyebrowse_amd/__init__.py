@@ -33,6 +33,7 @@ from .kernels import (argmax, argmax_workspace_floats, attn_decode, attn_decode_
                       LANE_OPS_ROWS, launch_selftest_lane_ops, attn_prefill_pv16,
                       launch_attn_prefill_pv16, launch_attn_prefill_pv16_ws,
                       linear_q4, linear_q4_multi, linear_q4_workspace_floats, launch_linear_q4,
+                      q4_packed_bytes, launch_q4_pack,
                       kv_write_i8, kv_read_i8, attn_decode_i8, attn_decode_step_i8,
                       attn_prefill_chunk_i8, attn_i8_workspace_floats, launch_kv_write_i8,
                       launch_kv_read_i8, launch_attn_decode_i8, launch_attn_prefill_chunk_i8,
@@ -59,7 +60,7 @@ __all__ = [
     "attn_decode_noalloc_max_floats", "rmsnorm", "rope", "Attention", "KvCache", "Linear", "Rope",
     "LANE_OPS_ROWS", "launch_selftest_lane_ops", "attn_prefill_pv16", "launch_attn_prefill_pv16",
     "launch_attn_prefill_pv16_ws", "LinearQ4", "CacheI8",
-    "linear_q4", "linear_q4_multi", "linear_q4_workspace_floats", "launch_linear_q4",
+    "linear_q4", "linear_q4_multi", "linear_q4_workspace_floats", "launch_linear_q4", "q4_packed_bytes", "launch_q4_pack",
     "kv_write_i8", "kv_read_i8", "attn_decode_i8", "attn_decode_step_i8",
     "attn_prefill_chunk_i8", "attn_i8_workspace_floats", "launch_kv_write_i8",
     "launch_kv_read_i8", "launch_attn_decode_i8", "launch_attn_prefill_chunk_i8", "sample",

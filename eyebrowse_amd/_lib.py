@@ -42,12 +42,11 @@ class AttentionDesc(ctypes.Structure):
 class Q4Weight(ctypes.Structure):
     """eb_q4_weight."""
     _fields_ = [
-        ("w", c_vp),
-        ("scales", c_vp),
-        ("zeros", c_vp),
+        ("packed", c_vp),
         ("in_f", c_size),
         ("out_f", c_size),
         ("group", c_size),
+        ("zeros", c_int),
     ]
 
 
@@ -234,8 +233,13 @@ SIGNATURES = {
     "eb_linear_q4_multi": (c_st, [c_vp, c_vp, c_size, ctypes.POINTER(Q4Weight),
                                   ctypes.POINTER(c_vp), c_size]),
     "eb_linear_q4_workspace_floats": (c_size, [c_size, c_size]),
-    "eb_launch_linear_q4": (c_st, [c_vp, c_vp, c_size, c_vp, c_size, c_vp, c_size, c_vp, c_size,
-                                   c_vp, c_size, c_size, c_size, c_size, c_size, c_vp, c_size]),
+    "eb_q4_packed_bytes": (c_size, [c_size, c_size, c_size, c_int]),
+    "eb_q4_pack": (c_st, [c_vp, c_vp, c_vp, c_vp, c_size, c_size, c_size,
+                          ctypes.POINTER(c_vp)]),
+    "eb_launch_q4_pack": (c_st, [c_vp, c_vp, c_size, c_vp, c_size, c_vp, c_size, c_size, c_size,
+                                 c_size, c_vp, c_size]),
+    "eb_launch_linear_q4": (c_st, [c_vp, c_vp, c_size, c_vp, c_size, c_vp, c_size, c_size, c_size,
+                                   c_size, c_size, c_int, c_vp, c_size]),
     "eb_attention_new_q4": (c_st, [ctypes.POINTER(AttentionDesc), ctypes.POINTER(Q4Weight),
                                    ctypes.POINTER(c_vp)]),
     "eb_kv_cache_new_i8": (c_st, [c_vp, ctypes.POINTER(c_size), c_size, c_size, c_size, c_size,

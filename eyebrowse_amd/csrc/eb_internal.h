@@ -231,11 +231,14 @@ eb_status launch_linear_f16w_multi(hipStream_t st, const float *x, const uint16_
 // linear_q4: nseg (1..kLinearMaxSegs) weight/output pairs that share x, in_f and group, with zero
 // points all or none; linear_q4_workspace_floats(m, in_f) floats, 16-byte aligned.
 struct Q4Weight {
-    const uint32_t *w;       // [out_f, in_f / 8]
-    const uint16_t *scales;  // [out_f, in_f / group]
-    const uint8_t *zeros;    // the same, or null
+    const uint8_t *packed;  // q4_packed_bytes, 16-byte aligned
     size_t in_f, out_f, group;
+    bool zeros;
 };
+// w [out_f, in_f / 8], scales [out_f, in_f / group], zeros the same or null.
+size_t q4_packed_bytes(size_t in_f, size_t out_f, size_t group, bool zeros);
+eb_status launch_q4_pack(hipStream_t st, const uint32_t *w, const uint16_t *scales, const uint8_t *zeros, uint8_t *packed,
+                         size_t in_f, size_t out_f, size_t group);
 size_t linear_q4_workspace_floats(size_t m, size_t in_f);
 eb_status launch_linear_q4(hipStream_t st, const float *x, const Q4Weight *w, float *const *y, int nseg, size_t m,
                            float *ws);

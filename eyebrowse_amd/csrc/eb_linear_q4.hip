@@ -1,16 +1,25 @@
 // Projections with 4-bit weights and group scales for gfx950:
 //   y[i, o] = sum_g s[o, g] sum_{k in g} x[i, k] (q[o, k] - z[o, g])
-// with x and y f32, q 4-bit codes (eight per word, lowest bits first), s half, z a byte (or 8).
+// with x and y f32, q 4-bit codes, s half, z a byte (or 8).
 //
-// Both forms run on the matrix cores. A code less its zero point is a whole number, exact in f16.
+// All forms run on the matrix cores. A code less its zero point is a whole number, exact in f16.
 // An x row is scaled by a power of two (its largest magnitude lands in [2^14, 2^15)) and split
 // into f16 halves hi + lo, 22 bits of it; each product is exact in f32. The sum over a group is
 // accumulated apart, then scaled and added in f32, so that no scale is rounded to f16.
 //
-// Unpacking a word gives four f16 pairs with nine instructions: (w & 0x000F000F) | 0x64006400 is
-// the pair (1024 + k0, 1024 + k4), from which 1024 + z is subtracted; (w & 0x00F000F0) |
-// 0x64006400 is (1024 + 16 k1, 1024 + 16 k5), times 1/16 less 64 + z; the same of w >> 8. So a
-// word's contraction order is k0 k4 k1 k5 k2 k6 k3 k7, and x's halves are laid out in it.
+// Weights are packed once (q4_pack_kernel) into tiles of 16 features, cut into blocks of 128 of the
+// contraction: 1 KiB of codes, which lane n + 16 g of a wave reads as 16 bytes: word j holds the
+// 8 codes of feature n from k = 32 j + 8 g on. So a product of 32 of the contraction (word j of
+// every lane) lies in one group whatever the group's size, a wave's load is 1 KiB of memory, and a
+// tile is one run of it. Read in the [out, in] layout, a wave's load was 16 pieces of 64 bytes in 16
+// rows, and as many lines again for scales and zero points: a head of 1024 x 151936 took 30 us (3.1
+// TB/s) whatever its instructions. Scales and zero points follow, [tile][block][16][128 / group]
+// each. The contraction is padded to whole blocks and the features to whole tiles, with zero scales.
+//
+// In a word, codes k0, k2, k4, k6 are the nibbles of the low half, k1, k3, k5, k7 of the high one.
+// Unpacking gives four f16 pairs in order with nine instructions: (w & 0x000F000F) | 0x64006400 is
+// the pair (1024 + k0, 1024 + k1), from which 1024 + z is subtracted; (w & 0x00F000F0) |
+// 0x64006400 is (1024 + 16 k2, 1024 + 16 k3), times 1/16 less 64 + z; the same of w >> 8.
 #include "eb_common.h"
 #include "eb_internal.h"
 
@@ -26,23 +35,31 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
+constexpr int kBlock = 128;       // of the contraction
+constexpr int kTileBytes = 1024;  // codes of a block of a tile
+constexpr int kFeatures = 16;     // of a tile
+
+// A packed weight: its planes, and the output.
 struct Seg {
-    const uint32_t *w;
-    const _Float16 *s;
-    const uint8_t *z;
+    const uint8_t *w;  // [tiles][blocks][1024]
+    const _Float16 *s; // [tiles][blocks][16][128 / group]
+    const uint8_t *z;  // the same, or null
     float *y;
     int n;      // features
-    int first;  // first 16-feature tile (or work unit) of the pair
+    int first;  // first work unit of the pair
 };
 struct Segs {
     Seg seg[eb::kLinearMaxSegs];
-    int nseg, total;  // tiles of all pairs
+    int nseg, total;  // units of all pairs
 };
-__device__ __forceinline__ int seg_of(const Segs &s, int u) {
-    int i = 0;
+// The pair of unit u, by selects on the kernel's arguments (an index that varies would load from
+// memory, and wait for it, wherever it is used).
+__device__ __forceinline__ Seg seg_at(const Segs &s, int u) {
+    Seg r = s.seg[0];
 #pragma unroll
-    for (int j = 1; j < eb::kLinearMaxSegs; ++j) i += (j < s.nseg && u >= s.seg[j].first) ? 1 : 0;
-    return i;
+    for (int j = 1; j < eb::kLinearMaxSegs; ++j)
+        if (j < s.nseg && u >= s.seg[j].first) r = s.seg[j];
+    return r;
 }
 
 // The four f16 pairs of a word: codes less their zero point.
@@ -58,17 +75,31 @@ __device__ __forceinline__ Zero zero_of(unsigned z4, int i) {
 }
 __device__ __forceinline__ f16x8 unpack(unsigned w, const Zero &z) {
     const f16x2 sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f};
+    // (the constant in a register: and + or are then one instruction, which takes no literals)
+    unsigned magic = 0x64006400u;
+    asm("" : "+v"(magic));
     const unsigned v = w >> 8;
-    const f16x2 a = __builtin_bit_cast(f16x2, (w & 0x000F000Fu) | 0x64006400u) + z.low;
-    const f16x2 b = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (w & 0x00F000F0u) | 0x64006400u), sixteenth, z.high);
-    const f16x2 c = __builtin_bit_cast(f16x2, (v & 0x000F000Fu) | 0x64006400u) + z.low;
-    const f16x2 d = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (v & 0x00F000F0u) | 0x64006400u), sixteenth, z.high);
+    const f16x2 a = __builtin_bit_cast(f16x2, (w & 0x000F000Fu) | magic) + z.low;
+    const f16x2 b = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (w & 0x00F000F0u) | magic), sixteenth, z.high);
+    const f16x2 c = __builtin_bit_cast(f16x2, (v & 0x000F000Fu) | magic) + z.low;
+    const f16x2 d = __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (v & 0x00F000F0u) | magic), sixteenth, z.high);
     return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
+__device__ __forceinline__ float half_of(unsigned w, int i) {
+    return (float)__builtin_bit_cast(_Float16, (unsigned short)(w >> (16 * i)));
+}
 
-// Eight values of a row (k0 .. k7), scaled by 2^-e, as hi and lo halves in a word's order.
+// Scales and zero points of a feature in a block, NG = 128 / group of each.
+template <int NG>
+struct Scales {
+    unsigned s[(NG + 1) / 2];
+    unsigned z;
+    __device__ __forceinline__ float scale(int i) const { return half_of(s[i / 2], i % 2); }
+};
+
+// Eight values of a row, scaled by 2^-e, as hi and lo halves.
 __device__ __forceinline__ void split8(f32x4 a, f32x4 b, int e, f16x8 &hi, f16x8 &lo) {
-    const float v[8] = {a[0], b[0], a[1], b[1], a[2], b[2], a[3], b[3]};
+    const float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const float x = ldexpf(v[i], -e);
@@ -92,104 +123,107 @@ __device__ __forceinline__ unsigned max_bits(unsigned top, f32x4 x) {
     return top;
 }
 
+// ------------------------------------------------------------------------ packing -------------
+// One workgroup per block of a tile.
+constexpr int kPackThreads = 256;
+__global__ __launch_bounds__(kPackThreads) void q4_pack_kernel(const uint32_t *__restrict__ w,
+                                                               const uint16_t *__restrict__ s,
+                                                               const uint8_t *__restrict__ z, uint32_t *__restrict__ pw,
+                                                               uint16_t *__restrict__ ps, uint8_t *__restrict__ pz, int N,
+                                                               int K, int G, int nb) {
+    const size_t at = blockIdx.x;  // tile * nb + block
+    const int tile = (int)(at / nb), b = (int)(at % nb), tid = threadIdx.x;
+    const int ng = kBlock / G, ngr = K / G, nw = K / 8;
+    {
+        const int lane = tid / 4, j = tid % 4, n = lane % 16, g = lane / 16;
+        const int o = tile * kFeatures + n, word = b * 16 + 4 * j + g;
+        uint32_t v = 0, r = 0;
+        if (o < N && word < nw) v = w[(size_t)o * nw + word];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r |= (v >> (4 * i) & 15u) << (16 * (i % 2) + 4 * (i / 2));
+        pw[at * (kTileBytes / 4) + tid] = r;
+    }
+    if (tid < kFeatures * ng) {
+        const int o = tile * kFeatures + tid / ng, gr = b * ng + tid % ng;
+        const bool in = o < N && gr < ngr;
+        ps[at * kFeatures * ng + tid] = in ? s[(size_t)o * ngr + gr] : (uint16_t)0;
+        if (pz) pz[at * kFeatures * ng + tid] = in && z ? z[(size_t)o * ngr + gr] : (uint8_t)0;
+    }
+}
+
 // ------------------------------------------------------------------------ up to 8 rows --------
-// A wave takes tiles of 16 features: B of v_mfma_f32_16x16x32_f16 is 16 features' codes (lane
-// (n, g) = lane n + 16 g: feature n), A the x rows, hi halves in rows 0..7 and lo halves in rows
-// 8..15, so that one product serves both. A block is 128 of the contraction, 16 words of a
-// feature: lane (n, g) loads words 4g .. 4g + 3 in one 16-byte load. Each of the block's four
-// products takes one word of every lane, and these must lie in one group: at group 128 any
-// word does; at 64 lane groups 0, 1 hold the first group and 2, 3 the second, and two swaps of
-// wave halves bring each group's words together; at 32 a 4 x 4 transpose over lane groups and
-// words does (four swaps). The rows' halves stay in LDS; a workgroup splits them once and then
-// walks its tiles; kw waves share a tile's contraction.
+// A wave takes tiles: B of v_mfma_f32_16x16x32_f16 is the 16 features' codes, A the x rows, hi halves
+// in rows 0..7 and lo halves in rows 8..15, so that one product serves both. The rows' halves stay in
+// LDS; a workgroup splits them once and then walks its tiles; kw waves share a tile's contraction.
 constexpr int kGemvWaves = 8;
 constexpr int kGemvThreads = kGemvWaves * 64;
 constexpr int kDepth = 4;  // blocks of weights in flight per wave
 
-template <int G>
+template <int NG>
 struct Block {
-    static constexpr int NG = 128 / G;  // groups
     unsigned w[4];
-    unsigned s[(NG + 1) / 2];  // scales, two halves a word
-    unsigned z;                // zero points, a byte each
+    Scales<NG> f;
 };
 
-// w[j] of lane group g for w[j'] of g', bit b of j and bit b of g exchanged (b = 1: wave halves,
-// b = 0: neighbouring 16-lane rows).
-__device__ __forceinline__ void swap_halves(unsigned &a, unsigned &b) {
-    const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
-    a = r[0];
-    b = r[1];
-}
-__device__ __forceinline__ void swap_rows(unsigned &a, unsigned &b) {
-    const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
-    a = r[0];
-    b = r[1];
-}
-
-// VEC: a block's scales and zero points lie aligned in one load each (K % 128 == 0, aligned bases).
-template <int G, bool ZERO, bool VEC>
-__global__ __launch_bounds__(kGemvThreads, 4) void q4_gemv_kernel(const float *__restrict__ x, Segs segs, int m,
-                                                                  int K, int kw) {
-    using B = Block<G>;
-    constexpr int NG = B::NG;
+template <int G, bool ZERO>
+__global__ __launch_bounds__(kGemvThreads, 4) void q4_gemv_kernel(const float *__restrict__ x, Segs segs, int m, int K,
+                                                                  int kw) {
+    constexpr int NG = kBlock / G;
+    using B = Block<NG>;
     extern __shared__ f16x8 lds[];  // [blocks * 16 chunks][2 m]: chunk c of row i: hi, then lo
     __shared__ unsigned s_top[kGemvWaves][8];
+    __shared__ int s_exp[8];
     __shared__ float s_part[kGemvWaves][8][16];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 15, g = lane >> 4;
-    const int nb = (K + 127) / 128;  // blocks of a row
-    const int ngr = K / G;           // groups of a row
-    const int nw = K / 8;            // words of a row
+    const int nb = (K + kBlock - 1) / kBlock;
+    const int nw = K / 8;  // chunks of a row
 
-    // This wave's walk: tiles t0, t0 + units, ..., of each `per` blocks from b0 on. (Blocks past the
-    // row's last and tiles past the last are skipped, but walked: waves that share a tile meet at
-    // its end, in barriers of the workgroup.)
+    // This wave's walk: tiles t0, t0 + units, ..., of each `per` blocks from b0 on. Blocks past the
+    // row's last and tiles past the last are walked too, against zeros of x and without a store:
+    // the loop has no branch around a load, so that kDepth of them stay in flight, and the waves
+    // that share a tile meet at its end, in barriers of the workgroup.
     const int units = (int)gridDim.x * (kGemvWaves / kw);
     const int t0 = (int)blockIdx.x * (kGemvWaves / kw) + wave / kw;
     const int per = (nb + kw - 1) / kw;
     const int b0 = wave % kw * per;
     const int steps = (segs.total + units - 1) / units * per;
 
+    // The next block to load; buffer resources over its tile (over nothing past the last).
     B ring[kDepth];
-    int lt = t0, lb = 0;  // the next block to load
+    int lt = t0, lb = 0;
+    __amdgpu_buffer_rsrc_t wres, sres, zres;
+    auto enter = [&] {
+        const Seg sg = seg_at(segs, lt);
+        const size_t at = (size_t)(lt - sg.first) * nb;
+        const int have = lt < segs.total ? nb : 0;
+        wres = eb::make_rsrc(sg.w + at * kTileBytes, have * kTileBytes);
+        sres = eb::make_rsrc(sg.s + at * (kFeatures * NG), have * kFeatures * NG * 2);
+        if constexpr (ZERO) zres = eb::make_rsrc(sg.z + at * (kFeatures * NG), have * kFeatures * NG);
+    };
+    enter();
     auto load = [&](B &r) {
-        if (lt < segs.total && b0 + lb < nb) {
-            const Seg &sg = segs.seg[seg_of(segs, lt)];
-            const int o = min((lt - sg.first) * 16 + n, sg.n - 1);
-            const int b = b0 + lb;
-            // (words past the row's end repeat its last ones, against zeros of x)
-            const int at = VEC ? 16 * b + 4 * g : min(16 * b + 4 * g, nw - 4);
-            const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(sg.w + (size_t)o * nw + at));
+        const int b = __builtin_amdgcn_readfirstlane(b0 + lb);
+        const u32x4 v = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(wres, 16 * lane, kTileBytes * b, 0));
 #pragma unroll
-            for (int j = 0; j < 4; ++j) r.w[j] = v[j];
-            const size_t gr = (size_t)o * ngr + b * NG;
-            if constexpr (VEC && NG == 4) {
-                const u32x2 q = *reinterpret_cast<const u32x2 *>(sg.s + gr);
-                r.s[0] = q[0];
-                r.s[1] = q[1];
-                if constexpr (ZERO) r.z = *reinterpret_cast<const unsigned *>(sg.z + gr);
-            } else if constexpr (VEC && NG == 2) {
-                r.s[0] = *reinterpret_cast<const unsigned *>(sg.s + gr);
-                if constexpr (ZERO) r.z = *reinterpret_cast<const uint16_t *>(sg.z + gr);
-            } else {
-                unsigned z = 0;
-                unsigned sc[(NG + 1) / 2] = {};
-#pragma unroll
-                for (int i = 0; i < NG; ++i) {
-                    const size_t gi = (size_t)o * ngr + min(b * NG + i, ngr - 1);
-                    sc[i / 2] |= (unsigned)__builtin_bit_cast(uint16_t, sg.s[gi]) << (16 * (i % 2));
-                    if constexpr (ZERO) z |= (unsigned)sg.z[gi] << (8 * i);
-                }
-#pragma unroll
-                for (int i = 0; i < (NG + 1) / 2; ++i) r.s[i] = sc[i];
-                r.z = z;
-            }
+        for (int j = 0; j < 4; ++j) r.w[j] = v[j];
+        if constexpr (NG == 4) {
+            const u32x2 q = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(sres, 8 * n, 128 * b, 0));
+            r.f.s[0] = q[0];
+            r.f.s[1] = q[1];
+            if constexpr (ZERO) r.f.z = __builtin_amdgcn_raw_buffer_load_b32(zres, 4 * n, 64 * b, 0);
+        } else if constexpr (NG == 2) {
+            r.f.s[0] = __builtin_amdgcn_raw_buffer_load_b32(sres, 4 * n, 64 * b, 0);
+            if constexpr (ZERO) r.f.z = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(zres, 2 * n, 32 * b, 0);
+        } else {
+            r.f.s[0] = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(sres, 2 * n, 32 * b, 0);
+            if constexpr (ZERO) r.f.z = (unsigned char)__builtin_amdgcn_raw_buffer_load_b8(zres, n, 16 * b, 0);
         }
         if (++lb == per) {
             lb = 0;
             lt += units;
+            enter();
         }
     };
 #pragma unroll
@@ -220,18 +254,19 @@ __global__ __launch_bounds__(kGemvThreads, 4) void q4_gemv_kernel(const float *_
         if (lane == 0) s_top[wave][i] = top;
     }
     __syncthreads();
-    auto exponent = [&](int i) {
+    if (tid < m) {
         unsigned top = 0;
 #pragma unroll
-        for (int w = 0; w < kGemvWaves; ++w) top = s_top[w][i] > top ? s_top[w][i] : top;
-        return row_exponent(top);
-    };
+        for (int w = 0; w < kGemvWaves; ++w) top = s_top[w][tid] > top ? s_top[w][tid] : top;
+        s_exp[tid] = row_exponent(top);
+    }
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         if (i >= m) break;
         const f32x4 *p = reinterpret_cast<const f32x4 *>(x + (size_t)i * K);
-        const int e = exponent(i);
-        for (int c = tid; c < nb * 16; c += kGemvThreads) {
+        const int e = s_exp[i];
+        for (int c = tid; c < kw * per * 16; c += kGemvThreads) {
             f16x8 hi = {}, lo = {};
             if (c == tid)
                 split8(keep[i][0], keep[i][1], e, hi, lo);  // (zeros past the row's end)
@@ -244,10 +279,7 @@ __global__ __launch_bounds__(kGemvThreads, 4) void q4_gemv_kernel(const float *_
     __syncthreads();
 
     const int row = (n < 8 ? 0 : m) + min(n & 7, m - 1);  // (rows past m: the last, not stored)
-    // The chunk of lane group g in product j: word 4 g' + j', bits of g and j exchanged.
-    const int gw = G == 128 ? 4 * g : G == 64 ? 4 * (g & 1) + (g & 2) : g;
-    auto word = [](int j) { return G == 128 ? j : G == 64 ? 4 * (j & 2) + (j & 1) : 4 * j; };
-    const f16x8 *xa = lds + gw * 2 * m + row;
+    const f16x8 *xa = lds + g * 2 * m + row;               // word j of lane group g is chunk 4 j + g
     f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
     int ct = t0, cb = 0;
     auto finish = [&] {
@@ -255,58 +287,47 @@ __global__ __launch_bounds__(kGemvThreads, 4) void q4_gemv_kernel(const float *_
         float v[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[r] = acc[r] + eb::lane_xor32(acc[r]);
+        const Seg sg = seg_at(segs, ct);
+        const int o = (ct - sg.first) * kFeatures + n;
+        const bool store = ct < segs.total && o < sg.n;
         if (kw == 1) {
-            if (ct < segs.total) {
-                const Seg &sg = segs.seg[seg_of(segs, ct)];
-                const int o = (ct - sg.first) * 16 + n;
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (g < 2 && o < sg.n && 4 * g + r < m)
-                        sg.y[(size_t)(4 * g + r) * sg.n + o] = ldexpf(v[r], exponent(4 * g + r));
-            }
+            for (int r = 0; r < 4; ++r)
+                if (store && g < 2 && 4 * g + r < m)
+                    sg.y[(size_t)(4 * g + r) * sg.n + o] = ldexpf(v[r], s_exp[4 * g + r]);
         } else {
             if (g < 2)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) s_part[wave][4 * g + r][n] = v[r];
             __syncthreads();
-            // The first wave of each tile's waves adds their sums: lane (n, g) rows g and g + 4.
-            if (wave % kw == 0 && ct < segs.total) {
-                const Seg &sg = segs.seg[seg_of(segs, ct)];
-                const int o = (ct - sg.first) * 16 + n;
-#pragma unroll
-                for (int i = g; i < 8; i += 4)
-                    if (i < m && o < sg.n) {
-                        float t = 0.0f;
-                        for (int w = 0; w < kw; ++w) t += s_part[wave + w][i][n];
-                        sg.y[(size_t)i * sg.n + o] = ldexpf(t, exponent(i));
-                    }
-            }
+            // The first of a tile's waves adds their sums: lane (n, g) rows g and g + 4.
+            if (wave % kw == 0 && store)
+                for (int i = g; i < m; i += 4) {
+                    float t = 0.0f;
+                    for (int w = 0; w < kw; ++w) t += s_part[wave + w][i][n];
+                    sg.y[(size_t)i * sg.n + o] = ldexpf(t, s_exp[i]);
+                }
             __syncthreads();
         }
         acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         ct += units;
     };
-    auto consume = [&](B &r) {
-        if (ct < segs.total && b0 + cb < nb) {
-            const f16x8 *xb = xa + (size_t)(b0 + cb) * 16 * 2 * m;
-            if constexpr (G <= 64) {
-                swap_halves(r.w[0], r.w[2]);
-                swap_halves(r.w[1], r.w[3]);
-            }
-            if constexpr (G == 32) {
-                swap_rows(r.w[0], r.w[1]);
-                swap_rows(r.w[2], r.w[3]);
-            }
+    auto consume = [&](const B &r) {
+        const f16x8 *xb = xa + (size_t)(b0 + cb) * 16 * 2 * m;
+        f16x8 xv[4];
 #pragma unroll
-            for (int i = 0; i < NG; ++i) {
-                const Zero z = zero_of(ZERO ? r.z : 0x08080808u, i);
-                f32x4 t = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int j = 0; j < 4; ++j) xv[j] = xb[4 * j * 2 * m];
+        f32x4 t[NG];
 #pragma unroll
-                for (int j = i * (4 / NG); j < (i + 1) * (4 / NG); ++j)
-                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(xb[word(j) * 2 * m], unpack(r.w[j], z), t, 0, 0, 0);
-                acc += t * (float)__builtin_bit_cast(_Float16, (unsigned short)(r.s[i / 2] >> (16 * (i % 2))));
-            }
+        for (int i = 0; i < NG; ++i) {
+            const Zero z = zero_of(ZERO ? r.f.z : 0x08080808u, i);
+            t[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int j = i * (4 / NG); j < (i + 1) * (4 / NG); ++j)
+                t[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xv[j], unpack(r.w[j], z), t[i], 0, 0, 0);
         }
+#pragma unroll
+        for (int i = 0; i < NG; ++i) acc += t[i] * r.f.scale(i);
         if (++cb == per) {
             cb = 0;
             finish();
@@ -314,11 +335,11 @@ __global__ __launch_bounds__(kGemvThreads, 4) void q4_gemv_kernel(const float *_
     };
     for (int s = 0; s < steps; s += kDepth) {
 #pragma unroll
-        for (int i = 0; i < kDepth; ++i)
-            if (s + i < steps) {  // (the same in every wave)
-                consume(ring[i]);
-                load(ring[i]);
-            }
+        for (int i = 0; i < kDepth; ++i) {
+            if (s + i >= steps) break;  // (the same in every wave)
+            consume(ring[i]);
+            load(ring[i]);
+        }
     }
 }
 
@@ -376,150 +397,281 @@ __global__ __launch_bounds__(kSplitThreads) void q4_split_kernel(const float *__
     for (int c = l + kSplitKept * L; c < KC; c += L) put(c, c < have ? p[2 * c] : z4, c < have ? p[2 * c + 1] : z4);
 }
 
-// Workgroup tile: 32 MB WM rows x 32 NB WN features, WM x WN waves of MB x NB blocks of 32 x 32
-// (v_mfma_f32_32x32x16_f16: A = x rows, lane (r, h): row r, chunk 2 step + h; B = codes, lane
-// (n, h): feature n). In a unit of U = min(G, 64) of the contraction, lane half h takes the U / 2
-// values h * U / 2 .. as U / 16 words, step j word j.
-template <int G, bool ZERO, int MB, int NB, int WM, int WN>
-__global__ __launch_bounds__(kThreads, 1) void q4_gemm_kernel(const f16x8 *__restrict__ hi,
-                                                              const f16x8 *__restrict__ lo,
-                                                              const float *__restrict__ ex, Segs segs, int M, int K,
-                                                              int KC) {
-    constexpr int U = G < 64 ? G : 64, W = U / 16;  // a unit, and its words (and steps) per lane
-    constexpr int S = 64 / U;                       // units per 64-deep stage
-    constexpr int BM = 32 * MB * WM;
-    constexpr int CH = 8 * BM;                      // chunks of a stage's plane
-    constexpr int NLD = 2 * CH / kThreads;
-    __shared__ f16x8 lds[2][2 * CH];                // hi then lo: [block][chunk][row]
+// B of v_mfma_f32_32x32x16_f16 for 32 features (two tiles): lane (n, h) is lane n + 32 h, feature n.
+// In a block, lane half h reads the 16 bytes of slots g = h and g = 2 + h of its feature: word j of
+// slot g is chunk 4 j + g, so product (q, j) takes chunk 4 j + 2 q + h of x, and lies in group j of
+// 128 / G.
+template <int NG>
+struct Wide {
+    unsigned w[2][4];  // slot 2 q + h, word j
+    Scales<NG> f;
+};
+template <int NG, bool ZERO>
+__device__ __forceinline__ void load_wide(Wide<NG> &r, const Seg &sg, int tile, int b, int nb, int n, int h) {
+    const size_t at = (size_t)tile * nb + b;
+    const u32x4 *p = reinterpret_cast<const u32x4 *>(sg.w + at * kTileBytes) + (n & 15) + 16 * h;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const u32x4 v = p[32 * q];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r.w[q][j] = v[j];
+    }
+    const size_t f = at * kFeatures + (n & 15);
+    if constexpr (NG == 4) {
+        const u32x2 q = *reinterpret_cast<const u32x2 *>(sg.s + f * 4);
+        r.f.s[0] = q[0];
+        r.f.s[1] = q[1];
+        if constexpr (ZERO) r.f.z = *reinterpret_cast<const unsigned *>(sg.z + f * 4);
+    } else if constexpr (NG == 2) {
+        r.f.s[0] = *reinterpret_cast<const unsigned *>(sg.s + f * 2);
+        if constexpr (ZERO) r.f.z = *reinterpret_cast<const uint16_t *>(sg.z + f * 2);
+    } else {
+        r.f.s[0] = *reinterpret_cast<const uint16_t *>(sg.s + f);
+        if constexpr (ZERO) r.f.z = sg.z[f];
+    }
+}
+
+// Four KiB from src (this lane's 16 bytes of the first) to LDS byte address dst, which m0 holds for
+// all of them. A wait state follows the write of m0 (inside an asm block the compiler adds none).
+__device__ __forceinline__ void copy_4kib(unsigned dst, const void *src) {
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\t"
+        "global_load_lds_dwordx4 %1, off offset:1024\n\tglobal_load_lds_dwordx4 %1, off offset:2048\n\t"
+        "global_load_lds_dwordx4 %1, off offset:3072"
+        :
+        : "s"(dst), "v"(src)
+        : "memory", "m0");
+}
+
+// Workgroup tile: 128 rows x 128 features, two sets of 2 x 2 waves (64 x 64 each); a stage is a
+// block of 128, whose slots 2 q + h of q = 0 are the first set's and of q = 1 the second's: two
+// waves on every SIMD, each with whole tiles of registers, where a launch has about one workgroup
+// per CU. The sets' sums meet in LDS at the end. x's halves are copied memory-to-LDS a stage ahead
+// (64 KiB; a wave copies one plane of one 32-row block), and the weights loaded a stage ahead. All
+// of a stage's loads are waited for at its start; the empty asm on the weights there keeps the
+// compiler from waiting for them, and with them for the next stage's copies, at their first use.
+constexpr int kTileRows = 128, kTileCols = 128;
+constexpr int kTileThreads = 512;
+template <int G, bool ZERO>
+__global__ __launch_bounds__(kTileThreads, 2) void q4_tile_kernel(const f16x8 *__restrict__ hi, const f16x8 *__restrict__ lo,
+                                                                  const float *__restrict__ ex, Segs segs, int M, int K,
+                                                                  int KC) {
+    constexpr int NG = kBlock / G;
+    constexpr int CH = 16 * kTileRows;  // chunks of a stage's plane: [row block][chunk][row]
+    extern __shared__ f16x8 lds[];      // [2][hi CH, lo CH]
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wm = wave / WN, wn = wave % WN;
+    const int q = wave >> 2, wm = (wave >> 1) & 1, wn = wave & 1;
     const int n = lane & 31, h = lane >> 5;
     const int mt = blockIdx.x / segs.total, u = blockIdx.x % segs.total;
-    const Seg &sg = segs.seg[seg_of(segs, u)];
-    const int m0 = mt * BM, n0 = (u - sg.first) * 32 * NB * WN + wn * 32 * NB;
-    const int ngr = K / G, nw = K / 8;
-    const int stages = (K + 63) / 64;
+    const Seg sg = seg_at(segs, u);
+    const int m0 = mt * kTileRows, n0 = (u - sg.first) * kTileCols + wn * 64;
+    const int nb = (K + kBlock - 1) / kBlock;
+    const int last = (sg.n + kFeatures - 1) / kFeatures - 1;
 
-    f16x8 rx[NLD];
-    auto load_x = [&](int st) {
+    // This wave's copies: plane wave / 4, row block wave % 4, 8 KiB a stage.
+    const f16x8 *src = (wave < 4 ? hi : lo) + (size_t)(m0 / 32 + wave % 4) * KC * 32 + lane;
+    const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
+    const unsigned dst0 = __builtin_amdgcn_readfirstlane(lds0 + ((wave / 4) * CH + (wave % 4) * 512) * 16);
+    auto copy_stage = [&](int st) {
+        const unsigned dst = dst0 + (st & 1) * 2 * CH * 16;
+        copy_4kib(dst, src + (size_t)st * 512);
+        copy_4kib(dst + 4096, src + (size_t)st * 512 + 256);
+    };
+    // This set's half of a block: slot 2 q + h of both blocks of 32 features.
+    struct Half {
+        unsigned w[4];
+        Scales<NG> f;
+    };
+    size_t tile_at[2];
 #pragma unroll
-        for (int i = 0; i < NLD; ++i) {
-            const int c = tid + i * kThreads;
-            const int at = c % CH;
-            const f16x8 *p = c < CH ? hi : lo;
-            rx[i] = p[((size_t)(m0 / 32 + at / 256) * KC + st * 8) * 32 + at % 256];
+    for (int b = 0; b < 2; ++b) tile_at[b] = (size_t)min((n0 + 32 * b + n) / kFeatures, last) * nb;
+    auto load_w = [&](int st, Half (&r)[2]) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            const size_t at = tile_at[b] + st;
+            const u32x4 v = reinterpret_cast<const u32x4 *>(sg.w + at * kTileBytes)[(n & 15) + 16 * (2 * q + h)];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r[b].w[j] = v[j];
+            const size_t f = at * kFeatures + (n & 15);
+            r[b].f.z = 0x08080808u;
+            if constexpr (NG == 4) {
+                const u32x2 s = *reinterpret_cast<const u32x2 *>(sg.s + f * 4);
+                r[b].f.s[0] = s[0];
+                r[b].f.s[1] = s[1];
+                if constexpr (ZERO) r[b].f.z = *reinterpret_cast<const unsigned *>(sg.z + f * 4);
+            } else if constexpr (NG == 2) {
+                r[b].f.s[0] = *reinterpret_cast<const unsigned *>(sg.s + f * 2);
+                if constexpr (ZERO) r[b].f.z = *reinterpret_cast<const uint16_t *>(sg.z + f * 2);
+            } else {
+                r[b].f.s[0] = *reinterpret_cast<const uint16_t *>(sg.s + f);
+                if constexpr (ZERO) r[b].f.z = sg.z[f];
+            }
         }
     };
-    auto store_x = [&](int buf) {
+    auto arrived = [&](Half (&r)[2]) {
 #pragma unroll
-        for (int i = 0; i < NLD; ++i) lds[buf][tid + i * kThreads] = rx[i];
+        for (int b = 0; b < 2; ++b) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) asm volatile("" : "+v"(r[b].w[j]));
+#pragma unroll
+            for (int i = 0; i < (NG + 1) / 2; ++i) asm volatile("" : "+v"(r[b].f.s[i]));
+            if constexpr (ZERO) asm volatile("" : "+v"(r[b].f.z));
+        }
     };
-    unsigned rw[2][NB][S][W];
-    auto load_w = [&](int st, unsigned (&r)[NB][S][W]) {
+    floatx16 acc[2][2] = {};
+    auto compute = [&](int buf, const Half (&r)[2]) {
+        const f16x8 *xb = lds + buf * 2 * CH + (wm * 2 * 16 + 2 * q + h) * 32 + n;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const int o = min(n0 + 32 * b + n, sg.n - 1);
+        for (int i = 0; i < NG; ++i) {
+            floatx16 t[2][2];
+            f16x8 w[2];
 #pragma unroll
-            for (int s = 0; s < S; ++s) {
-                const int k = min(st * 64 + s * U, K - U);  // (past K: against zeros of x)
-                const uint32_t *p = sg.w + (size_t)o * nw + k / 8 + h * W;
-                if constexpr (W == 4) {
-                    const u32x4 v = *reinterpret_cast<const u32x4 *>(p);
+            for (int j = i * (4 / NG); j < (i + 1) * (4 / NG); ++j) {
+                f16x8 ah[2], al[2];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) r[b][s][j] = v[j];
-                } else {
-                    const u32x2 v = *reinterpret_cast<const u32x2 *>(p);
-                    r[b][s][0] = v[0];
-                    r[b][s][1] = v[1];
+                for (int a = 0; a < 2; ++a) {
+                    ah[a] = xb[(a * 16 + 4 * j) * 32];
+                    al[a] = xb[CH + (a * 16 + 4 * j) * 32];
                 }
+#pragma unroll
+                for (int b = 0; b < 2; ++b) w[b] = unpack(r[b].w[j], zero_of(ZERO ? r[b].f.z : 0x08080808u, i));
+#pragma unroll
+                for (int a = 0; a < 2; ++a)
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+                        t[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                            ah[a], w[b], j == i * (4 / NG) ? floatx16{} : t[a][b], 0, 0, 0);
+#pragma unroll
+                for (int a = 0; a < 2; ++a)
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+                        t[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[a], w[b], t[a][b], 0, 0, 0);
             }
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+#pragma unroll
+                for (int b = 0; b < 2; ++b) acc[a][b] += t[a][b] * r[b].f.scale(i);
+            // (one group's sums at a time: two groups' do not fit the registers)
+            if constexpr (NG > 1) __builtin_amdgcn_sched_barrier(0);
         }
     };
-    floatx16 acc[MB][NB] = {}, t[MB][NB] = {};
-    auto compute = [&](int st, int buf, const unsigned (&r)[NB][S][W]) {
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
-            const int gr = min((st * 64 + s * U) / G, ngr - 1);
-            Zero z[NB];
-            float sc[NB];
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                const int o = min(n0 + 32 * b + n, sg.n - 1);
-                z[b] = zero_of(ZERO ? sg.z[(size_t)o * ngr + gr] : 8u, 0);
-                sc[b] = (float)sg.s[(size_t)o * ngr + gr];
-            }
-#pragma unroll
-            for (int j = 0; j < W; ++j) {
-                f16x8 ah[MB], al[MB];
-#pragma unroll
-                for (int a = 0; a < MB; ++a) {
-                    const int at = ((wm * MB + a) * 8 + s * (U / 8) + h * W + j) * 32 + n;
-                    ah[a] = lds[buf][at];
-                    al[a] = lds[buf][CH + at];
-                }
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    const f16x8 w = unpack(r[b][s][j], z[b]);
-#pragma unroll
-                    for (int a = 0; a < MB; ++a) {
-                        t[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[a], w, t[a][b], 0, 0, 0);
-                        t[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[a], w, t[a][b], 0, 0, 0);
-                    }
-                }
-            }
-            // The group's sum is complete (group 128: after its second stage).
-            if (G <= 64 || (st & 1) || st + 1 == stages) {
-#pragma unroll
-                for (int a = 0; a < MB; ++a)
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        acc[a][b] += t[a][b] * sc[b];
-                        t[a][b] = floatx16{};
-                    }
-            }
+    Half wa[2], wb[2];
+    copy_stage(0);
+    load_w(0, wa);
+    auto stage = [&](int st, Half (&now)[2], Half (&next)[2]) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        arrived(now);
+        __syncthreads();  // stage st is there, and nobody reads the other buffer any more
+        if (st + 1 < nb) {
+            copy_stage(st + 1);
+            load_w(st + 1, next);
         }
+        __builtin_amdgcn_sched_barrier(0);
+        compute(st & 1, now);
     };
-    load_x(0);
-    load_w(0, rw[0]);
-    store_x(0);
-    __syncthreads();
-    for (int st = 0; st < stages; ++st) {
-        if (st + 1 < stages) {
-            load_x(st + 1);
-            load_w(st + 1, rw[1]);
-        }
-        compute(st, st & 1, rw[0]);
-        if (st + 1 < stages) {
-            store_x((st & 1) ^ 1);
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int s = 0; s < S; ++s)
-#pragma unroll
-                    for (int j = 0; j < W; ++j) rw[0][b][s][j] = rw[1][b][s][j];
-        }
-        __syncthreads();
+    for (int st = 0; st < nb; st += 2) {
+        stage(st, wa, wb);
+        if (st + 1 < nb) stage(st + 1, wb, wa);
     }
+    // The second set's sums through LDS.
+    float *part = reinterpret_cast<float *>(lds);
+    __syncthreads();
+    if (q == 1)
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) part[(((wave & 3) * 4 + a * 2 + b) * 16 + r) * 64 + lane] = acc[a][b][r];
+    __syncthreads();
+    if (q == 1) return;
     // Lane (n, h) holds feature n, rows 8 (r / 4) + 4 h + r % 4 of each block.
 #pragma unroll
-    for (int a = 0; a < MB; ++a)
+    for (int a = 0; a < 2; ++a)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            const int row = m0 + (wm * MB + a) * 32 + 8 * (r >> 2) + 4 * h + (r & 3);
+            const int row = m0 + (wm * 2 + a) * 32 + 8 * (r >> 2) + 4 * h + (r & 3);
             if (row >= M) continue;
             const int e = (int)ex[row];
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
+            for (int b = 0; b < 2; ++b) {
                 const int o = n0 + 32 * b + n;
-                if (o < sg.n) sg.y[(size_t)row * sg.n + o] = ldexpf(acc[a][b][r], e);
+                const float v = acc[a][b][r] + part[((wave * 4 + a * 2 + b) * 16 + r) * 64 + lane];
+                if (o < sg.n) sg.y[(size_t)row * sg.n + o] = ldexpf(v, e);
             }
         }
 }
 
+// Fewer rows than fill the card with such tiles: 32 MB rows x 32 features a workgroup, its eight
+// waves sharing the contraction (wave w blocks w, w + 8, ...); x's halves come from L2 straight into
+// the products' registers, and the waves' sums meet in LDS.
+constexpr int kSlimWaves = 8;
+template <int G, bool ZERO, int MB>
+__global__ __launch_bounds__(kSlimWaves * 64, 2) void q4_slim_kernel(const f16x8 *__restrict__ hi,
+                                                                     const f16x8 *__restrict__ lo,
+                                                                     const float *__restrict__ ex, Segs segs, int M, int K,
+                                                                     int KC) {
+    constexpr int NG = kBlock / G;
+    __shared__ float part[kSlimWaves][MB * 16][64];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 31, h = lane >> 5;
+    const int mt = blockIdx.x / segs.total, u = blockIdx.x % segs.total;
+    const Seg sg = seg_at(segs, u);
+    const int m0 = mt * 32 * MB, n0 = (u - sg.first) * 32;
+    const int nb = (K + kBlock - 1) / kBlock;
+    const int last = (sg.n + kFeatures - 1) / kFeatures - 1;
+    const int tile = min((n0 + n) / kFeatures, last);
+    floatx16 acc[MB] = {};
+    Wide<NG> r;
+    if (wave < nb) load_wide<NG, ZERO>(r, sg, tile, wave, nb, n, h);
+    for (int b = wave; b < nb; b += kSlimWaves) {
+        Wide<NG> next = r;
+        if (b + kSlimWaves < nb) load_wide<NG, ZERO>(next, sg, tile, b + kSlimWaves, nb, n, h);
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            const Zero z = zero_of(ZERO ? r.f.z : 0x08080808u, i);
+            floatx16 t[MB] = {};
+#pragma unroll
+            for (int j = i * (4 / NG); j < (i + 1) * (4 / NG); ++j)
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const f16x8 w = unpack(r.w[q][j], z);
+#pragma unroll
+                    for (int a = 0; a < MB; ++a) {
+                        const size_t at = ((size_t)(m0 / 32 + a) * KC + b * 16 + 4 * j + 2 * q + h) * 32 + n;
+                        t[a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi[at], w, t[a], 0, 0, 0);
+                        t[a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lo[at], w, t[a], 0, 0, 0);
+                    }
+                }
+#pragma unroll
+            for (int a = 0; a < MB; ++a) acc[a] += t[a] * r.f.scale(i);
+        }
+        r = next;
+    }
+#pragma unroll
+    for (int a = 0; a < MB; ++a)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) part[wave][a * 16 + i][lane] = acc[a][i];
+    __syncthreads();
+    // Lane (n, h): feature n, rows 8 (i / 4) + 4 h + i % 4 of block a; wave w takes i = w, w + 8, ...
+#pragma unroll
+    for (int v = wave; v < MB * 16; v += kSlimWaves) {
+        const int i = v % 16, row = m0 + v / 16 * 32 + 8 * (i >> 2) + 4 * h + (i & 3), o = n0 + n;
+        float t = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kSlimWaves; ++w) t += part[w][v][lane];
+        if (row < M && o < sg.n) sg.y[(size_t)row * sg.n + o] = ldexpf(t, (int)ex[row]);
+    }
+}
+
 constexpr size_t kGemvLds = 144 * 1024;  // of the 160 KB, beside the kernel's own arrays
 constexpr size_t kGemvRows = 8;
-size_t gemv_lds(size_t m, size_t K) { return (K + 127) / 128 * 16 * 2 * m * 16; }
+// (the blocks rounded up to what kGemvWaves waves share)
+size_t gemv_lds(size_t m, size_t K) {
+    return ((K + kBlock - 1) / kBlock + kGemvWaves - 1) / kGemvWaves * kGemvWaves * 16 * 2 * m * 16;
+}
 bool gemv(size_t m, size_t K) { return m <= kGemvRows && gemv_lds(m, K) <= kGemvLds; }
 
 size_t round_up(size_t x, size_t to) { return (x + to - 1) / to * to; }
@@ -534,42 +686,41 @@ int number(Segs &s, int per) {
     return s.total = t;
 }
 
-// Waves that share a tile: the fewest that give every wave slot (two workgroups on a CU) a tile.
-template <int G, bool ZERO, bool VEC>
-hipError_t launch_gemv(hipStream_t st, const float *x, const Segs &s, int m, int K) {
-    static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&q4_gemv_kernel<G, ZERO, VEC>),
-                                                    hipFuncAttributeMaxDynamicSharedMemorySize, (int)kGemvLds);
-    if (e != hipSuccess) return e;
-    const int slots = 2 * eb::current_cu_count();
-    int kw = 1;
-    while (kw < kGemvWaves && s.total * kw < slots * kGemvWaves) kw *= 2;
-    const int tiles = kGemvWaves / kw;  // a workgroup's at a time
-    const int grid = std::min((s.total + tiles - 1) / tiles, slots);
-    q4_gemv_kernel<G, ZERO, VEC><<<grid, kGemvThreads, gemv_lds(m, K), st>>>(x, s, m, K, kw);
-    return hipSuccess;
-}
-
 template <int G, bool ZERO>
 hipError_t launch(hipStream_t st, const float *x, Segs s, int m, int K, float *ws) {
+    const int cus = eb::current_cu_count();
     if (gemv(m, K)) {
-        number(s, 16);
-        bool vec = K % 128 == 0;
-        for (int i = 0; i < s.nseg; ++i)
-            vec = vec && ((reinterpret_cast<uintptr_t>(s.seg[i].s) | 2 * reinterpret_cast<uintptr_t>(s.seg[i].z)) & 7) == 0;
-        return vec ? launch_gemv<G, ZERO, true>(st, x, s, m, K) : launch_gemv<G, ZERO, false>(st, x, s, m, K);
+        static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&q4_gemv_kernel<G, ZERO>),
+                                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)kGemvLds);
+        if (e != hipSuccess) return e;
+        // Waves that share a tile: the fewest that give every wave slot (two workgroups on a CU) one.
+        number(s, kFeatures);
+        const int slots = 2 * cus;
+        int kw = 1;
+        while (kw < kGemvWaves && s.total * kw < slots * kGemvWaves) kw *= 2;
+        const int tiles = kGemvWaves / kw;  // a workgroup's at a time
+        const int grid = std::min((s.total + tiles - 1) / tiles, slots);
+        q4_gemv_kernel<G, ZERO><<<grid, kGemvThreads, gemv_lds(m, K), st>>>(x, s, m, K, kw);
+        return hipSuccess;
     }
-    const size_t mp = round_up(m, kRowPad), kp = round_up(K, 64);
+    const size_t mp = round_up(m, kRowPad), kp = round_up(K, kBlock);
     f16x8 *hi = reinterpret_cast<f16x8 *>(ws + mp), *lo = hi + mp * kp / 8;
-    q4_split_kernel<<<(unsigned)(mp / 8), kSplitThreads, 0, st>>>(x, ws, hi, lo, m, K, (int)(kp / 8));
-    if (m <= 64) {
-        number(s, 128);
-        q4_gemm_kernel<G, ZERO, 1, 1, 1, 4>
-            <<<(unsigned)((m + 31) / 32 * s.total), kThreads, 0, st>>>(hi, lo, ws, s, m, K, (int)(kp / 8));
-    } else {
-        number(s, 128);
-        q4_gemm_kernel<G, ZERO, 2, 2, 2, 2>
-            <<<(unsigned)((m + 127) / 128 * s.total), kThreads, 0, st>>>(hi, lo, ws, s, m, K, (int)(kp / 8));
+    const int KC = (int)(kp / 8);
+    q4_split_kernel<<<(unsigned)(mp / 8), kSplitThreads, 0, st>>>(x, ws, hi, lo, m, K, KC);
+    const int tiles = (m + kTileRows - 1) / kTileRows * number(s, kTileCols);
+    if (tiles >= cus / 2) {
+        constexpr size_t lds = 2 * 2 * 16 * kTileRows * 16;
+        static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&q4_tile_kernel<G, ZERO>),
+                                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return e;
+        q4_tile_kernel<G, ZERO><<<(unsigned)tiles, kTileThreads, lds, st>>>(hi, lo, ws, s, m, K, KC);
+        return hipSuccess;
     }
+    number(s, 32);
+    if (m <= 32)
+        q4_slim_kernel<G, ZERO, 1><<<(unsigned)s.total, kSlimWaves * 64, 0, st>>>(hi, lo, ws, s, m, K, KC);
+    else
+        q4_slim_kernel<G, ZERO, 2><<<(unsigned)((m + 63) / 64 * s.total), kSlimWaves * 64, 0, st>>>(hi, lo, ws, s, m, K, KC);
     return hipSuccess;
 }
 
@@ -579,19 +730,39 @@ namespace eb {
 
 size_t linear_q4_workspace_floats(size_t m, size_t in_f) {
     if (m == 0 || in_f == 0 || gemv(m, in_f)) return 0;
-    return round_up(m, kRowPad) * (1 + round_up(in_f, 64));
+    return round_up(m, kRowPad) * (1 + round_up(in_f, kBlock));
+}
+
+// Planes: codes | scales | zero points; each a whole number of 16 bytes.
+size_t q4_packed_bytes(size_t in_f, size_t out_f, size_t group, bool zeros) {
+    const size_t blocks = (out_f + kFeatures - 1) / kFeatures * ((in_f + kBlock - 1) / kBlock);
+    return blocks * (kTileBytes + kFeatures * (kBlock / group) * (zeros ? 3 : 2));
+}
+
+eb_status launch_q4_pack(hipStream_t st, const uint32_t *w, const uint16_t *scales, const uint8_t *zeros, uint8_t *packed,
+                         size_t in_f, size_t out_f, size_t group) {
+    const size_t nb = (in_f + kBlock - 1) / kBlock, blocks = (out_f + kFeatures - 1) / kFeatures * nb;
+    if (blocks == 0) return EB_OK;
+    uint8_t *ps = packed + blocks * kTileBytes, *pz = ps + blocks * kFeatures * (kBlock / group) * 2;
+    q4_pack_kernel<<<(unsigned)blocks, kPackThreads, 0, st>>>(w, scales, zeros, reinterpret_cast<uint32_t *>(packed),
+                                                              reinterpret_cast<uint16_t *>(ps), zeros ? pz : nullptr,
+                                                              (int)out_f, (int)in_f, (int)group, (int)nb);
+    return check_launch("q4_pack");
 }
 
 eb_status launch_linear_q4(hipStream_t st, const float *x, const Q4Weight *w, float *const *y, int nseg, size_t m,
                            float *ws) {
     Segs s{};
-    for (int i = 0; i < nseg; ++i)
-        if (w[i].out_f > 0)
-            s.seg[s.nseg++] = Seg{w[i].w, reinterpret_cast<const _Float16 *>(w[i].scales), w[i].zeros, y[i],
-                                  (int)w[i].out_f, 0};
+    for (int i = 0; i < nseg; ++i) {
+        if (w[i].out_f == 0) continue;
+        const size_t blocks = (w[i].out_f + kFeatures - 1) / kFeatures * ((w[i].in_f + kBlock - 1) / kBlock);
+        const uint8_t *ps = w[i].packed + blocks * kTileBytes;
+        s.seg[s.nseg++] = Seg{w[i].packed, reinterpret_cast<const _Float16 *>(ps),
+                              ps + blocks * kFeatures * (kBlock / w[i].group) * 2, y[i], (int)w[i].out_f, 0};
+    }
     if (s.nseg == 0) return EB_OK;
     const int K = (int)w[0].in_f, M = (int)m;
-    const bool zero = w[0].zeros != nullptr;
+    const bool zero = w[0].zeros;
     hipError_t e = hipSuccess;
     switch (w[0].group) {
         case 32: e = zero ? launch<32, true>(st, x, s, M, K, ws) : launch<32, false>(st, x, s, M, K, ws); break;

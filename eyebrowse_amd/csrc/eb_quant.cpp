@@ -4,6 +4,7 @@
 // eb_sample.hip).
 #include <algorithm>
 #include <climits>
+#include <cstdint>
 #include <memory>
 #include <mutex>
 
@@ -406,34 +407,87 @@ eb_status eb_launch_attn_prefill_chunk_i8(void *stream, const float *q, size_t q
 
 // ---- 4-bit projections ------------------------------------------------------------------------
 
-static eb_status q4_checked(hipStream_t st, const Room &src, const float *a, size_t an, const eb::Q4Weight *w,
-                            const size_t *words, const size_t *scales, const size_t *zeros, float *const *c,
-                            const size_t *cn, int n, size_t m) {
-    const size_t in_f = w[0].in_f, group = w[0].group;
+// A weight's shape; its sizes are indexed with 32 bits.
+static eb_status q4_shape(size_t in_f, size_t out_f, size_t group) {
     if (group != 32 && group != 64 && group != 128)
-        return fail(EB_UNSUPPORTED_CONFIG, "linear_q4: group %zu (32, 64 or 128)", group);
+        return fail(EB_UNSUPPORTED_CONFIG, "4-bit weight: group %zu (32, 64 or 128)", group);
     if (in_f == 0 || in_f % group != 0)
-        return fail(EB_SHAPE_MISMATCH, "linear_q4: in_f %zu is not a positive multiple of the group %zu", in_f, group);
-    EB_TRY(eb::check_numel(an, {m, in_f}, "a"));
+        return fail(EB_SHAPE_MISMATCH, "4-bit weight: in_f %zu is not a positive multiple of the group %zu", in_f, group);
+    if (in_f > ((size_t)1 << 24)) return fail(EB_UNSUPPORTED_CONFIG, "4-bit weight: in_f %zu (at most 2^24)", in_f);
+    return eb::check_numel(SIZE_MAX, {out_f + 15, in_f / 8}, "4-bit weight");
+}
+
+size_t eb_q4_packed_bytes(size_t in_f, size_t out_f, size_t group, int zeros) {
+    return q4_shape(in_f, out_f, group) == EB_OK ? eb::q4_packed_bytes(in_f, out_f, group, zeros != 0) : 0;
+}
+
+static eb_status pack_checked(hipStream_t st, const uint32_t *w, size_t words, const uint16_t *scales, size_t sn,
+                              const uint8_t *zeros, size_t zn, size_t in_f, size_t out_f, size_t group, void *packed,
+                              size_t bytes) {
+    EB_TRY(q4_shape(in_f, out_f, group));
+    EB_TRY(eb::check_numel(words, {out_f, in_f / 8}, "w"));
+    EB_TRY(eb::check_numel(sn, {out_f, in_f / group}, "scales"));
+    if (zeros) EB_TRY(eb::check_numel(zn, {out_f, in_f / group}, "zeros"));
+    EB_TRY(holds(bytes, eb::q4_packed_bytes(in_f, out_f, group, zeros != nullptr), "packed"));
+    if (out_f == 0) return eb::ok();
+    EB_TRY(eb::check_ptr(w, "w"));
+    EB_TRY(eb::check_ptr(scales, "scales"));
+    EB_TRY(eb::check_ptr(packed, "packed"));
+    EB_TRY(aligned({w}, 4, "q4_pack: w"));
+    EB_TRY(aligned({scales}, 2, "q4_pack: scales"));
+    EB_TRY(aligned({packed}, 16, "q4_pack: packed"));
+    EB_TRY(eb::launch_q4_pack(st, w, scales, zeros, static_cast<uint8_t *>(packed), in_f, out_f, group));
+    return eb::ok();
+}
+
+eb_status eb_q4_pack(eb_recorder *rec, const eb_tensor *w, const eb_tensor *scales, const eb_tensor *zeros, size_t in_f,
+                     size_t out_f, size_t group, eb_tensor **packed) {
+    if (!packed) return fail(EB_OTHER, "q4_pack: out is null");
+    *packed = nullptr;
+    eb_device *dev;
+    EB_TRY(eb::recorder_ready(rec, &dev));
+    EB_TRY(eb::check_tensor(w, EB_U32, "w", dev));
+    EB_TRY(eb::check_tensor(scales, EB_F16, "scales", dev));
+    if (zeros) EB_TRY(eb::check_tensor(zeros, EB_U8, "zeros", dev));
+    EB_TRY(q4_shape(in_f, out_f, group));
+    const size_t bytes = eb::q4_packed_bytes(in_f, out_f, group, zeros != nullptr);
+    eb_tensor *t = nullptr;
+    EB_TRY(eb_tensor_empty(dev, &bytes, 1, EB_U8, &t));
+    Owned p(t);
+    EB_TRY(pack_checked(stream_of(dev), data<uint32_t>(w), eb_tensor_numel(w), data<uint16_t>(scales),
+                        eb_tensor_numel(scales), zeros ? data<uint8_t>(zeros) : nullptr, zeros ? eb_tensor_numel(zeros) : 0,
+                        in_f, out_f, group, data<void>(p.t), bytes));
+    *packed = p.release();
+    return eb::ok();
+}
+
+eb_status eb_launch_q4_pack(void *stream, const uint32_t *w, size_t w_words, const uint16_t *scales, size_t scales_numel,
+                            const uint8_t *zeros, size_t zeros_numel, size_t in_f, size_t out_f, size_t group,
+                            void *packed, size_t packed_bytes) {
+    return pack_checked((hipStream_t)stream, w, w_words, scales, scales_numel, zeros, zeros_numel, in_f, out_f, group,
+                        packed, packed_bytes);
+}
+
+static eb_status q4_checked(hipStream_t st, const Room &src, const float *a, size_t an, const eb::Q4Weight *w,
+                            const size_t *bytes, float *const *c, const size_t *cn, int n, size_t m) {
+    const size_t in_f = w[0].in_f, group = w[0].group;
     for (int i = 0; i < n; ++i) {
-        if (w[i].in_f != in_f || w[i].group != group || (w[i].zeros != nullptr) != (w[0].zeros != nullptr))
+        EB_TRY(q4_shape(w[i].in_f, w[i].out_f, w[i].group));
+        if (w[i].in_f != in_f || w[i].group != group || w[i].zeros != w[0].zeros)
             return fail(EB_SHAPE_MISMATCH, "linear_q4: the weights of a launch share in_f and group, and have zero "
                         "points all or none");
-        EB_TRY(eb::check_numel(words[i], {w[i].out_f, in_f / 8}, "w"));
-        EB_TRY(eb::check_numel(scales[i], {w[i].out_f, in_f / group}, "scales"));
-        if (w[i].zeros) EB_TRY(eb::check_numel(zeros[i], {w[i].out_f, in_f / group}, "zeros"));
+        EB_TRY(holds(bytes[i], eb::q4_packed_bytes(in_f, w[i].out_f, group, w[i].zeros), "packed"));
         EB_TRY(eb::check_numel(cn[i], {m, w[i].out_f}, "c"));
     }
+    EB_TRY(eb::check_numel(an, {m, in_f}, "a"));
     if (m == 0) return eb::ok();
     EB_TRY(eb::check_ptr(a, "a"));
     EB_TRY(aligned({a}, 16, "linear_q4: a"));
     for (int i = 0; i < n; ++i) {
         if (w[i].out_f == 0) continue;
-        EB_TRY(eb::check_ptr(w[i].w, "w"));
-        EB_TRY(eb::check_ptr(w[i].scales, "scales"));
+        EB_TRY(eb::check_ptr(w[i].packed, "packed"));
         EB_TRY(eb::check_ptr(c[i], "c"));
-        EB_TRY(aligned({w[i].w}, 16, "linear_q4: w"));
-        EB_TRY(aligned({w[i].scales}, 2, "linear_q4: scales"));
+        EB_TRY(aligned({w[i].packed}, 16, "linear_q4: packed"));
     }
     float *ws;
     WsLock lk;
@@ -451,22 +505,16 @@ eb_status eb_linear_q4_multi(eb_recorder *rec, const eb_tensor *a, size_t n, con
     EB_TRY(eb::check_tensor(a, EB_F32, "a", dev));
     eb::Q4Weight q[kMax];
     float *y[kMax];
-    size_t words[kMax], scales[kMax], zeros[kMax], cn[kMax];
+    size_t bytes[kMax], cn[kMax];
     for (size_t i = 0; i < n; ++i) {
-        EB_TRY(eb::check_tensor(w[i].w, EB_U32, "w", dev));
-        EB_TRY(eb::check_tensor(w[i].scales, EB_F16, "scales", dev));
-        if (w[i].zeros) EB_TRY(eb::check_tensor(w[i].zeros, EB_U8, "zeros", dev));
+        EB_TRY(eb::check_tensor(w[i].packed, EB_U8, "packed", dev));
         EB_TRY(eb::check_tensor(c[i], EB_F32, "c", dev));
-        q[i] = eb::Q4Weight{data<uint32_t>(w[i].w), data<uint16_t>(w[i].scales),
-                            w[i].zeros ? data<uint8_t>(w[i].zeros) : nullptr, w[i].in_f, w[i].out_f, w[i].group};
+        q[i] = eb::Q4Weight{data<uint8_t>(w[i].packed), w[i].in_f, w[i].out_f, w[i].group, w[i].zeros != 0};
         y[i] = data<float>(c[i]);
-        words[i] = eb_tensor_numel(w[i].w);
-        scales[i] = eb_tensor_numel(w[i].scales);
-        zeros[i] = w[i].zeros ? eb_tensor_numel(w[i].zeros) : 0;
+        bytes[i] = eb_tensor_numel(w[i].packed);
         cn[i] = eb_tensor_numel(c[i]);
     }
-    return q4_checked(stream_of(dev), Room{dev}, data<float>(a), eb_tensor_numel(a), q, words, scales, zeros, y, cn,
-                      (int)n, m);
+    return q4_checked(stream_of(dev), Room{dev}, data<float>(a), eb_tensor_numel(a), q, bytes, y, cn, (int)n, m);
 }
 
 eb_status eb_linear_q4(eb_recorder *rec, const eb_tensor *a, const eb_q4_weight *w, eb_tensor *c, size_t m) {
@@ -475,13 +523,12 @@ eb_status eb_linear_q4(eb_recorder *rec, const eb_tensor *a, const eb_q4_weight 
 
 size_t eb_linear_q4_workspace_floats(size_t m, size_t in_f) { return eb::linear_q4_workspace_floats(m, in_f); }
 
-eb_status eb_launch_linear_q4(void *stream, const float *a, size_t a_numel, const uint32_t *w, size_t w_words,
-                              const uint16_t *scales, size_t scales_numel, const uint8_t *zeros, size_t zeros_numel,
-                              float *c, size_t c_numel, size_t m, size_t in_f, size_t out_f, size_t group,
+eb_status eb_launch_linear_q4(void *stream, const float *a, size_t a_numel, const void *packed, size_t packed_bytes,
+                              float *c, size_t c_numel, size_t m, size_t in_f, size_t out_f, size_t group, int zeros,
                               float *workspace, size_t workspace_floats) {
-    const eb::Q4Weight q{w, scales, zeros, in_f, out_f, group};
-    return q4_checked((hipStream_t)stream, Room{nullptr, workspace, workspace_floats}, a, a_numel, &q, &w_words,
-                      &scales_numel, &zeros_numel, &c, &c_numel, 1, m);
+    const eb::Q4Weight q{static_cast<const uint8_t *>(packed), in_f, out_f, group, zeros != 0};
+    return q4_checked((hipStream_t)stream, Room{nullptr, workspace, workspace_floats}, a, a_numel, &q, &packed_bytes, &c,
+                      &c_numel, 1, m);
 }
 
 eb_status eb_attention_new_q4(const eb_attention_desc *desc, const eb_q4_weight proj[4], eb_attention **out) {
@@ -497,15 +544,11 @@ eb_status eb_attention_new_q4(const eb_attention_desc *desc, const eb_q4_weight 
         if (p.out_f != outs[i] || p.in_f != ins[i])
             return fail(EB_SHAPE_MISMATCH, "attention: projection %d is [%zu, %zu], must be [%zu, %zu]", i, p.out_f,
                         p.in_f, outs[i], ins[i]);
-        if ((p.group != 32 && p.group != 64 && p.group != 128) || p.in_f % p.group)
-            return fail(EB_UNSUPPORTED_CONFIG, "attention: projection %d: group %zu (32, 64 or 128, dividing %zu)", i,
-                        p.group, p.in_f);
-        const size_t per = outs[i] * (ins[i] / p.group);
-        if (!p.w || eb_tensor_dtype(p.w) != EB_U32 || eb_tensor_numel(p.w) != outs[i] * (ins[i] / 8) || !p.scales ||
-            eb_tensor_dtype(p.scales) != EB_F16 || eb_tensor_numel(p.scales) != per ||
-            (p.zeros && (eb_tensor_dtype(p.zeros) != EB_U8 || eb_tensor_numel(p.zeros) != per)))
-            return fail(EB_SHAPE_MISMATCH, "attention: projection %d: codes, scales or zero points do not fit", i);
-        if (i < 3 && (p.group != proj[0].group || (p.zeros != nullptr) != (proj[0].zeros != nullptr)))
+        EB_TRY(q4_shape(p.in_f, p.out_f, p.group));
+        if (!p.packed || eb_tensor_dtype(p.packed) != EB_U8 ||
+            eb_tensor_numel(p.packed) < eb::q4_packed_bytes(p.in_f, p.out_f, p.group, p.zeros != 0))
+            return fail(EB_SHAPE_MISMATCH, "attention: projection %d is not a packed 4-bit weight of its shape", i);
+        if (i < 3 && (p.group != proj[0].group || (p.zeros != 0) != (proj[0].zeros != 0)))
             return fail(EB_SHAPE_MISMATCH, "attention: q, k and v share a group, and have zero points all or none");
     }
     eb_attention *a = nullptr;

@@ -136,14 +136,26 @@ def linear_q4_workspace_floats(m: int, in_f: int) -> int:
     return int(lib().eb_linear_q4_workspace_floats(m, in_f))
 
 
-def launch_linear_q4(stream: int, a_ptr: int, a_numel: int, w_ptr: int, w_words: int,
-                     scales_ptr: int, scales_numel: int, zeros_ptr: int, zeros_numel: int,
+def q4_packed_bytes(in_f: int, out_f: int, group: int, zeros: bool) -> int:
+    return int(lib().eb_q4_packed_bytes(in_f, out_f, group, int(zeros)))
+
+
+def launch_q4_pack(stream: int, w_ptr: int, w_words: int, scales_ptr: int, scales_numel: int,
+                   zeros_ptr: int, zeros_numel: int, in_f: int, out_f: int, group: int,
+                   packed_ptr: int, packed_bytes: int) -> None:
+    """Lay a 4-bit weight out as linear_q4 reads it, on caller memory (zeros_ptr 0: none)."""
+    check(lib().eb_launch_q4_pack(c_vp(stream), w_ptr, w_words, scales_ptr, scales_numel,
+                                  zeros_ptr or None, zeros_numel, in_f, out_f, group, packed_ptr,
+                                  packed_bytes))
+
+
+def launch_linear_q4(stream: int, a_ptr: int, a_numel: int, packed_ptr: int, packed_bytes: int,
                      c_ptr: int, c_numel: int, m: int, in_f: int, out_f: int, group: int,
-                     ws_ptr: int = 0, ws_floats: int = 0) -> None:
-    """linear_q4 on caller memory (zeros_ptr 0: zero point 8)."""
-    check(lib().eb_launch_linear_q4(c_vp(stream), a_ptr, a_numel, w_ptr, w_words, scales_ptr,
-                                    scales_numel, zeros_ptr or None, zeros_numel, c_ptr, c_numel,
-                                    m, in_f, out_f, group, ws_ptr or None, ws_floats))
+                     zeros: bool, ws_ptr: int = 0, ws_floats: int = 0) -> None:
+    """linear_q4 on caller memory."""
+    check(lib().eb_launch_linear_q4(c_vp(stream), a_ptr, a_numel, packed_ptr, packed_bytes, c_ptr,
+                                    c_numel, m, in_f, out_f, group, int(zeros), ws_ptr or None,
+                                    ws_floats))
 
 
 def kv_write_i8(rec: Recorder, kv, layer: int, k: Tensor, v: Tensor, count: int,

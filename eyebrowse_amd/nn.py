@@ -91,18 +91,23 @@ class LinearQ4:
     """A bias-free projection with 4-bit codes and group scales (no counterpart in the reference):
     W[o, k] = (code[o, k] - zero[o, k // group]) * scale[o, k // group]. w: U32 [out_f, in_f / 8],
     eight codes per word along k, lowest bits first; scales: F16 [out_f, in_f / group]; zeros: U8 of
-    that shape, or None (8 everywhere). group is 32, 64 or 128 and divides in_f."""
+    that shape, or None (8 everywhere). group is 32, 64 or 128 and divides in_f. The weight is laid
+    out once, into `packed`, as the kernels read it; w, scales and zeros are not kept."""
 
     def __init__(self, w: Tensor, scales: Tensor, zeros: Optional[Tensor], in_f: int, out_f: int,
                  group: int):
-        self.w, self.scales, self.zeros = w, scales, zeros
-        self.in_f, self.out_f, self.group = in_f, out_f, group
+        out = c_vp()
+        rec = Recorder(w.dev)
+        check(lib().eb_q4_pack(rec.handle, w.handle, scales.handle,
+                               zeros.handle if zeros is not None else None, in_f, out_f, group,
+                               ctypes.byref(out)))
+        self.packed = Tensor(out.value, w.dev)
+        rec.submit()
+        self.in_f, self.out_f, self.group, self.zeros = in_f, out_f, group, zeros is not None
 
     @property
     def desc(self) -> Q4Weight:
-        return Q4Weight(self.w.handle, self.scales.handle,
-                        self.zeros.handle if self.zeros is not None else None, self.in_f,
-                        self.out_f, self.group)
+        return Q4Weight(self.packed.handle, self.in_f, self.out_f, self.group, int(self.zeros))
 
     @classmethod
     def from_f32(cls, dev: Device, weight, group: int = 128, symmetric: bool = True) -> "LinearQ4":

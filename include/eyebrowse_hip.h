@@ -570,32 +570,41 @@ eb_status eb_attention_forward(const eb_attention *attn, eb_recorder *rec, const
 
 /* ---- projections with 4-bit weights (no counterpart in the reference) ----------------
  * c [m, out_f] = a [m, in_f] . W^T with W[o, k] = (code[o, k] - zero[o, k / group]) *
- * scale[o, k / group]. Codes 0..15 are packed eight per u32 word along k, lowest bits first:
- * w is an EB_U32 tensor [out_f, in_f / 8]. scales is EB_F16 [out_f, in_f / group]; zeros is
- * EB_U8 of that shape, or NULL: 8 everywhere (symmetric codes). group is 32, 64 or 128 and
- * divides in_f; out_f is any size. a and c are f32. Every code less its zero point is exact
- * in f16; the products run on the matrix cores against a's rows split into two halves (about
- * f32 accuracy, as linear_f16w's many-row form), are summed in f32 within a group, and the
- * groups' sums are scaled and added in f32. The order of a sum depends on the shape alone. */
+ * scale[o, k / group]. Every code less its zero point is exact in f16; the products run on the
+ * matrix cores against a's rows split into two halves (about f32 accuracy, as linear_f16w's
+ * many-row form), are summed in f32 within a group, and the groups' sums are scaled and added
+ * in f32. The order of a sum depends on the shape alone.
+ *
+ * eb_q4_pack lays a weight out once, as the kernels read it: w holds codes 0..15 packed eight
+ * per u32 word along k, lowest bits first (EB_U32 [out_f, in_f / 8]), scales is EB_F16 [out_f,
+ * in_f / group], zeros EB_U8 of that shape, or NULL: 8 everywhere (symmetric codes). group is
+ * 32, 64 or 128 and divides in_f; out_f is any size. *packed is a new EB_U8 tensor of
+ * eb_q4_packed_bytes bytes (about what w, scales and zeros hold, which are no longer needed). */
 typedef struct eb_q4_weight {
-    const eb_tensor *w;
-    const eb_tensor *scales;
-    const eb_tensor *zeros; /* may be NULL */
+    const eb_tensor *packed;
     size_t in_f, out_f, group;
+    int zeros; /* 1: packed with zero points */
 } eb_q4_weight;
+size_t eb_q4_packed_bytes(size_t in_f, size_t out_f, size_t group, int zeros);
+eb_status eb_q4_pack(eb_recorder *rec, const eb_tensor *w, const eb_tensor *scales,
+                     const eb_tensor *zeros, size_t in_f, size_t out_f, size_t group,
+                     eb_tensor **packed);
 eb_status eb_linear_q4(eb_recorder *rec, const eb_tensor *a, const eb_q4_weight *w, eb_tensor *c,
                        size_t m);
 /* n (1..3) projections of the same a in one launch, e.g. a layer's q/k/v; the weights share
  * in_f and group, and have zero points all or none. */
 eb_status eb_linear_q4_multi(eb_recorder *rec, const eb_tensor *a, size_t n,
                              const eb_q4_weight *w, eb_tensor *const *c, size_t m);
-/* On caller memory. The workspace (16-byte aligned, no initialisation) holds the split rows;
- * launches that share one must not overlap. */
+/* On caller memory. packed is 16-byte aligned; the workspace (16-byte aligned, no
+ * initialisation) holds the split rows; launches that share one must not overlap. */
+eb_status eb_launch_q4_pack(void *stream, const uint32_t *w, size_t w_words,
+                            const uint16_t *scales, size_t scales_numel, const uint8_t *zeros,
+                            size_t zeros_numel, size_t in_f, size_t out_f, size_t group,
+                            void *packed, size_t packed_bytes);
 size_t eb_linear_q4_workspace_floats(size_t m, size_t in_f);
-eb_status eb_launch_linear_q4(void *stream, const float *a, size_t a_numel, const uint32_t *w,
-                              size_t w_words, const uint16_t *scales, size_t scales_numel,
-                              const uint8_t *zeros, size_t zeros_numel, float *c, size_t c_numel,
-                              size_t m, size_t in_f, size_t out_f, size_t group,
+eb_status eb_launch_linear_q4(void *stream, const float *a, size_t a_numel, const void *packed,
+                              size_t packed_bytes, float *c, size_t c_numel, size_t m,
+                              size_t in_f, size_t out_f, size_t group, int zeros,
                               float *workspace, size_t workspace_floats);
 /* eb_attention_new with 4-bit projections: proj[0..3] are q, k, v and o, of the shapes the
  * descriptor asks for; the descriptor's own projections are NULL, its hidden is set. */

@@ -80,6 +80,26 @@ def pack_q4(codes):
     return np.bitwise_or.reduce(c << (4 * np.arange(8, dtype=np.uint32)), axis=-1).astype(np.uint32)
 
 
+def unpack_q4(packed, in_f, out_f, group, zeros):
+    """(codes, scales, zero points or None) of a packed weight's bytes, and whether its padding (to
+    16 features, 128 of the contraction) is zeros."""
+    nt, nb, ng = -(-out_f // 16), -(-in_f // 128), 128 // group
+    b = np.frombuffer(packed, np.uint8)
+    planes = np.split(b, np.cumsum([nt * nb * 1024, nt * nb * 16 * ng * 2]))
+    w = planes[0].view(np.uint32).reshape(nt, nb, 4, 16, 4)  # tile, block, g, n, j
+    at = [16 * (i % 2) + 4 * (i // 2) for i in range(8)]
+    c = np.stack([(w >> np.uint32(a)) & 15 for a in at], -1)  # tile, block, g, n, j, k
+    codes = c.transpose(0, 3, 1, 4, 2, 5).reshape(nt * 16, nb * 128)
+    s = planes[1].view(np.float16).reshape(nt, nb, 16, ng).transpose(0, 2, 1, 3).reshape(nt * 16, nb * ng)
+    ngr = in_f // group
+    padding = s[out_f:].any() or s[:, ngr:].any() or codes[out_f:].any() or codes[:, in_f:].any()
+    z = None
+    if zeros:
+        z = planes[2].reshape(nt, nb, 16, ng).transpose(0, 2, 1, 3).reshape(nt * 16, nb * ng)[:out_f, :ngr]
+    assert planes[2].size == (nt * nb * 16 * ng if zeros else 0)
+    return codes[:out_f, :in_f].astype(np.int64), s[:out_f, :ngr], z, not padding
+
+
 def linear_q4_bound(a, codes, scales, zeros, group):
     """(a . W^T, bound on its error) in 64 bits: a keeps 22 bits, a group's products are summed in
     f32 and scaled, and the groups' sums added in f32 (the waves of a workgroup adding eight more)."""

@@ -5,7 +5,7 @@ import pytest
 
 import eyebrowse_amd as eb
 from tests._gpu import note
-from tests._quant import linear_q4_bound, pack_q4
+from tests._quant import linear_q4_bound, pack_q4, unpack_q4
 
 pytestmark = pytest.mark.gpu
 
@@ -53,7 +53,7 @@ def test_rows(dev, m, group, zeros):
 
 
 @pytest.mark.parametrize("m,in_f,out_f", [(1, 1024, 20000), (4, 4096, 5000), (8, 4736, 257), (8, 6144, 100), (1, 16384, 64),
-                                          (300, 1152, 777), (1, 40960, 33), (2, 1024, 9000)])
+                                          (300, 1152, 777), (1, 40960, 33), (2, 1024, 9000), (700, 1024, 3000), (129, 640, 16500)])
 def test_large(dev, m, in_f, out_f):
     note(f"q4 {m} rows {in_f} to {out_f}")
     rng = np.random.default_rng(in_f)
@@ -151,17 +151,51 @@ def test_graph_replays(dev):
             assert run(dev, a, w).tobytes() == out.to_f32().tobytes()
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_pack(dev, group):
+    """The packed layout holds the weight, and zeros besides."""
+    rng = np.random.default_rng(group)
+    for out_f, in_f in ((1, group), (16, 128), (50, 3 * group), (129, 1152)):
+        for zeros in (False, True):
+            codes, scales, z = weight(rng, out_f, in_f, group, zeros)
+            w = device_weight(dev, codes, scales, z, group)
+            assert w.packed.numel() == eb.q4_packed_bytes(in_f, out_f, group, zeros)
+            c, s, zz, clean = unpack_q4(w.packed.read_bytes(), in_f, out_f, group, zeros)
+            np.testing.assert_array_equal(c, codes)
+            assert s.tobytes() == scales.tobytes() and clean
+            if zeros:
+                np.testing.assert_array_equal(zz, z)
+
+
+def test_infinite_scales_stay_with_their_feature(dev):
+    rng = np.random.default_rng(12)
+    for m in (1, 20, 200):
+        codes, scales, z = weight(rng, 40, 160, 32, True)
+        scales[7, 4], scales[20, 0] = np.inf, np.nan
+        a = rng.standard_normal((m, 160)).astype(np.float32)
+        got = run(dev, a, device_weight(dev, codes, scales, z, 32))
+        assert not np.isfinite(got[:, [7, 20]]).any()
+        keep = [i for i in range(40) if i not in (7, 20)]
+        want, bound = linear_q4_bound(a, codes[keep], scales[keep], z[keep], 32)
+        close(got[:, keep], want, bound, "the other features")
+
+
 def test_raw_launch(dev):
     rng = np.random.default_rng(3)
     codes, scales, z = weight(rng, 65, 256, 64, True)
     w = device_weight(dev, codes, scales, z, 64)
-    for m in (1, 17):
+    wt, st, zt = (eb.Tensor.from_array(dev, x) for x in (pack_q4(codes), scales, z))
+    packed = eb.Tensor.empty(dev, (w.packed.numel(),), eb.DType.U8)
+    eb.launch_q4_pack(dev.stream, wt.data_ptr, wt.numel(), st.data_ptr, st.numel(), zt.data_ptr, zt.numel(), 256, 65, 64,
+                      packed.data_ptr, packed.numel())
+    dev.synchronize()
+    assert packed.read_bytes() == w.packed.read_bytes()
+    for m in (1, 17, 300):
         a = rng.standard_normal((m, 256)).astype(np.float32)
         at, out = eb.Tensor.from_array(dev, a), eb.Tensor.empty(dev, (m, 65))
         floats = eb.linear_q4_workspace_floats(m, 256)
         ws = eb.Tensor.empty(dev, (max(floats, 1),))
-        eb.launch_linear_q4(dev.stream, at.data_ptr, a.size, w.w.data_ptr, w.w.numel(), w.scales.data_ptr,
-                            w.scales.numel(), w.zeros.data_ptr, w.zeros.numel(), out.data_ptr, m * 65, m, 256, 65, 64,
-                            ws.data_ptr, floats)
+        eb.launch_linear_q4(dev.stream, at.data_ptr, a.size, packed.data_ptr, packed.numel(), out.data_ptr, m * 65, m, 256, 65,
+                            64, True, ws.data_ptr, floats)
         dev.synchronize()
         assert out.to_f32().tobytes() == run(dev, a, w).tobytes()

@@ -5,7 +5,7 @@ import pytest
 
 import eyebrowse_amd as eb
 from tests._gpu import note
-from tests._quant import CacheModel, sample_f64
+from tests._quant import CacheModel, sample_f64, unpack_q4
 from tests._textbook import attention_f64, rel_l2_f64, rmsnorm_f64, rope_f64
 
 pytestmark = pytest.mark.gpu
@@ -13,11 +13,9 @@ EPS, THETA = 1e-6, 1e4
 
 
 def dequantised(p):
-    words = np.frombuffer(p.w.read_bytes(), np.uint32).reshape(p.out_f, p.in_f // 8)
-    codes = (words[..., None] >> (4 * np.arange(8, dtype=np.uint32))) & 15
-    s = np.frombuffer(p.scales.read_bytes(), np.float16).reshape(p.out_f, -1).astype(np.float64)
-    z = 8.0 if p.zeros is None else np.frombuffer(p.zeros.read_bytes(), np.uint8).reshape(s.shape).astype(np.float64)[..., None]
-    return ((codes.reshape(*s.shape, p.group) - z) * s[..., None]).reshape(p.out_f, p.in_f)
+    codes, s, z, _ = unpack_q4(p.packed.read_bytes(), p.in_f, p.out_f, p.group, p.zeros)
+    z = np.full(s.shape, 8.0) if z is None else z.astype(np.float64)
+    return (codes - np.repeat(z, p.group, 1)) * np.repeat(s.astype(np.float64), p.group, 1)
 
 
 class Model:

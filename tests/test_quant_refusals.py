@@ -79,22 +79,33 @@ def test_rows_and_operands():
 
 def test_linear_q4():
     l = eb.lib()
+    bytes_ = eb.q4_packed_bytes(256, 10, 64, True)
+    assert bytes_ == 2 * (1024 + 16 * 2 * 3) and eb.q4_packed_bytes(256, 10, 64, False) == 2 * (1024 + 16 * 2 * 2)
+    assert eb.q4_packed_bytes(200, 10, 64, False) == 0 and eb.q4_packed_bytes(256, 10, 48, False) == 0
 
-    def call(a=P, an=256, w=P, words=10 * 32, s=P, sn=10 * 4, z=P, zn=10 * 4, c=P, cn=10, m=1, in_f=256, out_f=10, group=64,
-             ws=None, wsn=0):
-        return err(l.eb_launch_linear_q4, None, a, an, w, words, s, sn, z, zn, c, cn, m, in_f, out_f, group, ws, wsn)
+    def pack(w=P, words=10 * 32, s=P, sn=10 * 4, z=P, zn=10 * 4, in_f=256, out_f=10, group=64, packed=P, n=bytes_):
+        return err(l.eb_launch_q4_pack, None, w, words, s, sn, z, zn, in_f, out_f, group, packed, n)
 
-    for over, status, word in ((dict(group=16), 3, "group"), (dict(group=256), 3, "group"), (dict(group=0), 3, "group"),
-                               (dict(in_f=200), 4, "multiple"), (dict(in_f=0), 4, "multiple"), (dict(an=255), 4, "a holds"),
-                               (dict(words=319), 4, "w holds"), (dict(sn=39), 4, "scales holds"), (dict(zn=39), 4, "zeros holds"),
-                               (dict(cn=9), 4, "c holds"), (dict(a=None), 4, "null"), (dict(w=None), 4, "null"), (dict(s=None), 4, "null"),
-                               (dict(c=None), 4, "null"), (dict(a=P + 4), 3, "aligned"), (dict(w=P + 4), 3, "aligned"), (dict(s=P + 1), 3, "aligned"),
-                               (dict(out_f=1 << 62), 3, "overflows"),
+    def call(a=P, an=256, w=P, n=bytes_, c=P, cn=10, m=1, in_f=256, out_f=10, group=64, zeros=1, ws=None, wsn=0):
+        return err(l.eb_launch_linear_q4, None, a, an, w, n, c, cn, m, in_f, out_f, group, zeros, ws, wsn)
+
+    shapes = ((dict(group=16), 3, "group"), (dict(group=256), 3, "group"), (dict(group=0), 3, "group"),
+              (dict(in_f=200), 4, "multiple"), (dict(in_f=0), 4, "multiple"), (dict(out_f=1 << 62), 3, "overflows"),
+              (dict(in_f=1 << 25), 3, "in_f"), (dict(n=bytes_ - 1), 4, "packed holds"))
+    for over, status, word in (*shapes, (dict(words=319), 4, "w holds"), (dict(sn=39), 4, "scales holds"), (dict(zn=39), 4, "zeros holds"),
+                               (dict(w=None), 4, "null"), (dict(s=None), 4, "null"), (dict(packed=None), 4, "null"),
+                               (dict(packed=P + 8), 3, "aligned"), (dict(w=P + 2), 3, "aligned"), (dict(s=P + 1), 3, "aligned")):
+        over = {**over, **(dict(words=1 << 40, sn=1 << 40, zn=1 << 40) if "in_f" in over else {})}
+        st, msg = pack(**over)
+        assert st == status and word in msg, (over, msg)
+    for over, status, word in (*shapes, (dict(an=255), 4, "a holds"), (dict(cn=9), 4, "c holds"), (dict(a=None), 4, "null"),
+                               (dict(w=None), 4, "null"), (dict(c=None), 4, "null"), (dict(a=P + 4), 3, "aligned"), (dict(w=P + 4), 3, "aligned"),
                                (dict(m=40, an=40 * 256, cn=400), 4, "workspace")):
         st, msg = call(**over)
         assert st == status and word in msg, (over, msg)
     assert call(m=0, an=0, cn=0)[0] == 0
-    assert call(out_f=0, words=0, sn=0, zn=0, cn=0, w=None, s=None, c=None)[0] == 0
+    assert call(out_f=0, n=0, cn=0, w=None, c=None)[0] == 0
+    assert pack(out_f=0, words=0, sn=0, zn=0, n=0, w=None, s=None, packed=None)[0] == 0
     assert eb.linear_q4_workspace_floats(1, 1024) == 0
     assert eb.linear_q4_workspace_floats(100, 1024) >= 100 * 1024
 
@@ -123,9 +134,9 @@ def test_handles_refuse_null():
     assert l.eb_linear_q4(None, None, None, None, 1) == 6
     assert l.eb_kv_write_i8(None, None, 0, None, None, 1, 0) == 6
     d = _lib.AttentionDesc(4, 2, 64, 0.125, 1e-6, None, None, None, 0, None, None, None, None, 256)
-    proj = (_lib.Q4Weight * 4)(*[_lib.Q4Weight(None, None, None, i, o, 64) for i, o in ((256, 256), (256, 128), (256, 128), (256, 256))])
+    proj = (_lib.Q4Weight * 4)(*[_lib.Q4Weight(None, i, o, 64, 0) for i, o in ((256, 256), (256, 128), (256, 128), (256, 256))])
     assert l.eb_attention_new_q4(ctypes.byref(d), proj, ctypes.byref(out)) == 4
-    assert "codes" in l.eb_last_error().decode()
+    assert "not a packed" in l.eb_last_error().decode()
     proj[0].in_f = 128
     assert l.eb_attention_new_q4(ctypes.byref(d), proj, ctypes.byref(out)) == 4
     assert "projection 0 is" in l.eb_last_error().decode()
