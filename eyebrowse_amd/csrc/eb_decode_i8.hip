@@ -7,7 +7,7 @@
 // over the keys j that column c sees. A column is one query head of one row; the up to 16 columns
 // of a workgroup share a KV head, so that every key row is read once for all of them.
 //
-// Grid (hkv * nsub) x nsplit, 4 waves. A tile is 16 keys at an aligned position, hence inside one
+// Grid hkv x nsub x nsplit, 4 waves. A tile is 16 keys at an aligned position, hence inside one
 // block of the cache: its two scales are the same for the whole tile. Lane (n, g) is lane
 // n + 16 g.
 //  - Scores S[key][column] = K q^T on v_mfma_f32_16x16x32_f16. A: lane (n, g) holds 16 dims of
@@ -28,11 +28,13 @@
 //    nor the small ones' precision where the large ones have no weight.
 // The products sum in f32; the f16 pairs keep 22 bits of q and of the weights.
 //
-// Fused append (one row): the split with the fewest tiles owns the token's block. It normalises
-// and rotates the new K and V rows, writes their codes (and the block's earlier codes again where
-// the exponent grew), and then takes the block's tiles itself, from the cache; no other split
-// reads that block. With more than 16 columns several workgroups would read it, and the append is
-// a launch of its own.
+// Fused append (one row): the split with the fewest tiles owns the token's block; no other split
+// reads it. Its waves take the block's tiles first, loaded with q as any first tile. The workgroup
+// then normalises and rotates the new K and V rows and writes their codes, and the tile that holds
+// the new row gets it out of LDS; only where the exponent grew, and the block's earlier codes are
+// written again, are its tiles loaded again. Tiles beyond two per wave are loaded after the append
+// anyway. With more than 16 columns several workgroups would read the block, and the append is a
+// launch of its own.
 #include "eb_cache_i8.h"
 
 #include <algorithm>
@@ -60,10 +62,11 @@ struct Shape {
     static constexpr int VW = DV / 4;    // words per lane and V row
     static constexpr int QS = HD + 4;    // floats per LDS row (bank spread)
     // LDS (floats): q [kCols][QS], later the waves' accumulators [kWaves][ncol][QS]; then the new
-    // rows [2][HD]; column exponents [kCols]; m and l [kCols][kWaves] each.
+    // rows [2][HD]; column exponents [kCols]; m and l [kCols][kWaves] each; the new rows' codes
+    // [2][HD / 4 words]; their block's exponents before and after, [2][2].
     static constexpr size_t lds_floats(int ncol) {
         const int a = kCols * QS, b = kWaves * ncol * QS;
-        return (size_t)(a > b ? a : b) + 2 * HD + kCols + 2 * kCols * kWaves;
+        return (size_t)(a > b ? a : b) + 2 * HD + kCols + 2 * kCols * kWaves + 2 * HD / 4 + 4;
     }
 };
 
@@ -121,10 +124,10 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i8_kernel(Args a, int hd) 
     const int n = lane & 15;
     const int g4 = lane >> 4;
     const int hkv = (int)a.c.hkv;
-    const int kvh = blockIdx.x % hkv;
-    const int col0 = (int)(blockIdx.x / hkv) * kCols;
+    const int kvh = blockIdx.x;
+    const int col0 = (int)blockIdx.y * kCols;
     const int ncol = min(kCols, a.ncols - col0);
-    const int split = blockIdx.y;
+    const int split = blockIdx.z;
     const bool owner = a.knew != nullptr && split == a.owner;
     const int lds_rows = max(kCols, kWaves * ncol);
     float *s_q = smem;
@@ -132,6 +135,8 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i8_kernel(Args a, int hd) 
     int *s_qe = reinterpret_cast<int *>(s_new + 2 * HD);
     float *s_m = reinterpret_cast<float *>(s_qe + kCols);
     float *s_l = s_m + kCols * kWaves;
+    unsigned *s_code = reinterpret_cast<unsigned *>(s_l + kCols * kWaves);
+    unsigned *s_e = s_code + 2 * (HD / 4);
 
     // ---- tile loads ------------------------------------------------------------------------
     const int row_bytes = hkv * hd;
@@ -153,7 +158,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i8_kernel(Args a, int hd) 
         const __amdgpu_buffer_rsrc_t vres = eb::make_rsrc(vbase + off, nbytes);
 #pragma unroll
         for (int c = 0; c < KL; ++c) {
-            const u32x4 w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(kres, kvo, 64 * c, 0));
+            const u32x4 w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(kres, kvo + 64 * c, 0, 0));
 #pragma unroll
             for (int i = 0; i < 4; ++i) x.k[c][i] = w[i];
         }
@@ -176,134 +181,154 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i8_kernel(Args a, int hd) 
         x.ek = a.c.ks[b];
         x.ev = a.c.vs[b];
     };
-    // Local tile i of this wave (all waves and splits together walk one stretch of the cache).
+    // Local tile i of this wave (all waves and splits together walk one stretch of the cache); the
+    // owner's first ones are the new token's block.
+    const int own_steps = owner ? (a.tails + kWaves - 1) / kWaves : 0;
     auto tile_of = [&](int i) {
-        const int t = (i * kWaves + wave) * a.nsplit + split;
-        return t < a.tiles ? a.tile0 + t : INT_MAX / kTile;
+        const int w = i * kWaves + wave, t = (w - own_steps * kWaves) * a.nsplit + split;
+        const bool tail = i < own_steps;
+        return (tail ? w < a.tails : t < a.tiles) ? (tail ? a.tail0 + w : a.tile0 + t) : INT_MAX / kTile;
     };
 
-    // ---- q, its first loads, then the first two tiles' ---------------------------------------
-    for (int i = tid; i < kCols * (HD / 4); i += kThreads) {
-        const int c = i / (HD / 4), d = 4 * (i % (HD / 4));
-        const int cc = col0 + min(c, ncol - 1);
-        const size_t at = ((size_t)(cc / a.g) * a.h + kvh * a.g + cc % a.g) * hd + d;
-        const f32x4 x = d < hd ? *reinterpret_cast<const f32x4 *>(a.q + at) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        *reinterpret_cast<f32x4 *>(s_q + c * QS + d) = x;
-    }
-    if (owner)
-        for (int i = tid; i < 2 * (HD / 4); i += kThreads) {
-            const int d = 4 * (i % (HD / 4));
-            const float *src = (i < HD / 4 ? a.knew : a.vnew) + (size_t)kvh * hd + d;
-            *reinterpret_cast<f32x4 *>(s_new + (i / (HD / 4)) * HD + d) =
-                d < hd ? *reinterpret_cast<const f32x4 *>(src) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    // ---- every first load at once: q, the new rows, what transforms them, two tiles ------------
+    // Wave w takes columns w, w + 4, ... and, of the owner, wave 0 the new K row and wave 1 the new
+    // V row. A lane owns the dim pairs (p, p + hd/2), so that RMSNorm and RoPE never read another
+    // lane's dims. What is absent reads as zeros and is not used.
+    constexpr int NP = (HD / 2 + 63) / 64, NJ = kCols / kWaves;
+    const int half = hd / 2;
+    const bool newrow = owner && wave < 2;
+    float x1[NJ + 1][NP], x2[NJ + 1][NP], qw1[NP], qw2[NP], nw1[NP], nw2[NP], cs[NP], sn[NP];
+    const float *nw = wave ? a.vn_w : a.kn_w;
+    unsigned old_e = 0;
+    {
+        const int none = 0x7FFFFFF0;
+        const auto qres = eb::make_rsrc(a.q, a.rows * a.h * hd * 4);
+        const auto nres = eb::make_rsrc((wave ? a.vnew : a.knew) + (size_t)kvh * hd, newrow ? hd * 4 : 0);
+        const auto qwres = eb::make_rsrc(a.qn_w, a.prologue && a.qn_w ? hd * 4 : 0);
+        const auto nwres = eb::make_rsrc(nw, newrow && a.prologue && nw ? hd * 4 : 0);
+        const size_t trow = (size_t)a.pos0 * half;
+        const bool rope = a.prologue && a.rcos;
+        const auto cres = eb::make_rsrc(a.rcos + trow, rope ? half * 4 : 0);
+        const auto sres = eb::make_rsrc(a.rsin + trow, rope ? half * 4 : 0);
+        auto get = [&](__amdgpu_buffer_rsrc_t r, int vo) {
+            return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, vo, 0, 0));
+        };
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const int p = lane + 64 * i;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const int cc = col0 + j * kWaves + wave;
+                const int row = a.rows == 1 ? 0 : cc / a.g;
+                const int at = (row * a.h + kvh * a.g + cc - row * a.g) * hd * 4;
+                const bool have = j * kWaves + wave < ncol && p < half;
+                x1[j][i] = get(qres, have ? at + 4 * p : none);
+                x2[j][i] = get(qres, have ? at + 4 * (p + half) : none);
+            }
+            const int v1 = p < half ? 4 * p : none, v2 = p < half ? 4 * (p + half) : none;
+            x1[NJ][i] = get(nres, v1);
+            x2[NJ][i] = get(nres, v2);
+            qw1[i] = get(qwres, v1);
+            qw2[i] = get(qwres, v2);
+            nw1[i] = get(nwres, v1);
+            nw2[i] = get(nwres, v2);
+            cs[i] = get(cres, v1);
+            sn[i] = get(sres, v1);
         }
+        if (newrow) old_e = (wave ? a.c.vs : a.c.ks)[(size_t)(a.pos0 >> a.block_log2) * hkv + kvh];
+    }
     Tile ta, tb;
     load_tile(tile_of(0), ta);
     load_tile(tile_of(1), tb);
-    __syncthreads();
 
-    // Row jobs: the columns' q, then the new K and V rows. A lane owns the dim pairs (p, p + hd/2),
-    // so that RMSNorm and RoPE never read another lane's dims.
-    {
-        constexpr int NP = (HD / 2 + 63) / 64;
-        const int half = hd / 2;
-        const size_t trow = (size_t)a.pos0 * half;
-        const int njobs = owner ? ncol + 2 : ncol;
-        for (int job = wave; job < njobs; job += kWaves) {
-            float *x = job < ncol ? s_q + job * QS : s_new + (job - ncol) * HD;
-            const float *w = !a.prologue ? nullptr : job < ncol ? a.qn_w : job == ncol ? a.kn_w : a.vn_w;
-            const bool rope = a.prologue && a.rcos && job <= ncol;
-            float x1[NP], x2[NP];
+    // RMSNorm (x * (1 / sqrt(mean x^2 + eps)) * w), then RoPE, of a row's pairs.
+    auto transform = [&](float (&y1)[NP], float (&y2)[NP], bool norm, const float (&w1)[NP], const float (&w2)[NP],
+                         bool rope) {
+        if (norm) {
+            float ss = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NP; ++i) ss += y1[i] * y1[i] + y2[i] * y2[i];
+            ss = eb::class_reduce<1, false>(ss);
+            const float inv = 1.0f / sqrtf(ss / (float)hd + a.eps);
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
-                const int p = lane + 64 * i;
-                x1[i] = p < half ? x[p] : 0.0f;
-                x2[i] = p < half ? x[p + half] : 0.0f;
+                y1[i] = y1[i] * inv * w1[i];
+                y2[i] = y2[i] * inv * w2[i];
             }
-            if (w) {  // x * (1 / sqrt(mean x^2 + eps)) * w
-                float ss = 0.0f;
+        }
+        if (rope) {  // without fused multiply-adds as the row pass
 #pragma unroll
-                for (int i = 0; i < NP; ++i) ss += x1[i] * x1[i] + x2[i] * x2[i];
-                ss = eb::class_reduce<1, false>(ss);
-                const float inv = 1.0f / sqrtf(ss / (float)hd + a.eps);
-#pragma unroll
-                for (int i = 0; i < NP; ++i) {
-                    const int p = lane + 64 * i;
-                    if (p < half) {
-                        x1[i] = x1[i] * inv * w[p];
-                        x2[i] = x2[i] * inv * w[p + half];
-                    }
-                }
+            for (int i = 0; i < NP; ++i) {
+                const float z1 = __fsub_rn(__fmul_rn(y1[i], cs[i]), __fmul_rn(y2[i], sn[i]));
+                y2[i] = __fadd_rn(__fmul_rn(y2[i], cs[i]), __fmul_rn(y1[i], sn[i]));
+                y1[i] = z1;
             }
-            if (rope) {  // pairs (p, p + hd/2), without fused multiply-adds as the row pass
+        }
+    };
+    const bool rope = a.prologue && a.rcos;
 #pragma unroll
-                for (int i = 0; i < NP; ++i) {
-                    const int p = lane + 64 * i;
-                    if (p < half) {
-                        const float cs = a.rcos[trow + p], sn = a.rsin[trow + p];
-                        const float y1 = __fsub_rn(__fmul_rn(x1[i], cs), __fmul_rn(x2[i], sn));
-                        const float y2 = __fadd_rn(__fmul_rn(x2[i], cs), __fmul_rn(x1[i], sn));
-                        x1[i] = y1;
-                        x2[i] = y2;
-                    }
-                }
+    for (int j = 0; j < NJ; ++j) {
+        const int c = j * kWaves + wave;
+        if (c < ncol) {  // (uniform) q * scale * log2(e), then the column's power of two
+            transform(x1[j], x2[j], a.prologue && a.qn_w, qw1, qw2, rope);
+            float top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                x1[j][i] *= a.scale_log2;
+                x2[j][i] *= a.scale_log2;
+                top = fmaxf(top, fmaxf(fabsf(x1[j][i]), fabsf(x2[j][i])));
             }
+            top = eb::class_reduce<1, true>(top);
             int ex = 0;
-            if (job < ncol) {  // q * scale * log2(e), then the column's power of two
-                float top = 0.0f;
-#pragma unroll
-                for (int i = 0; i < NP; ++i) {
-                    x1[i] *= a.scale_log2;
-                    x2[i] *= a.scale_log2;
-                    top = fmaxf(top, fmaxf(fabsf(x1[i]), fabsf(x2[i])));
-                }
-                top = eb::class_reduce<1, true>(top);
-                if (top > 0.0f && top <= 3.0e38f) {
-                    frexpf(top, &ex);
-                    ex = 14 - ex;
-                }
-                if (lane == 0) s_qe[job] = -ex;
+            if (top > 0.0f && top <= 3.0e38f) {
+                frexpf(top, &ex);
+                ex = 14 - ex;
             }
+            if (lane == 0) s_qe[c] = -ex;
+            float *x = s_q + c * QS;
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
                 const int p = lane + 64 * i;
                 if (p < half) {
-                    x[p] = ldexpf(x1[i], ex);
-                    x[p + half] = ldexpf(x2[i], ex);
+                    x[p] = ldexpf(x1[j][i], ex);
+                    x[p + half] = ldexpf(x2[j][i], ex);
                 }
             }
+            for (int p = hd + lane; p < HD; p += 64) x[p] = 0.0f;
         }
     }
-    __syncthreads();
 
     // ---- the append ---------------------------------------------------------------------------
-    if (owner && wave < 2) {  // wave 0: K, wave 1: V
+    if (newrow) {  // wave 0: K, wave 1: V
+        transform(x1[NJ], x2[NJ], a.prologue && nw, nw1, nw2, rope && wave == 0);
         uint8_t *codes = (wave ? a.c.v : a.c.k) + (size_t)kvh * hd;
         uint8_t *exps = wave ? a.c.vs : a.c.ks;
-        const float *x = s_new + wave * HD;
+        float *x = s_new + wave * HD;
         const int b = a.pos0 >> a.block_log2, first = b << a.block_log2, lead = a.pos0 - first;
-        const unsigned old_e = lead ? exps[(size_t)b * hkv + kvh] : 0u;
-        const int d = 4 * lane;
-        f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (d < hd) y = *reinterpret_cast<const f32x4 *>(x + d);
+        if (!lead) old_e = 0;
         unsigned top = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const unsigned u = eb::magnitude_bits(y[i]);
-            top = u > top ? u : top;
+        for (int i = 0; i < NP; ++i) {
+            const int p = lane + 64 * i;
+            if (p < half) {
+                x[p] = x1[NJ][i];
+                x[p + half] = x2[NJ][i];
+            }
+            const unsigned u1 = eb::magnitude_bits(x1[NJ][i]), u2 = eb::magnitude_bits(x2[NJ][i]);
+            top = p < half ? max(top, max(u1, u2)) : top;
         }
 #pragma unroll
-        for (int m = 32; m > 0; m >>= 1) {
-            const unsigned o = __shfl_xor(top, m);
-            top = o > top ? o : top;
-        }
+        for (int m = 32; m > 0; m >>= 1) top = max(top, __shfl_xor(top, m));
         unsigned e = eb::i8_exponent(top);
         if (lead) e = eb::i8_join(old_e, e);
+        const int d = 4 * lane;
         if (d < hd) {
+            const f32x4 y = *reinterpret_cast<const f32x4 *>(x + d);  // (this wave's own row)
             unsigned w = 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i) w |= eb::i8_code(y[i], e) << (8 * i);
             *reinterpret_cast<unsigned *>(codes + (size_t)a.pos0 * row_bytes + d) = w;
+            s_code[wave * (HD / 4) + lane] = w;
         }
         if (lead && e != old_e && e != eb::kNanExponent) {
             const int per_row = hd / 4;
@@ -313,9 +338,39 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i8_kernel(Args a, int hd) 
                 *p = eb::i8_recode(*p, old_e, e);
             }
         }
-        if (lane == 0) exps[(size_t)b * hkv + kvh] = (uint8_t)e;
+        if (lane == 0) {
+            exps[(size_t)b * hkv + kvh] = (uint8_t)e;
+            s_e[2 * wave] = lead ? old_e : e;
+            s_e[2 * wave + 1] = e;
+        }
     }
-    // The block's tiles are loaded below, after a barrier that completes these stores.
+    if (owner) __threadfence_block();
+    __syncthreads();
+    if (owner) {  // (uniform over the workgroup)
+        const unsigned k0 = s_e[0], k1 = s_e[1], v0 = s_e[2], v1 = s_e[3];
+        auto appended = [&](int t, Tile &x) {
+            if (t < a.tail0 || t * kTile >= end) return;
+            if (k0 != k1 || v0 != v1) {
+                load_tile(t, x);
+                return;
+            }
+            const int at = a.pos0 - t * kTile;  // the new row, if in this tile
+#pragma unroll
+            for (int c = 0; c < KL; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (n == at) x.k[c][i] = s_code[16 * c + 4 * g4 + i];
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int i = 0; i < VW; ++i)
+                    if (4 * g4 + r == at) x.v[r][i] = s_code[HD / 4 + VW * n + i];
+            x.ek = k1;
+            x.ev = v1;
+        };
+        appended(tile_of(0), ta);
+        appended(tile_of(1), tb);
+    }
 
     // ---- operands and state -------------------------------------------------------------------
     const int own = min(n, ncol - 1);  // this lane's column (the last one, repeated, past ncol)
@@ -434,22 +489,13 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i8_kernel(Args a, int hd) 
 
     // ---- the tiles, in pairs, each buffer refilled once consumed --------------------------------
     const int mine = a.tiles > split ? (a.tiles - split + a.nsplit - 1) / a.nsplit : 0;
-    const int steps = (mine + kWaves - 1) / kWaves;
+    const int steps = own_steps + (mine + kWaves - 1) / kWaves;
     for (int i = 0; i < steps; i += 2) {
         consume(tile_of(i), ta);
         load_tile(tile_of(i + 2), ta);
         if (i + 1 < steps) consume(tile_of(i + 1), tb);
         load_tile(tile_of(i + 3), tb);
     }
-    if (owner) {  // (uniform over the workgroup)
-        __threadfence_block();
-        __syncthreads();
-        for (int t = wave; t < a.tails; t += kWaves) {
-            load_tile(a.tail0 + t, ta);
-            consume(a.tail0 + t, ta);
-        }
-    }
-
     // ---- the waves' states meet in LDS ----------------------------------------------------------
     l += eb::lane_xor16(l);
     l += eb::lane_xor32(l);
@@ -471,26 +517,28 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i8_kernel(Args a, int hd) 
         }
     }
     __syncthreads();
-    for (int i = tid; i < ncol * hd; i += kThreads) {
-        const int c = i / hd, d = i % hd;
+    for (int i = tid; i < ncol * (HD / 4); i += kThreads) {
+        const int c = i / (HD / 4), d = 4 * (i % (HD / 4));
+        if (d >= hd) continue;
         const f32x4 m4 = *reinterpret_cast<const f32x4 *>(s_m + c * kWaves);
         const f32x4 l4 = *reinterpret_cast<const f32x4 *>(s_l + c * kWaves);
         const float M = fmaxf(fmaxf(m4.x, m4.y), fmaxf(m4.z, m4.w));
         const float mref = M == -INFINITY ? 0.0f : M;
-        float A = 0.0f, L = 0.0f;
+        f32x4 A = {0.0f, 0.0f, 0.0f, 0.0f};
+        float L = 0.0f;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
             const float f = eb::fast_exp2(m4[w] - mref);
-            A += f * smem[(w * ncol + c) * QS + d];
+            A += f * *reinterpret_cast<const f32x4 *>(smem + (w * ncol + c) * QS + d);
             L += f * l4[w];
         }
-        const int cc = col0 + c;
-        const size_t at = (size_t)(cc / a.g) * a.h + kvh * a.g + cc % a.g;
+        const int cc = col0 + c, row = a.rows == 1 ? 0 : cc / a.g;
+        const size_t at = (size_t)row * a.h + kvh * a.g + cc - row * a.g;
         if (a.nsplit == 1) {
-            a.o[at * hd + d] = A / L;
+            *reinterpret_cast<f32x4 *>(a.o + at * hd + d) = A / L;
         } else {
             const size_t slot = (size_t)split * a.rows * a.h + at;
-            a.part_acc[slot * hd + d] = A;
+            *reinterpret_cast<f32x4 *>(a.part_acc + slot * hd + d) = A;
             if (d == 0) {
                 a.part_ml[slot * 2 + 0] = M;
                 a.part_ml[slot * 2 + 1] = L;
@@ -543,7 +591,7 @@ hipError_t launch(hipStream_t st, const Args &a, const Plan &p, size_t hd) {
                                                         hipFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);
         if (e != hipSuccess) return e;
     }
-    decode_i8_kernel<HD><<<dim3((unsigned)(a.c.hkv * p.nsub), (unsigned)p.nsplit), kThreads, lds, st>>>(a, (int)hd);
+    decode_i8_kernel<HD><<<dim3((unsigned)a.c.hkv, (unsigned)p.nsub, (unsigned)p.nsplit), kThreads, lds, st>>>(a, (int)hd);
     return hipSuccess;
 }
 

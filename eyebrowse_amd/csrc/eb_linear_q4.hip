@@ -204,21 +204,22 @@ __global__ __launch_bounds__(kGemvThreads, 4) void q4_gemv_kernel(const float *_
     };
     enter();
     auto load = [&](B &r) {
+        // (whole offsets in the vector operand: the scalar one is outside the range check)
         const int b = __builtin_amdgcn_readfirstlane(b0 + lb);
-        const u32x4 v = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(wres, 16 * lane, kTileBytes * b, 0));
+        const u32x4 v = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(wres, kTileBytes * b + 16 * lane, 0, 0));
 #pragma unroll
         for (int j = 0; j < 4; ++j) r.w[j] = v[j];
         if constexpr (NG == 4) {
-            const u32x2 q = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(sres, 8 * n, 128 * b, 0));
+            const u32x2 q = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(sres, 128 * b + 8 * n, 0, 0));
             r.f.s[0] = q[0];
             r.f.s[1] = q[1];
-            if constexpr (ZERO) r.f.z = __builtin_amdgcn_raw_buffer_load_b32(zres, 4 * n, 64 * b, 0);
+            if constexpr (ZERO) r.f.z = __builtin_amdgcn_raw_buffer_load_b32(zres, 64 * b + 4 * n, 0, 0);
         } else if constexpr (NG == 2) {
-            r.f.s[0] = __builtin_amdgcn_raw_buffer_load_b32(sres, 4 * n, 64 * b, 0);
-            if constexpr (ZERO) r.f.z = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(zres, 2 * n, 32 * b, 0);
+            r.f.s[0] = __builtin_amdgcn_raw_buffer_load_b32(sres, 64 * b + 4 * n, 0, 0);
+            if constexpr (ZERO) r.f.z = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(zres, 32 * b + 2 * n, 0, 0);
         } else {
-            r.f.s[0] = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(sres, 2 * n, 32 * b, 0);
-            if constexpr (ZERO) r.f.z = (unsigned char)__builtin_amdgcn_raw_buffer_load_b8(zres, n, 16 * b, 0);
+            r.f.s[0] = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(sres, 32 * b + 2 * n, 0, 0);
+            if constexpr (ZERO) r.f.z = (unsigned char)__builtin_amdgcn_raw_buffer_load_b8(zres, 16 * b + n, 0, 0);
         }
         if (++lb == per) {
             lb = 0;
