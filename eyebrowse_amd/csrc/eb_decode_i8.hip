@@ -80,7 +80,8 @@ struct Args {
     int pos0;               // position of row 0
     int window;             // 0: none
     int tile0, tiles;       // the tiles dealt to the splits: tile0 .. tile0 + tiles - 1
-    int owner, tail0, tails;  // the append's split and its block's tiles
+    int owner, tails;        // the append's split; its block's tiles, behind the others
+    unsigned g_inv;          // 2^32 / g, rounded up
     int nsplit, block_log2;
     float scale_log2;
     bool prologue;
@@ -129,6 +130,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i8_kernel(Args a, int hd) 
     const int ncol = min(kCols, a.ncols - col0);
     const int split = blockIdx.z;
     const bool owner = a.knew != nullptr && split == a.owner;
+    auto row_of = [&](int cc) { return a.g == 1 ? cc : (int)__umulhi((unsigned)cc, a.g_inv); };  // cc / g
     const int lds_rows = max(kCols, kWaves * ncol);
     float *s_q = smem;
     float *s_new = smem + lds_rows * QS;
@@ -181,13 +183,20 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i8_kernel(Args a, int hd) 
         x.ek = a.c.ks[b];
         x.ev = a.c.vs[b];
     };
-    // Local tile i of this wave (all waves and splits together walk one stretch of the cache); the
-    // owner's first ones are the new token's block.
-    const int own_steps = owner ? (a.tails + kWaves - 1) / kWaves : 0;
-    auto tile_of = [&](int i) {
-        const int w = i * kWaves + wave, t = (w - own_steps * kWaves) * a.nsplit + split;
-        const bool tail = i < own_steps;
-        return (tail ? w < a.tails : t < a.tiles) ? (tail ? a.tail0 + w : a.tile0 + t) : INT_MAX / kTile;
+    // This wave's tiles (all waves and splits together walk one stretch of the cache). The owner's
+    // first ones are the new token's block, right behind that stretch.
+    const int stretch = a.tile0 + a.tiles, stride = kWaves * a.nsplit;
+    const int first_tile = a.tile0 + wave * a.nsplit + split;
+    bool in_tail = owner && wave < a.tails;
+    int next = in_tail ? stretch + wave : first_tile;
+    // The next tile, or one past the last key; then one further.
+    auto advance = [&] {
+        const int t = in_tail || next < stretch ? next : INT_MAX / kTile;
+        const int up = next + (in_tail ? kWaves : stride);
+        const bool back = in_tail && up >= stretch + a.tails;
+        next = back ? first_tile : min(up, INT_MAX / kTile);
+        in_tail = in_tail && !back;
+        return t;
     };
 
     // ---- every first load at once: q, the new rows, what transforms them, two tiles ------------
@@ -218,8 +227,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i8_kernel(Args a, int hd) 
             const int p = lane + 64 * i;
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
-                const int cc = col0 + j * kWaves + wave;
-                const int row = a.rows == 1 ? 0 : cc / a.g;
+                const int cc = col0 + j * kWaves + wave, row = row_of(cc);
                 const int at = (row * a.h + kvh * a.g + cc - row * a.g) * hd * 4;
                 const bool have = j * kWaves + wave < ncol && p < half;
                 x1[j][i] = get(qres, have ? at + 4 * p : none);
@@ -235,11 +243,12 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i8_kernel(Args a, int hd) 
             cs[i] = get(cres, v1);
             sn[i] = get(sres, v1);
         }
-        if (newrow) old_e = (wave ? a.c.vs : a.c.ks)[(size_t)(a.pos0 >> a.block_log2) * hkv + kvh];
+        old_e = (wave ? a.c.vs : a.c.ks)[(size_t)(a.pos0 >> a.block_log2) * hkv + kvh];
     }
     Tile ta, tb;
-    load_tile(tile_of(0), ta);
-    load_tile(tile_of(1), tb);
+    int na = advance(), nb = advance();
+    load_tile(na, ta);
+    load_tile(nb, tb);
 
     // RMSNorm (x * (1 / sqrt(mean x^2 + eps)) * w), then RoPE, of a row's pairs.
     auto transform = [&](float (&y1)[NP], float (&y2)[NP], bool norm, const float (&w1)[NP], const float (&w2)[NP],
@@ -349,7 +358,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i8_kernel(Args a, int hd) 
     if (owner) {  // (uniform over the workgroup)
         const unsigned k0 = s_e[0], k1 = s_e[1], v0 = s_e[2], v1 = s_e[3];
         auto appended = [&](int t, Tile &x) {
-            if (t < a.tail0 || t * kTile >= end) return;
+            if (t < stretch || t >= stretch + a.tails) return;
             if (k0 != k1 || v0 != v1) {
                 load_tile(t, x);
                 return;
@@ -368,8 +377,8 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i8_kernel(Args a, int hd) 
             x.ek = k1;
             x.ev = v1;
         };
-        appended(tile_of(0), ta);
-        appended(tile_of(1), tb);
+        appended(na, ta);
+        appended(nb, tb);
     }
 
     // ---- operands and state -------------------------------------------------------------------
@@ -389,7 +398,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i8_kernel(Args a, int hd) 
             ql[c][j] = (_Float16)(v - (float)hi);
         }
     }
-    const int my_pos = a.pos0 + (col0 + own) / a.g;  // the column's last key
+    const int my_pos = a.pos0 + row_of(col0 + own);  // the column's last key
     const int my_first = a.window > 0 ? my_pos - a.window + 1 : 0;  // and its first
     // Tiles wholly inside every column's keys need no mask.
     const int safe_lo = a.window > 0 ? end - a.window : 0, safe_hi = a.pos0;
@@ -489,13 +498,16 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i8_kernel(Args a, int hd) 
 
     // ---- the tiles, in pairs, each buffer refilled once consumed --------------------------------
     const int mine = a.tiles > split ? (a.tiles - split + a.nsplit - 1) / a.nsplit : 0;
-    const int steps = own_steps + (mine + kWaves - 1) / kWaves;
+    const int steps = (mine + kWaves - 1) / kWaves + (owner ? (a.tails + kWaves - 1) / kWaves : 0);
     for (int i = 0; i < steps; i += 2) {
-        consume(tile_of(i), ta);
-        load_tile(tile_of(i + 2), ta);
-        if (i + 1 < steps) consume(tile_of(i + 1), tb);
-        load_tile(tile_of(i + 3), tb);
+        consume(na, ta);
+        na = advance();
+        load_tile(na, ta);
+        if (i + 1 < steps) consume(nb, tb);
+        nb = advance();
+        load_tile(nb, tb);
     }
+
     // ---- the waves' states meet in LDS ----------------------------------------------------------
     l += eb::lane_xor16(l);
     l += eb::lane_xor32(l);
@@ -532,7 +544,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i8_kernel(Args a, int hd) 
             A += f * *reinterpret_cast<const f32x4 *>(smem + (w * ncol + c) * QS + d);
             L += f * l4[w];
         }
-        const int cc = col0 + c, row = a.rows == 1 ? 0 : cc / a.g;
+        const int cc = col0 + c, row = row_of(cc);
         const size_t at = (size_t)row * a.h + kvh * a.g + cc - row * a.g;
         if (a.nsplit == 1) {
             *reinterpret_cast<f32x4 *>(a.o + at * hd + d) = A / L;
@@ -548,7 +560,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i8_kernel(Args a, int hd) 
 }
 
 struct Plan {
-    int nsub, nsplit, tile0, tiles, tail0, tails;
+    int nsub, nsplit, tile0, tiles, tails;
     bool fused;
 };
 
@@ -569,7 +581,6 @@ Plan plan_of(size_t h, size_t hkv, size_t pos0, size_t rows, size_t block, size_
     p.tile0 = (int)(first / kTile);
     if (p.fused) {
         const size_t b0 = std::max(pos0 / block * block / kTile, (size_t)p.tile0);
-        p.tail0 = (int)b0;
         p.tails = (int)(stop - b0);
         stop = b0;
     }
@@ -615,6 +626,9 @@ eb_status launch_attn_decode_i8(hipStream_t st, const float *q, const CacheI8 &c
                                 const float *vnew, float *o, size_t h, size_t pos0, size_t rows, float scale,
                                 size_t window, float *ws, size_t ws_floats, int cu_count,
                                 const DecodePrologue *pro) {
+    // (q's offsets are 32-bit; the division by g is a multiplication that is exact to 65535)
+    if (rows * h * c.hd >= (size_t)1 << 29 || rows * (h / c.hkv) > 65535)
+        return fail(EB_UNSUPPORTED_CONFIG, "attn_decode_i8: %zu rows of %zu heads of %zu", rows, h, c.hd);
     const Plan p = plan_of(h, c.hkv, pos0, rows, c.block, window, knew != nullptr, cu_count);
     if (knew && !p.fused) {
         if (pro) return fail(EB_OTHER, "attn_decode_i8: more than %d heads per KV head need the row pass", kCols);
@@ -634,6 +648,7 @@ eb_status launch_attn_decode_i8(hipStream_t st, const float *q, const CacheI8 &c
     a.part_ml = ws ? ws + (size_t)p.nsplit * rows * h * c.hd : nullptr;
     a.h = (int)h;
     a.g = (int)(h / c.hkv);
+    a.g_inv = (unsigned)((((uint64_t)1 << 32) + a.g - 1) / a.g);
     a.rows = (int)rows;
     a.ncols = (int)(rows * (h / c.hkv));
     a.pos0 = (int)pos0;
@@ -641,7 +656,6 @@ eb_status launch_attn_decode_i8(hipStream_t st, const float *q, const CacheI8 &c
     a.tile0 = p.tile0;
     a.tiles = p.tiles;
     a.owner = p.tiles % p.nsplit;  // (the first split that has one tile less, if any)
-    a.tail0 = p.tail0;
     a.tails = p.tails;
     a.nsplit = p.nsplit;
     while ((size_t)1 << a.block_log2 < c.block) ++a.block_log2;
