@@ -117,8 +117,12 @@ eb_status move_i8(hipStream_t st, const char *what, const eb::CacheI8 &c, const 
 }
 
 // Rows whose columns (rows x heads of a KV head) number at most this many run the few-row kernel,
-// which reads the cache once for 16 of them; more rows run the prefill kernels over records.
-constexpr size_t kFewRowCols = 64;
+// which reads the cache once for every 16 of them; more rows run the prefill kernels over records.
+// Both measured, few-row and prefill, at 32 heads over 8 KV heads of 128 (4 columns a row): 16 rows
+// behind 1000 keys 14.7 and 20.3 us, 48 rows 22.5 and 28.6; behind 8192 keys 20 rows 26.7 and 46.2,
+// 48 rows 46.8 and 52.7, 64 rows 57.2 and 56.5; behind 32000 keys 48 rows 130 and 144. 16 over 8
+// heads of 256, 8192 keys: 64 rows (128 columns) 56.1 and 74.7.
+constexpr size_t kFewRowCols = 192;
 
 size_t attn_workspace(size_t h, size_t hkv, size_t hd, size_t pos0, size_t rows, size_t window, size_t block, int cus) {
     if (rows * (h / hkv) <= kFewRowCols) return eb::decode_i8_workspace_floats(h, hkv, pos0, rows, hd, block, cus);
