@@ -456,7 +456,7 @@ constexpr int kTileThreads = 512;
 template <int G, bool ZERO>
 __global__ __launch_bounds__(kTileThreads, 2) void q4_tile_kernel(const f16x8 *__restrict__ hi, const f16x8 *__restrict__ lo,
                                                                   const float *__restrict__ ex, Segs segs, int M, int K,
-                                                                  int KC) {
+                                                                  int KC, float *__restrict__ parts) {
     constexpr int NG = kBlock / G;
     constexpr int CH = 16 * kTileRows;  // chunks of a stage's plane: [row block][chunk][row]
     extern __shared__ f16x8 lds[];      // [2][hi CH, lo CH]
@@ -469,6 +469,7 @@ __global__ __launch_bounds__(kTileThreads, 2) void q4_tile_kernel(const f16x8 *_
     const int m0 = mt * kTileRows, n0 = (u - sg.first) * kTileCols + wn * 64;
     const int nb = (K + kBlock - 1) / kBlock;
     const int last = (sg.n + kFeatures - 1) / kFeatures - 1;
+    const int st0 = (int)((long long)nb * blockIdx.y / gridDim.y), st1 = (int)((long long)nb * (blockIdx.y + 1) / gridDim.y);
 
     // This wave's copies: plane wave / 4, row block wave % 4, 8 KiB a stage.
     const f16x8 *src = (wave < 4 ? hi : lo) + (size_t)(m0 / 32 + wave % 4) * KC * 32 + lane;
@@ -558,73 +559,102 @@ __global__ __launch_bounds__(kTileThreads, 2) void q4_tile_kernel(const f16x8 *_
         }
     };
     Half wa[2], wb[2];
-    copy_stage(0);
-    load_w(0, wa);
+    copy_stage(st0);
+    load_w(st0, wa);
     auto stage = [&](int st, Half (&now)[2], Half (&next)[2]) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         arrived(now);
         __syncthreads();  // stage st is there, and nobody reads the other buffer any more
-        if (st + 1 < nb) {
+        if (st + 1 < st1) {
             copy_stage(st + 1);
             load_w(st + 1, next);
         }
         __builtin_amdgcn_sched_barrier(0);
         compute(st & 1, now);
     };
-    for (int st = 0; st < nb; st += 2) {
+    for (int st = st0; st < st1; st += 2) {
         stage(st, wa, wb);
-        if (st + 1 < nb) stage(st + 1, wb, wa);
+        if (st + 1 < st1) stage(st + 1, wb, wa);
     }
-    // The second set's sums through LDS.
+    // The sets' sums meet in LDS: each takes one of the two blocks of 32 rows.
     float *part = reinterpret_cast<float *>(lds);
     __syncthreads();
-    if (q == 1)
 #pragma unroll
-        for (int a = 0; a < 2; ++a)
+    for (int b = 0; b < 2; ++b) {
+        const floatx16 give = q ? acc[0][b] : acc[1][b];
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) part[(((wave & 3) * 4 + a * 2 + b) * 16 + r) * 64 + lane] = acc[a][b][r];
+        for (int r = 0; r < 16; ++r) part[((wave * 2 + b) * 16 + r) * 64 + lane] = give[r];
+    }
     __syncthreads();
-    if (q == 1) return;
     // Lane (n, h) holds feature n, rows 8 (r / 4) + 4 h + r % 4 of each block.
+    const int mr = (wm * 2 + q) * 32;
 #pragma unroll
-    for (int a = 0; a < 2; ++a)
+    for (int b = 0; b < 2; ++b) {
+        const floatx16 keep = q ? acc[1][b] : acc[0][b];
+        const int o = n0 + 32 * b + n;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            const int row = m0 + (wm * 2 + a) * 32 + 8 * (r >> 2) + 4 * h + (r & 3);
+            const int at = mr + 8 * (r >> 2) + 4 * h + (r & 3), row = m0 + at;
+            const float v = keep[r] + part[(((wave ^ 4) * 2 + b) * 16 + r) * 64 + lane];
             if (row >= M) continue;
-            const int e = (int)ex[row];
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const int o = n0 + 32 * b + n;
-                const float v = acc[a][b][r] + part[((wave * 4 + a * 2 + b) * 16 + r) * 64 + lane];
-                if (o < sg.n) sg.y[(size_t)row * sg.n + o] = ldexpf(v, e);
-            }
+            if (gridDim.y > 1)
+                parts[((size_t)blockIdx.y * gridDim.x + blockIdx.x) * kTileRows * kTileCols + at * kTileCols + wn * 64 +
+                      32 * b + n] = v;
+            else if (o < sg.n)
+                sg.y[(size_t)row * sg.n + o] = ldexpf(v, (int)ex[row]);
         }
+    }
 }
 
-// Fewer rows than fill the card with such tiles: 32 MB rows x 32 features a workgroup, its eight
-// waves sharing the contraction (wave w blocks w, w + 8, ...); x's halves come from L2 straight into
-// the products' registers, and the waves' sums meet in LDS.
+// The sums of a contraction that several workgroups shared, in their order. A workgroup takes eight
+// rows of a tile, a thread four features of one; up to kJoinBatch shares' sums are in flight.
+constexpr int kJoinRows = 8, kJoinThreads = 256, kJoinBatch = 8;
+__global__ __launch_bounds__(kJoinThreads) void q4_join_kernel(const float *__restrict__ parts,
+                                                               const float *__restrict__ ex, Segs segs, int M, int tiles,
+                                                               int shares) {
+    const int t = blockIdx.x, mt = t / segs.total, u = t % segs.total;
+    const Seg sg = seg_at(segs, u);
+    const int at = (int)blockIdx.y * kJoinRows + threadIdx.x / 32, row = mt * kTileRows + at;
+    const int col = 4 * (threadIdx.x % 32), o = (u - sg.first) * kTileCols + col;
+    if (row >= M || o >= sg.n) return;
+    const float *p = parts + (size_t)t * kTileRows * kTileCols + at * kTileCols + col;
+    const size_t step = (size_t)tiles * kTileRows * kTileCols;
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = 0; s < shares; s += kJoinBatch) {
+        f32x4 v[kJoinBatch];
+#pragma unroll
+        for (int i = 0; i < kJoinBatch; ++i)
+            v[i] = *reinterpret_cast<const f32x4 *>(p + (size_t)min(s + i, shares - 1) * step);
+#pragma unroll
+        for (int i = 0; i < kJoinBatch; ++i)
+            if (s + i < shares) sum += v[i];
+    }
+    const int e = (int)ex[row];
+    float *y = sg.y + (size_t)row * sg.n + o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (o + i < sg.n) y[i] = ldexpf(sum[i], e);
+}
+
+// Up to 32 rows: a workgroup takes them all and 32 features, its eight waves sharing the contraction
+// (wave w blocks w, w + 8, ...); x's halves come from L2 straight into the products' registers, and
+// the waves' sums meet in LDS.
 constexpr int kSlimWaves = 8;
-template <int G, bool ZERO, int MB>
+template <int G, bool ZERO>
 __global__ __launch_bounds__(kSlimWaves * 64, 2) void q4_slim_kernel(const f16x8 *__restrict__ hi,
                                                                      const f16x8 *__restrict__ lo,
-                                                                     const float *__restrict__ ex, Segs segs, int M, int K,
-                                                                     int KC) {
+                                                                     const float *__restrict__ ex, Segs segs, int M, int K) {
     constexpr int NG = kBlock / G;
-    __shared__ float part[kSlimWaves][MB * 16][64];
+    __shared__ float part[kSlimWaves][16][64];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = lane >> 5;
-    const int mt = blockIdx.x / segs.total, u = blockIdx.x % segs.total;
-    const Seg sg = seg_at(segs, u);
-    const int m0 = mt * 32 * MB, n0 = (u - sg.first) * 32;
+    const Seg sg = seg_at(segs, (int)blockIdx.x);
+    const int n0 = ((int)blockIdx.x - sg.first) * 32;
     const int nb = (K + kBlock - 1) / kBlock;
     const int last = (sg.n + kFeatures - 1) / kFeatures - 1;
     const int tile = min((n0 + n) / kFeatures, last);
-    floatx16 acc[MB] = {};
+    floatx16 acc = {};
     Wide<NG> r;
     if (wave < nb) load_wide<NG, ZERO>(r, sg, tile, wave, nb, n, h);
     for (int b = wave; b < nb; b += kSlimWaves) {
@@ -633,36 +663,30 @@ __global__ __launch_bounds__(kSlimWaves * 64, 2) void q4_slim_kernel(const f16x8
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
             const Zero z = zero_of(ZERO ? r.f.z : 0x08080808u, i);
-            floatx16 t[MB] = {};
+            floatx16 t = {};
 #pragma unroll
             for (int j = i * (4 / NG); j < (i + 1) * (4 / NG); ++j)
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
                     const f16x8 w = unpack(r.w[q][j], z);
-#pragma unroll
-                    for (int a = 0; a < MB; ++a) {
-                        const size_t at = ((size_t)(m0 / 32 + a) * KC + b * 16 + 4 * j + 2 * q + h) * 32 + n;
-                        t[a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi[at], w, t[a], 0, 0, 0);
-                        t[a] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lo[at], w, t[a], 0, 0, 0);
-                    }
+                    const int at = (b * 16 + 4 * j + 2 * q + h) * 32 + n;
+                    t = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi[at], w, t, 0, 0, 0);
+                    t = __builtin_amdgcn_mfma_f32_32x32x16_f16(lo[at], w, t, 0, 0, 0);
                 }
-#pragma unroll
-            for (int a = 0; a < MB; ++a) acc[a] += t[a] * r.f.scale(i);
+            acc += t * r.f.scale(i);
         }
         r = next;
     }
 #pragma unroll
-    for (int a = 0; a < MB; ++a)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) part[wave][a * 16 + i][lane] = acc[a][i];
+    for (int i = 0; i < 16; ++i) part[wave][i][lane] = acc[i];
     __syncthreads();
-    // Lane (n, h): feature n, rows 8 (i / 4) + 4 h + i % 4 of block a; wave w takes i = w, w + 8, ...
+    // Lane (n, h): feature n, rows 8 (i / 4) + 4 h + i % 4; wave w takes i = w, w + 8.
 #pragma unroll
-    for (int v = wave; v < MB * 16; v += kSlimWaves) {
-        const int i = v % 16, row = m0 + v / 16 * 32 + 8 * (i >> 2) + 4 * h + (i & 3), o = n0 + n;
+    for (int i = wave; i < 16; i += kSlimWaves) {
+        const int row = 8 * (i >> 2) + 4 * h + (i & 3), o = n0 + n;
         float t = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kSlimWaves; ++w) t += part[w][v][lane];
+        for (int w = 0; w < kSlimWaves; ++w) t += part[w][i][lane];
         if (row < M && o < sg.n) sg.y[(size_t)row * sg.n + o] = ldexpf(t, (int)ex[row]);
     }
 }
@@ -677,6 +701,16 @@ bool gemv(size_t m, size_t K) { return m <= kGemvRows && gemv_lds(m, K) <= kGemv
 
 size_t round_up(size_t x, size_t to) { return (x + to - 1) / to * to; }
 constexpr size_t kRowPad = 128;
+
+// Where the tiles are fewer than the CUs, workgroups share a tile's contraction, as many as the CUs
+// hold (one each, by its LDS), of at least kMinStages blocks of 128; kMaxParts bounds their sums.
+// 4096 to 4096 features: 500 rows (128 tiles) 64 us whole, 32 + 5 in two shares; 128 rows (32 tiles)
+// 17.5 + 4.7 in eight.
+constexpr int kMaxParts = 256, kMinStages = 2;
+// Up to this many rows the slim kernel: 16 rows of 4096 to 4096 features 9.1 us, against 17.5 + 4.7
+// in shared tiles; to 14336 features 15.2 against 36.7 + 5. With two blocks of rows (64) it took
+// 21.9 and 38.8, as the tiles do, and 60 for 200 rows of group 64 against 27.
+constexpr int kSlimRows = 32;
 
 int number(Segs &s, int per) {
     int t = 0;
@@ -708,20 +742,23 @@ hipError_t launch(hipStream_t st, const float *x, Segs s, int m, int K, float *w
     f16x8 *hi = reinterpret_cast<f16x8 *>(ws + mp), *lo = hi + mp * kp / 8;
     const int KC = (int)(kp / 8);
     q4_split_kernel<<<(unsigned)(mp / 8), kSplitThreads, 0, st>>>(x, ws, hi, lo, m, K, KC);
-    const int tiles = (m + kTileRows - 1) / kTileRows * number(s, kTileCols);
-    if (tiles >= cus / 2) {
+    if (m > kSlimRows) {
         constexpr size_t lds = 2 * 2 * 16 * kTileRows * 16;
         static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&q4_tile_kernel<G, ZERO>),
                                                         hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return e;
-        q4_tile_kernel<G, ZERO><<<(unsigned)tiles, kTileThreads, lds, st>>>(hi, lo, ws, s, m, K, KC);
+        const int tiles = (m + kTileRows - 1) / kTileRows * number(s, kTileCols);
+        const int shares = std::max(1, std::min(std::min(cus, kMaxParts) / tiles, KC / 16 / kMinStages));
+        float *parts = ws + mp * (1 + kp);
+        q4_tile_kernel<G, ZERO><<<dim3((unsigned)tiles, (unsigned)shares), kTileThreads, lds, st>>>(hi, lo, ws, s, m, K, KC,
+                                                                                                   parts);
+        if (shares > 1)
+            q4_join_kernel<<<dim3((unsigned)tiles, (std::min(m, kTileRows) + kJoinRows - 1) / kJoinRows), kJoinThreads, 0, st>>>(
+                parts, ws, s, m, tiles, shares);
         return hipSuccess;
     }
     number(s, 32);
-    if (m <= 32)
-        q4_slim_kernel<G, ZERO, 1><<<(unsigned)s.total, kSlimWaves * 64, 0, st>>>(hi, lo, ws, s, m, K, KC);
-    else
-        q4_slim_kernel<G, ZERO, 2><<<(unsigned)((m + 63) / 64 * s.total), kSlimWaves * 64, 0, st>>>(hi, lo, ws, s, m, K, KC);
+    q4_slim_kernel<G, ZERO><<<(unsigned)s.total, kSlimWaves * 64, 0, st>>>(hi, lo, ws, s, m, K);
     return hipSuccess;
 }
 
@@ -731,7 +768,8 @@ namespace eb {
 
 size_t linear_q4_workspace_floats(size_t m, size_t in_f) {
     if (m == 0 || in_f == 0 || gemv(m, in_f)) return 0;
-    return round_up(m, kRowPad) * (1 + round_up(in_f, kBlock));
+    const size_t parts = m > kSlimRows ? (size_t)kMaxParts * kTileRows * kTileCols : 0;
+    return round_up(m, kRowPad) * (1 + round_up(in_f, kBlock)) + parts;
 }
 
 // Planes: codes | scales | zero points; each a whole number of 16 bytes.

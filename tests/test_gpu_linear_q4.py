@@ -63,6 +63,21 @@ def test_large(dev, m, in_f, out_f):
     close(run(dev, a, device_weight(dev, codes, scales, z, 64)), want, bound, "large")
 
 
+@pytest.mark.parametrize("m,in_f,out_f,group", [(33, 8320, 130, 32), (40, 512, 128, 128), (128, 4128, 64, 32),
+                                                (129, 4096, 1000, 64), (257, 384, 5, 128), (200, 2112, 4096, 64)])
+def test_shared_contraction(dev, m, in_f, out_f, group):
+    """Few tiles of a long contraction: workgroups share it; the same bits every time."""
+    note(f"q4 {m} rows {in_f} to {out_f} group {group}")
+    rng = np.random.default_rng(in_f + m)
+    codes, scales, z = weight(rng, out_f, in_f, group, m % 2 == 0)
+    a = rng.standard_normal((m, in_f)).astype(np.float32)
+    want, bound = linear_q4_bound(a, codes, scales, z, group)
+    w = device_weight(dev, codes, scales, z, group)
+    got = run(dev, a, w)
+    close(got, want, bound, "shared")
+    assert run(dev, a, w).tobytes() == got.tobytes()
+
+
 @pytest.mark.parametrize("m", [1, 20, 100])
 def test_extreme_rows(dev, m):
     """Rows of zeros, of tiny and of huge values beside ordinary ones; a zero point above 15."""
