@@ -454,13 +454,22 @@ eb_status eb_q4_pack(eb_recorder *rec, const eb_tensor *w, const eb_tensor *scal
     EB_TRY(eb::check_tensor(scales, EB_F16, "scales", dev));
     if (zeros) EB_TRY(eb::check_tensor(zeros, EB_U8, "zeros", dev));
     EB_TRY(q4_shape(in_f, out_f, group));
+    // Like a tensor's write, complete when it returns, and ordered behind every stream: a weight is
+    // often filled by another library's stream, and its buffers are reused as soon as it is packed.
+    const hipStream_t st = stream_of(dev);
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    EB_HIP_TRY(hipStreamIsCapturing(st, &capture));
+    if (capture != hipStreamCaptureStatusNone)
+        return fail(EB_OTHER, "q4_pack: not allowed while the device's stream is being captured");
+    EB_HIP_TRY(hipDeviceSynchronize());
     const size_t bytes = eb::q4_packed_bytes(in_f, out_f, group, zeros != nullptr);
     eb_tensor *t = nullptr;
     EB_TRY(eb_tensor_empty(dev, &bytes, 1, EB_U8, &t));
     Owned p(t);
-    EB_TRY(pack_checked(stream_of(dev), data<uint32_t>(w), eb_tensor_numel(w), data<uint16_t>(scales),
+    EB_TRY(pack_checked(st, data<uint32_t>(w), eb_tensor_numel(w), data<uint16_t>(scales),
                         eb_tensor_numel(scales), zeros ? data<uint8_t>(zeros) : nullptr, zeros ? eb_tensor_numel(zeros) : 0,
                         in_f, out_f, group, data<void>(p.t), bytes));
+    EB_HIP_TRY(hipStreamSynchronize(st));
     *packed = p.release();
     return eb::ok();
 }

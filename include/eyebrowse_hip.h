@@ -579,7 +579,9 @@ eb_status eb_attention_forward(const eb_attention *attn, eb_recorder *rec, const
  * per u32 word along k, lowest bits first (EB_U32 [out_f, in_f / 8]), scales is EB_F16 [out_f,
  * in_f / group], zeros EB_U8 of that shape, or NULL: 8 everywhere (symmetric codes). group is
  * 32, 64 or 128 and divides in_f; out_f is any size. *packed is a new EB_U8 tensor of
- * eb_q4_packed_bytes bytes (about what w, scales and zeros hold, which are no longer needed). */
+ * eb_q4_packed_bytes bytes (about what w, scales and zeros hold, which are no longer needed). A
+ * set-up call, as eb_tensor_write: it waits for all earlier work on the device, its own included,
+ * and is refused during a capture. */
 typedef struct eb_q4_weight {
     const eb_tensor *packed;
     size_t in_f, out_f, group;
