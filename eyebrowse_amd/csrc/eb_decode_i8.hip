@@ -28,6 +28,12 @@
 //    nor the small ones' precision where the large ones have no weight.
 // The products sum in f32; the f16 pairs keep 22 bits of q and of the weights.
 //
+// Bound by HBM in long caches (32 heads over 8 of 128, 131071 keys: 49.5 us with the merge, 5.4
+// TB/s), by the instructions of a tile (about 220 a wave for 16 keys) beside the ramp below: 32767
+// keys 21.4, 8191 keys (16 heads) 13.1, 1000 keys 9.5; 100 keys, one launch on 8 workgroups, 6.8: a
+// chain of q, scores, softmax and output. So every first load is issued before the first wait.
+// Sixteen columns read the cache once: 4 rows at 8192 keys 15.0 us, 16 rows (64 columns) 23.2.
+//
 // Fused append (one row): the split with the fewest tiles owns the token's block; no other split
 // reads it. Its waves take the block's tiles first, loaded with q as any first tile. The workgroup
 // then normalises and rotates the new K and V rows and writes their codes, and the tile that holds
@@ -564,7 +570,8 @@ struct Plan {
     bool fused;
 };
 
-// Splits: enough workgroups for two on every CU, each wave with at least one tile; fewer than
+// Splits: enough workgroups for two on every CU (32767 keys 21.1 us; for three 22.0, for four 25.3:
+// a later workgroup's ramp), each wave with at least one tile; fewer than
 // kMinSplitKeys keys stay in one workgroup (a second launch costs more than the split saves).
 constexpr size_t kMinSplitKeys = 128;
 constexpr int kWgsPerCu = 2;

@@ -155,6 +155,10 @@ __global__ __launch_bounds__(kPackThreads) void q4_pack_kernel(const uint32_t *_
 // A wave takes tiles: B of v_mfma_f32_16x16x32_f16 is the 16 features' codes, A the x rows, hi halves
 // in rows 0..7 and lo halves in rows 8..15, so that one product serves both. The rows' halves stay in
 // LDS; a workgroup splits them once and then walks its tiles; kw waves share a tile's contraction.
+// Bound by HBM past some 30 MB of weights, by the ramp (x's halves, the first loads) below: 131072
+// features of 4096, group 128, 51 us (5.5 TB/s of weights); 151936 of 1024, group 32 with zero points,
+// 21.3 (4.4); 14336 of 4096 11.1; 14335 of 4096, three rows, group 64 with zero points, 13.3; 4096 of
+// 4096 5.9; 2048 of 1024 4.9.
 constexpr int kGemvWaves = 8;
 constexpr int kGemvThreads = kGemvWaves * 64;
 constexpr int kDepth = 4;  // blocks of weights in flight per wave
@@ -348,10 +352,10 @@ __global__ __launch_bounds__(kGemvThreads, 4) void q4_gemv_kernel(const float *_
 // The rows are split once into the workspace, as operands: hi halves of 32-row block b, chunk c
 // (8 of the contraction, in a word's order) and row r at chunk (b * KC + c) * 32 + r, the lo
 // halves a plane on; rows past M and the contraction past K are zeros.
-constexpr int kThreads = 256;
 
 // 8 rows a workgroup, 128 threads each; a thread's first kSplitKept chunks stay in registers
-// between the row's exponent and its halves (4096 of the contraction).
+// between the row's exponent and its halves (4096 of the contraction). 1000 rows of 4096: 10 us, 33
+// MB read and written; of few rows 8, the chain of a workgroup's loads.
 constexpr int kSplitThreads = 1024, kSplitKept = 4;
 __global__ __launch_bounds__(kSplitThreads) void q4_split_kernel(const float *__restrict__ x, float *__restrict__ ex,
                                                                  f16x8 *__restrict__ hi, f16x8 *__restrict__ lo, int M,
@@ -438,9 +442,9 @@ __device__ __forceinline__ void copy_4kib(unsigned dst, const void *src) {
     asm volatile(
         "s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\t"
         "global_load_lds_dwordx4 %1, off offset:1024\n\tglobal_load_lds_dwordx4 %1, off offset:2048\n\t"
-        "global_load_lds_dwordx4 %1, off offset:3072"
+        "global_load_lds_dwordx4 %1, off offset:%2"
         :
-        : "s"(dst), "v"(src)
+        : "s"(dst), "v"(src), "n"(3 * 1024)
         : "memory", "m0");
 }
 
@@ -451,6 +455,8 @@ __device__ __forceinline__ void copy_4kib(unsigned dst, const void *src) {
 // (64 KiB; a wave copies one plane of one 32-row block), and the weights loaded a stage ahead. All
 // of a stage's loads are waited for at its start; the empty asm on the weights there keeps the
 // compiler from waiting for them, and with them for the next stage's copies, at their first use.
+// Bound by the products: 1000 rows of 4096 to 4096 features, group 128, 70 to 76 us for 67 GFLOP of
+// halves (880 to 960 TFLOP/s; a library's f16 product of 8192^3 reaches 1134 here).
 constexpr int kTileRows = 128, kTileCols = 128;
 constexpr int kTileThreads = 512;
 template <int G, bool ZERO>
@@ -607,7 +613,8 @@ __global__ __launch_bounds__(kTileThreads, 2) void q4_tile_kernel(const f16x8 *_
 }
 
 // The sums of a contraction that several workgroups shared, in their order. A workgroup takes eight
-// rows of a tile, a thread four features of one; up to kJoinBatch shares' sums are in flight.
+// rows of a tile, a thread four features of one; up to kJoinBatch shares' sums are in flight: 4.7 us
+// for eight shares of 128 x 4096 (17.5 with a load, and a wait, a share at a time).
 constexpr int kJoinRows = 8, kJoinThreads = 256, kJoinBatch = 8;
 __global__ __launch_bounds__(kJoinThreads) void q4_join_kernel(const float *__restrict__ parts,
                                                                const float *__restrict__ ex, Segs segs, int M, int tiles,
@@ -709,7 +716,7 @@ constexpr size_t kRowPad = 128;
 constexpr int kMaxParts = 256, kMinStages = 2;
 // Up to this many rows the slim kernel: 16 rows of 4096 to 4096 features 9.1 us, against 17.5 + 4.7
 // in shared tiles; to 14336 features 15.2 against 36.7 + 5. With two blocks of rows (64) it took
-// 21.9 and 38.8, as the tiles do, and 60 for 200 rows of group 64 against 27.
+// 21.9 and 38.8, as the tiles do, and 200 rows of group 64 60 (the whole call 71, 41 in tiles).
 constexpr int kSlimRows = 32;
 
 int number(Segs &s, int per) {

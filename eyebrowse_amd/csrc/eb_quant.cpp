@@ -218,6 +218,9 @@ eb_status eb::attention_forward_i8(const eb_attention_desc &d, eb_recorder *rec,
     EB_TRY(check_tensor(v, EB_F32, "v", dev));
     CacheI8 c;
     EB_TRY(layer_of(kv, layer, dev, &c));
+    if (c.hkv != d.n_kv_heads || c.hd != d.head_dim)
+        return fail(EB_SHAPE_MISMATCH, "attention_forward: the block-scaled cache has %zu heads of %zu, not %zu of %zu",
+                    c.hkv, c.hd, d.n_kv_heads, d.head_dim);
     const size_t H = d.n_heads, hd = d.head_dim, g = H / c.hkv;
     DecodePrologue pro{};
     EB_TRY(prologue_of(d, rope, base_pos + rows - 1, dev, &pro));

@@ -15,12 +15,16 @@
 //  3. collect: every slice finds from the histogram the steps that can hold the cut, lists its
 //     tokens of those steps, and sums the kept weights of the steps above them;
 //  4. choose: one workgroup per row sorts the listed tokens, walks them to the exact cut, adds
-//     what is kept of them to their slices' sums, and finds the token in its slice. Up to 256
+//     what is kept of them to their slices' sums, and finds the token in its slice. Up to 512
 //     listed tokens (a language model's logits list a few, up to some hundred where the cut lies
 //     in the wide floor) are ranked by counting, a token per thread.
 // Steps 2 and 3 do nothing for rows that need only the best token. A row whose steps list more
 // than kListed tokens (many equal logits; logits of enormous range) is solved by the choosing
 // workgroup alone, by radix selection over the row.
+//
+// Bound by four dependent launches. One row of 151936 (top-k 50, top-p 0.9): 2.9, 5.1, 6.2 and 7.5
+// us under a profiler, 22.3 in all; 64 rows of 32768: 4.5, 7.5, 11.2 and 12.2, 36 in all (8.4 MB, 1.6
+// us of a large copy). With a row to one workgroup they took 444 and 184.
 #include "eb_common.h"
 #include "eb_internal.h"
 
@@ -462,9 +466,9 @@ struct Shared {
     u64 waves[kWaves];
     unsigned waves32[kWaves];
     unsigned digit;
-    u64 above_w, cut, left;
+    u64 above_w, cut;
     unsigned above_c, in_last;
-    int tile, last;
+    int last;
 };
 
 // A row by itself: its cut by radix selection (returned as the least rank that is kept), and the

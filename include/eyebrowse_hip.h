@@ -598,7 +598,9 @@ eb_status eb_linear_q4(eb_recorder *rec, const eb_tensor *a, const eb_q4_weight 
 eb_status eb_linear_q4_multi(eb_recorder *rec, const eb_tensor *a, size_t n,
                              const eb_q4_weight *w, eb_tensor *const *c, size_t m);
 /* On caller memory. packed is 16-byte aligned; the workspace (16-byte aligned, no
- * initialisation) holds the split rows; launches that share one must not overlap. */
+ * initialisation) holds the split rows of more than 8 rows, and of more than 32 the sums of
+ * workgroups that share a contraction; launches that share one must not overlap. The raw pack is
+ * ordered on its stream alone. */
 eb_status eb_launch_q4_pack(void *stream, const uint32_t *w, size_t w_words,
                             const uint16_t *scales, size_t scales_numel, const uint8_t *zeros,
                             size_t zeros_numel, size_t in_f, size_t out_f, size_t group,

@@ -162,3 +162,16 @@ def test_other_calls_refuse_a_block_scaled_cache(dev):
         with pytest.raises(eb.UnsupportedConfig):
             eb.KvCache.new_i8(dev, 1, 64, 2, bad[1], bad[0])
     rec.submit()
+
+
+@pytest.mark.parametrize("hkv,hd", [(2, 128), (8, 32)])
+@pytest.mark.parametrize("rows", [1, 5])
+def test_a_cache_of_other_heads_is_refused(dev, hkv, hd, rows):
+    """As many codes a position, in other heads: blocks and exponents lie elsewhere."""
+    attn = eb.Attention(8, 4, 64, 0.125, None, None, None)
+    kv = eb.KvCache.new_i8(dev, 1, 64, hkv, hd, 16)
+    q, k = eb.Tensor.empty(dev, (rows, 512)), eb.Tensor.empty(dev, (rows, 256))
+    for t in (q, k):
+        t.write(np.zeros(t.shape, np.float32))
+    with pytest.raises(eb.ShapeMismatch, match="block-scaled"):
+        attn.forward_qkv(eb.Recorder(dev), q, k, k, eb.Rope.build(dev, 64, 64, THETA), kv, 0, rows, 0)
