@@ -37,6 +37,15 @@ eb_status aligned(std::initializer_list<const void *> ps, uintptr_t n, const cha
     return EB_OK;
 }
 
+// A set-up call's work belongs to no graph.
+eb_status not_captured(hipStream_t st, const char *what) {
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    EB_HIP_TRY(hipStreamIsCapturing(st, &capture));
+    if (capture != hipStreamCaptureStatusNone)
+        return fail(EB_OTHER, "%s: not allowed while the device's stream is being captured", what);
+    return EB_OK;
+}
+
 // ---- block-scaled caches --------------------------------------------------------------------
 
 // Rows and elements of a row that the kernels index with 32 bits (a whole cache may pass 2^31).
@@ -274,6 +283,7 @@ eb_status eb_kv_cache_new_i8(eb_device *dev, const size_t *head_dims, size_t n_l
     *out = nullptr;
     for (size_t l = 0; l < n_layers; ++l) EB_TRY(shape_i8(max_seq, n_kv_heads, head_dims[l], block));
     if (n_layers == 0) EB_TRY(shape_i8(max_seq, n_kv_heads, 32, block));
+    EB_TRY(not_captured(stream_of(dev), "kv_cache"));  // (a replay would clear the exponents)
     struct Release {
         void operator()(eb_kv_cache *kv) const { eb_kv_cache_release(kv); }
     };
@@ -460,10 +470,7 @@ eb_status eb_q4_pack(eb_recorder *rec, const eb_tensor *w, const eb_tensor *scal
     // Like a tensor's write, complete when it returns, and ordered behind every stream: a weight is
     // often filled by another library's stream, and its buffers are reused as soon as it is packed.
     const hipStream_t st = stream_of(dev);
-    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
-    EB_HIP_TRY(hipStreamIsCapturing(st, &capture));
-    if (capture != hipStreamCaptureStatusNone)
-        return fail(EB_OTHER, "q4_pack: not allowed while the device's stream is being captured");
+    EB_TRY(not_captured(st, "q4_pack"));
     EB_HIP_TRY(hipDeviceSynchronize());
     const size_t bytes = eb::q4_packed_bytes(in_f, out_f, group, zeros != nullptr);
     eb_tensor *t = nullptr;

@@ -135,3 +135,13 @@ def test_two_graphs_share_the_workspace(dev):
         assert attend(dev, big, qb, 2999, hd ** -0.5).tobytes() == first.tobytes()
         for i in (0, 1):
             assert steps[i][1][3].to_f32().tobytes() == caches[i]
+
+
+def test_a_cache_is_made_outside_a_capture(dev):
+    dev.begin_capture()
+    try:
+        with pytest.raises(eb.EyebrowseError, match="captured"):
+            eb.KvCache.new_i8(dev, 1, 64, 2, 64, 16)
+    finally:
+        dev.end_capture()
+    assert set(eb.KvCache.new_i8(dev, 1, 64, 2, 64, 16).k_scale[0].read_bytes()) == {1}
