@@ -467,11 +467,12 @@ eb_status eb_q4_pack(eb_recorder *rec, const eb_tensor *w, const eb_tensor *scal
     EB_TRY(eb::check_tensor(scales, EB_F16, "scales", dev));
     if (zeros) EB_TRY(eb::check_tensor(zeros, EB_U8, "zeros", dev));
     EB_TRY(q4_shape(in_f, out_f, group));
-    // Like a tensor's write, complete when it returns, and ordered behind every stream: a weight is
-    // often filled by another library's stream, and its buffers are reused as soon as it is packed.
+    // Like a tensor's write, complete when it returns, and ordered behind the null stream, on which
+    // other libraries fill weights; the sources are reused as soon as they are packed. (Not behind
+    // every stream: a wait for the whole device would end a capture that another of its streams runs.)
     const hipStream_t st = stream_of(dev);
     EB_TRY(not_captured(st, "q4_pack"));
-    EB_HIP_TRY(hipDeviceSynchronize());
+    EB_HIP_TRY(hipStreamSynchronize(nullptr));
     const size_t bytes = eb::q4_packed_bytes(in_f, out_f, group, zeros != nullptr);
     eb_tensor *t = nullptr;
     EB_TRY(eb_tensor_empty(dev, &bytes, 1, EB_U8, &t));

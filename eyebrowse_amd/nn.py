@@ -93,7 +93,7 @@ class LinearQ4:
     eight codes per word along k, lowest bits first; scales: F16 [out_f, in_f / group]; zeros: U8 of
     that shape, or None (8 everywhere). group is 32, 64 or 128 and divides in_f. The weight is laid
     out once, into `packed`, as the kernels read it; w, scales and zeros are not kept, and are read
-    when the constructor returns (it waits for all earlier work on the device, on any stream)."""
+    when the constructor returns (it waits for earlier work on the null stream and the device's)."""
 
     def __init__(self, w: Tensor, scales: Tensor, zeros: Optional[Tensor], in_f: int, out_f: int,
                  group: int):

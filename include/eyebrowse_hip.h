@@ -580,8 +580,8 @@ eb_status eb_attention_forward(const eb_attention *attn, eb_recorder *rec, const
  * in_f / group], zeros EB_U8 of that shape, or NULL: 8 everywhere (symmetric codes). group is
  * 32, 64 or 128 and divides in_f; out_f is any size. *packed is a new EB_U8 tensor of
  * eb_q4_packed_bytes bytes (about what w, scales and zeros hold, which are no longer needed). A
- * set-up call, as eb_tensor_write: it waits for all earlier work on the device, its own included,
- * and is refused during a capture. */
+ * set-up call, as eb_tensor_write: it waits for earlier work on the null stream and on the device's
+ * own, is complete when it returns, and is refused during a capture of the device's stream. */
 typedef struct eb_q4_weight {
     const eb_tensor *packed;
     size_t in_f, out_f, group;

@@ -216,9 +216,9 @@ def test_raw_launch(dev):
         assert out.to_f32().tobytes() == run(dev, a, w).tobytes()
 
 
-def test_pack_waits_for_other_streams(dev):
-    """A weight that another stream is still filling is packed whole, and may be overwritten at once.
-    (The other stream writes the words as the codes of a block-scaled cache laid over them.)"""
+def test_pack_waits_for_the_null_stream(dev):
+    """A weight that the null stream is still filling is packed whole, and may be overwritten at once.
+    (It writes the words as the codes of a block-scaled cache laid over them.)"""
     rng = np.random.default_rng(21)
     out_f, in_f, hkv, hd, block = 600, 2048, 4, 256, 16
     b = rng.integers(-127, 128, (out_f, in_f // 2))
@@ -226,29 +226,29 @@ def test_pack_waits_for_other_streams(dev):
     words = b.astype(np.int8).view(np.uint32)
     codes = (words[..., None] >> (4 * np.arange(8, dtype=np.uint32)) & 15).reshape(out_f, in_f)
     _, scales, _ = weight(rng, out_f, in_f, 128, False)
-    other = eb.Device.new(0)
     wt, st = eb.Tensor.empty(dev, words.shape, eb.DType.U32), eb.Tensor.from_array(dev, scales)
     wt.write(np.zeros_like(words))
-    spare = eb.Tensor.empty(other, (out_f, hkv, hd), eb.DType.I8)
-    exps = [eb.Tensor.empty(other, ((out_f + block - 1) // block, hkv), eb.DType.U8) for _ in range(2)]
+    spare = eb.Tensor.empty(dev, (out_f, hkv, hd), eb.DType.I8)
+    exps = [eb.Tensor.empty(dev, ((out_f + block - 1) // block, hkv), eb.DType.U8) for _ in range(2)]
     cache = eb.CacheI8(wt.data_ptr, exps[0].data_ptr, spare.data_ptr, exps[1].data_ptr, spare.numel(), exps[0].numel(),
                        out_f, hkv, hd, block)
-    big = eb.KvCache.new_i8(other, 1, 16384, 8, 128, 64)
-    load = eb.Tensor.empty(other, (16384, 8, 128))
-    load.write(np.ones((16384, 8, 128), np.float32))
-    x, none = eb.Tensor.from_array(other, b.astype(np.float32)), eb.Tensor.from_array(other, np.zeros(b.shape, np.float32))
-    other.synchronize()
+    n = 16384
+    big = eb.KvCache.new_i8(dev, 1, n, 8, 128, 64)
+    long = eb.CacheI8(big.k[0].data_ptr, big.k_scale[0].data_ptr, big.v[0].data_ptr, big.v_scale[0].data_ptr,
+                      big.k[0].numel(), big.k_scale[0].numel(), n, 8, 128, 64)
+    load = eb.Tensor.empty(dev, (n, 8, 128))
+    load.write(np.ones((n, 8, 128), np.float32))
+    x, none = eb.Tensor.from_array(dev, b.astype(np.float32)), eb.Tensor.from_array(dev, np.zeros(b.shape, np.float32))
+    dev.synchronize()
     for _ in range(20):
-        rec = eb.Recorder(other)
-        eb.kv_write_i8(rec, big, 0, load, load, 16384, 0)
-        rec.submit()
-    eb.launch_kv_write_i8(other.stream, cache, x.data_ptr, x.data_ptr, b.size, out_f, 0)
+        eb.launch_kv_write_i8(0, long, load.data_ptr, load.data_ptr, load.numel(), n, 0)
+    eb.launch_kv_write_i8(0, cache, x.data_ptr, x.data_ptr, b.size, out_f, 0)
     w = eb.LinearQ4(wt, st, None, in_f, out_f, 128)
-    eb.launch_kv_write_i8(other.stream, cache, none.data_ptr, none.data_ptr, b.size, out_f, 0)
+    eb.launch_kv_write_i8(0, cache, none.data_ptr, none.data_ptr, b.size, out_f, 0)
     a = rng.standard_normal((2, in_f)).astype(np.float32)
     want, bound = linear_q4_bound(a, codes, scales, None, 128)
-    close(run(dev, a, w), want, bound, "packed behind another stream")
-    other.synchronize()
+    close(run(dev, a, w), want, bound, "packed behind the null stream")
+    eb.LinearQ4(wt, st, None, in_f, out_f, 128)  # (waits for the writes above, before their tensors go)
 
 
 def test_pack_during_a_capture_is_refused(dev):
@@ -261,3 +261,33 @@ def test_pack_during_a_capture_is_refused(dev):
             eb.LinearQ4(*ts, None, 128, 16, 64)
     finally:
         dev.end_capture()
+
+
+def test_pack_leaves_another_capture_alone(dev):
+    """Weights are loaded while another device's stream (of the same GPU) is being captured."""
+    rng = np.random.default_rng(23)
+    codes, scales, z = weight(rng, 48, 256, 64, True)
+    other = eb.Device.new(0)
+    w = device_weight(other, codes, scales, z, 64)
+    a = rng.standard_normal((2, 256)).astype(np.float32)
+    want, bound = linear_q4_bound(a, codes, scales, z, 64)
+    at, out = eb.Tensor.from_array(other, a), eb.Tensor.empty(other, (2, 48))
+
+    def step():
+        rec = eb.Recorder(other)
+        eb.linear_q4(rec, at, w, out, 2)
+        rec.submit()
+
+    step()
+    out.write(np.zeros((2, 48), np.float32))
+    other.begin_capture()
+    try:
+        mine = device_weight(dev, codes, scales, z, 64)
+        step()
+    finally:
+        graph = other.end_capture()
+    close(run(dev, a, mine), want, bound, "packed during the capture")
+    for _ in range(3):
+        graph.launch()
+        other.synchronize()
+        close(out.to_f32().reshape(2, 48), want, bound, "the captured call")
