@@ -87,7 +87,7 @@ struct Args {
     int window;             // 0: none
     int tile0, tiles;       // the tiles dealt to the splits: tile0 .. tile0 + tiles - 1
     int owner, tails;        // the append's split; its block's tiles, behind the others
-    unsigned g_inv;          // 2^32 / g, rounded up
+    unsigned g_inv;          // 2^32 / g, rounded up (exact below 65536 columns; a call has 192 at most)
     int nsplit, block_log2;
     float scale_log2;
     bool prologue;
@@ -633,9 +633,6 @@ eb_status launch_attn_decode_i8(hipStream_t st, const float *q, const CacheI8 &c
                                 const float *vnew, float *o, size_t h, size_t pos0, size_t rows, float scale,
                                 size_t window, float *ws, size_t ws_floats, int cu_count,
                                 const DecodePrologue *pro) {
-    // (q's offsets are 32-bit; the division by g is a multiplication that is exact to 65535)
-    if (rows * h * c.hd >= (size_t)1 << 29 || rows * (h / c.hkv) > 65535)
-        return fail(EB_UNSUPPORTED_CONFIG, "attn_decode_i8: %zu rows of %zu heads of %zu", rows, h, c.hd);
     const Plan p = plan_of(h, c.hkv, pos0, rows, c.block, window, knew != nullptr, cu_count);
     if (knew && !p.fused) {
         if (pro) return fail(EB_OTHER, "attn_decode_i8: more than %d heads per KV head need the row pass", kCols);

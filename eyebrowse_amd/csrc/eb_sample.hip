@@ -38,7 +38,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 512;   // of the choosing workgroup
 constexpr int kWaves = kThreads / 64;
-constexpr int kTile = 4096;     // tokens of a slice
+constexpr int kTile = 4096;     // tokens of a slice (of 2048: one row of 151936 22.0 -> 21.0 us, 64 rows 62.5 -> 93)
 constexpr int kSliceThreads = 512;
 constexpr int kPer = kTile / kSliceThreads;  // tokens per thread of a slice
 constexpr int kDigits = 256;    // of a radix pass
@@ -58,8 +58,9 @@ struct Args {
     eb::SampleArgs s;
     int frac;  // F
     int tiles;
+    int per, groups;  // slices of a workgroup, workgroups of a row
     // workspace
-    u64 *best;         // [rows, tiles] rank keys
+    u64 *best;         // [rows, groups] rank keys
     u64 *tile_sum;     // [rows, tiles]
     u64 *hist_w;       // [rows, kBins]
     unsigned *hist_c;  // [rows, kBins]
@@ -249,7 +250,7 @@ __device__ __forceinline__ u64 wave_scan(u64 x) {
     return x;
 }
 
-// ---- steps 1 to 3: one workgroup per slice -----------------------------------------------------
+// ---- steps 1 to 3: one workgroup per run of slices -----------------------------------------------------
 
 // The tokens of this thread in slice t: four at a time, NaN past the vocabulary.
 struct Slice {
@@ -276,29 +277,35 @@ struct Slice {
 // Step 1, and the clearing of the row's histogram and list.
 __global__ __launch_bounds__(kSliceThreads) void sample_max_kernel(Args a) {
     __shared__ u64 s_waves[kSliceThreads / 64];
-    const int t = blockIdx.x, tid = threadIdx.x;
+    const int g = blockIdx.x, tid = threadIdx.x;
     const size_t r = blockIdx.y;
-    const Slice s(a.s.logits + r * a.s.vocab, (int)a.s.vocab, t);
-    for (int i = t * kSliceThreads + tid; i < kBins; i += a.tiles * kSliceThreads) {
+    const float *row = a.s.logits + r * a.s.vocab;
+    const int t0 = g * a.per, t1 = min(t0 + a.per, a.tiles);
+    Slice s(row, (int)a.s.vocab, t0);
+    for (int i = g * kSliceThreads + tid; i < kBins; i += a.groups * kSliceThreads) {
         a.hist_w[r * kBins + i] = 0;
         a.hist_c[r * kBins + i] = 0;
     }
-    if (t == 0 && tid == 0) a.count[r] = 0;
+    if (g == 0 && tid == 0) a.count[r] = 0;
     u64 k = 0;
+    for (int t = t0;;) {
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-        const u64 o = rank_of(s.x[j], (unsigned)s.at(j));
-        k = o > k ? o : k;
+        for (int j = 0; j < kPer; ++j) {
+            const u64 o = rank_of(s.x[j], (unsigned)s.at(j));
+            k = o > k ? o : k;
+        }
+        if (++t >= t1) break;
+        s = Slice(row, (int)a.s.vocab, t);
     }
     k = block_best<kSliceThreads>(k, s_waves);
-    if (tid == 0) a.best[r * a.tiles + t] = k;
+    if (tid == 0) a.best[r * a.groups + g] = k;
 }
 
 // The row's largest rank key, from step 1's (every wave by itself: no barrier).
 __device__ __forceinline__ u64 row_best(const Args &a, size_t r) {
     u64 k = 0;
-    for (int i = threadIdx.x & 63; i < a.tiles; i += 64) {
-        const u64 o = a.best[r * a.tiles + i];
+    for (int i = threadIdx.x & 63; i < a.groups; i += 64) {
+        const u64 o = a.best[r * a.groups + i];
         k = o > k ? o : k;
     }
     return wave_best(k);
@@ -310,7 +317,9 @@ __global__ __launch_bounds__(kSliceThreads) void sample_histogram_kernel(Args a)
     __shared__ unsigned s_c[kBins];
     const int tid = threadIdx.x;
     const size_t r = blockIdx.y;
-    const Slice s(a.s.logits + r * a.s.vocab, (int)a.s.vocab, blockIdx.x);
+    const float *x = a.s.logits + r * a.s.vocab;
+    const int t0 = blockIdx.x * a.per, t1 = min(t0 + a.per, a.tiles);
+    Slice s(x, (int)a.s.vocab, t0);
     const Params params(a, r);
     for (int i = tid; i < kBins; i += kSliceThreads) {
         s_w[i] = 0;
@@ -319,15 +328,19 @@ __global__ __launch_bounds__(kSliceThreads) void sample_histogram_kernel(Args a)
     const Row row(a, params, (unsigned)(row_best(a, r) >> 32));
     if (row.none || row.best || !(row.use_k || row.use_p)) return;  // (uniform)
     __syncthreads();
+    for (int t = t0;;) {
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-        if (s.x[j] != s.x[j]) continue;
-        const int b = row.bin(s.x[j]);
-        atomicAdd(&s_c[b], 1u);
-        if (row.use_p) {
-            const u64 w = row.units(row.weight(s.x[j]));
-            if (w) atomicAdd(&s_w[b], w);
+        for (int j = 0; j < kPer; ++j) {
+            if (s.x[j] != s.x[j]) continue;
+            const int b = row.bin(s.x[j]);
+            atomicAdd(&s_c[b], 1u);
+            if (row.use_p) {
+                const u64 w = row.units(row.weight(s.x[j]));
+                if (w) atomicAdd(&s_w[b], w);
+            }
         }
+        if (++t >= t1) break;
+        s = Slice(x, (int)a.s.vocab, t);
     }
     __syncthreads();
     for (int i = tid; i < kBins; i += kSliceThreads) {
@@ -348,7 +361,9 @@ __global__ __launch_bounds__(kSliceThreads) void sample_collect_kernel(Args a) {
     __shared__ unsigned s_above, s_here, s_from;
     const int tid = threadIdx.x;
     const size_t r = blockIdx.y;
-    const Slice s(a.s.logits + r * a.s.vocab, (int)a.s.vocab, blockIdx.x);
+    const float *x = a.s.logits + r * a.s.vocab;
+    const int t0 = blockIdx.x * a.per, t1 = min(t0 + a.per, a.tiles);
+    Slice s(x, (int)a.s.vocab, t0);
     const Params params(a, r);
     unsigned c[PB];
     u64 w[PB];
@@ -422,38 +437,45 @@ __global__ __launch_bounds__(kSliceThreads) void sample_collect_kernel(Args a) {
         if (blockIdx.x == 0 && tid == 0)
             a.cut[r] = Cut{row.use_p ? s_before_cut : s_before_topk, s_before_topk, s_above, topk};
     }
-    u64 sum = 0;
-    unsigned mine = 0;
+    for (int t = t0;;) {
+        u64 sum = 0;
+        unsigned mine = 0;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-        if (s.x[j] != s.x[j]) continue;
-        const int b = row.bin(s.x[j]);
-        if (b < lo)
-            sum += row.units_kept(row.weight(s.x[j]));
-        else if (b <= hi || b == topk)
-            ++mine;
-    }
-    if (lo < kBins) {
-        // This slice's part of the list (in any order: it is sorted).
-        unsigned at = mine ? atomicAdd(&s_here, mine) : 0;
-        __syncthreads();
-        if (tid == 0) s_from = s_here ? atomicAdd(&a.count[r], s_here) : 0;
-        __syncthreads();
-        at += s_from;
-        if (mine) {
+        for (int j = 0; j < kPer; ++j) {
+            if (s.x[j] != s.x[j]) continue;
+            const int b = row.bin(s.x[j]);
+            if (b < lo)
+                sum += row.units_kept(row.weight(s.x[j]));
+            else if (b <= hi || b == topk)
+                ++mine;
+        }
+        if (lo < kBins) {
+            // This slice's part of the list (in any order: it is sorted).
+            unsigned at = mine ? atomicAdd(&s_here, mine) : 0;
+            __syncthreads();
+            if (tid == 0) {
+                s_from = s_here ? atomicAdd(&a.count[r], s_here) : 0;
+                s_here = 0;
+            }
+            __syncthreads();
+            at += s_from;
+            if (mine) {
 #pragma unroll
-            for (int j = 0; j < kPer; ++j) {
-                if (s.x[j] != s.x[j]) continue;
-                const int b = row.bin(s.x[j]);
-                if (b >= lo && (b <= hi || b == topk)) {
-                    if (at < kListed) a.listed[r * kListed + at] = rank_of(s.x[j], (unsigned)s.at(j));
-                    ++at;
+                for (int j = 0; j < kPer; ++j) {
+                    if (s.x[j] != s.x[j]) continue;
+                    const int b = row.bin(s.x[j]);
+                    if (b >= lo && (b <= hi || b == topk)) {
+                        if (at < kListed) a.listed[r * kListed + at] = rank_of(s.x[j], (unsigned)s.at(j));
+                        ++at;
+                    }
                 }
             }
         }
+        sum = block_total<kSliceThreads>(sum, s_waves);
+        if (tid == 0) a.tile_sum[r * a.tiles + t] = sum;
+        if (++t >= t1) break;
+        s = Slice(x, (int)a.s.vocab, t);
     }
-    sum = block_total<kSliceThreads>(sum, s_waves);
-    if (tid == 0) a.tile_sum[r * a.tiles + blockIdx.x] = sum;
 }
 
 // ---- step 4: one workgroup per row --------------------------------------------------------------
@@ -832,6 +854,10 @@ Layout layout_of(size_t rows, size_t tiles) {
 }
 
 constexpr size_t kMaxVocab = (size_t)1 << 24;
+// Where slices are more than this many for every CU, a workgroup of steps 1 to 3 takes several of a
+// row, so that a row's parameters, largest logit and cut are found by fewer. Rows of 151936, top-k 50
+// and top-p 0.9: 64 rows 57 us in runs of 2 and 65.5 a slice each, 256 rows 152 and 185.
+constexpr size_t kGroupsPerCu = 7;
 
 }  // namespace
 
@@ -848,6 +874,10 @@ eb_status launch_sample(hipStream_t st, const SampleArgs &s, float *ws) {
     while (((size_t)1 << (62 - a.frac)) < s.vocab) --a.frac;
     const size_t tiles = (s.vocab + kTile - 1) / kTile;
     a.tiles = (int)tiles;
+    const size_t per = (tiles * s.rows + kGroupsPerCu * current_cu_count() - 1) / (kGroupsPerCu * current_cu_count());
+    a.groups = (int)((tiles + per - 1) / per);
+    a.per = (a.tiles + a.groups - 1) / a.groups;
+    a.groups = (a.tiles + a.per - 1) / a.per;
     const size_t lds = tiles * 12 + 8;
     static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&sample_choose_kernel),
                                                     hipFuncAttributeMaxDynamicSharedMemorySize,
@@ -861,7 +891,7 @@ eb_status launch_sample(hipStream_t st, const SampleArgs &s, float *ws) {
     a.listed = reinterpret_cast<u64 *>(ws + l.listed);
     a.count = reinterpret_cast<unsigned *>(ws + l.count);
     a.cut = reinterpret_cast<Cut *>(ws + l.cut);
-    const dim3 grid((unsigned)tiles, (unsigned)s.rows);
+    const dim3 grid((unsigned)a.groups, (unsigned)s.rows);
     sample_max_kernel<<<grid, kSliceThreads, 0, st>>>(a);
     // (the parameters lie in device memory: which rows have a cut is known to the kernels alone)
     if (s.top_k || s.top_p) sample_histogram_kernel<<<grid, kSliceThreads, 0, st>>>(a);

@@ -175,3 +175,15 @@ def test_raw_launch(dev):
     eb.launch_sample(dev.stream, xt.data_ptr, x.size, ut.data_ptr, out.data_ptr, 2, 5000, ws_ptr=ws.data_ptr, ws_floats=floats)
     dev.synchronize()
     np.testing.assert_array_equal(np.frombuffer(out.read_bytes(), np.uint32), want(x, u))
+
+
+@pytest.mark.parametrize("choice", [dict(), dict(top_k=40, top_p=0.9), dict(top_p=0.95, min_p=0.02), dict(temperature=0.0)])
+@pytest.mark.parametrize("rows,vocab", [(900, 12289), (1900, 4100), (450, 20480)])
+def test_many_rows(dev, rows, vocab, choice):
+    """More slices than the card holds workgroups: a workgroup takes several of a row."""
+    note(f"sample {rows}x{vocab} {choice}")
+    rng = np.random.default_rng(vocab + rows)
+    x = (3 * rng.standard_normal((rows, vocab), dtype=np.float32))
+    x[:, vocab - 1] += np.float32(9)  # (kept tokens at the far end of a row too)
+    u = rng.random(rows).astype(np.float32)
+    np.testing.assert_array_equal(run(dev, x, u, **choice), want(x, u, **choice))
