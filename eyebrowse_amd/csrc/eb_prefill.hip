@@ -1437,7 +1437,8 @@ __global__ __attribute__((
 // Combines the key chunks of the query blocks that were split: o = sum_c w_c O_c /
 // sum_c w_c l_c with w_c = 2^(m_c - M), M the largest m_c, and O_c in units of 2^E_c
 // (brought to the largest E first, so nothing overflows). A chunk that saw no key of a
-// query has m = -inf and weight 0. Blocks of one chunk were written by the prefill itself.
+// query has m = -inf, l = 0 and weight 0. (One that saw NaN scores alone has m = -inf too, for
+// a maximum passes NaN by, but its l is NaN, and so is the sum.) Blocks of one chunk were written by the prefill itself.
 // Thread (pair, d4): four output dims of one (row, head) pair; the chunks' states are read
 // kMergeBatch at a time, all loads of a batch issued before any is used.
 constexpr int kMergeBatch = 8;
@@ -1449,13 +1450,14 @@ constexpr int kMergeBatch = 8;
 // term, so that a chunk of negligible weight but large V rows cannot push the others
 // below f32 range. d is clamped at -300: below that the term is under 2^-170 of any
 // finite E and rounds away in the sum.
+__device__ __forceinline__ bool merge_none(float4 ml) { return ml.x == -INFINITY && ml.y == 0.0f; }
 __device__ __forceinline__ int merge_exp(float4 ml, float Mr) {
-    if (ml.x == -INFINITY) return kZeroRowExp;  // a chunk that saw no key
+    if (merge_none(ml)) return kZeroRowExp;  // a chunk that saw no key
     return __float_as_int(ml.z) + (int)floorf(fmaxf(ml.x - Mr, -300.0f));
 }
 __device__ __forceinline__ void merge_add(float4 ml, float4 acc, float Mr, int EM, float4 &A,
                                           float &L) {
-    if (ml.x == -INFINITY) return;
+    if (merge_none(ml)) return;
     const float d = fmaxf(ml.x - Mr, -300.0f);
     const float fl = floorf(d);
     const float wf = eb::fast_exp2(d - fl);
