@@ -214,7 +214,7 @@ __device__ __forceinline__ int hv_chunk(int p, int c) { return C::KC + c * C::HD
 // values): conditionally written register arrays end up in scratch memory.
 // EB: bytes per k/v element: 4 (f32), 2 (IEEE half) or 1 (OCP FP8 E4M3), converted to f32
 // here (exactly); kCodes: the codes of a block-scaled cache with their exponents ks, vs, one for
-// 2^lb rows and a KV head (code * 2^(e - 127), exact in f32 too).
+// 2^lb rows and a KV head (code * 2^(e - 127), exact in f32 too; NaN for e = 255).
 constexpr int kCodes = -1;
 template <class C, int EB, bool NT = false>
 __device__ __forceinline__ void prefill_load_step(const void *__restrict__ k,
@@ -246,8 +246,13 @@ __device__ __forceinline__ void prefill_load_step(const void *__restrict__ k,
             vx = eb::f8x4_to_f32(
                 *reinterpret_cast<const unsigned *>(static_cast<const uint8_t *>(v) + off));
         } else if constexpr (EB == kCodes) {
+            // A NaN block's V rows are zeros here and their scores NaN instead: a query that sees
+            // one is NaN throughout either way, while one that does not has 0 for a score's weight
+            // and would have 0 * NaN from V, in whose product it shares a tile.
             const size_t b = (size_t)(min(key, T - 1) >> lb) * Hkv + kvh;
-            const float fk = eb::i8_scale(ks[b], 0), fv = eb::i8_scale(vs[b], 0);
+            const unsigned ev = vs[b];
+            const bool nan_v = ev == eb::kNanExponent;
+            const float fk = eb::i8_scale(nan_v ? ev : ks[b], 0), fv = nan_v ? 0.0f : eb::i8_scale(ev, 0);
             const unsigned wk = *reinterpret_cast<const unsigned *>(static_cast<const uint8_t *>(k) + off);
             const unsigned wv = *reinterpret_cast<const unsigned *>(static_cast<const uint8_t *>(v) + off);
 #pragma unroll

@@ -61,3 +61,25 @@ def test_k_rows_of_an_f32_cache_that_fill_a_share(dev, h, hkv, hd, bad):
     assert np.isnan(got[:, :h // hkv]).all()
     want = attention_f64(q, np.nan_to_num(k, nan=0.0), v, hd ** -0.5, q_offset=pos)
     assert_close(got[:, h // hkv:], want[:, h // hkv:], what="the other heads")
+
+
+@pytest.mark.parametrize("h,hkv,hd,block", [(4, 2, 256, 64), (4, 2, 64, 256), (8, 2, 128, 256), (3, 3, 32, 256)])
+def test_v_blocks_that_fill_a_share_of_the_keys(dev, h, hkv, hd, block):
+    note(f"i8 nan V share {h}/{hkv}x{hd} block {block}")
+    check(dev, h, hkv, hd, block, 640, 200, 0, [(1, block + 5, 0)])
+    check(dev, h, hkv, hd, block, 640, 200, 300, [(1, block + 5, 0)])
+
+
+@pytest.mark.parametrize("h,hkv,hd", [(4, 2, 64), (16, 8, 128), (4, 2, 256), (3, 3, 48)])
+@pytest.mark.parametrize("block", [16, 64])
+@pytest.mark.parametrize("pos,n", [(0, 200), (0, 33), (45, 210), (301, 200), (1000, 6)])
+@pytest.mark.parametrize("window", [0, 40])
+def test_rows_that_do_not_see_the_block(dev, h, hkv, hd, block, pos, n, window):
+    """A block among the chunk's own rows, one behind a window's start, and one in another head."""
+    note(f"i8 nan {h}/{hkv}x{hd} block {block} pos {pos} rows {n} window {window}")
+    last = pos + n - 1
+    for side in (0, 1):
+        bad = [(side, pos + n // 2, 0), (1 - side, last, hkv - 1)]
+        if window and pos > window:
+            bad.append((side, pos - window + 3, 1))
+        check(dev, h, hkv, hd, block, pos, n, window, bad)
