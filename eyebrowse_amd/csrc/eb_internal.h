@@ -56,9 +56,12 @@ struct CacheI8 {
 // The device that owns a tensor.
 eb_device *tensor_device(const eb_tensor *t);
 
-// Entry points outside eb_runtime.cpp: the recorder may record (its device becomes current and goes
-// to *dev), an operand of a type on that device, and the device's workspace, grown to hold
-// `floats` and handed out with its mutex held in *lk until the launch is enqueued.
+// Entry points outside eb_runtime.cpp: the device becomes the thread's current one (what a call
+// without a recorder does before it launches: a buffer from the pool comes without it), the
+// recorder may record (its device becomes current and goes to *dev), an operand of a type on that
+// device, and the device's workspace, grown to hold `floats` and handed out with its mutex held in
+// *lk until the launch is enqueued.
+eb_status make_current(eb_device *dev);
 eb_status recorder_ready(eb_recorder *rec, eb_device **dev);
 eb_status check_tensor(const eb_tensor *t, eb_dtype dt, const char *name, eb_device *dev);
 eb_status device_workspace(eb_device *dev, size_t floats, float **out, std::unique_lock<std::mutex> &lk);

@@ -283,6 +283,7 @@ eb_status eb_kv_cache_new_i8(eb_device *dev, const size_t *head_dims, size_t n_l
     *out = nullptr;
     for (size_t l = 0; l < n_layers; ++l) EB_TRY(shape_i8(max_seq, n_kv_heads, head_dims[l], block));
     if (n_layers == 0) EB_TRY(shape_i8(max_seq, n_kv_heads, 32, block));
+    EB_TRY(eb::make_current(dev));
     EB_TRY(not_captured(stream_of(dev), "kv_cache"));  // (a replay would clear the exponents)
     struct Release {
         void operator()(eb_kv_cache *kv) const { eb_kv_cache_release(kv); }

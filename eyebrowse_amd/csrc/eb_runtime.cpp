@@ -1039,6 +1039,11 @@ eb_status eb::device_workspace(eb_device *dev, size_t floats, float **out, WsLoc
     return ::device_workspace(dev, floats, out, lk);
 }
 
+eb_status eb::make_current(eb_device *dev) {
+    EB_HIP_TRY(hipSetDevice(dev->ordinal));
+    return EB_OK;
+}
+
 eb_status eb::recorder_ready(eb_recorder *rec, eb_device **dev) {
     EB_TRY(rec_ready(rec));
     *dev = rec->dev;
