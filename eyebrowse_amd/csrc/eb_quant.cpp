@@ -306,6 +306,9 @@ eb_status eb_kv_cache_new_i8(eb_device *dev, const size_t *head_dims, size_t n_l
                 EB_TRY(eb::launch_fill_u8(stream_of(dev), data<uint8_t>(t), 1, blocks * n_kv_heads));
         }
     }
+    // Complete, as a tensor's write is: the next one to touch the exponents may be another stream,
+    // which nothing orders behind this one.
+    EB_HIP_TRY(hipStreamSynchronize(stream_of(dev)));
     *out = kv.release();
     return eb::ok();
 }

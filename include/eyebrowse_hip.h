@@ -630,7 +630,8 @@ eb_status eb_attention_new_q4(const eb_attention_desc *desc, const eb_q4_weight 
  * finite makes e = 255: the block (of its head, K or V) reads as NaN until it is written from
  * its first row on; attention rows of that head that see one of its keys are NaN, the others
  * as they would be without it. Attention computes in f32 on the values the codes stand for. A new cache is
- * made outside a capture: its exponents are cleared by the call, not by a graph. */
+ * made outside a capture: its exponents are cleared by the call, not by a graph, and are clear when
+ * it returns. */
 eb_status eb_kv_cache_new_i8(eb_device *dev, const size_t *head_dims, size_t n_layers,
                              size_t max_seq, size_t n_kv_heads, size_t block,
                              eb_kv_cache **out);
