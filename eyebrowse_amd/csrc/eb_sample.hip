@@ -858,31 +858,22 @@ constexpr size_t kMaxVocab = (size_t)1 << 24;
 // row, so that a row's parameters, largest logit and cut are found by fewer. Rows of 151936, top-k 50
 // and top-p 0.9: 64 rows 57 us in runs of 2 and 65.5 a slice each, 256 rows 152 and 185.
 constexpr size_t kGroupsPerCu = 7;
+// A row's histogram and list take 45 KB whatever its vocabulary: rows beyond this many go through the
+// same workspace after the others (65535 rows would ask for 2.9 GB; these are 46 MB).
+constexpr size_t kBatchRows = 1024;
 
-}  // namespace
-
-namespace eb {
-
-size_t sample_workspace_floats(size_t rows, size_t vocab) {
-    return layout_of(rows, (vocab + kTile - 1) / kTile).floats;
-}
-
-eb_status launch_sample(hipStream_t st, const SampleArgs &s, float *ws) {
+eb_status launch_batch(hipStream_t st, const eb::SampleArgs &s, float *ws) {
     Args a{};
     a.s = s;
     a.frac = 44;
     while (((size_t)1 << (62 - a.frac)) < s.vocab) --a.frac;
-    const size_t tiles = (s.vocab + kTile - 1) / kTile;
+    const size_t tiles = (s.vocab + kTile - 1) / kTile, cus = (size_t)eb::current_cu_count();
     a.tiles = (int)tiles;
-    const size_t per = (tiles * s.rows + kGroupsPerCu * current_cu_count() - 1) / (kGroupsPerCu * current_cu_count());
+    const size_t per = (tiles * s.rows + kGroupsPerCu * cus - 1) / (kGroupsPerCu * cus);
     a.groups = (int)((tiles + per - 1) / per);
     a.per = (a.tiles + a.groups - 1) / a.groups;
     a.groups = (a.tiles + a.per - 1) / a.per;
     const size_t lds = tiles * 12 + 8;
-    static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&sample_choose_kernel),
-                                                    hipFuncAttributeMaxDynamicSharedMemorySize,
-                                                    (int)(kMaxVocab / kTile * 12 + 8));
-    if (e != hipSuccess) return hip_fail(e, "sample launch set-up");
     const Layout l = layout_of(s.rows, tiles);
     a.best = reinterpret_cast<u64 *>(ws + l.best);
     a.tile_sum = reinterpret_cast<u64 *>(ws + l.tile_sum);
@@ -897,7 +888,31 @@ eb_status launch_sample(hipStream_t st, const SampleArgs &s, float *ws) {
     if (s.top_k || s.top_p) sample_histogram_kernel<<<grid, kSliceThreads, 0, st>>>(a);
     sample_collect_kernel<<<grid, kSliceThreads, 0, st>>>(a);
     sample_choose_kernel<<<(unsigned)s.rows, kThreads, lds, st>>>(a);
-    return check_launch("sample");
+    return eb::check_launch("sample");
+}
+
+}  // namespace
+
+namespace eb {
+
+size_t sample_workspace_floats(size_t rows, size_t vocab) {
+    return layout_of(std::min(rows, kBatchRows), (vocab + kTile - 1) / kTile).floats;
+}
+
+eb_status launch_sample(hipStream_t st, const SampleArgs &s, float *ws) {
+    static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&sample_choose_kernel),
+                                                    hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                    (int)(kMaxVocab / kTile * 12 + 8));
+    if (e != hipSuccess) return hip_fail(e, "sample launch set-up");
+    for (size_t r = 0; r < s.rows; r += kBatchRows) {
+        auto from = [&](auto *p) { return p ? p + r : nullptr; };
+        const SampleArgs b{s.logits + r * s.vocab, s.u + r,         from(s.temperature),
+                           from(s.top_k),          from(s.top_p),   from(s.min_p),
+                           s.out + r,              std::min(kBatchRows, s.rows - r), s.vocab};
+        const eb_status status = launch_batch(st, b, ws);
+        if (status != EB_OK) return status;
+    }
+    return EB_OK;
 }
 
 }  // namespace eb
