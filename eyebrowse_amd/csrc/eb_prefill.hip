@@ -1620,10 +1620,15 @@ size_t presplit_floats(size_t hd, size_t h, size_t hkv, const PrefillRange &r) {
     const int qb_rows = kTile * prefill_shape(hd, (int)h, (int)(h / hkv), r.rows).wph;
     const int nqb = (r.rows + qb_rows - 1) / qb_rows;
     if (!r.ks && nqb < (hd > 128 ? kPresplitMinBlocks256 : kPresplitMinBlocks)) return 0;
-    const size_t rec = hd == 32    ? PrefillCfg<32, 4, 1, 1>::PS_FLOATS
-                       : hd == 64  ? PrefillCfg<64, 4, 1, 1>::PS_FLOATS
-                       : hd == 128 ? PrefillCfg<128, 4, 1, 1>::PS_FLOATS
-                                   : PrefillCfg<256, 4, 1, 1>::PS_FLOATS;
+    // (a block-scaled cache's are half images; the others' room is one size for every element type)
+    auto record = [&](auto cfg) {
+        using C = decltype(cfg);
+        return (size_t)(r.ks ? C::HIMG : C::PS_FLOATS);
+    };
+    const size_t rec = hd == 32    ? record(PrefillCfg<32, 4, 1, 1>{})
+                       : hd == 64  ? record(PrefillCfg<64, 4, 1, 1>{})
+                       : hd == 128 ? record(PrefillCfg<128, 4, 1, 1>{})
+                                   : record(PrefillCfg<256, 4, 1, 1>{});
     return hkv * (size_t)presplit_nt(r) * rec;
 }
 
