@@ -113,18 +113,22 @@ class LinearQ4:
     @classmethod
     def from_f32(cls, dev: Device, weight, group: int = 128, symmetric: bool = True) -> "LinearQ4":
         """Round weight [out_f, in_f] to the nearest codes. Symmetric: scale = largest |w| of the
-        group / 7, zero point 8; else scale = (largest - smallest) / 15 over the group and 0."""
+        group / 7, zero point 8; else scale = (largest - smallest) / 15 over the group and 0. A
+        group whose scale no f16 holds (above 65504, or not finite) is refused."""
         w = np.asarray(weight, np.float32)
         out_f, in_f = w.shape
         if group not in (32, 64, 128) or in_f % group:
             raise UnsupportedConfig(f"LinearQ4: group {group} for in_f {in_f}")
         x = w.reshape(out_f, in_f // group, group)
-        if symmetric:
-            s = (np.abs(x).max(-1) / 7).astype(np.float16)
-            z = np.full(s.shape, 8, np.uint8)
-        else:
-            lo, hi = np.minimum(x.min(-1), 0), np.maximum(x.max(-1), 0)
-            s = ((hi - lo) / 15).astype(np.float16)
+        with np.errstate(over="ignore", invalid="ignore"):
+            if symmetric:
+                s = (np.abs(x).max(-1) / 7).astype(np.float16)
+                z = np.full(s.shape, 8, np.uint8)
+            else:
+                lo, hi = np.minimum(x.min(-1), 0), np.maximum(x.max(-1), 0)
+                s = ((hi - lo) / 15).astype(np.float16)
+        if not np.isfinite(s).all():
+            raise UnsupportedConfig("LinearQ4: a group's scale is not a finite f16")
         d = np.where(s > 0, s, 1).astype(np.float32)  # (a group of zeros: scale 0, any code)
         if not symmetric:
             z = np.clip(np.rint(-lo / d), 0, 15).astype(np.uint8)

@@ -48,3 +48,13 @@ def test_from_f32_keeps_the_weight(dev, group, symmetric):
     rec.submit()
     want, bound = linear_q4_bound(x, codes, s, z, group)
     assert (np.abs(y.to_f32().reshape(3, 75) - want) <= bound).all()
+
+
+@pytest.mark.parametrize("symmetric", [True, False])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf, 1e6, -3e38])
+def test_from_f32_refuses_what_a_half_scale_cannot_hold(symmetric, bad):
+    """(refused before a device is needed)"""
+    w = np.ones((4, 128), np.float32)
+    w[2, 70] = bad
+    with pytest.raises(eb.UnsupportedConfig, match="scale"):
+        eb.LinearQ4.from_f32(None, w, 64, symmetric)
