@@ -28,8 +28,9 @@
 //    nor the small ones' precision where the large ones have no weight.
 // The products sum in f32; the f16 pairs keep 22 bits of q and of the weights.
 //
-// Bound by HBM in long caches (32 heads over 8 of 128, 131071 keys: 49.5 us with the merge, 5.4
-// TB/s), by the instructions of a tile (about 220 a wave for 16 keys) beside the ramp below: 32767
+// Bound by the codes' loads in long caches (32 heads over 8 of 128, 131071 keys: 49.5 us with the
+// merge, 5.4 TB/s, where a plain read reaches 6.4, and 7.1 with non-temporal loads, which were not
+// tried here), by the instructions of a tile (about 220 a wave for 16 keys) beside the ramp below: 32767
 // keys 21.4, 8191 keys (16 heads) 13.1, 1000 keys 9.5; 100 keys, one launch on 8 workgroups, 6.8: a
 // chain of q, scores, softmax and output. So every first load is issued before the first wait.
 // Sixteen columns read the cache once: 4 rows at 8192 keys 15.0 us, 16 rows (64 columns) 23.2.

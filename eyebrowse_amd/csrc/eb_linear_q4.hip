@@ -155,9 +155,10 @@ __global__ __launch_bounds__(kPackThreads) void q4_pack_kernel(const uint32_t *_
 // A wave takes tiles: B of v_mfma_f32_16x16x32_f16 is the 16 features' codes, A the x rows, hi halves
 // in rows 0..7 and lo halves in rows 8..15, so that one product serves both. The rows' halves stay in
 // LDS; a workgroup splits them once and then walks its tiles; kw waves share a tile's contraction.
-// Bound by HBM past some 30 MB of weights, by the ramp (x's halves, the first loads) below: 131072
-// features of 4096, group 128, 51 us (5.5 TB/s of weights); 151936 of 1024, group 32 with zero points,
-// 21.3 (4.4); 14336 of 4096 11.1; 14335 of 4096, three rows, group 64 with zero points, 13.3; 4096 of
+// Bound by its weights' loads past some 30 MB, by the ramp (x's halves, the first loads) below: 131072
+// features of 4096, group 128, 51 us (5.5 TB/s of weights; a plain read reaches 6.4, and 7.1 with
+// non-temporal loads, which were not tried here); 151936 of 1024, group 32 with zero points, 21.3 to
+// 22.1 (4.4); 14336 of 4096 11.1; 14335 of 4096, three rows, group 64 with zero points, 13.3; 4096 of
 // 4096 5.9; 2048 of 1024 4.9.
 constexpr int kGemvWaves = 8;
 constexpr int kGemvThreads = kGemvWaves * 64;
@@ -455,8 +456,8 @@ __device__ __forceinline__ void copy_4kib(unsigned dst, const void *src) {
 // (64 KiB; a wave copies one plane of one 32-row block), and the weights loaded a stage ahead. All
 // of a stage's loads are waited for at its start; the empty asm on the weights there keeps the
 // compiler from waiting for them, and with them for the next stage's copies, at their first use.
-// Bound by the products: 1000 rows of 4096 to 4096 features, group 128, 70 to 76 us for 67 GFLOP of
-// halves (880 to 960 TFLOP/s; a library's f16 product of 8192^3 reaches 1134 here).
+// Bound by the products: 1000 rows of 4096 to 4096 features, group 128, 74 to 76 us for 67 GFLOP of
+// halves (880 to 900 TFLOP/s; a library's f16 product of 8192^3 reaches 1134 here).
 constexpr int kTileRows = 128, kTileCols = 128;
 constexpr int kTileThreads = 512;
 template <int G, bool ZERO>

@@ -127,10 +127,14 @@ eb_status move_i8(hipStream_t st, const char *what, const eb::CacheI8 &c, const 
 
 // Rows whose columns (rows x heads of a KV head) number at most this many run the few-row kernel,
 // which reads the cache once for every 16 of them; more rows run the prefill kernels over records.
-// Both measured, few-row and prefill, at 32 heads over 8 KV heads of 128 (4 columns a row): 16 rows
-// behind 1000 keys 14.7 and 20.3 us, 48 rows 22.5 and 28.6; behind 8192 keys 20 rows 26.7 and 46.2,
-// 48 rows 46.8 and 52.7, 64 rows 57.2 and 56.5; behind 32000 keys 48 rows 130 and 144. 16 over 8
-// heads of 256, 8192 keys: 64 rows (128 columns) 56.1 and 74.7.
+// Both measured (us, few-row and prefill): 192 columns of 32 heads over 8 KV heads of 128 behind 1000
+// keys 22.5 and 29.1, 8192 keys 47.0 and 56.3, 32000 keys 129 and 145; 256 columns 26.4 and 31.1, 57.0
+// and 57.0, 157 and 150. One head per KV head, 8 of 128: 192 columns 22.6 and 30.0, 47.8 and 53.1, 128
+// and 138, 256 columns 26.8 and 31.9, 57.4 and 56.3, 158 and 149. 14 over 2 heads of 64, 6 over 2 of
+// 96: few-row the faster through 256 columns (32000 keys 35.9 and 65.9, 48.6 and 66.0). 16 over 8 of
+// 256, 8192 keys: 128 columns 56.1 and 74.7. Where KV heads are many and short the sides meet
+// earlier: 16 over 16 of 64, 128 columns 18.0 and 23.8, 40.6 and 44.6, 115 and 126, but 192 columns
+// 20.3 and 23.5, 63.4 and 53.7, 197 and 159.
 constexpr size_t kFewRowCols = 192;
 
 size_t attn_workspace(size_t h, size_t hkv, size_t hd, size_t pos0, size_t rows, size_t window, size_t block, int cus) {

@@ -19,8 +19,9 @@
 //     listed tokens (a language model's logits list a few, up to some hundred where the cut lies
 //     in the wide floor) are ranked by counting, a token per thread.
 // Steps 2 and 3 do nothing for rows that need only the best token. A row whose steps list more
-// than kListed tokens (many equal logits; logits of enormous range) is solved by the choosing
-// workgroup alone, by radix selection over the row.
+// than kListed tokens (many equal logits; logits of enormous range; a mask that leaves fewer tokens
+// above -inf than top-k asks for) is solved by the choosing workgroup alone, by radix selection over
+// the row: 10 live tokens of 151936, top-k 50, 0.67 ms, and 1.2 with top-p 0.9 (23 us at top-k 5).
 //
 // Bound by four dependent launches. One row of 151936 (top-k 50, top-p 0.9): 2.9, 5.1, 6.2 and 7.5
 // us under a profiler, 22.3 in all; 64 rows of 32768: 4.5, 7.5, 11.2 and 12.2, 36 in all (8.4 MB, 1.6

@@ -573,7 +573,10 @@ eb_status eb_attention_forward(const eb_attention *attn, eb_recorder *rec, const
  * scale[o, k / group]. Every code less its zero point is exact in f16; the products run on the
  * matrix cores against a's rows split into two halves (about f32 accuracy, as linear_f16w's
  * many-row form), are summed in f32 within a group, and the groups' sums are scaled and added
- * in f32. The order of a sum depends on the shape alone.
+ * in f32. The same call gives the same bits; how a sum is shared out depends on m, on all weights
+ * of the launch and on the device's CU count, so that one call for q, k and v and three calls may
+ * differ in the last bits. A row of a that holds an infinity or NaN gives NaN in all its outputs,
+ * the other rows as without it.
  *
  * eb_q4_pack lays a weight out once, as the kernels read it: w holds codes 0..15 packed eight
  * per u32 word along k, lowest bits first (EB_U32 [out_f, in_f / 8]), scales is EB_F16 [out_f,
@@ -598,8 +601,9 @@ eb_status eb_linear_q4(eb_recorder *rec, const eb_tensor *a, const eb_q4_weight 
 eb_status eb_linear_q4_multi(eb_recorder *rec, const eb_tensor *a, size_t n,
                              const eb_q4_weight *w, eb_tensor *const *c, size_t m);
 /* On caller memory. packed is 16-byte aligned; the workspace (16-byte aligned, no
- * initialisation) holds the split rows of more than 8 rows, and of more than 32 the sums of
- * workgroups that share a contraction; launches that share one must not overlap. The raw pack is
+ * initialisation) holds the split rows of more than 8 rows (of fewer, where the contraction is too
+ * long for LDS), and of more than 32 the sums of workgroups that share a contraction; launches that
+ * share one must not overlap. The raw pack is
  * ordered on its stream alone. */
 eb_status eb_launch_q4_pack(void *stream, const uint32_t *w, size_t w_words,
                             const uint16_t *scales, size_t scales_numel, const uint8_t *zeros,
