@@ -860,8 +860,10 @@ constexpr size_t kMaxVocab = (size_t)1 << 24;
 // and top-p 0.9: 64 rows 57 us in runs of 2 and 65.5 a slice each, 256 rows 152 and 185.
 constexpr size_t kGroupsPerCu = 7;
 // A row's histogram and list take 45 KB whatever its vocabulary: rows beyond this many go through the
-// same workspace after the others (65535 rows would ask for 2.9 GB; these are 46 MB).
-constexpr size_t kBatchRows = 1024;
+// same workspace after the others (65535 rows would ask for 3 GB; these take 185 MB). Another batch
+// costs its launches and its tail: in batches of 1024, 2048 rows of 500 took 94 us instead of 81, 4096
+// of 32000 616 instead of 547.
+constexpr size_t kBatchRows = 4096;
 
 eb_status launch_batch(hipStream_t st, const eb::SampleArgs &s, float *ws) {
     Args a{};
