@@ -9,6 +9,7 @@ reference's Rust interface:
   linear_f16w (the projections around attention), plus chunked / windowed attention, the
   fused decode step and IEEE-half and OCP FP8 E4M3 caches; and a quantised model's operators:
   4-bit projections (linear_q4), block-scaled 8-bit caches (kv_write_i8, attn_*_i8), sampling;
+  and the verification of a drafted tree (tree_plan, attn_tree, tree_accept, kv_compact, kv_fork);
 - ``nn``: Linear, LinearQ4, Rope, KvCache, Attention (crates/eyebrowse-nn).
 """
 from ._lib import LIB_PATH, lib
@@ -37,7 +38,11 @@ from .kernels import (argmax, argmax_workspace_floats, attn_decode, attn_decode_
                       kv_write_i8, kv_read_i8, attn_decode_i8, attn_decode_step_i8,
                       attn_prefill_chunk_i8, attn_i8_workspace_floats, launch_kv_write_i8,
                       launch_kv_read_i8, launch_attn_decode_i8, launch_attn_prefill_chunk_i8,
-                      sample, sample_workspace_floats, launch_sample)
+                      sample, sample_workspace_floats, launch_sample,
+                      TREE_MAX, tree_plan, attn_prologue_tree, attn_tree, attn_tree_i8,
+                      attn_tree_workspace_floats, tree_accept, kv_compact, kv_fork,
+                      launch_tree_plan, launch_tree_accept, launch_attn_prologue_tree,
+                      launch_attn_tree, launch_attn_tree_i8)
 from ._lib import CacheI8
 from .nn import Attention, KvCache, Linear, LinearQ4, Rope
 
@@ -65,4 +70,7 @@ __all__ = [
     "attn_prefill_chunk_i8", "attn_i8_workspace_floats", "launch_kv_write_i8",
     "launch_kv_read_i8", "launch_attn_decode_i8", "launch_attn_prefill_chunk_i8", "sample",
     "sample_workspace_floats", "launch_sample",
+    "TREE_MAX", "tree_plan", "attn_prologue_tree", "attn_tree", "attn_tree_i8",
+    "attn_tree_workspace_floats", "tree_accept", "kv_compact", "kv_fork", "launch_tree_plan",
+    "launch_tree_accept", "launch_attn_prologue_tree", "launch_attn_tree", "launch_attn_tree_i8",
 ]

@@ -50,6 +50,9 @@ SOURCES = [
     "eb_decode_i8.hip",
     "eb_linear_q4.hip",
     "eb_sample.hip",
+    "eb_draft.cpp",
+    "eb_tree.hip",
+    "eb_tree_attn.hip",
 ]
 
 
@@ -62,6 +65,7 @@ SOURCE_FLAGS = {
     "eb_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "eb_decode_i8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "eb_linear_q4.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "eb_tree_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

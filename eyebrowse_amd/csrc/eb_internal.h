@@ -53,6 +53,9 @@ struct CacheI8 {
     size_t max_seq, hkv, hd, block;
 };
 
+// The caller's description of one, its shape and its buffers' sizes checked.
+eb_status cache_i8_of(const eb_cache_i8 *c, CacheI8 *out);
+
 // The device that owns a tensor.
 eb_device *tensor_device(const eb_tensor *t);
 
@@ -209,13 +212,15 @@ eb_status attn_decode_step_fused(eb_recorder *rec, const eb_tensor *q, const eb_
 // Attention::prefill between the projections and the attention as one launch: q/k/v
 // RMSNorm (null gains: none), RoPE of q and k at base_pos (null tables: none), q into
 // q_out [rows, h, hd] and K / V into cache rows base_pos.. (f32 or IEEE-half caches).
-// Handle-level, used by eb_attention_forward_qkv.
+// Handle-level, used by eb_attention_forward_qkv. depths (u32 [rows]; null: none): RoPE at
+// base_pos + depth instead of base_pos + row, as a drafted tree needs.
 eb_status attn_rows_fused(eb_recorder *rec, const eb_tensor *q, const eb_tensor *k,
                           const eb_tensor *v, eb_tensor *q_out, eb_tensor *kcache,
                           eb_tensor *vcache, size_t rows, size_t h, size_t hkv, size_t hd,
                           size_t base_pos, size_t max_seq, const eb_tensor *q_norm,
                           const eb_tensor *k_norm, const eb_tensor *v_norm, float eps,
-                          const eb_tensor *rope_cos, const eb_tensor *rope_sin);
+                          const eb_tensor *rope_cos, const eb_tensor *rope_sin,
+                          const eb_tensor *depths = nullptr);
 // linear_f16w: y[i][m, o] = sum_k x[m, k] * w[i][o, k] for nseg (1..kLinearMaxSegs)
 // weight/output pairs sharing x; w IEEE half [out_f[i], in_f]. m <= kLinearGemvRows runs
 // the weight-streaming kernel; more rows run the split-f16 matrix-core GEMM, which needs
@@ -283,6 +288,7 @@ struct RowsArgs {
     float eps;
     const float *cosb, *sinb;  // [>= rope_row0 + rows, hd / 2], null without RoPE
     int rope_row0;
+    const uint32_t *depths;  // [rows] in device memory: RoPE at rope_row0 + depth; null: + token
     int start[4];  // set by launch_attn_rows: first head row of each segment
 };
 eb_status launch_attn_rows(hipStream_t st, const RowsArgs &a);

@@ -280,10 +280,11 @@ extern "C" eb_status eb_attention_forward_qkv(const eb_attention *attn, eb_recor
 
 // Attention::forward with the projections (attention.rs:30-45; prefill :49-117, decode
 // :120-185): q/k/v = x . W^T in one launch, the post-projection part above, then o_proj.
-extern "C" eb_status eb_attention_forward(const eb_attention *attn, eb_recorder *rec,
-                                          const eb_tensor *x, const eb_rope_tables *rope,
-                                          eb_kv_cache *kv, size_t layer, size_t rows,
-                                          size_t base_pos, eb_tensor **out) {
+// With masks (and depths) the rows are a drafted tree's nodes.
+static eb_status forward_whole(const eb_attention *attn, eb_recorder *rec, const eb_tensor *x,
+                               const eb_rope_tables *rope, eb_kv_cache *kv, size_t layer,
+                               const eb_tensor *masks, const eb_tensor *depths, size_t rows,
+                               size_t base_pos, eb_tensor **out) {
     if (!attn || !rec || !x || !out) return fail(EB_OTHER, "attention_forward: null argument");
     *out = nullptr;
     const eb_attention_desc &d = attn->d;
@@ -309,8 +310,12 @@ extern "C" eb_status eb_attention_forward(const eb_attention *attn, eb_recorder 
     else
         EB_TRY(eb_linear_f16w_multi(rec, x, 3, w, c, of, rows, d.hidden));
     eb_tensor *ot = nullptr;
-    EB_TRY(eb_attention_forward_qkv(attn, rec, q.t, k.t, v.t, rope, kv, layer, rows, base_pos,
-                                    &ot));
+    if (masks)
+        EB_TRY(eb_attention_forward_tree_qkv(attn, rec, q.t, k.t, v.t, rope, kv, layer, masks,
+                                             depths, rows, base_pos, &ot));
+    else
+        EB_TRY(eb_attention_forward_qkv(attn, rec, q.t, k.t, v.t, rope, kv, layer, rows, base_pos,
+                                        &ot));
     Owned o(ot);
     const size_t ys[2] = {rows, d.hidden};
     eb_tensor *yt = nullptr;
@@ -322,4 +327,20 @@ extern "C" eb_status eb_attention_forward(const eb_attention *attn, eb_recorder 
         EB_TRY(eb_linear_f16w(rec, o.t, d.o_proj, y.t, rows, qd, d.hidden));
     *out = y.release();
     return eb::ok();
+}
+
+extern "C" eb_status eb_attention_forward(const eb_attention *attn, eb_recorder *rec,
+                                          const eb_tensor *x, const eb_rope_tables *rope,
+                                          eb_kv_cache *kv, size_t layer, size_t rows,
+                                          size_t base_pos, eb_tensor **out) {
+    return forward_whole(attn, rec, x, rope, kv, layer, nullptr, nullptr, rows, base_pos, out);
+}
+
+extern "C" eb_status eb_attention_forward_tree(const eb_attention *attn, eb_recorder *rec,
+                                               const eb_tensor *x, const eb_rope_tables *rope,
+                                               eb_kv_cache *kv, size_t layer,
+                                               const eb_tensor *masks, const eb_tensor *depths,
+                                               size_t rows, size_t base_pos, eb_tensor **out) {
+    if (!masks || !depths) return fail(EB_OTHER, "attention_forward_tree: null argument");
+    return forward_whole(attn, rec, x, rope, kv, layer, masks, depths, rows, base_pos, out);
 }

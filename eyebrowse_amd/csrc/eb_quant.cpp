@@ -63,20 +63,6 @@ eb_status shape_i8(size_t max_seq, size_t hkv, size_t hd, size_t block) {
     return EB_OK;
 }
 
-eb_status cache_of(const eb_cache_i8 *c, eb::CacheI8 *out) {
-    if (!c) return fail(EB_SHAPE_MISMATCH, "cache is null");
-    EB_TRY(shape_i8(c->max_seq, c->hkv, c->hd, c->block));
-    const size_t codes = c->max_seq * c->hkv * c->hd;
-    const size_t exps = (c->max_seq + c->block - 1) / c->block * c->hkv;
-    if (c->code_numel < codes)
-        return fail(EB_SHAPE_MISMATCH, "the cache's codes hold %zu elements, the shape needs %zu", c->code_numel, codes);
-    if (c->exp_numel < exps)
-        return fail(EB_SHAPE_MISMATCH, "the cache's exponents hold %zu bytes, the shape needs %zu", c->exp_numel, exps);
-    *out = eb::CacheI8{reinterpret_cast<uint8_t *>(c->k), c->k_exp, reinterpret_cast<uint8_t *>(c->v), c->v_exp,
-                       c->max_seq, c->hkv, c->hd, c->block};
-    return EB_OK;
-}
-
 eb_status cache_ready(const eb::CacheI8 &c) {
     EB_TRY(eb::check_ptr(c.k, "k codes"));
     EB_TRY(eb::check_ptr(c.ks, "k exponents"));
@@ -220,6 +206,20 @@ eb_status prologue_of(const eb_attention_desc &d, const eb_rope_tables *rope, si
 }
 
 }  // namespace
+
+eb_status eb::cache_i8_of(const eb_cache_i8 *c, CacheI8 *out) {
+    if (!c) return fail(EB_SHAPE_MISMATCH, "cache is null");
+    EB_TRY(shape_i8(c->max_seq, c->hkv, c->hd, c->block));
+    const size_t codes = c->max_seq * c->hkv * c->hd;
+    const size_t exps = (c->max_seq + c->block - 1) / c->block * c->hkv;
+    if (c->code_numel < codes)
+        return fail(EB_SHAPE_MISMATCH, "the cache's codes hold %zu elements, the shape needs %zu", c->code_numel, codes);
+    if (c->exp_numel < exps)
+        return fail(EB_SHAPE_MISMATCH, "the cache's exponents hold %zu bytes, the shape needs %zu", c->exp_numel, exps);
+    *out = CacheI8{reinterpret_cast<uint8_t *>(c->k), c->k_exp, reinterpret_cast<uint8_t *>(c->v), c->v_exp,
+                       c->max_seq, c->hkv, c->hd, c->block};
+    return EB_OK;
+}
 
 eb_status eb::attention_forward_i8(const eb_attention_desc &d, eb_recorder *rec, const eb_tensor *q,
                                    const eb_tensor *k, const eb_tensor *v, const eb_rope_tables *rope,
@@ -389,14 +389,14 @@ eb_status eb_attn_prefill_chunk_i8(eb_recorder *rec, const eb_tensor *q, const e
 eb_status eb_launch_kv_write_i8(void *stream, const eb_cache_i8 *cache, const float *k, const float *v, size_t numel,
                                 size_t count, size_t dst_start) {
     eb::CacheI8 c;
-    EB_TRY(cache_of(cache, &c));
+    EB_TRY(eb::cache_i8_of(cache, &c));
     return move_i8((hipStream_t)stream, "kv_write_i8", c, k, v, numel, count, dst_start, nullptr, nullptr);
 }
 
 eb_status eb_launch_kv_read_i8(void *stream, const eb_cache_i8 *cache, float *k, float *v, size_t numel, size_t count,
                                size_t src_start) {
     eb::CacheI8 c;
-    EB_TRY(cache_of(cache, &c));
+    EB_TRY(eb::cache_i8_of(cache, &c));
     return move_i8((hipStream_t)stream, "kv_read_i8", c, k, v, numel, count, src_start, k, v);
 }
 
@@ -413,7 +413,7 @@ eb_status eb_launch_attn_decode_i8(void *stream, const float *q, size_t q_numel,
                                    size_t pos, float scale, size_t window, float *workspace, size_t workspace_floats,
                                    int cu_count) {
     eb::CacheI8 c;
-    EB_TRY(cache_of(cache, &c));
+    EB_TRY(eb::cache_i8_of(cache, &c));
     EB_TRY(attn_checked(c, q, q_numel, o, o_numel, h, pos, 1));
     if (knew || vnew) EB_TRY(step_checked(c, knew, vnew, new_numel));
     return attend_i8((hipStream_t)stream, Room{nullptr, workspace, workspace_floats}, cu_count > 0 ? cu_count : 256, c,
@@ -424,7 +424,7 @@ eb_status eb_launch_attn_prefill_chunk_i8(void *stream, const float *q, size_t q
                                           float *o, size_t o_numel, size_t h, size_t pos0, size_t rows, float scale,
                                           size_t window, float *workspace, size_t workspace_floats, int cu_count) {
     eb::CacheI8 c;
-    EB_TRY(cache_of(cache, &c));
+    EB_TRY(eb::cache_i8_of(cache, &c));
     EB_TRY(attn_checked(c, q, q_numel, o, o_numel, h, pos0, rows));
     return attend_i8((hipStream_t)stream, Room{nullptr, workspace, workspace_floats}, cu_count > 0 ? cu_count : 256, c,
                      q, nullptr, nullptr, o, h, pos0, rows, scale, window);

@@ -7,7 +7,8 @@
 // segments of head rows (q, k, v: [rows, nh, HD] each) and for each row does
 //  - RMSNorm with a gain when the segment has one: y = x * (1 / sqrt(sum x^2 / HD + eps)) * w
 //    (kernels/src/rmsnorm.rs:6-38, per head: rows * heads rows of HD),
-//  - RoPE at table row rope_row0 + token when the segment asks for it: dims p and p + HD/2
+//  - RoPE at table row rope_row0 + token (or + the token's depth, in a drafted tree) when the segment
+//    asks for it: dims p and p + HD/2
 //    become (x1 c - x2 s, x2 c + x1 s) with the table's angle p (kernels/src/rope.rs:6-32;
 //    pass-through pairs have c = 1, s = 0),
 //  - a store into row dst_row0 + token of a [*, nh, HD] destination of f32, IEEE-half or
@@ -22,6 +23,8 @@
 // and lane swaps. Other even head dims (and unaligned buffers) take one wave per head row.
 #include "eb_common.h"
 #include "eb_internal.h"
+
+#include <type_traits>
 
 namespace {
 
@@ -72,7 +75,10 @@ __device__ __forceinline__ SegView seg_of(const eb::RowsArgs &a, int t) {
 // and angles after it, a row took two memory latencies. Gemma-4 (us, whole call): 1000 rows into
 // E4M3 71.8 -> 69.6, 500 rows 44.6 -> 43.7, 2000 rows 177.8 -> 176.5 (two rows per lane 177.3).
 // Bound by HBM beyond that: 131 MB in 22 us at 2000 rows.
-template <int LPR>
+//
+// TREE: a token's table row is rope_row0 + its depth, read with the row (a.depths; the angles then
+// wait for it). A depth past the launch's rows, which no tree has, makes the rotated row NaN.
+template <int LPR, bool TREE>
 __global__ __launch_bounds__(kThreads) void rows_vec_kernel(eb::RowsArgs a) {
 #pragma clang fp contract(off)
     constexpr int RPW = 64 / LPR;  // head rows per wave
@@ -96,8 +102,15 @@ __global__ __launch_bounds__(kThreads) void rows_vec_kernel(eb::RowsArgs a) {
         g1 = *reinterpret_cast<const f32x4 *>(sv.gain + jj);
         g2 = *reinterpret_cast<const f32x4 *>(sv.gain + half + jj);
     }
+    bool off_table = false;
     if (sv.rope) {
-        const size_t trow = (size_t)(a.rope_row0 + tok) * half + jj;
+        int turn = tok;
+        if constexpr (TREE) {
+            const unsigned depth = a.depths[tok];
+            off_table = depth >= (unsigned)a.rows;
+            turn = off_table ? 0 : (int)depth;
+        }
+        const size_t trow = (size_t)(a.rope_row0 + turn) * half + jj;
         c = *reinterpret_cast<const f32x4 *>(a.cosb + trow);
         s = *reinterpret_cast<const f32x4 *>(a.sinb + trow);
     }
@@ -118,6 +131,8 @@ __global__ __launch_bounds__(kThreads) void rows_vec_kernel(eb::RowsArgs a) {
         const f32x4 y2 = x2 * c + x1 * s;
         x1 = y1;
         x2 = y2;
+        if constexpr (TREE)
+            if (off_table) x1 = x2 = z + __builtin_nanf("");
     }
     const size_t d = ((size_t)(sv.dst_row0 + tok) * sv.nh + hh) * hd + 4 * j;
     if (sv.elem == 2) {
@@ -136,6 +151,7 @@ __global__ __launch_bounds__(kThreads) void rows_vec_kernel(eb::RowsArgs a) {
 }
 
 // Any even head dim: one wave per head row, lanes striding its RoPE pairs.
+template <bool TREE>
 __global__ __launch_bounds__(kThreads) void rows_wave_kernel(eb::RowsArgs a) {
 #pragma clang fp contract(off)
     const int lane = threadIdx.x & 63;
@@ -155,7 +171,14 @@ __global__ __launch_bounds__(kThreads) void rows_wave_kernel(eb::RowsArgs a) {
         inv = 1.0f / sqrtf(ss / (float)hd + a.eps);
     }
     const size_t d = ((size_t)(sv.dst_row0 + tok) * sv.nh + hh) * hd;
-    const size_t trow = (size_t)(a.rope_row0 + tok) * half;
+    int turn = tok;
+    bool off_table = false;
+    if constexpr (TREE) {
+        const unsigned depth = a.depths[tok];
+        off_table = depth >= (unsigned)a.rows;
+        turn = off_table ? 0 : (int)depth;
+    }
+    const size_t trow = (size_t)(a.rope_row0 + turn) * half;
     for (int p = lane; p < half; p += 64) {
         float x1 = src[p], x2 = src[p + half];
         if (sv.gain) {
@@ -168,6 +191,8 @@ __global__ __launch_bounds__(kThreads) void rows_wave_kernel(eb::RowsArgs a) {
             const float y2 = x2 * c + x1 * s;
             x1 = y1;
             x2 = y2;
+            if constexpr (TREE)
+                if (off_table) x1 = x2 = __builtin_nanf("");
         }
         if (sv.elem == 2) {
             _Float16 *o = static_cast<_Float16 *>(sv.dst) + d;
@@ -205,20 +230,31 @@ eb_status launch_attn_rows(hipStream_t st, const RowsArgs &args) {
     }
     vec = vec && aligned(a.cosb, 16) && aligned(a.sinb, 16);
     if (!vec) {
-        rows_wave_kernel<<<(unsigned)((total + kWaves - 1) / kWaves), kThreads, 0, st>>>(a);
+        const unsigned waves = (unsigned)((total + kWaves - 1) / kWaves);
+        if (a.depths)
+            rows_wave_kernel<true><<<waves, kThreads, 0, st>>>(a);
+        else
+            rows_wave_kernel<false><<<waves, kThreads, 0, st>>>(a);
         return check_launch("attention rows");
     }
     int lpr = 1;
     while (lpr < a.hd / 8) lpr *= 2;
     const int per_block = kWaves * (64 / lpr);
     const unsigned grid = (unsigned)((total + per_block - 1) / per_block);
+    const auto run = [&](auto lanes) {
+        constexpr int LPR = decltype(lanes)::value;
+        if (a.depths)
+            rows_vec_kernel<LPR, true><<<grid, kThreads, 0, st>>>(a);
+        else
+            rows_vec_kernel<LPR, false><<<grid, kThreads, 0, st>>>(a);
+    };
     switch (lpr) {
-        case 1: rows_vec_kernel<1><<<grid, kThreads, 0, st>>>(a); break;
-        case 2: rows_vec_kernel<2><<<grid, kThreads, 0, st>>>(a); break;
-        case 4: rows_vec_kernel<4><<<grid, kThreads, 0, st>>>(a); break;
-        case 8: rows_vec_kernel<8><<<grid, kThreads, 0, st>>>(a); break;
-        case 16: rows_vec_kernel<16><<<grid, kThreads, 0, st>>>(a); break;
-        default: rows_vec_kernel<32><<<grid, kThreads, 0, st>>>(a); break;
+        case 1: run(std::integral_constant<int, 1>()); break;
+        case 2: run(std::integral_constant<int, 2>()); break;
+        case 4: run(std::integral_constant<int, 4>()); break;
+        case 8: run(std::integral_constant<int, 8>()); break;
+        case 16: run(std::integral_constant<int, 16>()); break;
+        default: run(std::integral_constant<int, 32>()); break;
     }
     return check_launch("attention rows");
 }

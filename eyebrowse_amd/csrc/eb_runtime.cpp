@@ -963,7 +963,8 @@ static eb_status prologue_checked(hipStream_t st, const float *q, size_t qn, con
                                   const float *gv, float eps, const float *rc, const float *rs,
                                   size_t tn, size_t base_pos, float *q_out, size_t qon,
                                   void *kc, size_t kcn, void *vc, size_t vcn, size_t max_seq,
-                                  eb::CacheElem ce) {
+                                  eb::CacheElem ce, const uint32_t *depths = nullptr,
+                                  size_t depths_n = 0) {
     EB_TRY(eb::check_heads(h, hkv));
     if (hd == 0 || hd % 2 != 0)
         return fail(EB_SHAPE_MISMATCH, "attention prologue: head_dim must be even and > 0");
@@ -978,6 +979,7 @@ static eb_status prologue_checked(hipStream_t st, const float *q, size_t qn, con
     EB_TRY(eb::check_numel(vcn, {max_seq, hkv, hd}, "vcache"));
     if ((rc == nullptr) != (rs == nullptr)) return fail(EB_OTHER, "RoPE needs both tables");
     if (rc) EB_TRY(eb::check_numel(tn, {(base_pos + rows), (hd / 2)}, "rope tables"));
+    if (depths) EB_TRY(eb::check_numel(depths_n, rows, "depths"));
     if (rows == 0) return eb::ok();
     EB_TRY(eb::check_ptr(q, "q"));
     EB_TRY(eb::check_ptr(k, "k"));
@@ -997,6 +999,7 @@ static eb_status prologue_checked(hipStream_t st, const float *q, size_t qn, con
     a.cosb = rc;
     a.sinb = rs;
     a.rope_row0 = (int)base_pos;
+    a.depths = depths;
     EB_TRY(eb::launch_attn_rows(st, a));
     return eb::ok();
 }
@@ -1430,8 +1433,10 @@ eb_status eb::attn_rows_fused(eb_recorder *rec, const eb_tensor *q, const eb_ten
                               eb_tensor *vcache, size_t rows, size_t h, size_t hkv, size_t hd,
                               size_t base_pos, size_t max_seq, const eb_tensor *q_norm,
                               const eb_tensor *k_norm, const eb_tensor *v_norm, float eps,
-                              const eb_tensor *rope_cos, const eb_tensor *rope_sin) {
+                              const eb_tensor *rope_cos, const eb_tensor *rope_sin,
+                              const eb_tensor *depths) {
     EB_TRY(rec_ready(rec));
+    if (depths) EB_TRY(check_tensor(depths, EB_U32, "depths", rec->dev));
     EB_TRY(tensor_f32(q, "q", rec->dev));
     EB_TRY(tensor_f32(k, "k", rec->dev));
     EB_TRY(tensor_f32(v, "v", rec->dev));
@@ -1463,7 +1468,9 @@ eb_status eb::attn_rows_fused(eb_recorder *rec, const eb_tensor *q, const eb_ten
         rope_cos ? static_cast<const float *>(rope_cos->ptr) : nullptr,
         rope_sin ? static_cast<const float *>(rope_sin->ptr) : nullptr, tn, base_pos,
         static_cast<float *>(q_out->ptr), eb_tensor_numel(q_out), kcache->ptr,
-        eb_tensor_numel(kcache), vcache->ptr, eb_tensor_numel(vcache), max_seq, ce);
+        eb_tensor_numel(kcache), vcache->ptr, eb_tensor_numel(vcache), max_seq, ce,
+        depths ? static_cast<const uint32_t *>(depths->ptr) : nullptr,
+        depths ? eb_tensor_numel(depths) : 0);
 }
 
 extern "C" {
@@ -1808,6 +1815,30 @@ eb_status eb_launch_attn_prologue(void *stream, const float *q, size_t q_numel, 
                             cache_dtype == EB_F16      ? eb::CacheElem::F16
                             : cache_dtype == EB_F8E4M3 ? eb::CacheElem::E4M3
                                                        : eb::CacheElem::F32);
+}
+
+eb_status eb_launch_attn_prologue_tree(void *stream, const float *q, size_t q_numel,
+                                       const float *k, size_t k_numel, const float *v,
+                                       size_t v_numel, size_t rows, size_t h, size_t hkv,
+                                       size_t hd, const float *q_norm, const float *k_norm,
+                                       const float *v_norm, float eps, const float *rope_cos,
+                                       const float *rope_sin, size_t table_numel,
+                                       size_t base_pos, const uint32_t *depths,
+                                       size_t depths_numel, float *q_out, size_t q_out_numel,
+                                       void *kcache, size_t kc_numel, void *vcache,
+                                       size_t vc_numel, size_t max_seq, eb_dtype cache_dtype) {
+    if (cache_dtype != EB_F32 && cache_dtype != EB_F16 && cache_dtype != EB_F8E4M3)
+        return fail(EB_UNSUPPORTED_CONFIG,
+                    "attention prologue: caches must be f32, f16 or f8e4m3");
+    if (rows > 0) EB_TRY(eb::check_ptr(depths, "depths"));
+    return prologue_checked((hipStream_t)stream, q, q_numel, k, k_numel, v, v_numel, rows, h, hkv,
+                            hd, q_norm, k_norm, v_norm, eps, rope_cos, rope_sin, table_numel,
+                            base_pos, q_out, q_out_numel, kcache, kc_numel, vcache, vc_numel,
+                            max_seq,
+                            cache_dtype == EB_F16      ? eb::CacheElem::F16
+                            : cache_dtype == EB_F8E4M3 ? eb::CacheElem::E4M3
+                                                       : eb::CacheElem::F32,
+                            depths, depths_numel);
 }
 
 eb_status eb_launch_rope(void *stream, const float *x, size_t x_numel, const float *cos,

@@ -1,0 +1,334 @@
+// A drafted tree's plan, the walk that accepts a branch of it, and the rows that are moved for that,
+// for gfx950.
+//
+// Plan and walk are integers of at most kTreeMax nodes: one workgroup, a node per thread, bound by
+// latency. Both follow parents by doubling: after r rounds a node knows its ancestors within 2^r
+// steps, so a tree of depth d takes log2(d) rounds of two barriers instead of d dependent reads.
+//
+// The copies are bound by HBM: every byte read once and written once.
+#include "eb_cache_i8.h"
+#include "eb_tree.h"
+
+#include <algorithm>
+
+namespace {
+
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kNodes = (int)eb::kTreeMax;
+constexpr int kWords = kNodes / 32;
+constexpr int kThreads = 256;
+constexpr unsigned kNobody = 0xFFFFFFFFu;
+
+static_assert(kNodes == kThreads, "a node per thread");
+
+// A parent is an earlier node; anything else is none.
+__device__ __forceinline__ int parent_of(const int *parents, int i) {
+    const int p = parents[i];
+    return p >= 0 && p < i ? p : -1;
+}
+
+// masks[i] = node i and its ancestors, as bits; depths[i] = how many ancestors it has.
+__global__ __launch_bounds__(kThreads) void tree_plan_kernel(const int *__restrict__ parents,
+                                                             unsigned *__restrict__ masks,
+                                                             unsigned *__restrict__ depths, int n) {
+    __shared__ unsigned s_mask[kWords][kNodes];
+    __shared__ int s_up[kNodes];
+    const int i = threadIdx.x;
+    const int words = (n + 31) / 32;
+    int up = i < n ? parent_of(parents, i) : -1;
+    unsigned mask[kWords];
+#pragma unroll
+    for (int w = 0; w < kWords; ++w) mask[w] = w == i / 32 ? 1u << (i % 32) : 0u;
+    while (__syncthreads_or(up >= 0)) {
+        s_up[i] = up;
+#pragma unroll
+        for (int w = 0; w < kWords; ++w)
+            if (w < words) s_mask[w][i] = mask[w];
+        __syncthreads();
+        if (up >= 0) {
+#pragma unroll
+            for (int w = 0; w < kWords; ++w)
+                if (w < words) mask[w] |= s_mask[w][up];
+            up = s_up[up];
+        }
+    }
+    if (i >= n) return;
+    int depth = -1;
+#pragma unroll
+    for (int w = 0; w < kWords; ++w) {
+        if (w >= words) continue;
+        masks[i * words + w] = mask[w];
+        depth += __popc(mask[w]);
+    }
+    depths[i] = (unsigned)depth;
+}
+
+// The branch that the model's own tokens follow from node 0: from a node on to its first child whose
+// token is the node's sampled one. path[j] = its j-th node, emitted[j] = that node's sampled token.
+__global__ __launch_bounds__(kThreads) void tree_accept_kernel(const unsigned *__restrict__ tokens,
+                                                               const int *__restrict__ parents,
+                                                               const unsigned *__restrict__ sampled,
+                                                               unsigned *__restrict__ path,
+                                                               unsigned *__restrict__ emitted,
+                                                               unsigned *__restrict__ count, int n) {
+    __shared__ unsigned s_sampled[kNodes], s_first[kNodes], s_ok[kNodes];
+    __shared__ int s_up[kNodes], s_dist[kNodes];
+    const int i = threadIdx.x;
+    const bool in = i < n;
+    int up = in && i > 0 ? parent_of(parents, i) : -1;
+    const unsigned token = in ? tokens[i] : 0u, mine = in ? sampled[i] : 0u;
+    s_sampled[i] = mine;
+    s_first[i] = kNobody;
+    __syncthreads();
+    if (up >= 0 && token == s_sampled[up]) atomicMin(&s_first[up], (unsigned)i);
+    __syncthreads();
+    // Taken from its parent; then from all ancestors up to node 0, `dist` steps away.
+    unsigned ok = i == 0 || (up >= 0 && s_first[up] == (unsigned)i);
+    int dist = up >= 0 ? 1 : 0;
+    while (__syncthreads_or(up >= 0)) {
+        s_ok[i] = ok;
+        s_dist[i] = dist;
+        s_up[i] = up;
+        __syncthreads();
+        if (up >= 0) {
+            ok &= s_ok[up];
+            dist += s_dist[up];
+            up = s_up[up];
+        }
+    }
+    const int accepted = __syncthreads_count(in && ok);
+    if (!in) return;
+    if (i >= accepted) path[i] = emitted[i] = kNobody;
+    if (ok) {
+        path[dist] = (unsigned)i;
+        emitted[dist] = mine;
+    }
+    if (i == 0) *count = (unsigned)accepted;
+}
+
+// A path of rows to move, as a kernel takes it: as long as its entries are nodes and increase, hence
+// path[j] >= j, and a row is read before, or by the same thread that, another one is moved onto it.
+// Returns its length; the entries are in s_path.
+__device__ __forceinline__ int load_path(const unsigned *path, const unsigned *count, int n, unsigned *s_path,
+                                         unsigned *s_end) {
+    const int i = threadIdx.x;
+    const unsigned c = *count;
+    if (i == 0) *s_end = c < (unsigned)n ? c : (unsigned)n;
+    const unsigned p = i < n ? path[i] : kNobody;
+    s_path[i] = p;
+    __syncthreads();
+    if (i < n && (p >= (unsigned)n || (i > 0 && p <= s_path[i - 1]))) atomicMin(s_end, (unsigned)i);
+    __syncthreads();
+    return (int)*s_end;
+}
+
+constexpr int kMaxLayers = (int)eb::kMoveLayers;
+struct CompactArgs {
+    eb::CacheRows layer[kMaxLayers];
+    const unsigned *path, *count;
+    size_t pos;
+    int n;
+};
+
+// Workgroup (x, layer and side): 256 vectors of V of each row. A thread moves its vector of every row,
+// kBatch rows read before the first is written.
+template <class V>
+__global__ __launch_bounds__(kThreads) void kv_compact_kernel(CompactArgs a) {
+    __shared__ unsigned s_path[kNodes];
+    __shared__ unsigned s_end;
+    constexpr int kBatch = 8;
+    const eb::CacheRows &layer = a.layer[blockIdx.y >> 1];
+    V *cache = static_cast<V *>(blockIdx.y & 1 ? layer.v : layer.k);
+    const size_t per_row = layer.row_bytes / sizeof(V);
+    const int end = load_path(a.path, a.count, a.n, s_path, &s_end);
+    const size_t x = (size_t)blockIdx.x * kThreads + threadIdx.x;
+    if (x >= per_row) return;
+    cache += a.pos * per_row + x;
+    int j = 0;
+    while (j < end && s_path[j] == (unsigned)j) ++j;  // (rows that stay)
+    for (; j < end; j += kBatch) {
+        V row[kBatch];
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b)
+            if (j + b < end) row[b] = cache[s_path[j + b] * per_row];
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b)
+            if (j + b < end) cache[(j + b) * per_row] = row[b];
+    }
+}
+
+struct CompactI8Args {
+    struct Layer {
+        uint8_t *codes[2], *exps[2];
+        int hd;
+    } layer[kMaxLayers];
+    const unsigned *path, *count;
+    size_t pos;
+    int n, hkv, block;
+};
+
+// Workgroup (head, layer and side): the branch's rows as the values they stand for, written at pos as
+// any rows are: block by block, with the least exponent that holds them and the block's earlier rows.
+// All codes and exponents are in LDS before the first is overwritten; no other workgroup touches them.
+__global__ __launch_bounds__(kThreads) void kv_compact_i8_kernel(CompactI8Args a) {
+    extern __shared__ unsigned s_code[];  // [n][hd / 4]
+    __shared__ unsigned s_path[kNodes], s_exp[kNodes];
+    __shared__ unsigned s_end, s_top;
+    const CompactI8Args::Layer &layer = a.layer[blockIdx.y >> 1];
+    const int side = blockIdx.y & 1, head = blockIdx.x, tid = threadIdx.x;
+    const int per_row = layer.hd / 4;
+    const size_t stride = (size_t)a.hkv * layer.hd;
+    uint8_t *codes = layer.codes[side] + (size_t)head * layer.hd;
+    uint8_t *exps = layer.exps[side] + head;
+    const int end = load_path(a.path, a.count, a.n, s_path, &s_end);
+    auto word = [&](size_t row, int w) { return reinterpret_cast<unsigned *>(codes + row * stride + 4 * w); };
+    for (int i = tid; i < end * per_row; i += kThreads) s_code[i] = *word(a.pos + s_path[i / per_row], i % per_row);
+    if (tid < end) s_exp[tid] = exps[(a.pos + s_path[tid]) / a.block * a.hkv];
+    __syncthreads();
+    for (int lo = 0; lo < end;) {
+        const size_t b = (a.pos + lo) / a.block, first = b * a.block;
+        const int hi = (int)(first + a.block - a.pos) < end ? (int)(first + a.block - a.pos) : end;
+        const int lead = lo == 0 ? (int)(a.pos - first) : 0;  // earlier rows of the block
+        if (tid == 0) s_top = 0;
+        __syncthreads();
+        unsigned top = 0;
+        for (int i = lo * per_row + tid; i < hi * per_row; i += kThreads) {
+            const float f = eb::i8_scale(s_exp[i / per_row], 0);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) top = max(top, eb::magnitude_bits(eb::i8_f32(s_code[i], c) * f));
+        }
+#pragma unroll
+        for (int m = 32; m > 0; m >>= 1) top = max(top, __shfl_xor(top, m));
+        if ((tid & 63) == 0) atomicMax(&s_top, top);
+        const unsigned old_e = lead ? exps[b * a.hkv] : 0u;
+        __syncthreads();
+        unsigned e = eb::i8_exponent(s_top);
+        if (lead) e = eb::i8_join(old_e, e);
+        for (int i = lo * per_row + tid; i < hi * per_row; i += kThreads) {
+            const float f = eb::i8_scale(s_exp[i / per_row], 0);
+            unsigned w = 0;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) w |= eb::i8_code(eb::i8_f32(s_code[i], c) * f, e) << (8 * c);
+            *word(a.pos + i / per_row, i % per_row) = w;
+        }
+        if (lead && e != old_e && e != eb::kNanExponent) {
+            for (int i = tid; i < lead * per_row; i += kThreads) {
+                unsigned *p = word(first + i / per_row, i % per_row);
+                *p = eb::i8_recode(*p, old_e, e);
+            }
+        }
+        __syncthreads();  // (every thread has read the old exponent and s_top)
+        if (tid == 0) exps[b * a.hkv] = (uint8_t)e;
+        lo = hi;
+    }
+}
+
+constexpr int kMaxRuns = 2 * kMaxLayers;
+constexpr int kRunUnroll = 8;
+constexpr size_t kRunChunk = (size_t)kThreads * 16 * kRunUnroll;  // bytes a workgroup copies
+struct RunArgs {
+    eb::ByteRun run[kMaxRuns];
+};
+
+// Workgroup (x, run): chunk x of the run, 16 bytes per lane and access, all of a thread's loads
+// before its stores; a run's last 15 bytes one by one.
+__global__ __launch_bounds__(kThreads) void copy_runs_kernel(RunArgs a) {
+    const eb::ByteRun &r = a.run[blockIdx.y];
+    const size_t at = (size_t)blockIdx.x * kRunChunk;
+    if (at >= r.bytes) return;
+    const size_t vecs = r.bytes / 16, v0 = at / 16 + threadIdx.x;
+    const u32x4 *src = static_cast<const u32x4 *>(r.src);
+    u32x4 *dst = static_cast<u32x4 *>(r.dst);
+    u32x4 x[kRunUnroll];
+#pragma unroll
+    for (int i = 0; i < kRunUnroll; ++i) {
+        const size_t v = v0 + (size_t)i * kThreads;
+        if (v < vecs) x[i] = __builtin_nontemporal_load(src + v);
+    }
+#pragma unroll
+    for (int i = 0; i < kRunUnroll; ++i) {
+        const size_t v = v0 + (size_t)i * kThreads;
+        if (v < vecs) __builtin_nontemporal_store(x[i], dst + v);
+    }
+    if (at + kRunChunk >= r.bytes && threadIdx.x < r.bytes % 16) {
+        const size_t t = vecs * 16 + threadIdx.x;
+        static_cast<uint8_t *>(r.dst)[t] = static_cast<const uint8_t *>(r.src)[t];
+    }
+}
+
+}  // namespace
+
+namespace eb {
+
+eb_status launch_tree_plan(hipStream_t st, const int32_t *parents, uint32_t *masks, uint32_t *depths, size_t n) {
+    tree_plan_kernel<<<1, kThreads, 0, st>>>(parents, masks, depths, (int)n);
+    return check_launch("tree_plan");
+}
+
+eb_status launch_tree_accept(hipStream_t st, const uint32_t *tokens, const int32_t *parents, const uint32_t *sampled,
+                             uint32_t *path, uint32_t *emitted, uint32_t *count, size_t n) {
+    tree_accept_kernel<<<1, kThreads, 0, st>>>(tokens, parents, sampled, path, emitted, count, (int)n);
+    return check_launch("tree_accept");
+}
+
+eb_status launch_kv_compact(hipStream_t st, const CacheRows *layers, size_t n_layers, const uint32_t *path,
+                            const uint32_t *count, size_t n, size_t pos) {
+    CompactArgs a{};
+    a.path = path;
+    a.count = count;
+    a.pos = pos;
+    a.n = (int)n;
+    size_t most = 0;
+    bool wide = true;
+    for (size_t l = 0; l < n_layers; ++l) {
+        a.layer[l] = layers[l];
+        most = std::max(most, layers[l].row_bytes);
+        wide = wide && layers[l].row_bytes % 16 == 0;
+    }
+    if (most == 0) return EB_OK;
+    const size_t per_wg = kThreads * (wide ? 16 : 4);
+    const dim3 grid((unsigned)((most + per_wg - 1) / per_wg), (unsigned)(2 * n_layers));
+    if (wide)
+        kv_compact_kernel<u32x4><<<grid, kThreads, 0, st>>>(a);
+    else
+        kv_compact_kernel<unsigned><<<grid, kThreads, 0, st>>>(a);
+    return check_launch("kv_compact");
+}
+
+eb_status launch_kv_compact_i8(hipStream_t st, const CacheI8 *layers, size_t n_layers, const uint32_t *path,
+                               const uint32_t *count, size_t n, size_t pos) {
+    CompactI8Args a{};
+    a.path = path;
+    a.count = count;
+    a.pos = pos;
+    a.n = (int)n;
+    size_t hd = 0;
+    for (size_t l = 0; l < n_layers; ++l) {
+        const CacheI8 &c = layers[l];
+        a.layer[l] = {{c.k, c.v}, {c.ks, c.vs}, (int)c.hd};
+        hd = std::max(hd, c.hd);
+    }
+    a.hkv = (int)layers[0].hkv;
+    a.block = (int)layers[0].block;
+    constexpr int kMost = kNodes * 256;  // (the widest tree and head: 64 KB, beside 2 KB of paths)
+    static const hipError_t room = hipFuncSetAttribute(reinterpret_cast<const void *>(&kv_compact_i8_kernel),
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, kMost);
+    if (room != hipSuccess) return hip_fail(room, "kv_compact_i8 launch set-up");
+    kv_compact_i8_kernel<<<dim3((unsigned)a.hkv, (unsigned)(2 * n_layers)), kThreads, n * hd, st>>>(a);
+    return check_launch("kv_compact_i8");
+}
+
+eb_status launch_copy_runs(hipStream_t st, const ByteRun *runs, size_t n) {
+    RunArgs a{};
+    size_t most = 0;
+    for (size_t r = 0; r < n; ++r) {
+        a.run[r] = runs[r];
+        most = std::max(most, runs[r].bytes);
+    }
+    if (most == 0) return EB_OK;
+    copy_runs_kernel<<<dim3((unsigned)((most + kRunChunk - 1) / kRunChunk), (unsigned)n), kThreads, 0, st>>>(a);
+    return check_launch("kv_fork");
+}
+
+}  // namespace eb

@@ -527,3 +527,124 @@ def launch_attn_decode_step_noalloc(stream: int, q: int, q_numel: int, knew: int
     check(lib().eb_launch_attn_decode_step_noalloc(stream, q, q_numel, knew, vnew, new_numel, kc,
                                                    kc_numel, vc, vc_numel, o, o_numel, h, hkv,
                                                    pos, hd, max_seq, scale, cu_count))
+
+
+# ---- a tree of drafted tokens (no counterpart in the reference) ------------------------------
+
+def _opt(t):
+    return t.handle if t is not None else None
+
+
+TREE_MAX = 256  # nodes of a drafted tree
+
+
+def tree_plan(rec: Recorder, parents: Tensor, masks: Tensor, depths: Tensor, n: int) -> None:
+    """parents (I32 [n]; -1: none) -> masks (U32 [n, ceil(n / 32)], each node and its ancestors as
+    bits) and depths (U32 [n])."""
+    check(lib().eb_tree_plan(rec.handle, parents.handle, masks.handle, depths.handle, n))
+
+
+def attn_prologue_tree(rec: Recorder, q: Tensor, k: Tensor, v: Tensor, depths: Tensor,
+                       q_out: Tensor, kcache: Tensor, vcache: Tensor, rows: int, h: int, hkv: int,
+                       hd: int, base_pos: int, max_seq: int, q_norm, k_norm, v_norm, eps: float,
+                       rope_cos, rope_sin) -> None:
+    """launch_attn_prologue's work for a drafted tree: node i's rotation at table row base_pos +
+    depths[i], its K and V into cache row base_pos + i. Gains and tables may be None."""
+    check(lib().eb_attn_prologue_tree(rec.handle, q.handle, k.handle, v.handle, depths.handle,
+                                      q_out.handle, kcache.handle, vcache.handle, rows, h, hkv, hd,
+                                      base_pos, max_seq, _opt(q_norm), _opt(k_norm), _opt(v_norm),
+                                      eps, _opt(rope_cos), _opt(rope_sin)))
+
+
+def attn_tree(rec: Recorder, q: Tensor, kcache: Tensor, vcache: Tensor, masks: Tensor, depths,
+              o: Tensor, h: int, hkv: int, pos: int, n: int, hd: int, max_seq: int, scale: float,
+              window: int = 0) -> None:
+    """q, o [n, h, hd]: node i attends cache rows 0..pos-1 and the drafted rows pos + j with bit j
+    of masks' row i; with a window, those above its position pos + depths[i] less window (depths
+    may be None without one). Caches f32, f16 or E4M3."""
+    check(lib().eb_attn_tree(rec.handle, q.handle, kcache.handle, vcache.handle, masks.handle,
+                             _opt(depths), o.handle, h, hkv, pos, n, hd, max_seq, scale, window))
+
+
+def attn_tree_i8(rec: Recorder, q: Tensor, kv, layer: int, masks: Tensor, depths, o: Tensor, h: int,
+                 pos: int, n: int, scale: float, window: int = 0) -> None:
+    """attn_tree over a block-scaled KvCache's layer."""
+    check(lib().eb_attn_tree_i8(rec.handle, q.handle, kv.handle, layer, masks.handle, _opt(depths),
+                                o.handle, h, pos, n, scale, window))
+
+
+def attn_tree_workspace_floats(h: int, hkv: int, pos: int, n: int, hd: int, dtype: int,
+                               cu_count: int = 256) -> int:
+    """Floats of workspace the raw tree attention needs, for any window (dtype: the cache's)."""
+    return int(lib().eb_attn_tree_workspace_floats(h, hkv, pos, n, hd, int(dtype), cu_count))
+
+
+def tree_accept(rec: Recorder, tokens: Tensor, parents: Tensor, sampled: Tensor, path: Tensor,
+                emitted: Tensor, count: Tensor, n: int) -> None:
+    """The branch that the sampled tokens (U32 [n], one per node) follow through the drafted ones:
+    path (its nodes), emitted (the step's tokens), both U32 [n], 0xFFFFFFFF past count (U32 [1])."""
+    check(lib().eb_tree_accept(rec.handle, tokens.handle, parents.handle, sampled.handle,
+                               path.handle, emitted.handle, count.handle, n))
+
+
+def kv_compact(rec: Recorder, kv, path: Tensor, count: Tensor, n: int, pos: int) -> None:
+    """Rows pos + path[j] of every layer of a KvCache to rows pos + j, j < count, in place."""
+    check(lib().eb_kv_compact(rec.handle, kv.handle, path.handle, count.handle, n, pos))
+
+
+def kv_fork(rec: Recorder, dst, src, count: int) -> None:
+    """Rows 0..count-1 of every layer of the KvCache src into dst."""
+    check(lib().eb_kv_fork(rec.handle, dst.handle, src.handle, count))
+
+
+def launch_tree_plan(stream: int, parents: int, parents_numel: int, masks: int, masks_numel: int,
+                     depths: int, depths_numel: int, n: int) -> None:
+    """eb_launch_tree_plan: device pointers and the elements they hold."""
+    check(lib().eb_launch_tree_plan(stream, parents, parents_numel, masks, masks_numel, depths,
+                                    depths_numel, n))
+
+
+def launch_tree_accept(stream: int, tokens: int, tokens_numel: int, parents: int,
+                       parents_numel: int, sampled: int, sampled_numel: int, path: int,
+                       path_numel: int, emitted: int, emitted_numel: int, count: int,
+                       n: int) -> None:
+    """eb_launch_tree_accept: device pointers and the elements they hold."""
+    check(lib().eb_launch_tree_accept(stream, tokens, tokens_numel, parents, parents_numel, sampled,
+                                      sampled_numel, path, path_numel, emitted, emitted_numel,
+                                      count, n))
+
+
+def launch_attn_prologue_tree(stream: int, q: int, q_numel: int, k: int, k_numel: int, v: int,
+                              v_numel: int, rows: int, h: int, hkv: int, hd: int, q_norm: int,
+                              k_norm: int, v_norm: int, eps: float, rope_cos: int, rope_sin: int,
+                              table_numel: int, base_pos: int, depths: int, depths_numel: int,
+                              q_out: int, q_out_numel: int, kcache: int, kc_numel: int, vcache: int,
+                              vc_numel: int, max_seq: int, cache_dtype: int) -> None:
+    """eb_launch_attn_prologue_tree: launch_attn_prologue with a depth per row."""
+    check(lib().eb_launch_attn_prologue_tree(stream, q, q_numel, k, k_numel, v, v_numel, rows, h,
+                                             hkv, hd, q_norm, k_norm, v_norm, eps, rope_cos,
+                                             rope_sin, table_numel, base_pos, depths, depths_numel,
+                                             q_out, q_out_numel, kcache, kc_numel, vcache,
+                                             vc_numel, max_seq, int(cache_dtype)))
+
+
+def launch_attn_tree(stream: int, q: int, q_numel: int, kc: int, kc_numel: int, vc: int,
+                     vc_numel: int, dtype: int, masks: int, masks_numel: int, depths: int,
+                     depths_numel: int, o: int, o_numel: int, h: int, hkv: int, pos: int, n: int,
+                     hd: int, max_seq: int, scale: float, window: int, workspace: int,
+                     workspace_floats: int, cu_count: int = 256) -> None:
+    """eb_launch_attn_tree: attn_tree on device pointers."""
+    check(lib().eb_launch_attn_tree(stream, q, q_numel, kc, kc_numel, vc, vc_numel, int(dtype),
+                                    masks, masks_numel, depths, depths_numel, o, o_numel, h, hkv,
+                                    pos, n, hd, max_seq, scale, window, workspace,
+                                    workspace_floats, cu_count))
+
+
+def launch_attn_tree_i8(stream: int, q: int, q_numel: int, cache: CacheI8, masks: int,
+                        masks_numel: int, depths: int, depths_numel: int, o: int, o_numel: int,
+                        h: int, pos: int, n: int, scale: float, window: int, workspace: int,
+                        workspace_floats: int, cu_count: int = 256) -> None:
+    """eb_launch_attn_tree_i8: attn_tree_i8 on device pointers."""
+    check(lib().eb_launch_attn_tree_i8(stream, q, q_numel, ctypes.byref(cache), masks, masks_numel,
+                                       depths, depths_numel, o, o_numel, h, pos, n, scale, window,
+                                       workspace, workspace_floats, cu_count))

@@ -269,6 +269,27 @@ class Attention:
                                          layer, rows, base_pos, ctypes.byref(out)))
         return Tensor(out.value, rec.dev)
 
+    def forward_tree_qkv(self, rec: Recorder, q: Tensor, k: Tensor, v: Tensor, rope: Rope,
+                         kv: KvCache, layer: int, masks: Tensor, depths: Tensor, rows: int,
+                         base_pos: int) -> Tensor:
+        """forward_qkv for the nodes of a drafted tree (no counterpart in the reference): node i at
+        position base_pos + depths[i], in cache row base_pos + i, seeing the cached keys and the
+        nodes of masks' row i (tree_plan gives both)."""
+        out = c_vp()
+        check(lib().eb_attention_forward_tree_qkv(self._h, rec.handle, q.handle, k.handle, v.handle,
+                                                  rope.handle, kv.handle, layer, masks.handle,
+                                                  depths.handle, rows, base_pos, ctypes.byref(out)))
+        return Tensor(out.value, rec.dev)
+
+    def forward_tree(self, rec: Recorder, x: Tensor, rope: Rope, kv: KvCache, layer: int,
+                     masks: Tensor, depths: Tensor, rows: int, base_pos: int) -> Tensor:
+        """forward for the nodes of a drafted tree: x [rows, hidden] -> [rows, hidden]."""
+        out = c_vp()
+        check(lib().eb_attention_forward_tree(self._h, rec.handle, x.handle, rope.handle, kv.handle,
+                                              layer, masks.handle, depths.handle, rows, base_pos,
+                                              ctypes.byref(out)))
+        return Tensor(out.value, rec.dev)
+
     def __del__(self):
         h = getattr(self, "_h", None)
         if h is not None and h.value:

@@ -718,6 +718,118 @@ eb_status eb_launch_sample(void *stream, const float *logits, size_t logits_nume
                            const float *temperature, const uint32_t *top_k, const float *top_p,
                            const float *min_p, float *workspace, size_t workspace_floats);
 
+/* ---- a tree of drafted tokens (no counterpart in the reference) --------------------------
+ * A draft proposes several continuations at once, and one pass over the cache answers for all of
+ * them. A tree has n nodes (1 to 256). Node 0 is its root: the last token that is certain, whose row
+ * the cache does not hold yet. parents[i] (EB_I32) is an earlier node, or -1; anything else counts
+ * as -1. Node i's K and V go to cache row pos + i, its position is pos + depth[i].
+ *
+ * A step: eb_tree_plan; per layer eb_attention_forward_tree; logits of all nodes; a token for each
+ * of them (eb_sample, one row per node; or the largest logit, at temperature 0); eb_tree_accept;
+ * eb_kv_compact. The cache then holds rows up to pos + count, and the last emitted token is the next
+ * root. The emitted tokens are the ones that decoding one by one would sample from the same numbers u
+ * at those nodes: a node is accepted exactly if the token sampled at its parent is its own.
+ * Trees, paths and counts are read from device memory when the work runs (a captured graph replays
+ * with another tree of n nodes); n and pos are arguments.
+ *
+ * eb_tree_plan: masks (EB_U32 [n, ceil(n / 32)]), row i = node i itself and its ancestors, node j as
+ * bit j % 32 of word j / 32; depths (EB_U32 [n]) = how many ancestors each has. */
+eb_status eb_tree_plan(eb_recorder *rec, const eb_tensor *parents, eb_tensor *masks,
+                       eb_tensor *depths, size_t n);
+eb_status eb_launch_tree_plan(void *stream, const int32_t *parents, size_t parents_numel,
+                              uint32_t *masks, size_t masks_numel, uint32_t *depths,
+                              size_t depths_numel, size_t n);
+/* eb_launch_attn_prologue's work (per-head RMSNorm where a gain is given, RoPE, K and V into cache
+ * rows base_pos.., q into q_out) with node i's rotation at table row base_pos + depths[i]. The tables
+ * reach base_pos + rows. A depth of rows or more, which no tree has, makes the node's rotated q and K
+ * NaN. Caches f32, f16 or E4M3. */
+eb_status eb_attn_prologue_tree(eb_recorder *rec, const eb_tensor *q, const eb_tensor *k,
+                                const eb_tensor *v, const eb_tensor *depths, eb_tensor *q_out,
+                                eb_tensor *kcache, eb_tensor *vcache, size_t rows, size_t h,
+                                size_t hkv, size_t hd, size_t base_pos, size_t max_seq,
+                                const eb_tensor *q_norm, const eb_tensor *k_norm,
+                                const eb_tensor *v_norm, float eps, const eb_tensor *rope_cos,
+                                const eb_tensor *rope_sin);
+eb_status eb_launch_attn_prologue_tree(void *stream, const float *q, size_t q_numel,
+                                       const float *k, size_t k_numel, const float *v,
+                                       size_t v_numel, size_t rows, size_t h, size_t hkv,
+                                       size_t hd, const float *q_norm, const float *k_norm,
+                                       const float *v_norm, float eps, const float *rope_cos,
+                                       const float *rope_sin, size_t table_numel,
+                                       size_t base_pos, const uint32_t *depths,
+                                       size_t depths_numel, float *q_out, size_t q_out_numel,
+                                       void *kcache, size_t kc_numel, void *vcache,
+                                       size_t vc_numel, size_t max_seq, eb_dtype cache_dtype);
+/* q, o [n, h, hd]: node i attends cache rows 0..pos - 1 and those rows pos + j whose bit j is set in
+ * row i of masks (any bits; those past n are ignored). With window > 0 it sees only rows whose
+ * position is above its own less window, a drafted row's position being pos + depths[j]; depths may
+ * be NULL without a window. A node that sees nothing gives zeros. f32 accuracy over every cache
+ * (f32, f16, E4M3; eb_attn_tree_i8: block-scaled): products on f16 matrix cores of f32 values in two
+ * halves, 22 bits. Values of K or V that are not finite reach the nodes that see their row, whose
+ * heads become NaN, and no others. At most 256 query heads per KV head. The same call gives the same
+ * bits. */
+eb_status eb_attn_tree(eb_recorder *rec, const eb_tensor *q, const eb_tensor *kcache,
+                       const eb_tensor *vcache, const eb_tensor *masks, const eb_tensor *depths,
+                       eb_tensor *o, size_t h, size_t hkv, size_t pos, size_t n, size_t hd,
+                       size_t max_seq, float scale, size_t window);
+eb_status eb_attn_tree_i8(eb_recorder *rec, const eb_tensor *q, const eb_kv_cache *kv,
+                          size_t layer, const eb_tensor *masks, const eb_tensor *depths,
+                          eb_tensor *o, size_t h, size_t pos, size_t n, float scale,
+                          size_t window);
+/* On caller memory: q, o, the caches and the workspace 16-byte aligned. dtype is the caches'
+ * (EB_I8 for the block-scaled form's workspace); a workspace serves any window, needs no
+ * initialisation, and launches that share one must not overlap. */
+size_t eb_attn_tree_workspace_floats(size_t h, size_t hkv, size_t pos, size_t n, size_t hd,
+                                     eb_dtype dtype, int cu_count);
+eb_status eb_launch_attn_tree(void *stream, const float *q, size_t q_numel, const void *kc,
+                              size_t kc_numel, const void *vc, size_t vc_numel, eb_dtype dtype,
+                              const uint32_t *masks, size_t masks_numel, const uint32_t *depths,
+                              size_t depths_numel, float *o, size_t o_numel, size_t h, size_t hkv,
+                              size_t pos, size_t n, size_t hd, size_t max_seq, float scale,
+                              size_t window, float *workspace, size_t workspace_floats,
+                              int cu_count);
+eb_status eb_launch_attn_tree_i8(void *stream, const float *q, size_t q_numel,
+                                 const eb_cache_i8 *cache, const uint32_t *masks,
+                                 size_t masks_numel, const uint32_t *depths, size_t depths_numel,
+                                 float *o, size_t o_numel, size_t h, size_t pos, size_t n,
+                                 float scale, size_t window, float *workspace,
+                                 size_t workspace_floats, int cu_count);
+/* eb_attention_forward[_qkv] for a tree: norms, RoPE at the nodes' positions, their rows into the
+ * cache at base_pos.., eb_attn_tree with the layer's window. x [rows, hidden], q [rows,
+ * n_heads*hd], k / v [rows, n_kv_heads*hd]; any cache. */
+eb_status eb_attention_forward_tree_qkv(const eb_attention *attn, eb_recorder *rec,
+                                        const eb_tensor *q, const eb_tensor *k,
+                                        const eb_tensor *v, const eb_rope_tables *rope,
+                                        eb_kv_cache *kv, size_t layer, const eb_tensor *masks,
+                                        const eb_tensor *depths, size_t rows, size_t base_pos,
+                                        eb_tensor **out);
+eb_status eb_attention_forward_tree(const eb_attention *attn, eb_recorder *rec,
+                                    const eb_tensor *x, const eb_rope_tables *rope,
+                                    eb_kv_cache *kv, size_t layer, const eb_tensor *masks,
+                                    const eb_tensor *depths, size_t rows, size_t base_pos,
+                                    eb_tensor **out);
+/* The branch that the sampled tokens follow (all EB_U32 [n] but parents): from node 0 on, a node's
+ * first child (the lowest index) whose token is sampled[node]. path[j] = its j-th node (path[0] = 0),
+ * emitted[j] = sampled[path[j]], count[0] = its nodes, 1 to n; path and emitted are 0xFFFFFFFF from
+ * count on. emitted[0..count) are the step's new tokens; the last of them has no row yet. */
+eb_status eb_tree_accept(eb_recorder *rec, const eb_tensor *tokens, const eb_tensor *parents,
+                         const eb_tensor *sampled, eb_tensor *path, eb_tensor *emitted,
+                         eb_tensor *count, size_t n);
+eb_status eb_launch_tree_accept(void *stream, const uint32_t *tokens, size_t tokens_numel,
+                                const int32_t *parents, size_t parents_numel,
+                                const uint32_t *sampled, size_t sampled_numel, uint32_t *path,
+                                size_t path_numel, uint32_t *emitted, size_t emitted_numel,
+                                uint32_t *count, size_t n);
+/* Moves rows pos + path[j] of every layer's K and V to rows pos + j, j < min(count[0], n), in place.
+ * The path counts up to its first entry that is not below n or not above the one before. The rows
+ * behind keep what they hold. Any cache; a block-scaled one is read and written as eb_kv_read_i8 and
+ * eb_kv_write_i8 do. */
+eb_status eb_kv_compact(eb_recorder *rec, eb_kv_cache *kv, const eb_tensor *path,
+                        const eb_tensor *count, size_t n, size_t pos);
+/* Rows 0..count - 1 of every layer's K and V of src into dst: the same prompt continued twice. The
+ * caches have the same layers, heads, elements and block; their max_seq may differ. Bit-exact. */
+eb_status eb_kv_fork(eb_recorder *rec, eb_kv_cache *dst, const eb_kv_cache *src, size_t count);
+
 /* ---- self-check (no counterpart in the reference) ----------------------------------
  * One wave applies the lane exchanges that every wave reduction in the kernels is built
  * from (16- and 32-lane swaps, DPP row rotations and mirrors) to in[0..64) = a and
