@@ -52,12 +52,24 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 using eb::TreeElem;
 
-constexpr int kWaves = 4;
-constexpr int kThreads = kWaves * 64;
 constexpr float kSlack = 8.0f;     // log2 units a score may exceed its reference by
 constexpr float kTop = 32768.0f;   // largest weight of a term (f16 holds 65504)
 constexpr float kUnit = 7.0f;      // log2 of a weight at its reference
-constexpr int kNone = 0x7FFFFFF0;  // a byte offset past any tile
+constexpr float kNoRef = -1.0e30f;  // a reference below all scores: no key yet
+constexpr unsigned kNone = 0x7FFFFFF0u;  // a byte offset past any tile
+
+// Waves of a workgroup, and 32-key groups of a tile. About 32 KB of the cache are in flight for every
+// four waves. One wave's columns (cw 1): the waves share the tile's keys. Up to 64: each wave has its
+// own 16. More: 32 columns to a wave, eight waves, the halves of the tile's keys to four each, so that
+// what is staged, and what a split leaves for the merge, serves twice the columns.
+constexpr int waves_of(int nset) { return nset == 2 ? 8 : 4; }
+constexpr int key_groups(int hdp, TreeElem e, int cw, int nset) {
+    const bool f32 = e == TreeElem::F32, f16 = e == TreeElem::F16;
+    if (hdp == 256) return f32 || (f16 && cw > 1) ? 1 : 2;
+    if (cw == 1) return f32 ? hdp == 64 ? 2 : 1 : 4;
+    if (nset == 2) return f32 ? 2 : f16 && hdp == 128 ? 2 : 4;
+    return f32 ? hdp == 64 ? 2 : 1 : f16 && hdp == 128 ? 2 : 4;
+}
 
 template <int HDP, TreeElem E, int CW, int NSET>
 struct Shape {
@@ -65,27 +77,33 @@ struct Shape {
     static constexpr bool SCALED = E == TreeElem::F32 || E == TreeElem::I8;
     static constexpr int ES = F32 ? 4 : E == TreeElem::F16 ? 2 : 1;  // bytes of an element
     static constexpr int PL = F32 ? 2 : 1;                           // f16 planes
-    // 32-key groups per tile: about 32 KB of cache in flight per workgroup, at most 64 KB of LDS.
-    static constexpr int KG = F32 ? (HDP == 64 ? 2 : 1) : HDP == 256 ? 2 : (ES == 2 && HDP == 128) ? 2 : 4;
+    static constexpr int WAVES = waves_of(NSET), THREADS = WAVES * 64, HT = THREADS / 2;
+    static constexpr int KG = key_groups(HDP, E, CW, NSET);
     static constexpr int T = 32 * KG;
-    static constexpr int KW = std::min(KG, kWaves / CW);  // waves that share a column's tile
+    static constexpr int KW = std::min(KG, WAVES / CW);  // waves that share a column's tile
     static constexpr int COLS = CW * NSET * 16;
-    static constexpr int PLANE = T * HDP * 2;  // bytes of one plane of K, and of V
-    static constexpr int TILE = 2 * PL * PLANE + 2 * T * 4;
-    static constexpr int NBUF = TILE > 40 * 1024 ? 1 : 2;
     static constexpr int NC = HDP / 32;  // 32-dim steps of a score
     static constexpr int ND = HDP / 16;  // 16-dim groups of an output
-    static constexpr int CH = HDP / 8;   // 8-dim chunks of a K row
+    static constexpr int CH = HDP / 8;   // 8-dim chunks of a K row in LDS
     static constexpr int SW = (CH < 16 ? CH : 16) - 1;
-    static constexpr int HT = kThreads / 2;
-    static constexpr int KU = T * CH / HT;  // K chunks per thread
-    static constexpr int VD = F32 ? 4 : 8;  // dims of a V unit (8 keys)
+    static constexpr int PLANE = T * HDP * 2;  // bytes of one plane of K, and of V
+    static constexpr int TILE = 2 * PL * PLANE + 2 * T * 4;
+    // q's low halves of 32 columns over f32 caches: in LDS, the registers do not hold them.
+    static constexpr bool QLDS = F32 && NSET == 2;
+    static constexpr int QBYTES = QLDS ? CW * NSET * NC * 1024 : 0;
+    static constexpr int NBUF = TILE > (NSET == 2 ? 64 : 40) * 1024 ? 1 : F32 && NSET == 2 ? 1 : 2;
+    static constexpr int WGS = NSET == 2 || (F32 && HDP == 256) ? 1 : 2;  // workgroups per CU
+    static constexpr int LD = 16 / ES;               // dims of a 16-byte load
+    static constexpr int KL = HDP / (F32 ? 8 : LD);  // K units of a row: 8 dims (f32), or a load
+    static constexpr int KU = T * KL / HT;           // and per thread
+    // V units: 8 keys by VD dims, a row's in VB bytes.
+    static constexpr int VD = NSET == 2 && !F32 ? LD / 2 : LD;
+    static constexpr int VW = VD * ES / 4;  // words of a unit's row
     static constexpr int VC = HDP / VD;
     static constexpr int VUNITS = 4 * KG * VC;
     static constexpr int VU = (VUNITS + HT - 1) / HT;
-    static constexpr int RW = ES == 1 ? 2 : 4;  // words of a load
-    static constexpr int NR = std::max(KU * (F32 ? 2 : 1), VU * 8);
-    static_assert(KW == 1 || (KW - 1) * CW * NSET * (ND * 1024 + 768) <= TILE * NBUF, "room to join waves");
+    static constexpr int NR = std::max(KU * (F32 ? 8 : 4), VU * 8 * VW);
+    static_assert((KW - 1) * CW * (ND * 1024 + 512) <= TILE * NBUF, "room to join waves");
 };
 
 struct Args {
@@ -102,12 +120,13 @@ struct Args {
     float scale_log2;
 };
 
-// The largest of N neighbouring lanes' values (N a power of two from 8 to 64), in each of them.
+// The largest of N neighbouring lanes' values, in each of them.
 template <int N>
 __device__ __forceinline__ float lanes_max(float x) {
     x = fmaxf(x, eb::dpp<eb::kDppQuadXor1>(x));
     x = fmaxf(x, eb::dpp<eb::kDppQuadXor2>(x));
-    x = fmaxf(x, eb::dpp<eb::kDppRowHalfMirror>(x));
+    static_assert(N == 4 || N == 8 || N == 16 || N == 32 || N == 64, "a power of two from 4 to 64");
+    if constexpr (N >= 8) x = fmaxf(x, eb::dpp<eb::kDppRowHalfMirror>(x));
     if constexpr (N >= 16) x = fmaxf(x, eb::dpp<eb::kDppRowMirror>(x));
     if constexpr (N >= 32) x = fmaxf(x, eb::lane_xor16(x));
     if constexpr (N >= 64) x = fmaxf(x, eb::lane_xor32(x));
@@ -139,16 +158,19 @@ __device__ __forceinline__ u32x2 narrow_f16(unsigned w) {
     }
 }
 
-// x as two halves, each rounded to nearest: 22 bits.
+// x as two halves, each rounded to nearest: 22 bits. (A fused multiply-add takes the half as it is.)
 __device__ __forceinline__ void split(f32x8 x, f16x8 &hi, f16x8 &lo) {
     hi = __builtin_convertvector(x, f16x8);
-    lo = __builtin_convertvector(x - __builtin_convertvector(hi, f32x8), f16x8);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __builtin_fmaf((float)hi[i], -1.0f, x[i]);
+    lo = __builtin_convertvector(x, f16x8);
 }
 
 template <int HDP, TreeElem E, int CW, int NSET>
-__global__ __launch_bounds__(kThreads, 2) void tree_attn_kernel(Args a) {
+__global__ __launch_bounds__(waves_of(NSET) * 64, (Shape<HDP, E, CW, NSET>::WGS * waves_of(NSET) / 4)) void tree_attn_kernel(Args a) {
     using S = Shape<HDP, E, CW, NSET>;
     constexpr int ES = S::ES, T = S::T, KW = S::KW, PL = S::PL, PLANE = S::PLANE, HT = S::HT;
+    constexpr int kWaves = S::WAVES, kThreads = S::THREADS;
     extern __shared__ char smem[];
     // Consecutive workgroups of an XCD (dealt round robin) take the column blocks of one KV head and
     // split, which then share that XCD's L2.
@@ -166,7 +188,8 @@ __global__ __launch_bounds__(kThreads, 2) void tree_attn_kernel(Args a) {
     const int col0 = cb * S::COLS;
     const int node0 = node_of(col0);
     const int nodes = node_of(min(col0 + S::COLS, a.ncols) - 1) - node0 + 1;  // of this workgroup's columns
-    unsigned *s_mask = reinterpret_cast<unsigned *>(smem + S::NBUF * S::TILE);  // [nodes][words]
+    char *s_ql = smem + S::NBUF * S::TILE;  // [CW][NSET][NC][lane]
+    unsigned *s_mask = reinterpret_cast<unsigned *>(s_ql + S::QBYTES);          // [nodes][words]
     int *s_depth = reinterpret_cast<int *>(s_mask + nodes * a.words);           // [n] (with a window)
 
     // ---- tiles: fetched into registers, then stored as operands -----------------------------------
@@ -174,45 +197,52 @@ __global__ __launch_bounds__(kThreads, 2) void tree_attn_kernel(Args a) {
     const int ht = tid % HT;
     const size_t row_bytes = (size_t)a.hkv * hd * ES;
     const char *base = (vside ? a.v : a.k) + (size_t)kvh * hd * ES;
-    unsigned raw[S::NR][S::RW];
+    unsigned raw[S::NR];
     unsigned raw_e = 127;  // I8: the exponent of key ht (1 past the last)
     auto fetch = [&](int t) {
         const int r0 = a.key0 + t * T;
         const int left = min(end - r0, T);
         const int nbytes = left > 0 ? (int)((left - 1) * row_bytes) + hd * ES : 0;
         const __amdgpu_buffer_rsrc_t res = eb::make_rsrc(base + (left > 0 ? (size_t)r0 * row_bytes : 0), nbytes);
-        auto get = [&](int i, int off) {
-            if constexpr (S::RW == 4) {
-                const u32x4 w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(res, off, 0, 0));
+        auto get = [&](int at, unsigned off) {
+            const u32x4 w = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(res, off, 0, 0));
 #pragma unroll
-                for (int j = 0; j < 4; ++j) raw[i][j] = w[j];
-            } else {
-                const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(res, off, 0, 0));
-#pragma unroll
-                for (int j = 0; j < 2; ++j) raw[i][j] = w[j];
-            }
+            for (int i = 0; i < 4; ++i) raw[at + i] = w[i];
         };
-        const int rb = (int)row_bytes;
+        // A lane whose dims the row does not have reads past the end from its first row on (unsigned
+        // offsets do not wrap: kNone plus a tile's bytes).
+        const unsigned rb = (unsigned)row_bytes;
         if (!vside) {
-            const int c = ht % S::CH, r = ht / S::CH;
+            const int c = ht % S::KL, r = ht / S::KL;
+            if constexpr (S::F32) {
+                const unsigned o0 = 8 * c < hd ? r * rb + c * 32 : kNone, o1 = 8 * c + 4 < hd ? o0 + 16 : kNone;
 #pragma unroll
-            for (int j = 0; j < S::KU; ++j) {
-                const int off = (r + j * (HT / S::CH)) * rb + c * 8 * ES;
-                if constexpr (S::F32) {
-                    get(2 * j, 8 * c < hd ? off : kNone);
-                    get(2 * j + 1, 8 * c + 4 < hd ? off + 16 : kNone);
-                } else {
-                    get(j, 8 * c < hd ? off : kNone);
+                for (int j = 0; j < S::KU; ++j) {
+                    get(8 * j, o0 + j * (HT / S::KL) * rb);
+                    get(8 * j + 4, o1 + j * (HT / S::KL) * rb);
                 }
+            } else {
+                const unsigned o0 = c * S::LD < hd ? r * rb + c * 16 : kNone;
+#pragma unroll
+                for (int j = 0; j < S::KU; ++j) get(4 * j, o0 + j * (HT / S::KL) * rb);
             }
         } else {
 #pragma unroll
             for (int j = 0; j < S::VU; ++j) {
                 const int u = ht + j * HT, c = u % S::VC, sb = u / S::VC;
-                const bool in = u < S::VUNITS && c * S::VD < hd;
-                const int off = (32 * (sb / 4) + 4 * (sb % 4)) * rb + c * S::VD * ES;
+                const unsigned o0 = u < S::VUNITS && c * S::VD < hd ? (32 * (sb / 4) + 4 * (sb % 4)) * rb + c * S::VW * 4 : kNone;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) get(8 * j + i, in ? off + (i + (i & 4) * 3) * rb : kNone);
+                for (int i = 0; i < 8; ++i) {
+                    const unsigned off = o0 + (i + (i & 4) * 3) * rb;
+                    const int at = (8 * j + i) * S::VW;
+                    if constexpr (S::VW == 4) {
+                        get(at, off);
+                    } else {
+                        const u32x2 w = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(res, off, 0, 0));
+                        raw[at] = w[0];
+                        raw[at + 1] = w[1];
+                    }
+                }
             }
         }
         if constexpr (E == TreeElem::I8) {
@@ -224,30 +254,36 @@ __global__ __launch_bounds__(kThreads, 2) void tree_attn_kernel(Args a) {
     auto store = [&](char *buf, bool edge) {
         float *s_scale = reinterpret_cast<float *>(buf + 2 * PL * PLANE);
         if (!vside) {
-            const int c = ht % S::CH, r0 = ht / S::CH;
+            const int c = ht % S::KL, r0 = ht / S::KL;
 #pragma unroll
             for (int j = 0; j < S::KU; ++j) {
-                const int r = r0 + j * (HT / S::CH);
-                char *at = buf + (r * S::CH + (c ^ (r & S::SW))) * 16;
+                const int r = r0 + j * (HT / S::KL);
+                auto at = [&](int chunk) { return buf + (r * S::CH + (chunk ^ (r & S::SW))) * 16; };
                 if constexpr (S::F32) {
                     f32x8 x;
                     float top = 0.0f;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        x[i] = __uint_as_float(raw[2 * j + i / 4][i % 4]);
-                        top = fmaxf(top, __uint_as_float(raw[2 * j + i / 4][i % 4] & 0x7FFFFFFFu));
+                        x[i] = __uint_as_float(raw[8 * j + i]);
+                        top = fmaxf(top, __uint_as_float(raw[8 * j + i] & 0x7FFFFFFFu));
                     }
-                    const unsigned e = biased_exponent(lanes_max<S::CH>(top));
+                    const unsigned e = biased_exponent(lanes_max<S::KL>(top));
                     f16x8 hi, lo;
                     split(x * pow2_biased(267u - e), hi, lo);
-                    *reinterpret_cast<f16x8 *>(at) = hi;
-                    *reinterpret_cast<f16x8 *>(at + PLANE) = lo;
+                    *reinterpret_cast<f16x8 *>(at(c)) = hi;
+                    *reinterpret_cast<f16x8 *>(at(c) + PLANE) = lo;
                     if (c == 0) s_scale[r] = pow2_biased(e - 13u);
                 } else if constexpr (ES == 2) {
-                    *reinterpret_cast<u32x4 *>(at) = u32x4{raw[j][0], raw[j][1], raw[j][2], raw[j][3]};
+                    *reinterpret_cast<u32x4 *>(at(c)) = u32x4{raw[4 * j], raw[4 * j + 1], raw[4 * j + 2], raw[4 * j + 3]};
                 } else {
-                    const u32x2 x = narrow_f16<E>(raw[j][0]), y = narrow_f16<E>(raw[j][1]);
-                    *reinterpret_cast<u32x4 *>(at) = u32x4{x[0], x[1], y[0], y[1]};
+                    const bool whole = E == TreeElem::I8 || 16 * c + 8 < hd;  // (else the next head's)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const u32x2 x = narrow_f16<E>(raw[4 * j + 2 * half]), y = narrow_f16<E>(raw[4 * j + 2 * half + 1]);
+                        u32x4 w = {x[0], x[1], y[0], y[1]};
+                        if (half && !whole) w = u32x4{0u, 0u, 0u, 0u};
+                        *reinterpret_cast<u32x4 *>(at(2 * c + half)) = w;
+                    }
                 }
             }
         } else {
@@ -263,7 +299,7 @@ __global__ __launch_bounds__(kThreads, 2) void tree_attn_kernel(Args a) {
                     float back[8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const unsigned *w = raw[8 * j + i];
+                        const unsigned *w = raw + (8 * j + i) * 4;
                         x[i] = f32x4{__uint_as_float(w[0]), __uint_as_float(w[1]), __uint_as_float(w[2]),
                                      __uint_as_float(w[3])};
                         unsigned bits = 0;  // (as whole numbers: NaN is above infinity)
@@ -292,32 +328,25 @@ __global__ __launch_bounds__(kThreads, 2) void tree_attn_kernel(Args a) {
                         *reinterpret_cast<f16x8 *>(at + PLANE) = lo;
                     }
                 } else {
-                    unsigned x[8][4];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        if constexpr (ES == 2) {
-#pragma unroll
-                            for (int d = 0; d < 4; ++d) x[i][d] = raw[8 * j + i][d];
-                        } else {
-                            const u32x2 p = narrow_f16<E>(raw[8 * j + i][0]), q = narrow_f16<E>(raw[8 * j + i][1]);
-                            x[i][0] = p[0];
-                            x[i][1] = p[1];
-                            x[i][2] = q[0];
-                            x[i][3] = q[1];
-                        }
-                    }
                     if constexpr (E != TreeElem::I8) {
-                        if (edge) {
+                        if (edge) {  // rows that are not finite: zeros, and NaN for the weight
                             float back[8];
 #pragma unroll
                             for (int i = 0; i < 8; ++i) {
+                                unsigned *w = raw + (8 * j + i) * S::VW;
                                 bool bad = false;
 #pragma unroll
-                                for (int d = 0; d < 4; ++d)
-                                    bad = bad || (x[i][d] & 0x7C00u) == 0x7C00u || (x[i][d] & 0x7C000000u) == 0x7C000000u;
+                                for (int d = 0; d < S::VW; ++d) {
+                                    if constexpr (ES == 2) {
+                                        bad = bad | ((w[d] & 0x7C00u) == 0x7C00u) | ((w[d] & 0x7C000000u) == 0x7C000000u);
+                                    } else {  // (dims from hd on are the next head's)
+                                        const unsigned m = w[d] & 0x7F7F7F7Fu;  // NaN is 0x7F: a carry into the sign bit
+                                        bad = bad | ((((m + 0x01010101u) & 0x80808080u) != 0u) & (c * S::VD + 4 * d < hd));
+                                    }
+                                }
                                 bad = lanes_max<S::VC>(bad ? 1.0f : 0.0f) > 0.0f;
 #pragma unroll
-                                for (int d = 0; d < 4; ++d) x[i][d] = bad ? 0u : x[i][d];
+                                for (int d = 0; d < S::VW; ++d) w[d] = bad ? 0u : w[d];
                                 back[i] = bad ? __builtin_nanf("") : 1.0f;
                             }
                             if (c == 0) {
@@ -327,13 +356,30 @@ __global__ __launch_bounds__(kThreads, 2) void tree_attn_kernel(Args a) {
                         }
                     }
 #pragma unroll
-                    for (int d = 0; d < 8; ++d) {
-                        const unsigned sel = d % 2 ? 0x07060302u : 0x05040100u;
-                        u32x4 w;
+                    for (int d0 = 0; d0 < S::VD; d0 += 4) {  // four dims: two words of f16 for each key
+                        unsigned x[8][2];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(x[2 * i + 1][d / 2], x[2 * i][d / 2], sel);
-                        const int dim = 8 * c + d;
-                        *reinterpret_cast<u32x4 *>(vt + dim * 64 + ((g ^ ((dim >> 2) & 3)) * 16)) = w;
+                        for (int i = 0; i < 8; ++i) {
+                            const unsigned *w = raw + (8 * j + i) * S::VW;
+                            if constexpr (ES == 2) {
+                                x[i][0] = w[d0 / 2];
+                                x[i][1] = w[d0 / 2 + 1];
+                            } else {
+                                const u32x2 p = narrow_f16<E>(w[d0 / 4]);
+                                x[i][0] = p[0];
+                                x[i][1] = p[1];
+                            }
+                        }
+#pragma unroll
+                        for (int d = 0; d < 4; ++d) {
+                            const unsigned sel = d % 2 ? 0x07060302u : 0x05040100u;
+                            u32x4 w;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                w[i] = __builtin_amdgcn_perm(x[2 * i + 1][d / 2], x[2 * i][d / 2], sel);
+                            const int dim = S::VD * c + d0 + d;
+                            *reinterpret_cast<u32x4 *>(vt + dim * 64 + ((g ^ ((dim >> 2) & 3)) * 16)) = w;
+                        }
                     }
                 }
             }
@@ -347,9 +393,14 @@ __global__ __launch_bounds__(kThreads, 2) void tree_attn_kernel(Args a) {
     fetch(t);
 
     // ---- the columns' queries, masks and first keys -------------------------------------------------
+    const unsigned first_mask = tid < nodes * a.words ? a.masks[(size_t)node0 * a.words + tid] : 0u;
+    auto put_mask = [&](int i, unsigned w) {
+        if (i % a.words == a.words - 1 && a.n % 32) w &= (1u << (a.n % 32)) - 1u;  // (no nodes past n)
+        s_mask[i] = w;
+    };
     const int cw = wave % CW, kw = wave / CW;
     const bool worker = kw < KW;  // (the others fetch and store only)
-    f16x8 qh[NSET][S::NC], ql[NSET][S::NC];
+    f16x8 qh[NSET][S::NC], ql[NSET][S::QLDS ? 1 : S::NC];
     float qs[NSET];
     int my_node[NSET], my_first[NSET];
 #pragma unroll
@@ -366,46 +417,62 @@ __global__ __launch_bounds__(kThreads, 2) void tree_attn_kernel(Args a) {
         for (int i = 0; i < S::NC; ++i) {
             const int d = 32 * i + 8 * g4;
             const f32x4 lo = __builtin_bit_cast(
-                f32x4, __builtin_amdgcn_raw_buffer_load_b128(res, have && d < hd ? (at + d) * 4 : kNone, 0, 0));
+                f32x4, __builtin_amdgcn_raw_buffer_load_b128(res, have && d < hd ? (unsigned)(at + d) * 4u : kNone, 0, 0));
             const f32x4 hi = __builtin_bit_cast(
-                f32x4, __builtin_amdgcn_raw_buffer_load_b128(res, have && d + 4 < hd ? (at + d + 4) * 4 : kNone, 0, 0));
+                f32x4, __builtin_amdgcn_raw_buffer_load_b128(res, have && d + 4 < hd ? (unsigned)(at + d + 4) * 4u : kNone, 0, 0));
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                x[i][j] = (j < 4 ? lo[j % 4] : hi[j % 4]) * a.scale_log2;
+                x[i][j] = j < 4 ? lo[j % 4] : hi[j % 4];
                 top = fmaxf(top, fabsf(x[i][j]));
             }
         }
         top = fmaxf(top, eb::lane_xor16(top));
         top = fmaxf(top, eb::lane_xor32(top));
-        const unsigned e = biased_exponent(top);
+        // (q times scale log2(e), its largest in [2^13, 2^14) or, if the product rounds up, at 2^14)
+        const unsigned e = biased_exponent(fabsf(top * a.scale_log2));
         qs[s] = pow2_biased(e - 13u);
+        const float f = a.scale_log2 * pow2_biased(267u - e);
 #pragma unroll
-        for (int i = 0; i < S::NC; ++i) split(x[i] * pow2_biased(267u - e), qh[s][i], ql[s][i]);
+        for (int i = 0; i < S::NC; ++i) {
+            f16x8 lo;
+            split(x[i] * f, qh[s][i], lo);
+            if constexpr (S::QLDS) {
+                if (kw == 0) *reinterpret_cast<f16x8 *>(s_ql + ((cw * NSET + s) * S::NC + i) * 1024 + lane * 16) = lo;
+            } else {
+                ql[s][i] = lo;
+            }
+        }
     }
-    for (int i = tid; i < nodes * a.words; i += kThreads) s_mask[i] = a.masks[(size_t)node0 * a.words + i];
+    for (int i = tid; i < nodes * a.words; i += kThreads) put_mask(i, i == tid ? first_mask : a.masks[(size_t)node0 * a.words + i]);
     if (a.window > 0)
         for (int i = tid; i < a.n; i += kThreads) s_depth[i] = (int)min(a.depths[i], 1u << 27);
     __syncthreads();
     int safe_lo = 0;  // keys below it may be behind some column's window
+    bool shallow = true;  // no drafted key is behind any node's window
     if (a.window > 0) {
         int deepest = 0;
         for (int i = lane; i < nodes; i += 64) deepest = max(deepest, s_depth[node0 + i]);
 #pragma unroll
         for (int m = 32; m > 0; m >>= 1) deepest = max(deepest, __shfl_xor(deepest, m));
-        safe_lo = __builtin_amdgcn_readfirstlane(a.pos + deepest - a.window + 1);
+        deepest = __builtin_amdgcn_readfirstlane(deepest);
+        safe_lo = a.pos + deepest - a.window + 1;
+        shallow = deepest < a.window;
     }
 #pragma unroll
     for (int s = 0; s < NSET; ++s)
         my_first[s] = a.window > 0 ? a.pos + s_depth[node0 + my_node[s]] - a.window + 1 : 0;
 
     // ---- state --------------------------------------------------------------------------------------
-    f32x4 acc[NSET][S::ND];
-    float m[NSET], l[NSET], lcu[NSET];
+    // ref: what a score's exponent is taken against (unscaled: less kUnit, so that weights and sums are
+    // in units of 2^-kUnit); lcu: the unit of scaled weights.
+    f32x4 acc[NSET][S::ND], lacc[NSET];
+    float ref[NSET], l[NSET], lcu[NSET];
 #pragma unroll
     for (int s = 0; s < NSET; ++s) {
-        m[s] = -INFINITY;
+        ref[s] = kNoRef;
         l[s] = 0.0f;
         lcu[s] = 0.0f;
+        lacc[s] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int e = 0; e < S::ND; ++e) acc[s][e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
@@ -418,6 +485,14 @@ __global__ __launch_bounds__(kThreads, 2) void tree_attn_kernel(Args a) {
         for (int s = 0; s < NSET; ++s) sc[s][0] = sc[s][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < S::NC; ++i) {
+            f16x8 lo[NSET];
+#pragma unroll
+            for (int s = 0; s < NSET; ++s) {
+                if constexpr (S::QLDS)
+                    lo[s] = *reinterpret_cast<const f16x8 *>(s_ql + ((cw * NSET + s) * S::NC + i) * 1024 + lane * 16);
+                else
+                    lo[s] = ql[s][i];
+            }
 #pragma unroll
             for (int sub = 0; sub < 2; ++sub) {
                 const int r = 32 * kg + 16 * sub + n;
@@ -428,113 +503,139 @@ __global__ __launch_bounds__(kThreads, 2) void tree_attn_kernel(Args a) {
 #pragma unroll
                 for (int s = 0; s < NSET; ++s) {
                     sc[s][sub] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[s][i], sc[s][sub], 0, 0, 0);
-                    sc[s][sub] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[s][i], sc[s][sub], 0, 0, 0);
+                    sc[s][sub] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, lo[s], sc[s][sub], 0, 0, 0);
                     if constexpr (PL == 2)
                         sc[s][sub] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[s][i], sc[s][sub], 0, 0, 0);
                 }
             }
         }
+        // Scales of the keys: one each (f32), or of their block, which 16 keys share.
         f32x4 ks[2], vs[2];
         if constexpr (S::SCALED) {
 #pragma unroll
             for (int sub = 0; sub < 2; ++sub) {
-                ks[sub] = *reinterpret_cast<const f32x4 *>(s_scale + 32 * kg + 16 * sub + 4 * g4);
-                vs[sub] = *reinterpret_cast<const f32x4 *>(s_scale + T + 32 * kg + 16 * sub + 4 * g4);
+                const float *at = s_scale + 32 * kg + 16 * sub;
+                if constexpr (S::F32) {
+                    ks[sub] = *reinterpret_cast<const f32x4 *>(at + 4 * g4);
+                    vs[sub] = *reinterpret_cast<const f32x4 *>(at + T + 4 * g4);
+                } else {
+                    ks[sub] = f32x4{at[0], at[0], at[0], at[0]};
+                    vs[sub] = f32x4{at[T], at[T], at[T], at[T]};
+                }
             }
         }
         f16x8 ph[NSET], pl[NSET];
 #pragma unroll
         for (int s = 0; s < NSET; ++s) {
-            float x[8], w[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[i] = sc[s][i / 4][i % 4];
-                if constexpr (S::SCALED) x[i] *= ks[i / 4][i % 4];
-                // (An infinite half of K meets q's two halves, whose signs may agree: infinity times 0
-                // is NaN whatever they gave. f32 rows' split made it NaN, E4M3 has no infinity.)
-                if constexpr (E == TreeElem::F16)
-                    x[i] = __builtin_fmaf(x[i], qs[s], x[i] * 0.0f);
-                else
-                    x[i] *= qs[s];
-            }
             unsigned seen = 0xFFu;
             if (edge) {
                 const unsigned *mask = s_mask + my_node[s] * a.words;
+                seen = 0u;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int key = k0 + 16 * (i / 4) + 4 * g4 + i % 4, j = key - a.pos;
-                    bool ok;
-                    if (j < 0) {
-                        ok = key >= my_first[s];
-                    } else {
-                        const int jj = min(j, a.n - 1);
-                        ok = j < a.n && (mask[jj >> 5] >> (jj & 31)) & 1u;
-                        if (a.window > 0) ok = ok && a.pos + s_depth[jj] >= my_first[s];
+                for (int sub = 0; sub < 2; ++sub) {  // four neighbouring keys; drafted from j = 0 on
+                    const int key = k0 + 16 * sub + 4 * g4, j = key - a.pos, at = j >> 5;
+                    const unsigned lo = at >= 0 && at < a.words ? mask[max(at, 0)] : 0u;
+                    const unsigned hi = at + 1 >= 0 && at + 1 < a.words ? mask[max(at + 1, 0)] : 0u;
+                    unsigned bits = __builtin_amdgcn_alignbit(hi, lo, (unsigned)j & 31u) & 15u;
+                    if (!shallow) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int jj = min(max(j + i, 0), a.n - 1);
+                            if (a.pos + s_depth[jj] < my_first[s]) bits &= ~(1u << i);
+                        }
                     }
-                    if (!ok) {
-                        x[i] = -INFINITY;
-                        seen &= ~(1u << i);
-                    }
+                    const unsigned cached = (1u << min(max(-j, 0), 4)) - 1u;
+                    const unsigned before = (1u << min(max(my_first[s] - key, 0), 4)) - 1u;
+                    seen |= ((bits & ~cached) | (cached & ~before)) << (4 * sub);
                 }
             }
-            const float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-            // Weights against the present reference and unit; true where they do not serve.
-            float sum = 0.0f;
-            auto weigh = [&] {
-                const float ref = m[s] == -INFINITY ? 0.0f : S::SCALED ? m[s] : m[s] - kUnit;
-                const float cu = ldexpf(1.0f, (int)lcu[s]);
-                float most = 0.0f;
+            float y[8], w[8], sum = 0.0f;  // y: scores before their column's factor
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                y[i] = sc[s][i / 4][i % 4];
+                if constexpr (S::F32) y[i] *= ks[i / 4][i % 4];
+            }
+            const float qk[2] = {E == TreeElem::I8 ? qs[s] * ks[0][0] : qs[s], E == TreeElem::I8 ? qs[s] * ks[1][0] : qs[s]};
+            // Weights against the present reference and unit; where those do not serve, once more.
+            for (bool again = true;; again = false) {
+                const float cu = S::SCALED ? ldexpf(1.0f, (int)lcu[s]) : 1.0f;
+                const float vc[2] = {S::SCALED ? vs[0][0] * cu : cu, S::SCALED ? vs[1][0] * cu : cu};
+                float top = -INFINITY, least = INFINITY, most = 0.0f;
                 sum = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float p = eb::fast_exp2(x[i] - ref);
-                    sum += p;
-                    w[i] = p;
+                    w[i] = __builtin_fmaf(y[i], qk[i / 4], -ref[s]);
+                    if constexpr (E == TreeElem::F16) least = fminf(least, w[i]);
+                }
+                if (edge) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) w[i] = (seen >> i) & 1u ? w[i] : -INFINITY;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    top = fmaxf(top, w[i]);
+                    w[i] = eb::fast_exp2(w[i]);
                     if constexpr (S::SCALED) {
-                        w[i] = p * vs[i / 4][i % 4] * cu;
+                        sum += w[i];
+                        w[i] *= S::F32 ? vs[i / 4][i % 4] * cu : vc[i / 4];
                         most = fmaxf(most, w[i]);
                     }
                 }
-                return top > m[s] + kSlack || (m[s] == -INFINITY && top > -INFINITY) || most > kTop;
-            };
-            if (__builtin_amdgcn_ballot_w64(weigh()) != 0) {
-                float t1 = fmaxf(top, eb::lane_xor16(top));
+                const bool over = (top > (S::SCALED ? kSlack : kSlack + kUnit)) | (most > kTop) | (least == -INFINITY);
+                if (!again || __builtin_amdgcn_ballot_w64(over) == 0) break;
+                float t1 = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    // (An infinite half of K meets q's two halves, whose signs may agree: infinity times 0
+                    // is NaN whatever they gave. f32 rows' split made it NaN, E4M3 has no infinity.)
+                    if constexpr (E == TreeElem::F16) y[i] = __builtin_fmaf(y[i], 0.0f, y[i]);
+                    t1 = fmaxf(t1, (seen >> i) & 1u ? y[i] * qk[i / 4] : -INFINITY);
+                }
+                t1 = fmaxf(t1, eb::lane_xor16(t1));
                 t1 = fmaxf(t1, eb::lane_xor32(t1));  // the column's largest score of the group
-                const float mn = m[s] == -INFINITY || t1 > m[s] + kSlack ? t1 : m[s];
-                const float d = mn == m[s] ? 0.0f : m[s] - mn;  // (infinite at the column's first keys)
+                if constexpr (!S::SCALED) t1 -= kUnit;
+                const float rn = t1 > ref[s] + kSlack ? t1 : ref[s];
+                const float d = ref[s] - rn;  // (-1e30 or so at the column's first keys)
                 float f = d;
                 if constexpr (S::SCALED) {
-                    const float ref = mn == -INFINITY ? 0.0f : mn;
-                    float y = 0.0f;  // the group's largest term
+                    float big = 0.0f;  // the group's largest term
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) y = fmaxf(y, eb::fast_exp2(x[i] - ref) * vs[i / 4][i % 4]);
-                    y = fmaxf(y, eb::lane_xor16(y));
-                    y = fmaxf(y, eb::lane_xor32(y));
+                    for (int i = 0; i < 8; ++i) {
+                        const float p = eb::fast_exp2(__builtin_fmaf(y[i], qk[i / 4], -rn)) * vs[i / 4][i % 4];
+                        big = fmaxf(big, (seen >> i) & 1u ? p : 0.0f);
+                    }
+                    big = fmaxf(big, eb::lane_xor16(big));
+                    big = fmaxf(big, eb::lane_xor32(big));
                     // Earlier terms lose 2^d: as much the unit may grow. Where this group's would pass
                     // 2^15 in it, its largest term becomes 2^6 to 2^7.
                     float unit = fminf(lcu[s] + floorf(-d), 120.0f);
-                    const float ey = (float)__builtin_amdgcn_frexp_expf(y);
-                    if (y > 0.0f && ey + unit > 15.0f) unit = 7.0f - ey;
+                    const float eb2 = (float)__builtin_amdgcn_frexp_expf(big);
+                    if (big > 0.0f && eb2 + unit > 15.0f) unit = 7.0f - eb2;
                     f = d + (unit - lcu[s]);
                     lcu[s] = unit;
+                    l[s] *= eb::fast_exp2(d);
                 }
-                f = d < -1.0e6f ? 0.0f : eb::fast_exp2(f);
-                l[s] *= d < -1.0e6f ? 0.0f : eb::fast_exp2(d);
-                m[s] = mn;
+                f = eb::fast_exp2(f);
+                ref[s] = rn;
+                lacc[s] *= f;
 #pragma unroll
                 for (int e = 0; e < S::ND; ++e) acc[s][e] *= f;
-                (void)weigh();
             }
             l[s] += sum;
             if (edge) {  // (a NaN scale does not reach what a column does not see)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    if constexpr (!S::SCALED)
-                        w[i] *= s_scale[T + 32 * kg + 16 * (i / 4) + 4 * g4 + i % 4];
+                    if constexpr (!S::SCALED) w[i] *= s_scale[T + 32 * kg + 16 * (i / 4) + 4 * g4 + i % 4];
                     if (!((seen >> i) & 1u)) w[i] = 0.0f;
                 }
             }
             split(f32x8{w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]}, ph[s], pl[s]);
+            if constexpr (!S::SCALED) {  // the weights' sum, as one more dim whose values are ones
+                const _Float16 one = (_Float16)1.0f;
+                const f16x8 ones = {one, one, one, one, one, one, one, one};
+                lacc[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, ph[s], lacc[s], 0, 0, 0);
+                lacc[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pl[s], lacc[s], 0, 0, 0);
+            }
         }
         const char *vt = buf + PL * PLANE + kg * (HDP * 64);
 #pragma unroll
@@ -572,10 +673,15 @@ __global__ __launch_bounds__(kThreads, 2) void tree_attn_kernel(Args a) {
     }
 
     // ---- the waves' states meet ---------------------------------------------------------------------
+    if constexpr (!S::SCALED) {
 #pragma unroll
-    for (int s = 0; s < NSET; ++s) {
-        l[s] += eb::lane_xor16(l[s]);
-        l[s] += eb::lane_xor32(l[s]);
+        for (int s = 0; s < NSET; ++s) l[s] = lacc[s][0];
+    } else {
+#pragma unroll
+        for (int s = 0; s < NSET; ++s) {
+            l[s] += eb::lane_xor16(l[s]);
+            l[s] += eb::lane_xor32(l[s]);
+        }
     }
     if constexpr (S::SCALED) {  // out of the columns' units
 #pragma unroll
@@ -585,39 +691,36 @@ __global__ __launch_bounds__(kThreads, 2) void tree_attn_kernel(Args a) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) acc[s][e][r] = ldexpf(acc[s][e][r], -(int)lcu[s]);
     }
-    if constexpr (KW > 1) {
-        constexpr int SLOT = NSET * (S::ND * 1024 + 512);  // bytes a wave leaves
-        __syncthreads();
-        if (worker && kw > 0) {
-            char *at = smem + ((kw - 1) * CW + cw) * SLOT;
+    if constexpr (KW > 1) {  // a set at a time: into LDS, and to the first of the waves
+        constexpr int SLOT = S::ND * 1024 + 512;  // bytes a wave leaves
 #pragma unroll
-            for (int s = 0; s < NSET; ++s) {
+        for (int s = 0; s < NSET; ++s) {
+            __syncthreads();
+            if (worker && kw > 0) {
+                char *at = smem + ((kw - 1) * CW + cw) * SLOT;
 #pragma unroll
-                for (int e = 0; e < S::ND; ++e)
-                    *reinterpret_cast<f32x4 *>(at + (s * S::ND + e) * 1024 + lane * 16) = acc[s][e];
-                float *ml = reinterpret_cast<float *>(at + NSET * S::ND * 1024 + s * 512);
-                ml[lane] = m[s];
+                for (int e = 0; e < S::ND; ++e) *reinterpret_cast<f32x4 *>(at + e * 1024 + lane * 16) = acc[s][e];
+                float *ml = reinterpret_cast<float *>(at + S::ND * 1024);
+                ml[lane] = ref[s];
                 ml[64 + lane] = l[s];
             }
-        }
-        __syncthreads();
-        if (kw > 0) return;
+            __syncthreads();
+            if (kw == 0) {
 #pragma unroll
-        for (int w = 1; w < KW; ++w) {
-            const char *at = smem + ((w - 1) * CW + cw) * SLOT;
+                for (int w = 1; w < KW; ++w) {
+                    const char *at = smem + ((w - 1) * CW + cw) * SLOT;
+                    const float *ml = reinterpret_cast<const float *>(at + S::ND * 1024);
+                    const float r2 = ml[lane], rn = fmaxf(ref[s], r2);
+                    const float f1 = eb::fast_exp2(ref[s] - rn), f2 = eb::fast_exp2(r2 - rn);
+                    l[s] = l[s] * f1 + ml[64 + lane] * f2;
+                    ref[s] = rn;
 #pragma unroll
-            for (int s = 0; s < NSET; ++s) {
-                const float *ml = reinterpret_cast<const float *>(at + NSET * S::ND * 1024 + s * 512);
-                const float m2 = ml[lane], mn = fmaxf(m[s], m2), ref = mn == -INFINITY ? 0.0f : mn;
-                const float f1 = eb::fast_exp2(m[s] - ref), f2 = eb::fast_exp2(m2 - ref);
-                l[s] = l[s] * f1 + ml[64 + lane] * f2;
-                m[s] = mn;
-#pragma unroll
-                for (int e = 0; e < S::ND; ++e)
-                    acc[s][e] = acc[s][e] * f1 +
-                                f2 * *reinterpret_cast<const f32x4 *>(at + (s * S::ND + e) * 1024 + lane * 16);
+                    for (int e = 0; e < S::ND; ++e)
+                        acc[s][e] = acc[s][e] * f1 + f2 * *reinterpret_cast<const f32x4 *>(at + e * 1024 + lane * 16);
+                }
             }
         }
+        if (kw > 0) return;
     }
     if (!worker) return;
 #pragma unroll
@@ -638,7 +741,7 @@ __global__ __launch_bounds__(kThreads, 2) void tree_attn_kernel(Args a) {
             for (int e = 0; e < S::ND; ++e)
                 if (16 * e + 4 * g4 < hd) *reinterpret_cast<f32x4 *>(a.part_acc + at * hd + 16 * e + 4 * g4) = acc[s][e];
             if (g4 == 0) {
-                a.part_ml[at * 2] = m[s];
+                a.part_ml[at * 2] = ref[s];
                 a.part_ml[at * 2 + 1] = l[s];
             }
         }
@@ -647,16 +750,17 @@ __global__ __launch_bounds__(kThreads, 2) void tree_attn_kernel(Args a) {
 
 // o[row] = sum of the splits' sums, at one reference. Workgroup: one row (node and head); a group of
 // lanes holds the row's dims, four each, the groups share the splits, four at a time in flight.
-__global__ __launch_bounds__(kThreads) void tree_merge_kernel(const float *__restrict__ part_acc,
+constexpr int kMergeThreads = 256;
+__global__ __launch_bounds__(kMergeThreads) void tree_merge_kernel(const float *__restrict__ part_acc,
                                                               const float *__restrict__ part_ml, float *__restrict__ o,
                                                               int rows, int hd, int nsplit, int lanes_log2) {
-    __shared__ float s_m[kThreads], s_l[kThreads];
-    __shared__ f32x4 s_a[kThreads];
+    __shared__ float s_m[kMergeThreads], s_l[kMergeThreads];
+    __shared__ f32x4 s_a[kMergeThreads];
     const int tid = threadIdx.x, row = blockIdx.x;
-    const int groups = kThreads >> lanes_log2;
+    const int groups = kMergeThreads >> lanes_log2;
     const int grp = tid >> lanes_log2, d = (tid & ((1 << lanes_log2) - 1)) * 4;
     const int at_d = d < hd ? d : 0;
-    float M = -INFINITY, L = 0.0f;
+    float M = kNoRef, L = 0.0f;
     f32x4 A = {0.0f, 0.0f, 0.0f, 0.0f};
     constexpr int B = 4;
     for (int s0 = grp; s0 < nsplit; s0 += groups * B) {
@@ -675,14 +779,13 @@ __global__ __launch_bounds__(kThreads) void tree_merge_kernel(const float *__res
 #pragma unroll
         for (int j = 0; j < B; ++j)
             if (s0 + j * groups < nsplit) mn = fmaxf(mn, bm[j]);
-        const float ref = mn == -INFINITY ? 0.0f : mn;
-        const float c = eb::fast_exp2(M - ref);
+        const float c = eb::fast_exp2(M - mn);
         L *= c;
         A *= c;
 #pragma unroll
         for (int j = 0; j < B; ++j) {
             if (s0 + j * groups >= nsplit) continue;
-            const float w = eb::fast_exp2(bm[j] - ref);
+            const float w = eb::fast_exp2(bm[j] - mn);
             L += w * bl[j];
             A += w * ba[j];
         }
@@ -695,12 +798,11 @@ __global__ __launch_bounds__(kThreads) void tree_merge_kernel(const float *__res
     if (grp > 0 || d >= hd) return;
     float mt = M;
     for (int g = 1; g < groups; ++g) mt = fmaxf(mt, s_m[(g << lanes_log2) + tid]);
-    const float ref = mt == -INFINITY ? 0.0f : mt;
     float Lt = 0.0f;
     f32x4 At = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int g = 0; g < groups; ++g) {
         const int i = (g << lanes_log2) + tid;
-        const float w = eb::fast_exp2(s_m[i] - ref);
+        const float w = eb::fast_exp2(s_m[i] - mt);
         Lt += w * s_l[i];
         At += w * s_a[i];
     }
@@ -709,16 +811,8 @@ __global__ __launch_bounds__(kThreads) void tree_merge_kernel(const float *__res
 }
 
 struct Plan {
-    int hdp, cols, ncb, T, key0, tiles, nsplit;
+    int hdp, cols, ncb, key0, tiles, nsplit;
 };
-
-int keys_per_tile(int hdp, TreeElem e) {
-    switch (e) {
-        case TreeElem::F32: return hdp == 64 ? 64 : 32;
-        case TreeElem::F16: return hdp == 64 ? 128 : 64;
-        default: return hdp == 256 ? 64 : 128;
-    }
-}
 
 constexpr size_t kMinSplitKeys = 128;
 constexpr int kWgsPerCu = 2;
@@ -728,11 +822,11 @@ Plan plan_of(size_t h, size_t hkv, size_t hd, size_t pos, size_t n, size_t windo
     const size_t cols = n * (h / hkv);
     p.cols = cols <= 16 ? 16 : cols <= 64 || p.hdp == 256 ? 64 : 128;
     p.ncb = (int)((cols + p.cols - 1) / p.cols);
-    p.T = keys_per_tile(p.hdp, elem);
+    const int T = 32 * key_groups(p.hdp, elem, p.cols == 16 ? 1 : 4, p.cols == 128 ? 2 : 1);
     const size_t first = window > 0 && pos + 1 > window ? pos + 1 - window : 0;
     p.key0 = (int)(first & ~(size_t)15);
-    p.tiles = (int)((pos + n - p.key0 + p.T - 1) / p.T);
-    size_t nsplit = std::max<size_t>(1, (size_t)cu_count * kWgsPerCu / (hkv * p.ncb));
+    p.tiles = (int)((pos + n - p.key0 + T - 1) / T);
+    size_t nsplit = std::max<size_t>(1, (size_t)cu_count * (p.cols == 128 ? 1 : kWgsPerCu) / (hkv * p.ncb));
     nsplit = std::min(nsplit, (size_t)p.tiles);
     if (pos + n - first <= kMinSplitKeys) nsplit = 1;
     p.nsplit = (int)nsplit;
@@ -743,15 +837,16 @@ template <int HDP, TreeElem E, int CW, int NSET>
 hipError_t launch(hipStream_t st, const Args &a) {
     using S = Shape<HDP, E, CW, NSET>;
     const size_t nodes = std::min<size_t>(a.n, S::COLS);
-    const size_t lds = (size_t)S::NBUF * S::TILE + (nodes * a.words + (a.window > 0 ? a.n : 0)) * 4;
+    const size_t lds = (size_t)S::NBUF * S::TILE + S::QBYTES + (nodes * a.words + (a.window > 0 ? a.n : 0)) * 4;
+    constexpr size_t kMost = S::NBUF * S::TILE + S::QBYTES + (S::COLS * 8 + 256) * 4;
+    static_assert(kMost <= 160 * 1024 / S::WGS, "LDS of a CU");
     if (lds > 64 * 1024) {
         static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&tree_attn_kernel<HDP, E, CW, NSET>),
-                                                        hipFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);
+                                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)kMost);
         if (e != hipSuccess) return e;
     }
-    static_assert(S::NBUF * S::TILE + (S::COLS * 8 + 256) * 4 <= 80 * 1024, "two workgroups per CU");
     const unsigned grid = (unsigned)((a.pairs + 7) / 8 * 8 * a.ncb);
-    tree_attn_kernel<HDP, E, CW, NSET><<<grid, kThreads, lds, st>>>(a);
+    tree_attn_kernel<HDP, E, CW, NSET><<<grid, S::THREADS, lds, st>>>(a);
     return hipSuccess;
 }
 
@@ -824,7 +919,7 @@ eb_status launch_attn_tree(hipStream_t st, const TreeAttn &x, float *ws, size_t 
     if (s != EB_OK || p.nsplit == 1) return s;
     int lanes_log2 = 0;
     while ((size_t)4 << lanes_log2 < x.hd) ++lanes_log2;
-    tree_merge_kernel<<<(unsigned)rows, kThreads, 0, st>>>(a.part_acc, a.part_ml, x.o, (int)rows, (int)x.hd, p.nsplit,
+    tree_merge_kernel<<<(unsigned)rows, kMergeThreads, 0, st>>>(a.part_acc, a.part_ml, x.o, (int)rows, (int)x.hd, p.nsplit,
                                                            lanes_log2);
     return check_launch("attn_tree (merge)");
 }
