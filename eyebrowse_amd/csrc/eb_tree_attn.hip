@@ -91,8 +91,11 @@ struct Shape {
     // q's low halves of 32 columns over f32 caches: in LDS, the registers do not hold them.
     static constexpr bool QLDS = F32 && NSET == 2;
     static constexpr int QBYTES = QLDS ? CW * NSET * NC * 1024 : 0;
-    static constexpr int NBUF = TILE > (NSET == 2 ? 64 : 40) * 1024 ? 1 : F32 && NSET == 2 ? 1 : 2;
+    static constexpr int NBUF = TILE > (NSET == 2 ? 66 : 40) * 1024 ? 1 : F32 && NSET == 2 ? 1 : 2;
     static constexpr int WGS = NSET == 2 || (F32 && HDP == 256) ? 1 : 2;  // workgroups per CU
+    // Operand reads from LDS that are on their way at once: units of two (16-key halves of a 32-dim
+    // step, or two 16-dim groups of V), 8 registers each and plane.
+    static constexpr int AHEAD = std::min(NC, HDP == 256 ? 1 : F32 ? (NSET == 2 ? 1 : 2) : NSET == 2 ? (ES == 1 ? 1 : 2) : 4);
     static constexpr int LD = 16 / ES;               // dims of a 16-byte load
     static constexpr int KL = HDP / (F32 ? 8 : LD);  // K units of a row: 8 dims (f32), or a load
     static constexpr int KU = T * KL / HT;           // and per thread
@@ -103,6 +106,7 @@ struct Shape {
     static constexpr int VUNITS = 4 * KG * VC;
     static constexpr int VU = (VUNITS + HT - 1) / HT;
     static constexpr int NR = std::max(KU * (F32 ? 8 : 4), VU * 8 * VW);
+    static_assert(NC % AHEAD == 0, "whole rounds");
     static_assert((KW - 1) * CW * (ND * 1024 + 512) <= TILE * NBUF, "room to join waves");
 };
 
@@ -156,6 +160,15 @@ __device__ __forceinline__ u32x2 narrow_f16(unsigned w) {
         const unsigned hi = __builtin_amdgcn_perm(0x64646464u, f, 0x04030402u);
         return u32x2{f16x2_bits(__builtin_bit_cast(f16x2, lo) + off), f16x2_bits(__builtin_bit_cast(f16x2, hi) + off)};
     }
+}
+
+// Where slot g (the keys of lane group g) of a dim lies in V's transposed rows of 64 bytes. Row
+// (dim % 4) HDP / 4 + dim / 4: neighbouring lanes, whose dims are 4 apart where they store, and 4
+// apart again where they read, meet neighbouring rows; the slots are xor-ed with the row.
+template <int HDP>
+__device__ __forceinline__ int v_row(int dim, int g) {
+    const int row = (dim % 4) * (HDP / 4) + dim / 4;
+    return row * 64 + ((g ^ ((row >> 2) & 3)) * 16);
 }
 
 // x as two halves, each rounded to nearest: 22 bits. (A fused multiply-add takes the half as it is.)
@@ -299,7 +312,9 @@ __global__ __launch_bounds__(waves_of(NSET) * 64, (Shape<HDP, E, CW, NSET>::WGS 
                     float back[8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const unsigned *w = raw + (8 * j + i) * 4;
+                        unsigned w[4];
+#pragma unroll
+                        for (int d = 0; d < 4; ++d) w[d] = raw[(8 * j + i) * 4 + d];
                         x[i] = f32x4{__uint_as_float(w[0]), __uint_as_float(w[1]), __uint_as_float(w[2]),
                                      __uint_as_float(w[3])};
                         unsigned bits = 0;  // (as whole numbers: NaN is above infinity)
@@ -323,30 +338,34 @@ __global__ __launch_bounds__(waves_of(NSET) * 64, (Shape<HDP, E, CW, NSET>::WGS 
                         const f32x8 col = {x[0][d], x[1][d], x[2][d], x[3][d], x[4][d], x[5][d], x[6][d], x[7][d]};
                         f16x8 hi, lo;
                         split(col, hi, lo);
-                        char *at = vt + (4 * c + d) * 64 + ((g ^ (c & 3)) * 16);
+                        char *at = vt + v_row<HDP>(4 * c + d, g);
                         *reinterpret_cast<f16x8 *>(at) = hi;
                         *reinterpret_cast<f16x8 *>(at + PLANE) = lo;
                     }
                 } else {
+                    unsigned in[8][S::VW];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+#pragma unroll
+                        for (int d = 0; d < S::VW; ++d) in[i][d] = raw[(8 * j + i) * S::VW + d];
                     if constexpr (E != TreeElem::I8) {
                         if (edge) {  // rows that are not finite: zeros, and NaN for the weight
                             float back[8];
 #pragma unroll
                             for (int i = 0; i < 8; ++i) {
-                                unsigned *w = raw + (8 * j + i) * S::VW;
                                 bool bad = false;
 #pragma unroll
                                 for (int d = 0; d < S::VW; ++d) {
                                     if constexpr (ES == 2) {
-                                        bad = bad | ((w[d] & 0x7C00u) == 0x7C00u) | ((w[d] & 0x7C000000u) == 0x7C000000u);
+                                        bad = bad | ((in[i][d] & 0x7C00u) == 0x7C00u) | ((in[i][d] & 0x7C000000u) == 0x7C000000u);
                                     } else {  // (dims from hd on are the next head's)
-                                        const unsigned m = w[d] & 0x7F7F7F7Fu;  // NaN is 0x7F: a carry into the sign bit
+                                        const unsigned m = in[i][d] & 0x7F7F7F7Fu;  // NaN is 0x7F: a carry into the sign bit
                                         bad = bad | ((((m + 0x01010101u) & 0x80808080u) != 0u) & (c * S::VD + 4 * d < hd));
                                     }
                                 }
                                 bad = lanes_max<S::VC>(bad ? 1.0f : 0.0f) > 0.0f;
 #pragma unroll
-                                for (int d = 0; d < S::VW; ++d) w[d] = bad ? 0u : w[d];
+                                for (int d = 0; d < S::VW; ++d) in[i][d] = bad ? 0u : in[i][d];
                                 back[i] = bad ? __builtin_nanf("") : 1.0f;
                             }
                             if (c == 0) {
@@ -360,12 +379,11 @@ __global__ __launch_bounds__(waves_of(NSET) * 64, (Shape<HDP, E, CW, NSET>::WGS 
                         unsigned x[8][2];
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
-                            const unsigned *w = raw + (8 * j + i) * S::VW;
                             if constexpr (ES == 2) {
-                                x[i][0] = w[d0 / 2];
-                                x[i][1] = w[d0 / 2 + 1];
+                                x[i][0] = in[i][d0 / 2];
+                                x[i][1] = in[i][d0 / 2 + 1];
                             } else {
-                                const u32x2 p = narrow_f16<E>(w[d0 / 4]);
+                                const u32x2 p = narrow_f16<E>(in[i][d0 / 4]);
                                 x[i][0] = p[0];
                                 x[i][1] = p[1];
                             }
@@ -378,7 +396,7 @@ __global__ __launch_bounds__(waves_of(NSET) * 64, (Shape<HDP, E, CW, NSET>::WGS 
                             for (int i = 0; i < 4; ++i)
                                 w[i] = __builtin_amdgcn_perm(x[2 * i + 1][d / 2], x[2 * i][d / 2], sel);
                             const int dim = S::VD * c + d0 + d;
-                            *reinterpret_cast<u32x4 *>(vt + dim * 64 + ((g ^ ((dim >> 2) & 3)) * 16)) = w;
+                            *reinterpret_cast<u32x4 *>(vt + v_row<HDP>(dim, g)) = w;
                         }
                     }
                 }
@@ -483,6 +501,30 @@ __global__ __launch_bounds__(waves_of(NSET) * 64, (Shape<HDP, E, CW, NSET>::WGS 
         f32x4 sc[NSET][2];
 #pragma unroll
         for (int s = 0; s < NSET; ++s) sc[s][0] = sc[s][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        constexpr int AHEAD = S::AHEAD;
+        f16x8 fr[AHEAD][2][PL];
+        auto read_k = [&](int i) {
+#pragma unroll
+            for (int sub = 0; sub < 2; ++sub) {
+                const int r = 32 * kg + 16 * sub + n;
+                const char *at = buf + (r * S::CH + ((4 * i + g4) ^ (r & S::SW))) * 16;
+#pragma unroll
+                for (int p = 0; p < PL; ++p) fr[i % AHEAD][sub][p] = *reinterpret_cast<const f16x8 *>(at + p * PLANE);
+            }
+        };
+        // Output group e = 4 q + d is dims 4 (16 q + n) + d, lane n's row of V.
+        const char *vt = buf + PL * PLANE + kg * (HDP * 64) + v_row<HDP>(4 * n, g4);
+        auto read_v = [&](int u) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int p = 0; p < PL; ++p)
+                    fr[u % AHEAD][e][p] = *reinterpret_cast<const f16x8 *>(vt + ((2 * u + e) % 4 * (HDP / 4) + (2 * u + e) / 4 * 16) * 64 + p * PLANE);
+        };
+        auto mfma = [](f16x8 x, f16x8 y, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0); };
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) read_k(i);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < S::NC; ++i) {
             f16x8 lo[NSET];
@@ -493,22 +535,26 @@ __global__ __launch_bounds__(waves_of(NSET) * 64, (Shape<HDP, E, CW, NSET>::WGS 
                 else
                     lo[s] = ql[s][i];
             }
+            const auto &k = fr[i % AHEAD];
 #pragma unroll
-            for (int sub = 0; sub < 2; ++sub) {
-                const int r = 32 * kg + 16 * sub + n;
-                const char *at = buf + (r * S::CH + ((4 * i + g4) ^ (r & S::SW))) * 16;
-                const f16x8 kh = *reinterpret_cast<const f16x8 *>(at);
-                f16x8 kl;
-                if constexpr (PL == 2) kl = *reinterpret_cast<const f16x8 *>(at + PLANE);
+            for (int s = 0; s < NSET; ++s)
 #pragma unroll
-                for (int s = 0; s < NSET; ++s) {
-                    sc[s][sub] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[s][i], sc[s][sub], 0, 0, 0);
-                    sc[s][sub] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, lo[s], sc[s][sub], 0, 0, 0);
-                    if constexpr (PL == 2)
-                        sc[s][sub] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[s][i], sc[s][sub], 0, 0, 0);
-                }
+                for (int sub = 0; sub < 2; ++sub) sc[s][sub] = mfma(k[sub][0], qh[s][i], sc[s][sub]);
+            if constexpr (PL == 2) {
+#pragma unroll
+                for (int s = 0; s < NSET; ++s)
+#pragma unroll
+                    for (int sub = 0; sub < 2; ++sub) sc[s][sub] = mfma(k[sub][PL - 1], qh[s][i], sc[s][sub]);
             }
+#pragma unroll
+            for (int s = 0; s < NSET; ++s)
+#pragma unroll
+                for (int sub = 0; sub < 2; ++sub) sc[s][sub] = mfma(k[sub][0], lo[s], sc[s][sub]);
+            if (i + AHEAD < S::NC) read_k(i + AHEAD);
         }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) read_v(u);
+        __builtin_amdgcn_sched_barrier(0);  // (on their way while the weights are formed)
         // Scales of the keys: one each (f32), or of their block, which 16 keys share.
         f32x4 ks[2], vs[2];
         if constexpr (S::SCALED) {
@@ -637,20 +683,24 @@ __global__ __launch_bounds__(waves_of(NSET) * 64, (Shape<HDP, E, CW, NSET>::WGS 
                 lacc[s] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pl[s], lacc[s], 0, 0, 0);
             }
         }
-        const char *vt = buf + PL * PLANE + kg * (HDP * 64);
 #pragma unroll
-        for (int e = 0; e < S::ND; ++e) {
-            const char *at = vt + (16 * e + n) * 64 + ((g4 ^ ((n >> 2) & 3)) * 16);
-            const f16x8 vh = *reinterpret_cast<const f16x8 *>(at);
-            f16x8 vl;
-            if constexpr (PL == 2) vl = *reinterpret_cast<const f16x8 *>(at + PLANE);
+        for (int u = 0; u < S::ND / 2; ++u) {
+            const auto &v = fr[u % AHEAD];
 #pragma unroll
-            for (int s = 0; s < NSET; ++s) {
-                acc[s][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph[s], acc[s][e], 0, 0, 0);
-                acc[s][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl[s], acc[s][e], 0, 0, 0);
-                if constexpr (PL == 2)
-                    acc[s][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[s], acc[s][e], 0, 0, 0);
+            for (int s = 0; s < NSET; ++s)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) acc[s][2 * u + e] = mfma(v[e][0], ph[s], acc[s][2 * u + e]);
+            if constexpr (PL == 2) {
+#pragma unroll
+                for (int s = 0; s < NSET; ++s)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) acc[s][2 * u + e] = mfma(v[e][PL - 1], ph[s], acc[s][2 * u + e]);
             }
+#pragma unroll
+            for (int s = 0; s < NSET; ++s)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) acc[s][2 * u + e] = mfma(v[e][0], pl[s], acc[s][2 * u + e]);
+            if (u + AHEAD < S::ND / 2) read_v(u + AHEAD);
         }
     };
 
@@ -729,21 +779,21 @@ __global__ __launch_bounds__(waves_of(NSET) * 64, (Shape<HDP, E, CW, NSET>::WGS 
         if (c >= a.ncols) continue;
         const int node = node0 + my_node[s];
         const size_t row = (size_t)node * a.h + kvh * a.g + c - node * a.g;
-        if (a.nsplit == 1) {
-            const float inv = l[s] == 0.0f ? 0.0f : 1.0f / l[s];
+        const size_t at = a.nsplit == 1 ? row : (size_t)split_id * a.n * a.h + row;
+        float *out = (a.nsplit == 1 ? a.o : a.part_acc) + at * hd;
+        const float f = a.nsplit > 1 ? 1.0f : l[s] == 0.0f ? 0.0f : 1.0f / l[s];
 #pragma unroll
-            for (int e = 0; e < S::ND; ++e)
-                if (16 * e + 4 * g4 < hd)
-                    *reinterpret_cast<f32x4 *>(a.o + row * hd + 16 * e + 4 * g4) = acc[s][e] * inv;
-        } else {
-            const size_t at = (size_t)split_id * a.n * a.h + row;
+        for (int q = 0; q < S::ND / 4; ++q)
 #pragma unroll
-            for (int e = 0; e < S::ND; ++e)
-                if (16 * e + 4 * g4 < hd) *reinterpret_cast<f32x4 *>(a.part_acc + at * hd + 16 * e + 4 * g4) = acc[s][e];
-            if (g4 == 0) {
-                a.part_ml[at * 2] = ref[s];
-                a.part_ml[at * 2 + 1] = l[s];
+            for (int r = 0; r < 4; ++r) {
+                const int d = 64 * q + 16 * g4 + 4 * r;
+                if (d < hd)
+                    *reinterpret_cast<f32x4 *>(out + d) = f32x4{acc[s][4 * q][r] * f, acc[s][4 * q + 1][r] * f,
+                                                                acc[s][4 * q + 2][r] * f, acc[s][4 * q + 3][r] * f};
             }
+        if (a.nsplit > 1 && g4 == 0) {
+            a.part_ml[at * 2] = ref[s];
+            a.part_ml[at * 2 + 1] = l[s];
         }
     }
 }
