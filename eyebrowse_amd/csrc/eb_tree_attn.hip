@@ -45,6 +45,8 @@ namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -58,54 +60,65 @@ constexpr float kUnit = 7.0f;      // log2 of a weight at its reference
 constexpr float kNoRef = -1.0e30f;  // a reference below all scores: no key yet
 constexpr unsigned kNone = 0x7FFFFFF0u;  // a byte offset past any tile
 
-// Waves of a workgroup, and 32-key groups of a tile. About 32 KB of the cache are in flight for every
-// four waves. One wave's columns (cw 1): the waves share the tile's keys. Up to 64: each wave has its
-// own 16. More: 32 columns to a wave, eight waves, the halves of the tile's keys to four each, so that
-// what is staged, and what a split leaves for the merge, serves twice the columns.
-constexpr int waves_of(int nset) { return nset == 2 ? 8 : 4; }
-constexpr int key_groups(int hdp, TreeElem e, int cw, int nset) {
+// How a call is run: COPY moves the cache's rows to LDS as they are (half rows, E4M3 rows of whole
+// 16-byte pieces, block-scaled codes); otherwise they pass through registers and become f16 there (f32
+// rows, whose halves are the same for all columns; E4M3 rows that end inside a piece).
+//
+// Waves of a workgroup, and 32-key groups of a tile. One wave's columns (cw 1): the waves share the
+// tile's keys. Up to 64: each wave has its own 16; more: its own 32. With eight waves the halves of a
+// tile's keys go to four each, so that a split leaves half as much for the merge.
+constexpr int waves_of(int cw, int nset, bool copy) { return nset == 2 || (copy && cw > 1) ? 8 : 4; }
+constexpr int key_groups(int hdp, TreeElem e, int cw, int nset, bool copy) {
     const bool f32 = e == TreeElem::F32, f16 = e == TreeElem::F16;
-    if (hdp == 256) return f32 || (f16 && cw > 1) ? 1 : 2;
-    if (cw == 1) return f32 ? hdp == 64 ? 2 : 1 : 4;
-    if (nset == 2) return f32 ? 2 : f16 && hdp == 128 ? 2 : 4;
-    return f32 ? hdp == 64 ? 2 : 1 : f16 && hdp == 128 ? 2 : 4;
+    if (copy) return f16 ? hdp == 64 ? 4 : hdp == 128 || cw > 1 ? 2 : 1 : hdp == 256 ? 2 : 4;
+    if (hdp == 256) return 1;
+    if (f32) return hdp == 64 || nset == 2 ? 2 : 1;
+    return 4;
 }
 
-template <int HDP, TreeElem E, int CW, int NSET>
+template <int HDP, TreeElem E, int CW, int NSET, bool COPY>
 struct Shape {
     static constexpr bool F32 = E == TreeElem::F32;
     static constexpr bool SCALED = E == TreeElem::F32 || E == TreeElem::I8;
     static constexpr int ES = F32 ? 4 : E == TreeElem::F16 ? 2 : 1;  // bytes of an element
     static constexpr int PL = F32 ? 2 : 1;                           // f16 planes
-    static constexpr int WAVES = waves_of(NSET), THREADS = WAVES * 64, HT = THREADS / 2;
-    static constexpr int KG = key_groups(HDP, E, CW, NSET);
+    static constexpr int WAVES = waves_of(CW, NSET, COPY), THREADS = WAVES * 64, HT = THREADS / 2;
+    static constexpr int KG = key_groups(HDP, E, CW, NSET, COPY);
     static constexpr int T = 32 * KG;
     static constexpr int KW = std::min(KG, WAVES / CW);  // waves that share a column's tile
     static constexpr int COLS = CW * NSET * 16;
     static constexpr int NC = HDP / 32;  // 32-dim steps of a score
     static constexpr int ND = HDP / 16;  // 16-dim groups of an output
-    static constexpr int CH = HDP / 8;   // 8-dim chunks of a K row in LDS
+    static constexpr int LD = 16 / ES;   // dims of a 16-byte piece
+    // ---- rows copied to LDS
+    static constexpr int RB = HDP * ES, CR = RB / 16;             // bytes and pieces of a row
+    static constexpr int CPW = T * CR / 64 / (WAVES / 2);         // copies per wave and tile
+    static constexpr int CPT = CPW + (E == TreeElem::I8 ? 1 : 0);  // with the exponents'
+    // ---- rows stored as operands
+    static constexpr int CH = HDP / 8;  // 8-dim chunks of a K row in LDS
     static constexpr int SW = (CH < 16 ? CH : 16) - 1;
     static constexpr int PLANE = T * HDP * 2;  // bytes of one plane of K, and of V
-    static constexpr int TILE = 2 * PL * PLANE + 2 * T * 4;
-    // q's low halves of 32 columns over f32 caches: in LDS, the registers do not hold them.
-    static constexpr bool QLDS = F32 && NSET == 2;
-    static constexpr int QBYTES = QLDS ? CW * NSET * NC * 1024 : 0;
-    static constexpr int NBUF = TILE > (NSET == 2 ? 66 : 40) * 1024 ? 1 : F32 && NSET == 2 ? 1 : 2;
-    static constexpr int WGS = NSET == 2 || (F32 && HDP == 256) ? 1 : 2;  // workgroups per CU
-    // Operand reads from LDS that are on their way at once: units of two (16-key halves of a 32-dim
-    // step, or two 16-dim groups of V), 8 registers each and plane.
-    static constexpr int AHEAD = std::min(NC, HDP == 256 ? 1 : F32 ? (NSET == 2 ? 1 : 2) : NSET == 2 ? (ES == 1 ? 1 : 2) : 4);
-    static constexpr int LD = 16 / ES;               // dims of a 16-byte load
     static constexpr int KL = HDP / (F32 ? 8 : LD);  // K units of a row: 8 dims (f32), or a load
     static constexpr int KU = T * KL / HT;           // and per thread
-    // V units: 8 keys by VD dims, a row's in VB bytes.
+    // V units: 8 keys by VD dims, VW words of a row.
     static constexpr int VD = NSET == 2 && !F32 ? LD / 2 : LD;
-    static constexpr int VW = VD * ES / 4;  // words of a unit's row
+    static constexpr int VW = VD * ES / 4;
     static constexpr int VC = HDP / VD;
     static constexpr int VUNITS = 4 * KG * VC;
     static constexpr int VU = (VUNITS + HT - 1) / HT;
-    static constexpr int NR = std::max(KU * (F32 ? 8 : 4), VU * 8 * VW);
+    static constexpr int NR = COPY ? 1 : std::max(KU * (F32 ? 8 : 4), VU * 8 * VW);
+    // ---- LDS
+    static constexpr int TILE = COPY ? 2 * T * RB + (E == TreeElem::I8 ? 512 : 0) : 2 * PL * PLANE + 2 * T * 4;
+    static constexpr int NBUF = COPY ? (WAVES == 8 && TILE <= 33 * 1024 ? 4 : 2)
+                                : TILE > (NSET == 2 ? 66 : 40) * 1024 || (F32 && NSET == 2) ? 1 : 2;
+    // q's low halves of 32 columns over f32 caches: in LDS, the registers do not hold them.
+    static constexpr bool QLDS = F32 && NSET == 2;
+    static constexpr int QBYTES = QLDS ? CW * NSET * NC * 1024 : 0;
+    static constexpr int WGS = WAVES == 8 || (F32 && HDP == 256) ? 1 : 2;  // workgroups per CU
+    // Operand reads from LDS that are on their way at once: units of two (16-key halves of a 32-dim
+    // step, or two 16-dim groups of V), 8 registers each and plane.
+    static constexpr int AHEAD = COPY ? (NSET == 2 || HDP == 256 ? 2 : std::min(NC, 4))
+                                 : std::min(NC, HDP == 256 || NSET == 2 ? 1 : F32 ? 2 : 4);
     static_assert(NC % AHEAD == 0, "whole rounds");
     static_assert((KW - 1) * CW * (ND * 1024 + 512) <= TILE * NBUF, "room to join waves");
 };
@@ -144,6 +157,10 @@ __device__ __forceinline__ unsigned biased_exponent(float magnitude) {
     return e < 14u ? 14u : e;
 }
 __device__ __forceinline__ float pow2_biased(unsigned e) { return __builtin_bit_cast(float, e << 23); }
+// The scale of a block's exponent byte: 2^(e - 127), NaN for 255.
+__device__ __forceinline__ float exponent_scale(unsigned e) {
+    return __builtin_bit_cast(float, e == eb::kNanExponent ? 0x7FC00000u : e << 23);
+}
 
 __device__ __forceinline__ unsigned f16x2_bits(f16x2 x) { return __builtin_bit_cast(unsigned, x); }
 
@@ -171,6 +188,12 @@ __device__ __forceinline__ int v_row(int dim, int g) {
     return row * 64 + ((g ^ ((row >> 2) & 3)) * 16);
 }
 
+// Whether one of four E4M3 patterns is NaN (0x7F and 0xFF: one more carries into the sign bit).
+__device__ __forceinline__ bool has_nan_e4m3(unsigned w) { return (((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) != 0u; }
+__device__ __forceinline__ bool has_nonfinite_f16(unsigned w) {
+    return ((w & 0x7C00u) == 0x7C00u) | ((w & 0x7C000000u) == 0x7C000000u);
+}
+
 // x as two halves, each rounded to nearest: 22 bits. (A fused multiply-add takes the half as it is.)
 __device__ __forceinline__ void split(f32x8 x, f16x8 &hi, f16x8 &lo) {
     hi = __builtin_convertvector(x, f16x8);
@@ -179,9 +202,27 @@ __device__ __forceinline__ void split(f32x8 x, f16x8 &hi, f16x8 &lo) {
     lo = __builtin_convertvector(x, f16x8);
 }
 
-template <int HDP, TreeElem E, int CW, int NSET>
-__global__ __launch_bounds__(waves_of(NSET) * 64, (Shape<HDP, E, CW, NSET>::WGS * waves_of(NSET) / 4)) void tree_attn_kernel(Args a) {
-    using S = Shape<HDP, E, CW, NSET>;
+// Copies to LDS are inline assembly, which the compiler's wait counting does not see; they complete
+// in issue order, so a tile is there when at most the later tiles' copies of this wave are under way
+// (and, after a barrier, the other waves'). What the compiler itself waits for is then at worst waited
+// for longer.
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// Where piece c of row r lies in a copied row of RB bytes (in pieces): xor-ed with the row, so that
+// neither 16 rows at one piece nor 4 rows at two meet a bank more often than their bytes ask for.
+template <int RB>
+__device__ __forceinline__ int piece_xor(int r) {
+    return RB >= 256 ? r & 15 : RB == 128 ? (r >> 1) & 7 : (r >> 2) & 3;
+}
+
+template <int HDP, TreeElem E, int CW, int NSET, bool COPY>
+__global__ __launch_bounds__((Shape<HDP, E, CW, NSET, COPY>::THREADS),
+                             (Shape<HDP, E, CW, NSET, COPY>::WGS * Shape<HDP, E, CW, NSET, COPY>::WAVES / 4))
+void tree_attn_kernel(Args a) {
+    using S = Shape<HDP, E, CW, NSET, COPY>;
     constexpr int ES = S::ES, T = S::T, KW = S::KW, PL = S::PL, PLANE = S::PLANE, HT = S::HT;
     constexpr int kWaves = S::WAVES, kThreads = S::THREADS;
     extern __shared__ char smem[];
@@ -202,7 +243,8 @@ __global__ __launch_bounds__(waves_of(NSET) * 64, (Shape<HDP, E, CW, NSET>::WGS 
     const int node0 = node_of(col0);
     const int nodes = node_of(min(col0 + S::COLS, a.ncols) - 1) - node0 + 1;  // of this workgroup's columns
     char *s_ql = smem + S::NBUF * S::TILE;  // [CW][NSET][NC][lane]
-    unsigned *s_mask = reinterpret_cast<unsigned *>(s_ql + S::QBYTES);          // [nodes][words]
+    float *s_bad = reinterpret_cast<float *>(s_ql + S::QBYTES);  // [T] (copied rows: 1, or NaN)
+    unsigned *s_mask = reinterpret_cast<unsigned *>(s_bad + (COPY ? T : 0));    // [nodes][words]
     int *s_depth = reinterpret_cast<int *>(s_mask + nodes * a.words);           // [n] (with a window)
 
     // ---- tiles: fetched into registers, then stored as operands -----------------------------------
@@ -210,8 +252,42 @@ __global__ __launch_bounds__(waves_of(NSET) * 64, (Shape<HDP, E, CW, NSET>::WGS 
     const int ht = tid % HT;
     const size_t row_bytes = (size_t)a.hkv * hd * ES;
     const char *base = (vside ? a.v : a.k) + (size_t)kvh * hd * ES;
+    const unsigned lds0 = (unsigned)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)smem);
+    unsigned piece[COPY ? S::CPW : 1];  // where this lane's pieces lie in a tile's rows
+    if constexpr (COPY) {
+#pragma unroll
+        for (int i = 0; i < S::CPW; ++i) {
+            const int at = ((wave % (kWaves / 2)) * S::CPW + i) * 64 + lane, r = at / S::CR;
+            const int c = (at % S::CR) ^ piece_xor<S::RB>(r);
+            piece[i] = c * S::LD < hd ? r * (unsigned)row_bytes + c * 16 : kNone;
+        }
+    }
+    // Tile t to buffer b: rows [T][RB] of K, then of V; then the exponents of their 16-key pieces, [64]
+    // words each. Past the last key, and past a row's dims, LDS gets zeros.
+    auto copy = [&](int t, int b) {
+        const int r0 = a.key0 + t * T;
+        const int left = min(end - r0, T);
+        const int nbytes = left > 0 ? (int)((left - 1) * row_bytes) + hd * ES : 0;
+        const __amdgpu_buffer_rsrc_t res = eb::make_rsrc(base + (left > 0 ? (size_t)r0 * row_bytes : 0), nbytes);
+        const unsigned dst = lds0 + b * S::TILE + (vside ? T * S::RB : 0) + (wave % (kWaves / 2)) * S::CPW * 1024;
+#pragma unroll
+        for (int i = 0; i < S::CPW; ++i)  // (a copy may read m0 one wait state after its write at the soonest)
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst + i * 1024),
+                         "v"(piece[i]), "s"(res)
+                         : "memory", "m0");
+        if constexpr (E == TreeElem::I8) {  // (every wave the same words: the counts stay alike)
+            const size_t b0 = left > 0 ? (size_t)(r0 >> a.block_log2) : 0;
+            const int last = left > 0 ? (r0 + left - 1) >> a.block_log2 : 0;
+            const __amdgpu_buffer_rsrc_t eres = eb::make_rsrc(
+                (vside ? a.vs : a.ks) + b0 * a.hkv, left > 0 ? (last - (int)b0) * a.hkv + kvh + 1 : 0);
+            const unsigned off = 16 * lane < left ? (((r0 + 16 * lane) >> a.block_log2) - (int)b0) * a.hkv + kvh : kNone;
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_ubyte %1, %2, 0 offen lds" ::"s"(
+                             lds0 + b * S::TILE + 2 * T * S::RB + (vside ? 256 : 0)),
+                         "v"(off), "s"(eres)
+                         : "memory", "m0");
+        }
+    };
     unsigned raw[S::NR];
-    unsigned raw_e = 127;  // I8: the exponent of key ht (1 past the last)
     auto fetch = [&](int t) {
         const int r0 = a.key0 + t * T;
         const int left = min(end - r0, T);
@@ -258,10 +334,6 @@ __global__ __launch_bounds__(waves_of(NSET) * 64, (Shape<HDP, E, CW, NSET>::WGS 
                 }
             }
         }
-        if constexpr (E == TreeElem::I8) {
-            const int key = min(r0 + min(ht, T - 1), end - 1);
-            raw_e = (vside ? a.vs : a.ks)[(size_t)(key >> a.block_log2) * a.hkv + kvh];
-        }
     };
     // The operands of a tile in LDS: K [planes][T][HDP], V [planes][KG][HDP][32], scales [2][T].
     auto store = [&](char *buf, bool edge) {
@@ -286,10 +358,8 @@ __global__ __launch_bounds__(waves_of(NSET) * 64, (Shape<HDP, E, CW, NSET>::WGS 
                     *reinterpret_cast<f16x8 *>(at(c)) = hi;
                     *reinterpret_cast<f16x8 *>(at(c) + PLANE) = lo;
                     if (c == 0) s_scale[r] = pow2_biased(e - 13u);
-                } else if constexpr (ES == 2) {
-                    *reinterpret_cast<u32x4 *>(at(c)) = u32x4{raw[4 * j], raw[4 * j + 1], raw[4 * j + 2], raw[4 * j + 3]};
                 } else {
-                    const bool whole = E == TreeElem::I8 || 16 * c + 8 < hd;  // (else the next head's)
+                    const bool whole = 16 * c + 8 < hd;  // (else the next head's)
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         const u32x2 x = narrow_f16<E>(raw[4 * j + 2 * half]), y = narrow_f16<E>(raw[4 * j + 2 * half + 1]);
@@ -348,30 +418,22 @@ __global__ __launch_bounds__(waves_of(NSET) * 64, (Shape<HDP, E, CW, NSET>::WGS 
                     for (int i = 0; i < 8; ++i)
 #pragma unroll
                         for (int d = 0; d < S::VW; ++d) in[i][d] = raw[(8 * j + i) * S::VW + d];
-                    if constexpr (E != TreeElem::I8) {
-                        if (edge) {  // rows that are not finite: zeros, and NaN for the weight
-                            float back[8];
+                    if (edge) {  // rows that are not finite: zeros, and NaN for the weight
+                        float back[8];
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                bool bad = false;
+                        for (int i = 0; i < 8; ++i) {
+                            bool bad = false;
 #pragma unroll
-                                for (int d = 0; d < S::VW; ++d) {
-                                    if constexpr (ES == 2) {
-                                        bad = bad | ((in[i][d] & 0x7C00u) == 0x7C00u) | ((in[i][d] & 0x7C000000u) == 0x7C000000u);
-                                    } else {  // (dims from hd on are the next head's)
-                                        const unsigned m = in[i][d] & 0x7F7F7F7Fu;  // NaN is 0x7F: a carry into the sign bit
-                                        bad = bad | ((((m + 0x01010101u) & 0x80808080u) != 0u) & (c * S::VD + 4 * d < hd));
-                                    }
-                                }
-                                bad = lanes_max<S::VC>(bad ? 1.0f : 0.0f) > 0.0f;
+                            for (int d = 0; d < S::VW; ++d)  // (dims from hd on are the next head's)
+                                bad = bad | (has_nan_e4m3(in[i][d]) & (c * S::VD + 4 * d < hd));
+                            bad = lanes_max<S::VC>(bad ? 1.0f : 0.0f) > 0.0f;
 #pragma unroll
-                                for (int d = 0; d < S::VW; ++d) in[i][d] = bad ? 0u : in[i][d];
-                                back[i] = bad ? __builtin_nanf("") : 1.0f;
-                            }
-                            if (c == 0) {
-                                *reinterpret_cast<f32x4 *>(vs) = f32x4{back[0], back[1], back[2], back[3]};
-                                *reinterpret_cast<f32x4 *>(vs + 16) = f32x4{back[4], back[5], back[6], back[7]};
-                            }
+                            for (int d = 0; d < S::VW; ++d) in[i][d] = bad ? 0u : in[i][d];
+                            back[i] = bad ? __builtin_nanf("") : 1.0f;
+                        }
+                        if (c == 0) {
+                            *reinterpret_cast<f32x4 *>(vs) = f32x4{back[0], back[1], back[2], back[3]};
+                            *reinterpret_cast<f32x4 *>(vs + 16) = f32x4{back[4], back[5], back[6], back[7]};
                         }
                     }
 #pragma unroll
@@ -379,14 +441,9 @@ __global__ __launch_bounds__(waves_of(NSET) * 64, (Shape<HDP, E, CW, NSET>::WGS 
                         unsigned x[8][2];
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
-                            if constexpr (ES == 2) {
-                                x[i][0] = in[i][d0 / 2];
-                                x[i][1] = in[i][d0 / 2 + 1];
-                            } else {
-                                const u32x2 p = narrow_f16<E>(in[i][d0 / 4]);
-                                x[i][0] = p[0];
-                                x[i][1] = p[1];
-                            }
+                            const u32x2 p = narrow_f16<E>(in[i][d0 / 4]);
+                            x[i][0] = p[0];
+                            x[i][1] = p[1];
                         }
 #pragma unroll
                         for (int d = 0; d < 4; ++d) {
@@ -402,13 +459,13 @@ __global__ __launch_bounds__(waves_of(NSET) * 64, (Shape<HDP, E, CW, NSET>::WGS 
                 }
             }
         }
-        if constexpr (E == TreeElem::I8) {
-            if (ht < T) s_scale[(vside ? T : 0) + ht] = eb::i8_scale(raw_e, 0);
-        }
     };
 
     int t = split_id;
-    fetch(t);
+    if constexpr (COPY)
+        copy(t, 0);
+    else
+        fetch(t);
 
     // ---- the columns' queries, masks and first keys -------------------------------------------------
     const unsigned first_mask = tid < nodes * a.words ? a.masks[(size_t)node0 * a.words + tid] : 0u;
@@ -418,6 +475,9 @@ __global__ __launch_bounds__(waves_of(NSET) * 64, (Shape<HDP, E, CW, NSET>::WGS 
     };
     const int cw = wave % CW, kw = wave / CW;
     const bool worker = kw < KW;  // (the others fetch and store only)
+    // First of the 8 dims that a lane multiplies in 32-dim step i (copied bytes: a 16-byte piece holds
+    // those of two steps).
+    auto chunk_dim = [&](int i) { return COPY && ES == 1 ? 64 * (i / 2) + 16 * g4 + 8 * (i % 2) : 32 * i + 8 * g4; };
     f16x8 qh[NSET][S::NC], ql[NSET][S::QLDS ? 1 : S::NC];
     float qs[NSET];
     int my_node[NSET], my_first[NSET];
@@ -433,7 +493,7 @@ __global__ __launch_bounds__(waves_of(NSET) * 64, (Shape<HDP, E, CW, NSET>::WGS 
         float top = 0.0f;
 #pragma unroll
         for (int i = 0; i < S::NC; ++i) {
-            const int d = 32 * i + 8 * g4;
+            const int d = chunk_dim(i);
             const f32x4 lo = __builtin_bit_cast(
                 f32x4, __builtin_amdgcn_raw_buffer_load_b128(res, have && d < hd ? (unsigned)(at + d) * 4u : kNone, 0, 0));
             const f32x4 hi = __builtin_bit_cast(
@@ -497,29 +557,82 @@ __global__ __launch_bounds__(waves_of(NSET) * 64, (Shape<HDP, E, CW, NSET>::WGS 
 
     // One group of 32 keys from k0 on, in buf.
     auto consume = [&](const char *buf, int kg, int k0, bool edge) {
-        const float *s_scale = reinterpret_cast<const float *>(buf + 2 * PL * PLANE);
+        const float *s_scale = reinterpret_cast<const float *>(buf + 2 * PL * PLANE);  // (stored rows)
+        const unsigned *s_exp = reinterpret_cast<const unsigned *>(buf + 2 * T * S::RB);  // (copied codes)
         f32x4 sc[NSET][2];
 #pragma unroll
         for (int s = 0; s < NSET; ++s) sc[s][0] = sc[s][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         constexpr int AHEAD = S::AHEAD;
-        f16x8 fr[AHEAD][2][PL];
+        constexpr bool BYTES = COPY && ES == 1;
+        // Reads on their way: [unit][two][plane], as they lie in LDS (copied bytes: a K unit is the 16
+        // dims of two steps, a V unit 8 bytes).
+        u32x4 fr[AHEAD][2][PL];
         auto read_k = [&](int i) {
 #pragma unroll
             for (int sub = 0; sub < 2; ++sub) {
                 const int r = 32 * kg + 16 * sub + n;
-                const char *at = buf + (r * S::CH + ((4 * i + g4) ^ (r & S::SW))) * 16;
+                if constexpr (COPY) {
+                    const int c = 4 * (BYTES ? i / 2 : i) + g4;
+                    if (!BYTES || i % 2 == 0)
+                        fr[i % AHEAD][sub][0] =
+                            *reinterpret_cast<const u32x4 *>(buf + r * S::RB + ((c ^ piece_xor<S::RB>(n)) * 16));
+                } else {
+                    const char *at = buf + (r * S::CH + ((4 * i + g4) ^ (r & S::SW))) * 16;
 #pragma unroll
-                for (int p = 0; p < PL; ++p) fr[i % AHEAD][sub][p] = *reinterpret_cast<const f16x8 *>(at + p * PLANE);
+                    for (int p = 0; p < PL; ++p) fr[i % AHEAD][sub][p] = *reinterpret_cast<const u32x4 *>(at + p * PLANE);
+                }
             }
         };
-        // Output group e = 4 q + d is dims 4 (16 q + n) + d, lane n's row of V.
-        const char *vt = buf + PL * PLANE + kg * (HDP * 64) + v_row<HDP>(4 * n, g4);
+        auto k_operand = [&](int i, int sub, int p) {
+            if constexpr (BYTES) {
+                const u32x4 w = fr[(i - i % 2) % AHEAD][sub][0];
+                const u32x2 x = narrow_f16<E>(w[i % 2 * 2]), y = narrow_f16<E>(w[i % 2 * 2 + 1]);
+                return __builtin_bit_cast(f16x8, u32x4{x[0], x[1], y[0], y[1]});
+            } else {
+                return __builtin_bit_cast(f16x8, fr[i % AHEAD][sub][p]);
+            }
+        };
+        // V by keys in the lane's order: stored so (output group e = 4 q + d is dims 4 (16 q + n) + d, lane
+        // n's row of V), or copied rows read across: 16 lanes read 16 dims of 4 keys (halves) or of 8 (bytes)
+        // and get their own dim of each.
+        const char *vt = COPY ? buf + T * S::RB + 32 * kg * S::RB + (n & 1) * 8
+                              : buf + PL * PLANE + kg * (HDP * 64) + v_row<HDP>(4 * n, g4);
         auto read_v = [&](int u) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
+            for (int e = 0; e < 2; ++e) {
+                if constexpr (BYTES) {
+                    const int r = 4 * g4 + ((n >> 1) & 3), key = r + (n >> 3) * 16;
+                    const int c = (2 * u + e) ^ piece_xor<S::RB>(r);
+                    const auto w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                        (__attribute__((address_space(3))) i32x2 *)(vt + key * S::RB + c * 16));
+                    fr[u % AHEAD][e][0][0] = w[0];
+                    fr[u % AHEAD][e][0][1] = w[1];
+                } else if constexpr (COPY) {
+                    const int r = 4 * g4 + (n >> 2), c = (2 * (2 * u + e) + ((n >> 1) & 1)) ^ piece_xor<S::RB>(r);
 #pragma unroll
-                for (int p = 0; p < PL; ++p)
-                    fr[u % AHEAD][e][p] = *reinterpret_cast<const f16x8 *>(vt + ((2 * u + e) % 4 * (HDP / 4) + (2 * u + e) / 4 * 16) * 64 + p * PLANE);
+                    for (int sub = 0; sub < 2; ++sub) {
+                        const auto w = __builtin_bit_cast(
+                            u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                       (__attribute__((address_space(3))) i16x4 *)(vt + (16 * sub + r) * S::RB + c * 16)));
+                        fr[u % AHEAD][e][0][2 * sub] = w[0];
+                        fr[u % AHEAD][e][0][2 * sub + 1] = w[1];
+                    }
+                } else {
+#pragma unroll
+                    for (int p = 0; p < PL; ++p)
+                        fr[u % AHEAD][e][p] = *reinterpret_cast<const u32x4 *>(
+                            vt + ((2 * u + e) % 4 * (HDP / 4) + (2 * u + e) / 4 * 16) * 64 + p * PLANE);
+                }
+            }
+        };
+        auto v_operand = [&](int u, int e, int p) {
+            if constexpr (BYTES) {
+                const u32x4 w = fr[u % AHEAD][e][0];
+                const u32x2 x = narrow_f16<E>(w[0]), y = narrow_f16<E>(w[1]);
+                return __builtin_bit_cast(f16x8, u32x4{x[0], x[1], y[0], y[1]});
+            } else {
+                return __builtin_bit_cast(f16x8, fr[u % AHEAD][e][p]);
+            }
         };
         auto mfma = [](f16x8 x, f16x8 y, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0); };
 #pragma unroll
@@ -535,7 +648,11 @@ __global__ __launch_bounds__(waves_of(NSET) * 64, (Shape<HDP, E, CW, NSET>::WGS 
                 else
                     lo[s] = ql[s][i];
             }
-            const auto &k = fr[i % AHEAD];
+            f16x8 k[2][PL];
+#pragma unroll
+            for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+                for (int p = 0; p < PL; ++p) k[sub][p] = k_operand(i, sub, p);
 #pragma unroll
             for (int s = 0; s < NSET; ++s)
 #pragma unroll
@@ -550,7 +667,11 @@ __global__ __launch_bounds__(waves_of(NSET) * 64, (Shape<HDP, E, CW, NSET>::WGS 
             for (int s = 0; s < NSET; ++s)
 #pragma unroll
                 for (int sub = 0; sub < 2; ++sub) sc[s][sub] = mfma(k[sub][0], lo[s], sc[s][sub]);
-            if (i + AHEAD < S::NC) read_k(i + AHEAD);
+            if constexpr (BYTES) {  // (a piece's second step frees it)
+                if (i % 2 && i - 1 + AHEAD < S::NC) read_k(i - 1 + AHEAD);
+            } else {
+                if (i + AHEAD < S::NC) read_k(i + AHEAD);
+            }
         }
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) read_v(u);
@@ -565,8 +686,9 @@ __global__ __launch_bounds__(waves_of(NSET) * 64, (Shape<HDP, E, CW, NSET>::WGS 
                     ks[sub] = *reinterpret_cast<const f32x4 *>(at + 4 * g4);
                     vs[sub] = *reinterpret_cast<const f32x4 *>(at + T + 4 * g4);
                 } else {
-                    ks[sub] = f32x4{at[0], at[0], at[0], at[0]};
-                    vs[sub] = f32x4{at[T], at[T], at[T], at[T]};
+                    const float k1 = exponent_scale(s_exp[2 * kg + sub]), v1 = exponent_scale(s_exp[64 + 2 * kg + sub]);
+                    ks[sub] = f32x4{k1, k1, k1, k1};
+                    vs[sub] = f32x4{v1, v1, v1, v1};
                 }
             }
         }
@@ -671,7 +793,8 @@ __global__ __launch_bounds__(waves_of(NSET) * 64, (Shape<HDP, E, CW, NSET>::WGS 
             if (edge) {  // (a NaN scale does not reach what a column does not see)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    if constexpr (!S::SCALED) w[i] *= s_scale[T + 32 * kg + 16 * (i / 4) + 4 * g4 + i % 4];
+                    if constexpr (!S::SCALED)
+                        w[i] *= (COPY ? s_bad : s_scale + T)[32 * kg + 16 * (i / 4) + 4 * g4 + i % 4];
                     if (!((seen >> i) & 1u)) w[i] = 0.0f;
                 }
             }
@@ -685,7 +808,11 @@ __global__ __launch_bounds__(waves_of(NSET) * 64, (Shape<HDP, E, CW, NSET>::WGS 
         }
 #pragma unroll
         for (int u = 0; u < S::ND / 2; ++u) {
-            const auto &v = fr[u % AHEAD];
+            f16x8 v[2][PL];
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int p = 0; p < PL; ++p) v[e][p] = v_operand(u, e, p);
 #pragma unroll
             for (int s = 0; s < NSET; ++s)
 #pragma unroll
@@ -705,21 +832,59 @@ __global__ __launch_bounds__(waves_of(NSET) * 64, (Shape<HDP, E, CW, NSET>::WGS 
     };
 
     // ---- the tiles ----------------------------------------------------------------------------------
-    for (int b = 0; t < a.tiles; t += a.nsplit, b ^= 1) {
-        char *buf = smem + (S::NBUF == 2 && b ? S::TILE : 0);
-        const int r0 = a.key0 + t * T;
-        const bool edge = r0 + T > a.pos || r0 < safe_lo;  // (uniform)
-        store(buf, edge);
-        if (t + a.nsplit < a.tiles) fetch(t + a.nsplit);
-        __syncthreads();
-        if (worker) {
+    auto multiply = [&](const char *buf, int r0, bool edge) {
+        if (!worker) return;
 #pragma unroll 1
-            for (int kg = kw; kg < S::KG; kg += KW) {
-                if (r0 + 32 * kg >= end) break;
-                consume(buf, kg, r0 + 32 * kg, edge);
-            }
+        for (int kg = kw; kg < S::KG; kg += KW) {
+            if (r0 + 32 * kg >= end) break;
+            consume(buf, kg, r0 + 32 * kg, edge);
         }
-        if constexpr (S::NBUF == 1) __syncthreads();
+    };
+    if constexpr (COPY) {
+        constexpr int NB = S::NBUF;
+        int b = 0;
+#pragma unroll
+        for (int i = 1; i < NB - 1; ++i) copy(t + i * a.nsplit, i);
+        for (; t < a.tiles; t += a.nsplit) {
+            char *buf = smem + b * S::TILE;
+            const int r0 = a.key0 + t * T;
+            const bool edge = r0 + T > a.pos || r0 < safe_lo;  // (uniform)
+            wait_copies<(NB - 2) * S::CPT>();
+            __syncthreads();  // tile t is there; tile t - 1's buffer is read no more
+            copy(t + (NB - 1) * a.nsplit, b == 0 ? NB - 1 : b - 1);  // (past the last tile: of no keys)
+            if constexpr (!S::SCALED) {
+                if (edge) {  // V rows that are not finite: zeros, and NaN for the weight
+                    for (int i = tid; i < T; i += kThreads) s_bad[i] = 1.0f;
+                    __syncthreads();
+                    u32x4 *v = reinterpret_cast<u32x4 *>(buf + T * S::RB);
+                    for (int i = tid; i < T * S::CR; i += kThreads) {
+                        const u32x4 w = v[i];
+                        bool bad = false;
+#pragma unroll
+                        for (int d = 0; d < 4; ++d) bad = bad | (ES == 2 ? has_nonfinite_f16(w[d]) : has_nan_e4m3(w[d]));
+                        if (bad) s_bad[i / S::CR] = __builtin_nanf("");
+                    }
+                    __syncthreads();
+                    for (int i = tid; i < T * S::CR; i += kThreads)
+                        if (s_bad[i / S::CR] != 1.0f) v[i] = u32x4{0u, 0u, 0u, 0u};
+                    __syncthreads();
+                }
+            }
+            multiply(buf, r0, edge);
+            b = b == NB - 1 ? 0 : b + 1;
+        }
+        wait_copies<0>();  // (of no keys, but they write zeros to LDS)
+    } else {
+        for (int b = 0; t < a.tiles; t += a.nsplit, b ^= 1) {
+            char *buf = smem + (S::NBUF == 2 && b ? S::TILE : 0);
+            const int r0 = a.key0 + t * T;
+            const bool edge = r0 + T > a.pos || r0 < safe_lo;
+            store(buf, edge);
+            if (t + a.nsplit < a.tiles) fetch(t + a.nsplit);
+            __syncthreads();
+            multiply(buf, r0, edge);
+            if constexpr (S::NBUF == 1) __syncthreads();
+        }
     }
 
     // ---- the waves' states meet ---------------------------------------------------------------------
@@ -782,15 +947,21 @@ __global__ __launch_bounds__(waves_of(NSET) * 64, (Shape<HDP, E, CW, NSET>::WGS 
         const size_t at = a.nsplit == 1 ? row : (size_t)split_id * a.n * a.h + row;
         float *out = (a.nsplit == 1 ? a.o : a.part_acc) + at * hd;
         const float f = a.nsplit > 1 ? 1.0f : l[s] == 0.0f ? 0.0f : 1.0f / l[s];
+        if constexpr (COPY) {
 #pragma unroll
-        for (int q = 0; q < S::ND / 4; ++q)
+            for (int e = 0; e < S::ND; ++e)
+                if (16 * e + 4 * g4 < hd) *reinterpret_cast<f32x4 *>(out + 16 * e + 4 * g4) = acc[s][e] * f;
+        } else {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int d = 64 * q + 16 * g4 + 4 * r;
-                if (d < hd)
-                    *reinterpret_cast<f32x4 *>(out + d) = f32x4{acc[s][4 * q][r] * f, acc[s][4 * q + 1][r] * f,
-                                                                acc[s][4 * q + 2][r] * f, acc[s][4 * q + 3][r] * f};
-            }
+            for (int q = 0; q < S::ND / 4; ++q)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int d = 64 * q + 16 * g4 + 4 * r;
+                    if (d < hd)
+                        *reinterpret_cast<f32x4 *>(out + d) = f32x4{acc[s][4 * q][r] * f, acc[s][4 * q + 1][r] * f,
+                                                                    acc[s][4 * q + 2][r] * f, acc[s][4 * q + 3][r] * f};
+                }
+        }
         if (a.nsplit > 1 && g4 == 0) {
             a.part_ml[at * 2] = ref[s];
             a.part_ml[at * 2 + 1] = l[s];
@@ -862,57 +1033,63 @@ __global__ __launch_bounds__(kMergeThreads) void tree_merge_kernel(const float *
 
 struct Plan {
     int hdp, cols, ncb, key0, tiles, nsplit;
+    bool copy;
 };
 
 constexpr size_t kMinSplitKeys = 128;
-constexpr int kWgsPerCu = 2;
 Plan plan_of(size_t h, size_t hkv, size_t hd, size_t pos, size_t n, size_t window, TreeElem elem, int cu_count) {
     Plan p{};
     p.hdp = hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
+    p.copy = elem != TreeElem::F32 && (elem != TreeElem::E4M3 || hd % 16 == 0);
     const size_t cols = n * (h / hkv);
     p.cols = cols <= 16 ? 16 : cols <= 64 || p.hdp == 256 ? 64 : 128;
     p.ncb = (int)((cols + p.cols - 1) / p.cols);
-    const int T = 32 * key_groups(p.hdp, elem, p.cols == 16 ? 1 : 4, p.cols == 128 ? 2 : 1);
+    const int cw = p.cols == 16 ? 1 : 4, nset = p.cols == 128 ? 2 : 1;
+    const int T = 32 * key_groups(p.hdp, elem, cw, nset, p.copy);
     const size_t first = window > 0 && pos + 1 > window ? pos + 1 - window : 0;
     p.key0 = (int)(first & ~(size_t)15);
     p.tiles = (int)((pos + n - p.key0 + T - 1) / T);
-    size_t nsplit = std::max<size_t>(1, (size_t)cu_count * (p.cols == 128 ? 1 : kWgsPerCu) / (hkv * p.ncb));
+    const int wgs = waves_of(cw, nset, p.copy) == 8 ? 1 : 2;
+    size_t nsplit = std::max<size_t>(1, (size_t)cu_count * wgs / (hkv * p.ncb));
     nsplit = std::min(nsplit, (size_t)p.tiles);
     if (pos + n - first <= kMinSplitKeys) nsplit = 1;
     p.nsplit = (int)nsplit;
     return p;
 }
 
-template <int HDP, TreeElem E, int CW, int NSET>
+template <int HDP, TreeElem E, int CW, int NSET, bool COPY>
 hipError_t launch(hipStream_t st, const Args &a) {
-    using S = Shape<HDP, E, CW, NSET>;
+    using S = Shape<HDP, E, CW, NSET, COPY>;
+    constexpr size_t kTiles = (size_t)S::NBUF * S::TILE + S::QBYTES + (COPY ? S::T * 4 : 0);
     const size_t nodes = std::min<size_t>(a.n, S::COLS);
-    const size_t lds = (size_t)S::NBUF * S::TILE + S::QBYTES + (nodes * a.words + (a.window > 0 ? a.n : 0)) * 4;
-    constexpr size_t kMost = S::NBUF * S::TILE + S::QBYTES + (S::COLS * 8 + 256) * 4;
+    const size_t lds = kTiles + (nodes * a.words + (a.window > 0 ? a.n : 0)) * 4;
+    constexpr size_t kMost = kTiles + (S::COLS * 8 + 256) * 4;
     static_assert(kMost <= 160 * 1024 / S::WGS, "LDS of a CU");
+    const auto kernel = &tree_attn_kernel<HDP, E, CW, NSET, COPY>;
     if (lds > 64 * 1024) {
-        static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(&tree_attn_kernel<HDP, E, CW, NSET>),
+        static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
                                                         hipFuncAttributeMaxDynamicSharedMemorySize, (int)kMost);
         if (e != hipSuccess) return e;
     }
     const unsigned grid = (unsigned)((a.pairs + 7) / 8 * 8 * a.ncb);
-    tree_attn_kernel<HDP, E, CW, NSET><<<grid, S::THREADS, lds, st>>>(a);
+    kernel<<<grid, S::THREADS, lds, st>>>(a);
     return hipSuccess;
 }
 
-template <int HDP, TreeElem E>
+template <int HDP, TreeElem E, bool COPY>
 hipError_t launch_cols(hipStream_t st, const Args &a, int cols) {
-    if (cols == 16) return launch<HDP, E, 1, 1>(st, a);
+    if (cols == 16) return launch<HDP, E, 1, 1, COPY>(st, a);
     if constexpr (HDP < 256)
-        if (cols == 128) return launch<HDP, E, 4, 2>(st, a);
-    return launch<HDP, E, 4, 1>(st, a);
+        if (cols == 128) return launch<HDP, E, 4, 2, COPY>(st, a);
+    return launch<HDP, E, 4, 1, COPY>(st, a);
 }
 
-template <TreeElem E>
+template <TreeElem E, bool COPY>
 hipError_t launch_elem(hipStream_t st, const Args &a, const Plan &p) {
-    return p.hdp == 64 ? launch_cols<64, E>(st, a, p.cols)
-           : p.hdp == 128 ? launch_cols<128, E>(st, a, p.cols)
-                          : launch_cols<256, E>(st, a, p.cols);
+    if (p.hdp == 64) return launch_cols<64, E, COPY>(st, a, p.cols);
+    if constexpr (COPY || E == TreeElem::F32)  // (E4M3 rows that end inside a piece: at most 120 dims)
+        if (p.hdp == 256) return launch_cols<256, E, COPY>(st, a, p.cols);
+    return launch_cols<128, E, COPY>(st, a, p.cols);
 }
 
 }  // namespace
@@ -960,10 +1137,11 @@ eb_status launch_attn_tree(hipStream_t st, const TreeAttn &x, float *ws, size_t 
     a.pairs = (int)x.hkv * p.nsplit;
     while (x.block > 0 && (size_t)1 << a.block_log2 < x.block) ++a.block_log2;
     a.scale_log2 = x.scale * kLog2e;
-    const hipError_t e = x.elem == TreeElem::F32    ? launch_elem<TreeElem::F32>(st, a, p)
-                         : x.elem == TreeElem::F16  ? launch_elem<TreeElem::F16>(st, a, p)
-                         : x.elem == TreeElem::E4M3 ? launch_elem<TreeElem::E4M3>(st, a, p)
-                                                    : launch_elem<TreeElem::I8>(st, a, p);
+    const hipError_t e = x.elem == TreeElem::F32   ? launch_elem<TreeElem::F32, false>(st, a, p)
+                         : x.elem == TreeElem::F16 ? launch_elem<TreeElem::F16, true>(st, a, p)
+                         : x.elem == TreeElem::I8  ? launch_elem<TreeElem::I8, true>(st, a, p)
+                         : p.copy                  ? launch_elem<TreeElem::E4M3, true>(st, a, p)
+                                                   : launch_elem<TreeElem::E4M3, false>(st, a, p);
     if (e != hipSuccess) return hip_fail(e, "attn_tree launch set-up");
     const eb_status s = check_launch("attn_tree");
     if (s != EB_OK || p.nsplit == 1) return s;
