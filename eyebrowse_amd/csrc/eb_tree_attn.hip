@@ -194,11 +194,34 @@ __device__ __forceinline__ bool has_nonfinite_f16(unsigned w) {
     return ((w & 0x7C00u) == 0x7C00u) | ((w & 0x7C000000u) == 0x7C000000u);
 }
 
-// x as two halves, each rounded to nearest: 22 bits. (A fused multiply-add takes the half as it is.)
+// x, computed here and not earlier: keeps what only rare branches need out of the common path.
+template <class T>
+__device__ __forceinline__ T here(T x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+// x less the low (or high) half of h, one instruction (the compiler takes two).
+__device__ __forceinline__ float less_low(float x, f16x2 h) {
+    float r;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
+    return r;
+}
+__device__ __forceinline__ float less_high(float x, f16x2 h) {
+    float r;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
+    return r;
+}
+// x as two halves, each rounded to nearest: 22 bits. x comes from ordinary vector instructions (no
+// matrix instruction's result, which inline assembly would not wait for).
 __device__ __forceinline__ void split(f32x8 x, f16x8 &hi, f16x8 &lo) {
     hi = __builtin_convertvector(x, f16x8);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = __builtin_fmaf((float)hi[i], -1.0f, x[i]);
+    for (int i = 0; i < 8; i += 2) {
+        const f16x2 h = {hi[i], hi[i + 1]};
+        x[i] = less_low(x[i], h);
+        x[i + 1] = less_high(x[i + 1], h);
+    }
     lo = __builtin_convertvector(x, f16x8);
 }
 
@@ -555,7 +578,7 @@ void tree_attn_kernel(Args a) {
         for (int e = 0; e < S::ND; ++e) acc[s][e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    // One group of 32 keys from k0 on, in buf.
+    // One group of 32 keys from k0 on, in buf; edge: some may be hidden from some column.
     auto consume = [&](const char *buf, int kg, int k0, bool edge) {
         const float *s_scale = reinterpret_cast<const float *>(buf + 2 * PL * PLANE);  // (stored rows)
         const unsigned *s_exp = reinterpret_cast<const unsigned *>(buf + 2 * T * S::RB);  // (copied codes)
@@ -567,15 +590,21 @@ void tree_attn_kernel(Args a) {
         // Reads on their way: [unit][two][plane], as they lie in LDS (copied bytes: a K unit is the 16
         // dims of two steps, a V unit 8 bytes).
         u32x4 fr[AHEAD][2][PL];
+        // Copied rows: piece c of a row is at its exclusive or with the row (piece_xor); a lane's own pieces
+        // are those of step 0 (K) or group 0 (V) with the step's bits flipped, rows being aligned.
+        typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+        const unsigned tile0 = (unsigned)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const char *)buf);
+        const int vr = BYTES ? 4 * g4 + ((n >> 1) & 3) : 4 * g4 + (n >> 2);  // (its row of the first 16)
+        const unsigned k_at = tile0 + (32 * kg + n) * S::RB + ((g4 ^ piece_xor<S::RB>(n)) * 16);
+        const unsigned v_at = tile0 + (T + 32 * kg + vr + (BYTES ? (n >> 3) * 16 : 0)) * S::RB + (n & 1) * 8 +
+                              (((BYTES ? 0 : (n >> 1) & 1) ^ piece_xor<S::RB>(vr)) * 16);
         auto read_k = [&](int i) {
 #pragma unroll
             for (int sub = 0; sub < 2; ++sub) {
                 const int r = 32 * kg + 16 * sub + n;
                 if constexpr (COPY) {
-                    const int c = 4 * (BYTES ? i / 2 : i) + g4;
                     if (!BYTES || i % 2 == 0)
-                        fr[i % AHEAD][sub][0] =
-                            *reinterpret_cast<const u32x4 *>(buf + r * S::RB + ((c ^ piece_xor<S::RB>(n)) * 16));
+                        fr[i % AHEAD][sub][0] = *(const lds_u32x4 *)((k_at ^ (64 * (BYTES ? i / 2 : i))) + 16 * sub * S::RB);
                 } else {
                     const char *at = buf + (r * S::CH + ((4 * i + g4) ^ (r & S::SW))) * 16;
 #pragma unroll
@@ -595,25 +624,21 @@ void tree_attn_kernel(Args a) {
         // V by keys in the lane's order: stored so (output group e = 4 q + d is dims 4 (16 q + n) + d, lane
         // n's row of V), or copied rows read across: 16 lanes read 16 dims of 4 keys (halves) or of 8 (bytes)
         // and get their own dim of each.
-        const char *vt = COPY ? buf + T * S::RB + 32 * kg * S::RB + (n & 1) * 8
-                              : buf + PL * PLANE + kg * (HDP * 64) + v_row<HDP>(4 * n, g4);
+        const char *vt = buf + PL * PLANE + kg * (HDP * 64) + v_row<HDP>(4 * n, g4);  // (stored)
         auto read_v = [&](int u) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 if constexpr (BYTES) {
-                    const int r = 4 * g4 + ((n >> 1) & 3), key = r + (n >> 3) * 16;
-                    const int c = (2 * u + e) ^ piece_xor<S::RB>(r);
                     const auto w = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                        (__attribute__((address_space(3))) i32x2 *)(vt + key * S::RB + c * 16));
+                        (__attribute__((address_space(3))) i32x2 *)(v_at ^ (16 * (2 * u + e))));
                     fr[u % AHEAD][e][0][0] = w[0];
                     fr[u % AHEAD][e][0][1] = w[1];
                 } else if constexpr (COPY) {
-                    const int r = 4 * g4 + (n >> 2), c = (2 * (2 * u + e) + ((n >> 1) & 1)) ^ piece_xor<S::RB>(r);
 #pragma unroll
                     for (int sub = 0; sub < 2; ++sub) {
                         const auto w = __builtin_bit_cast(
-                            u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                       (__attribute__((address_space(3))) i16x4 *)(vt + (16 * sub + r) * S::RB + c * 16)));
+                            u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((
+                                       address_space(3))) i16x4 *)((v_at ^ (32 * (2 * u + e))) + 16 * sub * S::RB)));
                         fr[u % AHEAD][e][0][2 * sub] = w[0];
                         fr[u % AHEAD][e][0][2 * sub + 1] = w[1];
                     }
@@ -735,9 +760,11 @@ void tree_attn_kernel(Args a) {
                     w[i] = __builtin_fmaf(y[i], qk[i / 4], -ref[s]);
                     if constexpr (E == TreeElem::F16) least = fminf(least, w[i]);
                 }
+                if constexpr (E == TreeElem::F16) least = here(least);
                 if (edge) {
+                    const unsigned bits = here(seen);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) w[i] = (seen >> i) & 1u ? w[i] : -INFINITY;
+                    for (int i = 0; i < 8; ++i) w[i] = (bits >> i) & 1u ? w[i] : -INFINITY;
                 }
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -752,12 +779,13 @@ void tree_attn_kernel(Args a) {
                 const bool over = (top > (S::SCALED ? kSlack : kSlack + kUnit)) | (most > kTop) | (least == -INFINITY);
                 if (!again || __builtin_amdgcn_ballot_w64(over) == 0) break;
                 float t1 = -INFINITY;
+                const unsigned bits = here(seen);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     // (An infinite half of K meets q's two halves, whose signs may agree: infinity times 0
                     // is NaN whatever they gave. f32 rows' split made it NaN, E4M3 has no infinity.)
                     if constexpr (E == TreeElem::F16) y[i] = __builtin_fmaf(y[i], 0.0f, y[i]);
-                    t1 = fmaxf(t1, (seen >> i) & 1u ? y[i] * qk[i / 4] : -INFINITY);
+                    t1 = fmaxf(t1, (bits >> i) & 1u ? y[i] * qk[i / 4] : -INFINITY);
                 }
                 t1 = fmaxf(t1, eb::lane_xor16(t1));
                 t1 = fmaxf(t1, eb::lane_xor32(t1));  // the column's largest score of the group
@@ -770,7 +798,7 @@ void tree_attn_kernel(Args a) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const float p = eb::fast_exp2(__builtin_fmaf(y[i], qk[i / 4], -rn)) * vs[i / 4][i % 4];
-                        big = fmaxf(big, (seen >> i) & 1u ? p : 0.0f);
+                        big = fmaxf(big, (bits >> i) & 1u ? p : 0.0f);
                     }
                     big = fmaxf(big, eb::lane_xor16(big));
                     big = fmaxf(big, eb::lane_xor32(big));
@@ -791,11 +819,12 @@ void tree_attn_kernel(Args a) {
             }
             l[s] += sum;
             if (edge) {  // (a NaN scale does not reach what a column does not see)
+                const unsigned bits = here(seen);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     if constexpr (!S::SCALED)
                         w[i] *= (COPY ? s_bad : s_scale + T)[32 * kg + 16 * (i / 4) + 4 * g4 + i % 4];
-                    if (!((seen >> i) & 1u)) w[i] = 0.0f;
+                    if (!((bits >> i) & 1u)) w[i] = 0.0f;
                 }
             }
             split(f32x8{w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]}, ph[s], pl[s]);
