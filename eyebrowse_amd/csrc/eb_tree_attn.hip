@@ -1065,25 +1065,90 @@ struct Plan {
     bool copy;
 };
 
-constexpr size_t kMinSplitKeys = 128;
+// How many columns share a workgroup, and how many workgroups share the keys, by an estimate of the
+// whole call's time (us): launch and a workgroup's start (queries, first tile), its tiles one after
+// the other, and for several splits the merge's launch and what is written for it and read again. A
+// tile costs its 32-key groups times 16-column sets at `set` each, times the workgroups that share the
+// CU, but at least `chain` a group that one wave takes. Few columns start sooner and spread wider, many
+// convert and read each key for more of them. Both sides measured (us; 32 heads over 8 of 128 unless
+// said), estimate in brackets:
+//   21 nodes behind 8191 block-scaled keys: 16 columns, 10 splits 23.5 (23.6); 64, 16 splits 27.5 (28);
+//   128, 32 splits 30.8 (30). 64 behind 1000 half keys: 16 columns 16.4 (17), 64 18.0, 128 25.2 (20).
+//   64 behind 32000 half keys: 16 columns 152, 64 86, 128 78. 16 behind 8000 f32 keys: 16 columns 41.7,
+//   64 29.7, 128 33.1. 16 nodes (32 columns) behind 200 E4M3 keys: one split 8.3 (7.5), two 10.2 (10).
+struct Cost {
+    float set, chain;
+};
+Cost cost_of(int hdp, TreeElem e, int cols) {
+    const int c = cols == 16 ? 0 : cols == 64 ? 1 : 2;
+    static const Cost f32[3] = {{0.96f, 1.6f}, {0.335f, 1.6f}, {0.296f, 2.4f}};
+    static const Cost f16[3] = {{0.28f, 1.3f}, {0.148f, 1.3f}, {0.112f, 2.0f}};
+    static const Cost e4[3] = {{0.22f, 1.3f}, {0.15f, 1.3f}, {0.12f, 2.0f}};
+    static const Cost i8[3] = {{0.24f, 1.5f}, {0.2f, 1.5f}, {0.15f, 2.2f}};
+    const Cost *t = e == TreeElem::F32 ? f32 : e == TreeElem::F16 ? f16 : e == TreeElem::E4M3 ? e4 : i8;
+    const float dims = (float)(hdp + 64) / 192.0f;  // (the products grow with the dims, the softmax does not)
+    return Cost{t[c].set * dims, t[c].chain * dims};
+}
+
+bool copies(TreeElem e, size_t hd) { return e != TreeElem::F32 && (e != TreeElem::E4M3 || hd % 16 == 0); }
+
+// The columns a workgroup may take, the largest number of splits, and the keys of a tile.
+struct Width {
+    int cols, cw, nset, wgs, T;
+    size_t most;
+};
+int widths_of(size_t cols, size_t hkv, size_t hd, TreeElem e, int cu_count, Width (&w)[3]) {
+    const int hdp = hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
+    const bool copy = copies(e, hd);
+    int n = 0;
+    for (const int c : {16, 64, 128}) {
+        if ((c == 64 && cols <= 16) || (c == 128 && (cols <= 64 || hdp == 256))) continue;
+        Width x{c, c == 16 ? 1 : 4, c == 128 ? 2 : 1, 0, 0, 0};
+        x.wgs = waves_of(x.cw, x.nset, copy) == 8 || (e == TreeElem::F32 && hdp == 256) ? 1 : 2;
+        x.T = 32 * key_groups(hdp, e, x.cw, x.nset, copy);
+        x.most = std::max<size_t>(1, (size_t)cu_count * x.wgs / (hkv * ((cols + c - 1) / c)));
+        w[n++] = x;
+    }
+    return n;
+}
+
 Plan plan_of(size_t h, size_t hkv, size_t hd, size_t pos, size_t n, size_t window, TreeElem elem, int cu_count) {
-    Plan p{};
-    p.hdp = hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
-    p.copy = elem != TreeElem::F32 && (elem != TreeElem::E4M3 || hd % 16 == 0);
     const size_t cols = n * (h / hkv);
-    p.cols = cols <= 16 ? 16 : cols <= 64 || p.hdp == 256 ? 64 : 128;
-    p.ncb = (int)((cols + p.cols - 1) / p.cols);
-    const int cw = p.cols == 16 ? 1 : 4, nset = p.cols == 128 ? 2 : 1;
-    const int T = 32 * key_groups(p.hdp, elem, cw, nset, p.copy);
     const size_t first = window > 0 && pos + 1 > window ? pos + 1 - window : 0;
-    p.key0 = (int)(first & ~(size_t)15);
-    p.tiles = (int)((pos + n - p.key0 + T - 1) / T);
-    const int wgs = waves_of(cw, nset, p.copy) == 8 ? 1 : 2;
-    size_t nsplit = std::max<size_t>(1, (size_t)cu_count * wgs / (hkv * p.ncb));
-    nsplit = std::min(nsplit, (size_t)p.tiles);
-    if (pos + n - first <= kMinSplitKeys) nsplit = 1;
-    p.nsplit = (int)nsplit;
-    return p;
+    Plan best{};
+    best.hdp = hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
+    best.copy = copies(elem, hd);
+    best.key0 = (int)(first & ~(size_t)15);
+    const size_t keys = pos + n - best.key0;
+    float least = 0.0f;
+    Width widths[3];
+    const int nw = widths_of(cols, hkv, hd, elem, cu_count, widths);
+    for (int i = 0; i < nw; ++i) {
+        const Width &w = widths[i];
+        const size_t ncb = (cols + w.cols - 1) / w.cols, tiles = (keys + w.T - 1) / w.T;
+        const Cost c = cost_of(best.hdp, elem, w.cols);
+        const int sets = (int)std::min<size_t>(w.cols / 16, (cols + 15) / 16), kw = std::min(w.T / 32, w.cw == 1 ? 4 : w.nset == 2 || best.copy ? 2 : 1);
+        const float start = 2.0f + (w.cols == 16 ? 2.5f : w.cols == 64 ? 3.5f : 4.5f);
+        const size_t tries[] = {w.most, w.most * 3 / 4, w.most / 2, w.most / 3, w.most / 4, 4, 3, 2, 1};
+        for (size_t s : tries) {
+            s = std::min(std::min(std::max<size_t>(s, 1), w.most), tiles);
+            const size_t per = (tiles + s - 1) / s;  // tiles of a split
+            s = (tiles + per - 1) / per;
+            const size_t wgs = hkv * ncb * s, room = (size_t)cu_count * w.wgs;
+            const float shared = (float)std::min<size_t>(w.wgs, (wgs + cu_count - 1) / cu_count);
+            const float tile = std::max(c.chain * (float)(w.T / 32 / kw), c.set * (float)(w.T / 32 * sets) * shared);
+            float us = start + (float)((wgs + room - 1) / room) * tile * (float)per;
+            if (s > 1) us += 4.0f + 8.0f * (float)(s * n * h * hd) / 4.0e6f;
+            if (best.cols == 0 || us < least) {
+                least = us;
+                best.cols = w.cols;
+                best.ncb = (int)ncb;
+                best.tiles = (int)tiles;
+                best.nsplit = (int)s;
+            }
+        }
+    }
+    return best;
 }
 
 template <int HDP, TreeElem E, int CW, int NSET, bool COPY>
@@ -1125,11 +1190,15 @@ hipError_t launch_elem(hipStream_t st, const Args &a, const Plan &p) {
 
 namespace eb {
 
-// part_acc [nsplit, n * h, hd], part_ml [nsplit, n * h, 2]; a window only lowers the splits.
+// part_acc [nsplit, n * h, hd], part_ml [nsplit, n * h, 2], for the most splits that a call with any
+// window may take.
 size_t tree_attn_workspace_floats(size_t h, size_t hkv, size_t hd, size_t pos, size_t n, TreeElem elem, int cu_count) {
     if (n == 0) return 0;
-    const Plan p = plan_of(h, hkv, hd, pos, n, 0, elem, cu_count);
-    return p.nsplit > 1 ? (size_t)p.nsplit * n * h * (hd + 2) : 0;
+    Width w[3];
+    size_t splits = 1;
+    for (int i = widths_of(n * (h / hkv), hkv, hd, elem, cu_count, w) - 1; i >= 0; --i)
+        splits = std::max(splits, std::min(w[i].most, (pos + n + w[i].T - 1) / w[i].T));
+    return splits > 1 ? splits * n * h * (hd + 2) : 0;
 }
 
 eb_status launch_attn_tree(hipStream_t st, const TreeAttn &x, float *ws, size_t ws_floats, int cu_count) {
