@@ -3,7 +3,8 @@
 //
 // Plan and walk are integers of at most kTreeMax nodes: one workgroup, a node per thread, bound by
 // latency. Both follow parents by doubling: after r rounds a node knows its ancestors within 2^r
-// steps, so a tree of depth d takes log2(d) rounds of two barriers instead of d dependent reads.
+// steps, so a tree of depth d takes log2(d) rounds instead of d dependent reads. A round reads what it wrote to
+// one half of LDS and the next one writes to the other, so one barrier parts them.
 //
 // The copies are bound by HBM: every byte read once and written once.
 #include "eb_cache_i8.h"
@@ -32,25 +33,25 @@ __device__ __forceinline__ int parent_of(const int *parents, int i) {
 __global__ __launch_bounds__(kThreads) void tree_plan_kernel(const int *__restrict__ parents,
                                                              unsigned *__restrict__ masks,
                                                              unsigned *__restrict__ depths, int n) {
-    __shared__ unsigned s_mask[kWords][kNodes];
-    __shared__ int s_up[kNodes];
+    __shared__ unsigned s_mask[2][kWords][kNodes];
+    __shared__ int s_up[2][kNodes];
     const int i = threadIdx.x;
     const int words = (n + 31) / 32;
     int up = i < n ? parent_of(parents, i) : -1;
     unsigned mask[kWords];
 #pragma unroll
     for (int w = 0; w < kWords; ++w) mask[w] = w == i / 32 ? 1u << (i % 32) : 0u;
-    while (__syncthreads_or(up >= 0)) {
-        s_up[i] = up;
+    for (int r = 0;; r ^= 1) {
+        s_up[r][i] = up;
 #pragma unroll
         for (int w = 0; w < kWords; ++w)
-            if (w < words) s_mask[w][i] = mask[w];
-        __syncthreads();
+            if (w < words) s_mask[r][w][i] = mask[w];
+        if (!__syncthreads_or(up >= 0)) break;
         if (up >= 0) {
 #pragma unroll
             for (int w = 0; w < kWords; ++w)
-                if (w < words) mask[w] |= s_mask[w][up];
-            up = s_up[up];
+                if (w < words) mask[w] |= s_mask[r][w][up];
+            up = s_up[r][up];
         }
     }
     if (i >= n) return;
@@ -72,8 +73,9 @@ __global__ __launch_bounds__(kThreads) void tree_accept_kernel(const unsigned *_
                                                                unsigned *__restrict__ path,
                                                                unsigned *__restrict__ emitted,
                                                                unsigned *__restrict__ count, int n) {
-    __shared__ unsigned s_sampled[kNodes], s_first[kNodes], s_ok[kNodes];
-    __shared__ int s_up[kNodes], s_dist[kNodes];
+    __shared__ unsigned s_sampled[kNodes], s_first[kNodes];
+    __shared__ unsigned s_state[2][kNodes];  // whether taken so far, and the distance to `up`
+    __shared__ int s_up[2][kNodes];
     const int i = threadIdx.x;
     const bool in = i < n;
     int up = in && i > 0 ? parent_of(parents, i) : -1;
@@ -85,16 +87,16 @@ __global__ __launch_bounds__(kThreads) void tree_accept_kernel(const unsigned *_
     __syncthreads();
     // Taken from its parent; then from all ancestors up to node 0, `dist` steps away.
     unsigned ok = i == 0 || (up >= 0 && s_first[up] == (unsigned)i);
-    int dist = up >= 0 ? 1 : 0;
-    while (__syncthreads_or(up >= 0)) {
-        s_ok[i] = ok;
-        s_dist[i] = dist;
-        s_up[i] = up;
-        __syncthreads();
+    unsigned dist = up >= 0 ? 1 : 0;
+    for (int r = 0;; r ^= 1) {
+        s_state[r][i] = dist * 2 + ok;
+        s_up[r][i] = up;
+        if (!__syncthreads_or(up >= 0)) break;
         if (up >= 0) {
-            ok &= s_ok[up];
-            dist += s_dist[up];
-            up = s_up[up];
+            const unsigned state = s_state[r][up];
+            ok &= state;
+            dist += state >> 1;
+            up = s_up[r][up];
         }
     }
     const int accepted = __syncthreads_count(in && ok);
@@ -225,32 +227,23 @@ __global__ __launch_bounds__(kThreads) void kv_compact_i8_kernel(CompactI8Args a
 }
 
 constexpr int kMaxRuns = 2 * kMaxLayers;
-constexpr int kRunUnroll = 8;
-constexpr size_t kRunChunk = (size_t)kThreads * 16 * kRunUnroll;  // bytes a workgroup copies
+constexpr size_t kRunChunk = (size_t)kThreads * 16;  // bytes a workgroup copies
 struct RunArgs {
     eb::ByteRun run[kMaxRuns];
 };
 
-// Workgroup (x, run): chunk x of the run, 16 bytes per lane and access, all of a thread's loads
-// before its stores; a run's last 15 bytes one by one.
+// Workgroup (x, run): chunk x of the run, one 16-byte vector a thread; a run's last 15 bytes one by
+// one. The stores are non-temporal: nothing reads the copy soon. One vector a thread keeps more waves
+// with a load on the way than several do: 64 runs of 16.4 MB (an 8000-row f16 cache of 32 layers) take
+// 331 us (6.3 TB/s), with 2 vectors 354, with 4 337 to 368, with 8 493; 56 runs of 1.4 MB 23.0 us, with
+// 8 vectors 43.4; stores that stay in the caches 342 and 22.7.
 __global__ __launch_bounds__(kThreads) void copy_runs_kernel(RunArgs a) {
     const eb::ByteRun &r = a.run[blockIdx.y];
     const size_t at = (size_t)blockIdx.x * kRunChunk;
     if (at >= r.bytes) return;
-    const size_t vecs = r.bytes / 16, v0 = at / 16 + threadIdx.x;
-    const u32x4 *src = static_cast<const u32x4 *>(r.src);
-    u32x4 *dst = static_cast<u32x4 *>(r.dst);
-    u32x4 x[kRunUnroll];
-#pragma unroll
-    for (int i = 0; i < kRunUnroll; ++i) {
-        const size_t v = v0 + (size_t)i * kThreads;
-        if (v < vecs) x[i] = __builtin_nontemporal_load(src + v);
-    }
-#pragma unroll
-    for (int i = 0; i < kRunUnroll; ++i) {
-        const size_t v = v0 + (size_t)i * kThreads;
-        if (v < vecs) __builtin_nontemporal_store(x[i], dst + v);
-    }
+    const size_t vecs = r.bytes / 16, v = at / 16 + threadIdx.x;
+    if (v < vecs)
+        __builtin_nontemporal_store(static_cast<const u32x4 *>(r.src)[v], static_cast<u32x4 *>(r.dst) + v);
     if (at + kRunChunk >= r.bytes && threadIdx.x < r.bytes % 16) {
         const size_t t = vecs * 16 + threadIdx.x;
         static_cast<uint8_t *>(r.dst)[t] = static_cast<const uint8_t *>(r.src)[t];
@@ -261,14 +254,16 @@ __global__ __launch_bounds__(kThreads) void copy_runs_kernel(RunArgs a) {
 
 namespace eb {
 
+static unsigned threads_of(size_t n) { return (unsigned)((n + 63) / 64 * 64); }
+
 eb_status launch_tree_plan(hipStream_t st, const int32_t *parents, uint32_t *masks, uint32_t *depths, size_t n) {
-    tree_plan_kernel<<<1, kThreads, 0, st>>>(parents, masks, depths, (int)n);
+    tree_plan_kernel<<<1, threads_of(n), 0, st>>>(parents, masks, depths, (int)n);
     return check_launch("tree_plan");
 }
 
 eb_status launch_tree_accept(hipStream_t st, const uint32_t *tokens, const int32_t *parents, const uint32_t *sampled,
                              uint32_t *path, uint32_t *emitted, uint32_t *count, size_t n) {
-    tree_accept_kernel<<<1, kThreads, 0, st>>>(tokens, parents, sampled, path, emitted, count, (int)n);
+    tree_accept_kernel<<<1, threads_of(n), 0, st>>>(tokens, parents, sampled, path, emitted, count, (int)n);
     return check_launch("tree_accept");
 }
 
