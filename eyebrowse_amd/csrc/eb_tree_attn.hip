@@ -5,36 +5,46 @@
 //   o[c] = sum_j 2^(s_cj - m) v_j / sum_j 2^(s_cj - m),   s_cj = scale log2(e) q_c . k_j
 //
 // over the keys j that column c sees; a column is one query head of one node. All columns of a KV
-// head read the same keys: a workgroup takes up to 128 of them, so that each key is fetched from
-// memory, and brought into the matrix cores' format, once for all. Split keys, then a log-sum-exp
-// merge.
+// head read the same keys: a workgroup takes 16, 64 or 128 of them, so that each key is fetched from
+// memory once for all of those. Split keys, then a log-sum-exp merge.
 //
-// A workgroup walks tiles of T keys. Half of its waves fetch K, half V, a tile ahead, into
-// registers; they become f16 operands on their way into LDS:
-//  - f32 rows: scaled by a power of two (the row's largest element in [2^13, 2^14)) and split into
-//    two halves, each rounded to nearest (22 bits; the product of the two low halves is left out:
-//    three matrix products per result); the power comes back with the score (K) or in the weight (V);
-//  - half and E4M3 rows, and the codes of a block-scaled cache: exact as they are (two products,
-//    for the two halves of q or of the weight); a block's scales come back as those powers do.
-// K lies in LDS by rows, V transposed, so that both are 16-byte operand reads; chunks are xor-ed
-// with the row (K) or the dim (V), which spreads eight neighbouring lanes over the banks.
+// A workgroup walks tiles of T keys; half of its waves fetch K, half V. Two ways to the matrix cores'
+// f16 operands:
+//  - Copied rows (half, E4M3 of whole 16-byte pieces, block-scaled codes) go from memory to LDS as they
+//    are, up to four tiles ahead, no register on the way. K's pieces are the score's operand as read; V
+//    is read across (16 lanes get 16 dims of 4 or 8 keys, each its own dim of all). Bytes become f16 at
+//    use. Pieces are xor-ed with the row, against bank conflicts.
+//  - Stored rows (f32; E4M3 rows that end inside a piece) pass through registers, a tile ahead, and
+//    become f16 on their way into LDS, once for all columns. An f32 row is scaled by a power of two (its
+//    largest element in [2^13, 2^14)) and split into two halves, each rounded to nearest (22 bits; the
+//    product of the two low halves is left out: three matrix products per result); the power comes back
+//    with the score (K) or in the weight (V). K lies by rows, V transposed.
+// Half, E4M3 and code values are exact in f16 (two products, for the two halves of q or of the
+// weight); a block's scales come back as those powers do.
 //
 // Lane (n, g) is lane n + 16 g of a wave; a wave owns 16 or 32 columns.
 //  - Scores S[key][column] on v_mfma_f32_16x16x32_f16: lane (n, g) ends with keys 4g .. 4g + 3 of
 //    each of two 16-key halves of a 32-key group, for column n.
 //  - O^T[dim][column] += V^T P^T, the 32 contracted indices being the group's keys in the order in
-//    which lane (n, g) holds them: its own scores are the operand, no lane exchange. V's transposed
-//    rows are stored in that order. Lane (n, g) ends with dims 4g .. 4g + 3 (+ 16 e) of column n, so
-//    that m, l and every rescale belong to the lane's own column.
+//    which lane (n, g) holds them: its own scores are the operand, no lane exchange; V comes in that
+//    order. Lane (n, g) ends with four dims of every 16 of column n, so that m, l and every rescale
+//    belong to the lane's own column.
 //  - Online softmax with a reference m per column that moves only when a score exceeds it by more
 //    than kSlack. Where V rows have powers of two of their own (f32, block-scaled), the weights carry
 //    them, in a unit per column (2^lcu) that moves when a term would pass 2^15: a row of large
 //    values that a column does not see costs it nothing.
 //
 // A key that a column does not see has weight exactly 0, and its V row is finite where any column
-// of the workgroup may not see it: in tiles with masked keys a row that is not finite is stored as
-// zeros and its weight made NaN, which reaches the columns that see it and no others. A column
-// that sees nothing gives zeros.
+// of the workgroup may not see it: in tiles with masked keys a row that is not finite becomes zeros
+// and its weight NaN, which reaches the columns that see it and no others. A column that sees nothing
+// gives zeros.
+//
+// What binds it, with 32 heads over 8 of 128 (whole calls in a graph): 4 nodes, the cache's bytes (behind
+// 30000 f32 keys 48 us, 5.1 TB/s, the rate of a large copy); 64 nodes, matrix instructions and the
+// softmax and conversions beside them, which two waves to a SIMD overlap in part (behind 32000 half keys
+// 76 us, 440 TFLOP/s of the formula's products and 880 of those issued; 30000 E4M3 71, block-scaled 87,
+// f32 133 us); between, both, and the call's fixed parts: 3 to 5 us until a workgroup's first tile is
+// there, 4 to 6 us for the merge and its launch (21 nodes behind 8191 block-scaled keys 23.6 us).
 #include "eb_cache_i8.h"
 #include "eb_tree.h"
 
@@ -999,7 +1009,8 @@ void tree_attn_kernel(Args a) {
 }
 
 // o[row] = sum of the splits' sums, at one reference. Workgroup: one row (node and head); a group of
-// lanes holds the row's dims, four each, the groups share the splits, four at a time in flight.
+// lanes holds the row's dims, four each, the groups share the splits, four at a time in flight. Bound
+// by latency and its launch: 128 rows of 63 splits 3.9 us in a trace, 2048 rows of 16 (17 MB) 5.8.
 constexpr int kMergeThreads = 256;
 __global__ __launch_bounds__(kMergeThreads) void tree_merge_kernel(const float *__restrict__ part_acc,
                                                               const float *__restrict__ part_ml, float *__restrict__ o,
@@ -1070,12 +1081,16 @@ struct Plan {
 // the other, and for several splits the merge's launch and what is written for it and read again. A
 // tile costs its 32-key groups times 16-column sets at `set` each, times the workgroups that share the
 // CU, but at least `chain` a group that one wave takes. Few columns start sooner and spread wider, many
-// convert and read each key for more of them. Both sides measured (us; 32 heads over 8 of 128 unless
-// said), estimate in brackets:
-//   21 nodes behind 8191 block-scaled keys: 16 columns, 10 splits 23.5 (23.6); 64, 16 splits 27.5 (28);
-//   128, 32 splits 30.8 (30). 64 behind 1000 half keys: 16 columns 16.4 (17), 64 18.0, 128 25.2 (20).
-//   64 behind 32000 half keys: 16 columns 152, 64 86, 128 78. 16 behind 8000 f32 keys: 16 columns 41.7,
-//   64 29.7, 128 33.1. 16 nodes (32 columns) behind 200 E4M3 keys: one split 8.3 (7.5), two 10.2 (10).
+// read each f32 key's operands and each half row for more of them. All sides measured (us; 32 heads over
+// 8 of 128 unless said; in brackets the estimates for 16, 64 and 128 columns):
+//   21 nodes behind 8191 block-scaled keys: 23.5, 27.5, 30.8 (23.7, 27.7, 27.5)
+//   64 nodes behind  1000 half keys:        16.4, 18.0, 25.2 (17.1, 16.5, 19.2)
+//   64 nodes behind 32000 half keys:         152,   86,   78 (174, 95.6, 82.9)
+//   16 nodes behind 30000 half keys:          51, 35.3       (49.6, 33.2)
+//   64 nodes behind  8000 f32 keys:                58.9, 52.9 (131, 60.8, 56.8)
+//   16 nodes behind  8000 f32 keys:         41.7, 29.7       (41.3, 26.5)
+//   16 nodes of 16 heads behind 200 E4M3 keys: 8.3 with one split, 10.9 with 64 columns (7.1, 10.7)
+//   8 nodes of 16 heads behind 100 f32 keys: 10.5 with one split, 9.2 with four (16 columns)
 struct Cost {
     float set, chain;
 };
@@ -1100,6 +1115,7 @@ struct Width {
 int widths_of(size_t cols, size_t hkv, size_t hd, TreeElem e, int cu_count, Width (&w)[3]) {
     const int hdp = hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
     const bool copy = copies(e, hd);
+    cu_count = std::min(cu_count, 1024);  // (a caller's number)
     int n = 0;
     for (const int c : {16, 64, 128}) {
         if ((c == 64 && cols <= 16) || (c == 128 && (cols <= 64 || hdp == 256))) continue;

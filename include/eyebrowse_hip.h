@@ -823,11 +823,14 @@ eb_status eb_launch_tree_accept(void *stream, const uint32_t *tokens, size_t tok
 /* Moves rows pos + path[j] of every layer's K and V to rows pos + j, j < min(count[0], n), in place.
  * The path counts up to its first entry that is not below n or not above the one before. The rows
  * behind keep what they hold. Any cache; a block-scaled one is read and written as eb_kv_read_i8 and
- * eb_kv_write_i8 do. */
+ * eb_kv_write_i8 do (the rows behind keep their codes; those in the last moved row's block take its
+ * new exponent). */
 eb_status eb_kv_compact(eb_recorder *rec, eb_kv_cache *kv, const eb_tensor *path,
                         const eb_tensor *count, size_t n, size_t pos);
 /* Rows 0..count - 1 of every layer's K and V of src into dst: the same prompt continued twice. The
- * caches have the same layers, heads, elements and block; their max_seq may differ. Bit-exact. */
+ * caches have the same layers, heads, elements and block; their max_seq may differ. Bit-exact. dst's
+ * rows from count on keep what they hold (block-scaled: their codes; the last copied block's exponents
+ * are src's). */
 eb_status eb_kv_fork(eb_recorder *rec, eb_kv_cache *dst, const eb_kv_cache *src, size_t count);
 
 /* ---- self-check (no counterpart in the reference) ----------------------------------
