@@ -277,7 +277,8 @@ void tree_attn_kernel(Args a) {
     const int nodes = node_of(min(col0 + S::COLS, a.ncols) - 1) - node0 + 1;  // of this workgroup's columns
     char *s_ql = smem + S::NBUF * S::TILE;  // [CW][NSET][NC][lane]
     float *s_bad = reinterpret_cast<float *>(s_ql + S::QBYTES);  // [T] (copied rows: 1, or NaN)
-    unsigned *s_mask = reinterpret_cast<unsigned *>(s_bad + (COPY ? T : 0));    // [nodes][words]
+    int *s_any = reinterpret_cast<int *>(s_bad + T);  // (copied rows) a tile that has a row with NaN
+    unsigned *s_mask = reinterpret_cast<unsigned *>(s_bad + (COPY ? T + 1 : 0));  // [nodes][words]
     int *s_depth = reinterpret_cast<int *>(s_mask + nodes * a.words);           // [n] (with a window)
 
     // ---- tiles: fetched into registers, then stored as operands -----------------------------------
@@ -502,6 +503,7 @@ void tree_attn_kernel(Args a) {
 
     // ---- the columns' queries, masks and first keys -------------------------------------------------
     const unsigned first_mask = tid < nodes * a.words ? a.masks[(size_t)node0 * a.words + tid] : 0u;
+    const unsigned first_depth = a.window > 0 && tid < a.n ? a.depths[tid] : 0u;
     auto put_mask = [&](int i, unsigned w) {
         if (i % a.words == a.words - 1 && a.n % 32) w &= (1u << (a.n % 32)) - 1u;  // (no nodes past n)
         s_mask[i] = w;
@@ -555,8 +557,9 @@ void tree_attn_kernel(Args a) {
         }
     }
     for (int i = tid; i < nodes * a.words; i += kThreads) put_mask(i, i == tid ? first_mask : a.masks[(size_t)node0 * a.words + i]);
+    if (COPY && tid == 0) *s_any = -1;
     if (a.window > 0)
-        for (int i = tid; i < a.n; i += kThreads) s_depth[i] = (int)min(a.depths[i], 1u << 27);
+        if (tid < a.n) s_depth[tid] = (int)min(first_depth, 1u << 27);  // (a node per thread at most)
     __syncthreads();
     int safe_lo = 0;  // keys below it may be behind some column's window
     bool shallow = true;  // no drafted key is behind any node's window
@@ -894,19 +897,27 @@ void tree_attn_kernel(Args a) {
             if constexpr (!S::SCALED) {
                 if (edge) {  // V rows that are not finite: zeros, and NaN for the weight
                     for (int i = tid; i < T; i += kThreads) s_bad[i] = 1.0f;
-                    __syncthreads();
                     u32x4 *v = reinterpret_cast<u32x4 *>(buf + T * S::RB);
-                    for (int i = tid; i < T * S::CR; i += kThreads) {
+                    auto is_bad = [&](int i) {
                         const u32x4 w = v[i];
                         bool bad = false;
 #pragma unroll
                         for (int d = 0; d < 4; ++d) bad = bad | (ES == 2 ? has_nonfinite_f16(w[d]) : has_nan_e4m3(w[d]));
-                        if (bad) s_bad[i / S::CR] = __builtin_nanf("");
+                        return bad;
+                    };
+                    bool any = false;
+#pragma unroll
+                    for (int i = 0; i < T * S::CR / kThreads; ++i) any = any | is_bad(i * kThreads + tid);
+                    if (any) *s_any = t;
+                    __syncthreads();
+                    if (*s_any == t) {
+                        for (int i = tid; i < T * S::CR; i += kThreads)
+                            if (is_bad(i)) s_bad[i / S::CR] = __builtin_nanf("");
+                        __syncthreads();
+                        for (int i = tid; i < T * S::CR; i += kThreads)
+                            if (s_bad[i / S::CR] != 1.0f) v[i] = u32x4{0u, 0u, 0u, 0u};
+                        __syncthreads();
                     }
-                    __syncthreads();
-                    for (int i = tid; i < T * S::CR; i += kThreads)
-                        if (s_bad[i / S::CR] != 1.0f) v[i] = u32x4{0u, 0u, 0u, 0u};
-                    __syncthreads();
                 }
             }
             multiply(buf, r0, edge);
@@ -1170,7 +1181,7 @@ Plan plan_of(size_t h, size_t hkv, size_t hd, size_t pos, size_t n, size_t windo
 template <int HDP, TreeElem E, int CW, int NSET, bool COPY>
 hipError_t launch(hipStream_t st, const Args &a) {
     using S = Shape<HDP, E, CW, NSET, COPY>;
-    constexpr size_t kTiles = (size_t)S::NBUF * S::TILE + S::QBYTES + (COPY ? S::T * 4 : 0);
+    constexpr size_t kTiles = (size_t)S::NBUF * S::TILE + S::QBYTES + (COPY ? S::T * 4 + 4 : 0);
     const size_t nodes = std::min<size_t>(a.n, S::COLS);
     const size_t lds = kTiles + (nodes * a.words + (a.window > 0 ? a.n : 0)) * 4;
     constexpr size_t kMost = kTiles + (S::COLS * 8 + 256) * 4;
