@@ -544,11 +544,11 @@ void tree_attn_kernel(Args a) {
         // (q times scale log2(e), its largest in [2^13, 2^14) or, if the product rounds up, at 2^14)
         const unsigned e = biased_exponent(fabsf(top * a.scale_log2));
         qs[s] = pow2_biased(e - 13u);
-        const float f = a.scale_log2 * pow2_biased(267u - e);
+        const float f = pow2_biased(267u - e);  // (beside a scale of 4 and more it could pass f32's range)
 #pragma unroll
         for (int i = 0; i < S::NC; ++i) {
             f16x8 lo;
-            split(x[i] * f, qh[s][i], lo);
+            split(x[i] * a.scale_log2 * f, qh[s][i], lo);
             if constexpr (S::QLDS) {
                 if (kw == 0) *reinterpret_cast<f16x8 *>(s_ql + ((cw * NSET + s) * S::NC + i) * 1024 + lane * 16) = lo;
             } else {

@@ -109,3 +109,41 @@ def test_same_call_same_bits(dev):
         first = c.attend(dev, q, nodes, pos, 0.1).tobytes()
         for _ in range(3):
             assert c.attend(dev, q, nodes, pos, 0.1).tobytes() == first, elem
+
+
+@pytest.mark.parametrize("elem", ["f32", "f16", "e4m3", "i8"])
+@pytest.mark.parametrize("n,pos", [(9, 0), (9, 2500), (70, 300)])
+def test_queries_that_are_not_finite(dev, elem, n, pos):
+    """They make their own head of their node NaN, where it sees a key, and change no other bit."""
+    note(f"tree plans, queries {elem} {n} {pos}")
+    rng = np.random.default_rng(6)
+    h, hkv, hd = 8, 2, 128
+    seen = Nodes(dev, random_parents(n, rng)).seen
+    seen[4] = False
+    nodes = Nodes(dev, seen=seen, depths=seen.sum(1))
+    c = Cache(dev, elem, pos + n, hkv, hd, rows(rng, pos + n, hkv, hd), rows(rng, pos + n, hkv, hd))
+    q = rng.standard_normal((n, h, hd)).astype(np.float32)
+    want = c.attend(dev, q, nodes, pos, 0.1)
+    q[0, 1, 5], q[3, 7, 127], q[n - 1, 2, 0], q[4, 0, 3] = np.nan, np.inf, -np.inf, np.nan
+    got = c.attend(dev, q, nodes, pos, 0.1)
+    bad = np.zeros((n, h), bool)
+    bad[0, 1] = bad[3, 7] = bad[n - 1, 2] = True
+    bad[4, 0] = pos > 0  # (otherwise it sees nothing: zeros)
+    assert np.isnan(got[bad]).all()
+    assert got[~bad].tobytes() == want[~bad].tobytes()
+
+
+@pytest.mark.parametrize("elem", ["f32", "f16", "e4m3", "i8"])
+@pytest.mark.parametrize("scale", [0.0, -0.1, 1e-30, 30.0])
+def test_scales(dev, elem, scale):
+    """All keys alike, the least alike key first, all nearly alike, one key with all the weight; and a node of zeros."""
+    note(f"tree plans, scale {elem} {scale}")
+    rng = np.random.default_rng(7)
+    h, hkv, hd, n, pos = 8, 2, 64, 11, 1300
+    nodes = Nodes(dev, random_parents(n, rng))
+    c = Cache(dev, elem, pos + n, hkv, hd, rows(rng, pos + n, hkv, hd), rows(rng, pos + n, hkv, hd))
+    q = rng.standard_normal((n, h, hd)).astype(np.float32)
+    q[2] = 0
+    got = c.attend(dev, q, nodes, pos, scale)
+    want, bound = attention(q, c.k, c.v, visible(nodes.seen, nodes.depth, pos, 0), np.float64(np.float32(scale)))
+    assert np.isfinite(got).all() and (np.abs(got - want) <= bound).all(), (np.abs(got - want) / bound).max()
