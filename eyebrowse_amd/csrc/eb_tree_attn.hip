@@ -147,6 +147,9 @@ struct Args {
     float scale_log2;
 };
 
+// 1 / l (to a step of f32: five of them meet in a result at most) for a sum of weights, which is at
+// least about 1; 0 where no key was seen.
+__device__ __forceinline__ float inverse(float l) { return l == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(l); }
 // The largest of N neighbouring lanes' values, in each of them.
 template <int N>
 __device__ __forceinline__ float lanes_max(float x) {
@@ -948,14 +951,21 @@ void tree_attn_kernel(Args a) {
             l[s] += eb::lane_xor32(l[s]);
         }
     }
-    if constexpr (S::SCALED) {  // out of the columns' units
+    // A set's averages, out of their units. Where V may be of any size (SCALED) they are formed before
+    // the waves' are joined: from there on nothing passes the size of V's own values.
+    auto average = [&](int s) {
+        const float inv = inverse(l[s]);
 #pragma unroll
-        for (int s = 0; s < NSET; ++s)
-#pragma unroll
-            for (int e = 0; e < S::ND; ++e)
+        for (int e = 0; e < S::ND; ++e) {
+            acc[s][e] *= inv;
+            if constexpr (S::SCALED)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) acc[s][e][r] = ldexpf(acc[s][e][r], -(int)lcu[s]);
-    }
+        }
+    };
+    if constexpr (S::SCALED)
+#pragma unroll
+        for (int s = 0; s < NSET; ++s) average(s);
     if constexpr (KW > 1) {  // a set at a time: into LDS, and to the first of the waves
         constexpr int SLOT = S::ND * 1024 + 512;  // bytes a wave leaves
 #pragma unroll
@@ -976,9 +986,15 @@ void tree_attn_kernel(Args a) {
                     const char *at = smem + ((w - 1) * CW + cw) * SLOT;
                     const float *ml = reinterpret_cast<const float *>(at + S::ND * 1024);
                     const float r2 = ml[lane], rn = fmaxf(ref[s], r2);
-                    const float f1 = eb::fast_exp2(ref[s] - rn), f2 = eb::fast_exp2(r2 - rn);
-                    l[s] = l[s] * f1 + ml[64 + lane] * f2;
+                    float f1 = eb::fast_exp2(ref[s] - rn), f2 = eb::fast_exp2(r2 - rn);
+                    const float l1 = l[s] * f1, l2 = ml[64 + lane] * f2;
+                    l[s] = l1 + l2;
                     ref[s] = rn;
+                    if constexpr (S::SCALED) {
+                        const float inv = inverse(l[s]);
+                        f1 = l1 * inv;
+                        f2 = l2 * inv;
+                    }
 #pragma unroll
                     for (int e = 0; e < S::ND; ++e)
                         acc[s][e] = acc[s][e] * f1 + f2 * *reinterpret_cast<const f32x4 *>(at + e * 1024 + lane * 16);
@@ -992,15 +1008,15 @@ void tree_attn_kernel(Args a) {
     for (int s = 0; s < NSET; ++s) {
         const int c = col0 + (cw * NSET + s) * 16 + n;
         if (c >= a.ncols) continue;
+        if constexpr (!S::SCALED) average(s);
         const int node = node0 + my_node[s];
         const size_t row = (size_t)node * a.h + kvh * a.g + c - node * a.g;
         const size_t at = a.nsplit == 1 ? row : (size_t)split_id * a.n * a.h + row;
         float *out = (a.nsplit == 1 ? a.o : a.part_acc) + at * hd;
-        const float f = a.nsplit > 1 ? 1.0f : l[s] == 0.0f ? 0.0f : 1.0f / l[s];
         if constexpr (COPY) {
 #pragma unroll
             for (int e = 0; e < S::ND; ++e)
-                if (16 * e + 4 * g4 < hd) *reinterpret_cast<f32x4 *>(out + 16 * e + 4 * g4) = acc[s][e] * f;
+                if (16 * e + 4 * g4 < hd) *reinterpret_cast<f32x4 *>(out + 16 * e + 4 * g4) = acc[s][e];
         } else {
 #pragma unroll
             for (int q = 0; q < S::ND / 4; ++q)
@@ -1008,8 +1024,8 @@ void tree_attn_kernel(Args a) {
                 for (int r = 0; r < 4; ++r) {
                     const int d = 64 * q + 16 * g4 + 4 * r;
                     if (d < hd)
-                        *reinterpret_cast<f32x4 *>(out + d) = f32x4{acc[s][4 * q][r] * f, acc[s][4 * q + 1][r] * f,
-                                                                    acc[s][4 * q + 2][r] * f, acc[s][4 * q + 3][r] * f};
+                        *reinterpret_cast<f32x4 *>(out + d) = f32x4{acc[s][4 * q][r], acc[s][4 * q + 1][r],
+                                                                    acc[s][4 * q + 2][r], acc[s][4 * q + 3][r]};
                 }
         }
         if (a.nsplit > 1 && g4 == 0) {
@@ -1019,7 +1035,7 @@ void tree_attn_kernel(Args a) {
     }
 }
 
-// o[row] = sum of the splits' sums, at one reference. Workgroup: one row (node and head); a group of
+// o[row] = average of the splits' averages, each weighed by its sum of weights at one reference. Workgroup: one row (node and head); a group of
 // lanes holds the row's dims, four each, the groups share the splits, four at a time in flight. Bound
 // by latency and its launch: 128 rows of 63 splits 3.9 us in a trace, 2048 rows of 16 (17 MB) 5.8.
 constexpr int kMergeThreads = 256;
@@ -1051,17 +1067,20 @@ __global__ __launch_bounds__(kMergeThreads) void tree_merge_kernel(const float *
 #pragma unroll
         for (int j = 0; j < B; ++j)
             if (s0 + j * groups < nsplit) mn = fmaxf(mn, bm[j]);
-        const float c = eb::fast_exp2(M - mn);
-        L *= c;
-        A *= c;
+        float Ln = L * eb::fast_exp2(M - mn);
+        const float had = Ln;
 #pragma unroll
         for (int j = 0; j < B; ++j) {
-            if (s0 + j * groups >= nsplit) continue;
-            const float w = eb::fast_exp2(bm[j] - mn);
-            L += w * bl[j];
-            A += w * ba[j];
+            bl[j] = s0 + j * groups < nsplit ? bl[j] * eb::fast_exp2(bm[j] - mn) : 0.0f;
+            Ln += bl[j];
         }
+        const float inv = inverse(Ln);
+        A *= had * inv;
+#pragma unroll
+        for (int j = 0; j < B; ++j)
+            if (s0 + j * groups < nsplit) A += (bl[j] * inv) * ba[j];
         M = mn;
+        L = Ln;
     }
     s_m[tid] = M;
     s_l[tid] = L;
@@ -1071,15 +1090,17 @@ __global__ __launch_bounds__(kMergeThreads) void tree_merge_kernel(const float *
     float mt = M;
     for (int g = 1; g < groups; ++g) mt = fmaxf(mt, s_m[(g << lanes_log2) + tid]);
     float Lt = 0.0f;
+    for (int g = 0; g < groups; ++g) {
+        const int i = (g << lanes_log2) + tid;
+        Lt += eb::fast_exp2(s_m[i] - mt) * s_l[i];
+    }
+    const float inv = inverse(Lt);  // (no key seen: zeros)
     f32x4 At = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int g = 0; g < groups; ++g) {
         const int i = (g << lanes_log2) + tid;
-        const float w = eb::fast_exp2(s_m[i] - mt);
-        Lt += w * s_l[i];
-        At += w * s_a[i];
+        At += (eb::fast_exp2(s_m[i] - mt) * s_l[i] * inv) * s_a[i];
     }
-    const float inv = Lt == 0.0f ? 0.0f : 1.0f / Lt;  // (no key seen: zeros)
-    *reinterpret_cast<f32x4 *>(o + (size_t)row * hd + d) = At * inv;
+    *reinterpret_cast<f32x4 *>(o + (size_t)row * hd + d) = At;
 }
 
 struct Plan {

@@ -147,3 +147,25 @@ def test_scales(dev, elem, scale):
     got = c.attend(dev, q, nodes, pos, scale)
     want, bound = attention(q, c.k, c.v, visible(nodes.seen, nodes.depth, pos, 0), np.float64(np.float32(scale)))
     assert np.isfinite(got).all() and (np.abs(got - want) <= bound).all(), (np.abs(got - want) / bound).max()
+
+
+@pytest.mark.parametrize("size", [1e-41, 1e-30, 1e30, 3e37])
+def test_sizes_of_rows(dev, size):
+    """f32 rows at the ends of their range, in K (against queries of the other end) and in V."""
+    note(f"tree plans, rows of {size}")
+    rng = np.random.default_rng(8)
+    h, hkv, hd, n, pos = 4, 2, 64, 9, 500
+    nodes = Nodes(dev, random_parents(n, rng))
+    k = rows(rng, pos + n, hkv, hd)
+    v = np.clip(rng.standard_normal((pos + n, hkv, hd)), -3, 3).astype(np.float32)
+    q = rng.standard_normal((n, h, hd)).astype(np.float32)
+    plain = Cache(dev, "f32", pos + n, hkv, hd, k, v)
+    c = Cache(dev, "f32", pos + n, hkv, hd, k, (v.astype(np.float64) * size).astype(np.float32))
+    got = c.attend(dev, q, nodes, pos, 0.1)
+    want, bound = attention(q, c.k, c.v, visible(nodes.seen, nodes.depth, pos, 0), 0.1)
+    # (a value or a result below 2^-126 may be taken for zero)
+    assert np.isfinite(got).all() and (np.abs(got - want) <= bound + 2 * 2.0 ** -126).all()
+    if size > 1e-40:
+        c = Cache(dev, "f32", pos + n, hkv, hd, (k * np.float32(2.0 ** np.round(np.log2(size) / 2))).astype(np.float32), v)
+        small = (q * np.float32(2.0 ** -np.round(np.log2(size) / 2))).astype(np.float32)
+        assert c.attend(dev, small, nodes, pos, 0.1).tobytes() == plain.attend(dev, q, nodes, pos, 0.1).tobytes()
