@@ -67,7 +67,7 @@ using eb::TreeElem;
 constexpr float kSlack = 8.0f;     // log2 units a score may exceed its reference by
 constexpr float kTop = 32768.0f;   // largest weight of a term (f16 holds 65504)
 constexpr float kUnit = 7.0f;      // log2 of a weight at its reference
-constexpr float kNoRef = -1.0e30f;  // a reference below all scores: no key yet
+constexpr float kNoRef = -3.0e38f;  // a reference below all scores: no key yet
 constexpr unsigned kNone = 0x7FFFFFF0u;  // a byte offset past any tile
 
 // How a call is run: COPY moves the cache's rows to LDS as they are (half rows, E4M3 rows of whole
@@ -807,7 +807,7 @@ void tree_attn_kernel(Args a) {
                 t1 = fmaxf(t1, eb::lane_xor32(t1));  // the column's largest score of the group
                 if constexpr (!S::SCALED) t1 -= kUnit;
                 const float rn = t1 > ref[s] + kSlack ? t1 : ref[s];
-                const float d = ref[s] - rn;  // (-1e30 or so at the column's first keys)
+                const float d = ref[s] - rn;  // (-3e38 or so, or -inf, at the column's first keys)
                 float f = d;
                 if constexpr (S::SCALED) {
                     float big = 0.0f;  // the group's largest term

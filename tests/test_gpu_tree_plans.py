@@ -169,3 +169,21 @@ def test_sizes_of_rows(dev, size):
         c = Cache(dev, "f32", pos + n, hkv, hd, (k * np.float32(2.0 ** np.round(np.log2(size) / 2))).astype(np.float32), v)
         small = (q * np.float32(2.0 ** -np.round(np.log2(size) / 2))).astype(np.float32)
         assert c.attend(dev, small, nodes, pos, 0.1).tobytes() == plain.attend(dev, q, nodes, pos, 0.1).tobytes()
+
+
+@pytest.mark.parametrize("elem", ["f32", "f16"])
+@pytest.mark.parametrize("size", [1e25, -1e25, -1e31, 1e31])
+def test_large_scores(dev, elem, size):
+    """All keys alike, with scores near the ends of f32's range: V's average."""
+    note(f"tree plans, scores of {size} {elem}")
+    rng = np.random.default_rng(9)
+    h, hkv, hd, n, pos = 4, 2, 64, 5, 700
+    nodes = Nodes(dev, random_parents(n, rng))
+    k = np.broadcast_to(np.sign(rng.standard_normal((1, hkv, hd))), (pos + n, hkv, hd)).astype(np.float32) * np.float32(64)
+    v = rng.standard_normal((pos + n, hkv, hd)).astype(np.float32)
+    c = Cache(dev, elem, pos + n, hkv, hd, k, v)
+    q = np.repeat(k[:n], h // hkv, 1) * np.float32(size / 64 ** 2)
+    got = c.attend(dev, q, nodes, pos, 1.0)
+    # (alike keys have the same score to the bit, so the weights are alike whatever the scores' error)
+    want, bound = attention(np.zeros_like(q), c.k, c.v, visible(nodes.seen, nodes.depth, pos, 0), 1.0)
+    check(got, want, bound, f"{elem} {size}")
