@@ -78,6 +78,8 @@ __device__ __forceinline__ SegView seg_of(const eb::RowsArgs &a, int t) {
 //
 // TREE: a token's table row is rope_row0 + its depth, read with the row (a.depths; the angles then
 // wait for it). A depth past the launch's rows, which no tree has, makes the rotated row NaN.
+// 16 nodes of 16/8 heads of 128 into f32 2.8 us (a launch), 256 of 32/8 into half 4.7 (11.7 MB; 3.7 in a
+// trace).
 template <int LPR, bool TREE>
 __global__ __launch_bounds__(kThreads) void rows_vec_kernel(eb::RowsArgs a) {
 #pragma clang fp contract(off)

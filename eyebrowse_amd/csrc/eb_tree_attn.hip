@@ -40,11 +40,12 @@
 // gives zeros.
 //
 // What binds it, with 32 heads over 8 of 128 (whole calls in a graph): 4 nodes, the cache's bytes (behind
-// 30000 f32 keys 48 us, 5.1 TB/s, the rate of a large copy); 64 nodes, matrix instructions and the
+// 30000 f32 keys 48 to 49 us, 5.1 TB/s, the rate of a large copy); 64 nodes, matrix instructions and the
 // softmax and conversions beside them, which two waves to a SIMD overlap in part (behind 32000 half keys
-// 76 us, 440 TFLOP/s of the formula's products and 880 of those issued; 30000 E4M3 71, block-scaled 87,
-// f32 133 us); between, both, and the call's fixed parts: 3 to 5 us until a workgroup's first tile is
-// there, 4 to 6 us for the merge and its launch (21 nodes behind 8191 block-scaled keys 23.6 us).
+// 76 to 81 us, 416 to 440 TFLOP/s of the formula's products, twice that issued; 30000 E4M3 71 to 74,
+// block-scaled 87 to 89, f32 133 to 139 us); between, both, and the call's fixed parts: 3 to 5 us until
+// a workgroup's first tile is there, 4 to 6 us for the merge and its launch (21 nodes behind 8191
+// block-scaled keys 24 us).
 #include "eb_cache_i8.h"
 #include "eb_tree.h"
 
@@ -1037,7 +1038,7 @@ void tree_attn_kernel(Args a) {
 
 // o[row] = average of the splits' averages, each weighed by its sum of weights at one reference. Workgroup: one row (node and head); a group of
 // lanes holds the row's dims, four each, the groups share the splits, four at a time in flight. Bound
-// by latency and its launch: 128 rows of 63 splits 3.9 us in a trace, 2048 rows of 16 (17 MB) 5.8.
+// by latency and its launch: 480 rows of 9 splits 4.0 us in a trace, 2048 rows of 16 (17 MB) 6.1 to 6.8.
 constexpr int kMergeThreads = 256;
 __global__ __launch_bounds__(kMergeThreads) void tree_merge_kernel(const float *__restrict__ part_acc,
                                                               const float *__restrict__ part_ml, float *__restrict__ o,
