@@ -604,6 +604,7 @@ void tree_attn_kernel(Args a) {
         for (int s = 0; s < NSET; ++s) sc[s][0] = sc[s][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         constexpr int AHEAD = S::AHEAD;
         constexpr bool BYTES = COPY && ES == 1;
+        constexpr int VSHIFT = E == TreeElem::I8 ? 8 : 0;
         // Reads on their way: [unit][two][plane], as they lie in LDS (copied bytes: a K unit is the 16
         // dims of two steps, a V unit 8 bytes).
         u32x4 fr[AHEAD][2][PL];
@@ -718,7 +719,8 @@ void tree_attn_kernel(Args a) {
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) read_v(u);
         __builtin_amdgcn_sched_barrier(0);  // (on their way while the weights are formed)
-        // Scales of the keys: one each (f32), or of their block, which 16 keys share.
+        // Scales of the keys: one each (f32), or of their block, which 16 keys share (V's then times 2^-VSHIFT,
+        // which the column's unit has instead: a weight of up to 2^8 times a scale of up to 2^122 stays finite).
         f32x4 ks[2], vs[2];
         if constexpr (S::SCALED) {
 #pragma unroll
@@ -728,7 +730,8 @@ void tree_attn_kernel(Args a) {
                     ks[sub] = *reinterpret_cast<const f32x4 *>(at + 4 * g4);
                     vs[sub] = *reinterpret_cast<const f32x4 *>(at + T + 4 * g4);
                 } else {
-                    const float k1 = exponent_scale(s_exp[2 * kg + sub]), v1 = exponent_scale(s_exp[64 + 2 * kg + sub]);
+                    const float k1 = exponent_scale(s_exp[2 * kg + sub]);
+                    const float v1 = exponent_scale(s_exp[64 + 2 * kg + sub]) * 0x1p-8f;
                     ks[sub] = f32x4{k1, k1, k1, k1};
                     vs[sub] = f32x4{v1, v1, v1, v1};
                 }
@@ -768,8 +771,7 @@ void tree_attn_kernel(Args a) {
             const float qk[2] = {E == TreeElem::I8 ? qs[s] * ks[0][0] : qs[s], E == TreeElem::I8 ? qs[s] * ks[1][0] : qs[s]};
             // Weights against the present reference and unit; where those do not serve, once more.
             for (bool again = true;; again = false) {
-                const float cu = S::SCALED ? ldexpf(1.0f, (int)lcu[s]) : 1.0f;
-                const float vc[2] = {S::SCALED ? vs[0][0] * cu : cu, S::SCALED ? vs[1][0] * cu : cu};
+                const float cu = S::SCALED ? ldexpf(1.0f, (int)lcu[s] + VSHIFT) : 1.0f;
                 float top = -INFINITY, least = INFINITY, most = 0.0f;
                 sum = 0.0f;
 #pragma unroll
@@ -789,7 +791,11 @@ void tree_attn_kernel(Args a) {
                     w[i] = eb::fast_exp2(w[i]);
                     if constexpr (S::SCALED) {
                         sum += w[i];
-                        w[i] *= S::F32 ? vs[i / 4][i % 4] * cu : vc[i / 4];
+                        // In this order: a row's scale and the column's unit together may pass f32's range
+                        // beside a weight of zero or near it. What the first product loses below 2^-126 is, times
+                        // the unit of at most 2^127, less than f16's least step. (Block-scaled rows: eight products
+                        // more a group than by a common factor, 0.5 to 2 % of a call.)
+                        w[i] = w[i] * vs[i / 4][i % 4] * cu;
                         most = fmaxf(most, w[i]);
                     }
                 }
@@ -821,8 +827,8 @@ void tree_attn_kernel(Args a) {
                     big = fmaxf(big, eb::lane_xor32(big));
                     // Earlier terms lose 2^d: as much the unit may grow. Where this group's would pass
                     // 2^15 in it, its largest term becomes 2^6 to 2^7.
-                    float unit = fminf(lcu[s] + floorf(-d), 120.0f);
-                    const float eb2 = (float)__builtin_amdgcn_frexp_expf(big);
+                    float unit = fminf(lcu[s] + floorf(-d), S::F32 ? 120.0f : 119.0f);
+                    const float eb2 = (float)(__builtin_amdgcn_frexp_expf(big) + VSHIFT);
                     if (big > 0.0f && eb2 + unit > 15.0f) unit = 7.0f - eb2;
                     f = d + (unit - lcu[s]);
                     lcu[s] = unit;
