@@ -70,6 +70,11 @@ constexpr float kTop = 32768.0f;   // largest weight of a term (f16 holds 65504)
 constexpr float kUnit = 7.0f;      // log2 of a weight at its reference
 constexpr float kNoRef = -3.0e38f;  // a reference below all scores: no key yet
 constexpr unsigned kNone = 0x7FFFFFF0u;  // a byte offset past any tile
+// f32 K: a sum of up to 256 products of 2^14 times 2^14 times a row's power of two (2^-126 to 2^114) passes
+// f32's range although the column's power, which comes last, brings it back: the rows' powers are kept times
+// this (2^-149 at least, which f32 holds), the columns' times its inverse.
+constexpr float kScoreShift = 0x1p-23f;
+constexpr unsigned kScoreShiftLog2 = 23;
 
 // How a call is run: COPY moves the cache's rows to LDS as they are (half rows, E4M3 rows of whole
 // 16-byte pieces, block-scaled codes); otherwise they pass through registers and become f16 there (f32
@@ -125,6 +130,7 @@ struct Shape {
     // q's low halves of 32 columns over f32 caches: in LDS, the registers do not hold them.
     static constexpr bool QLDS = F32 && NSET == 2;
     static constexpr int QBYTES = QLDS ? CW * NSET * NC * 1024 : 0;
+    static constexpr int STEEP = F32 ? COLS * 4 : 0;  // what large queries leave of their power of two
     static constexpr int WGS = WAVES == 8 || (F32 && HDP == 256) ? 1 : 2;  // workgroups per CU
     // Operand reads from LDS that are on their way at once: units of two (16-key halves of a 32-dim
     // step, or two 16-dim groups of V), 8 registers each and plane.
@@ -280,7 +286,8 @@ void tree_attn_kernel(Args a) {
     const int node0 = node_of(col0);
     const int nodes = node_of(min(col0 + S::COLS, a.ncols) - 1) - node0 + 1;  // of this workgroup's columns
     char *s_ql = smem + S::NBUF * S::TILE;  // [CW][NSET][NC][lane]
-    float *s_bad = reinterpret_cast<float *>(s_ql + S::QBYTES);  // [T] (copied rows: 1, or NaN)
+    float *s_steep = reinterpret_cast<float *>(s_ql + S::QBYTES);  // [columns] (f32 K)
+    float *s_bad = reinterpret_cast<float *>(s_ql + S::QBYTES + S::STEEP);  // [T] (copied rows: 1, or NaN)
     int *s_any = reinterpret_cast<int *>(s_bad + T);  // (copied rows) a tile that has a row with NaN
     unsigned *s_mask = reinterpret_cast<unsigned *>(s_bad + (COPY ? T + 1 : 0));  // [nodes][words]
     int *s_depth = reinterpret_cast<int *>(s_mask + nodes * a.words);           // [n] (with a window)
@@ -395,7 +402,7 @@ void tree_attn_kernel(Args a) {
                     split(x * pow2_biased(267u - e), hi, lo);
                     *reinterpret_cast<f16x8 *>(at(c)) = hi;
                     *reinterpret_cast<f16x8 *>(at(c) + PLANE) = lo;
-                    if (c == 0) s_scale[r] = pow2_biased(e - 13u);
+                    if (c == 0) s_scale[r] = pow2_biased(e - 13u) * kScoreShift;
                 } else {
                     const bool whole = 16 * c + 8 < hd;  // (else the next head's)
 #pragma unroll
@@ -519,6 +526,7 @@ void tree_attn_kernel(Args a) {
     auto chunk_dim = [&](int i) { return COPY && ES == 1 ? 64 * (i / 2) + 16 * g4 + 8 * (i % 2) : 32 * i + 8 * g4; };
     f16x8 qh[NSET][S::NC], ql[NSET][S::QLDS ? 1 : S::NC];
     float qs[NSET];
+    bool steep = false;  // (f32 K) a column's power of two, shifted, passes f32's range: s_steep has the rest
     int my_node[NSET], my_first[NSET];
 #pragma unroll
     for (int s = 0; s < NSET; ++s) {
@@ -547,7 +555,14 @@ void tree_attn_kernel(Args a) {
         top = fmaxf(top, eb::lane_xor32(top));
         // (q times scale log2(e), its largest in [2^13, 2^14) or, if the product rounds up, at 2^14)
         const unsigned e = biased_exponent(fabsf(top * a.scale_log2));
-        qs[s] = pow2_biased(e - 13u);
+        if constexpr (S::F32) {
+            const unsigned shifted = e - 13u + kScoreShiftLog2, most = min(shifted, 254u);
+            qs[s] = pow2_biased(most);
+            steep = steep | (shifted > 254u);
+            if (g4 == 0 && kw == 0) s_steep[(cw * NSET + s) * 16 + n] = pow2_biased(127u + shifted - most);
+        } else {
+            qs[s] = pow2_biased(e - 13u);
+        }
         const float f = pow2_biased(267u - e);  // (beside a scale of 4 and more it could pass f32's range)
 #pragma unroll
         for (int i = 0; i < S::NC; ++i) {
@@ -560,6 +575,7 @@ void tree_attn_kernel(Args a) {
             }
         }
     }
+    steep = __builtin_amdgcn_ballot_w64(steep) != 0;
     for (int i = tid; i < nodes * a.words; i += kThreads) put_mask(i, i == tid ? first_mask : a.masks[(size_t)node0 * a.words + i]);
     if (COPY && tid == 0) *s_any = -1;
     if (a.window > 0)
@@ -768,7 +784,17 @@ void tree_attn_kernel(Args a) {
                 y[i] = sc[s][i / 4][i % 4];
                 if constexpr (S::F32) y[i] *= ks[i / 4][i % 4];
             }
-            const float qk[2] = {E == TreeElem::I8 ? qs[s] * ks[0][0] : qs[s], E == TreeElem::I8 ? qs[s] * ks[1][0] : qs[s]};
+            if constexpr (S::F32)
+                if (steep) {
+                    const float rest = s_steep[(cw * NSET + s) * 16 + n];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) y[i] *= rest;
+                }
+            // (Finite, so that a score of zero stays zero; a NaN block's stays NaN.)
+            float qk[2] = {qs[s], qs[s]};
+            if constexpr (E == TreeElem::I8)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) qk[i] = __builtin_elementwise_minimum(qs[s] * ks[i][0], 0x1p127f);
             // Weights against the present reference and unit; where those do not serve, once more.
             for (bool again = true;; again = false) {
                 const float cu = S::SCALED ? ldexpf(1.0f, (int)lcu[s] + VSHIFT) : 1.0f;
@@ -792,9 +818,9 @@ void tree_attn_kernel(Args a) {
                     if constexpr (S::SCALED) {
                         sum += w[i];
                         // In this order: a row's scale and the column's unit together may pass f32's range
-                        // beside a weight of zero or near it. What the first product loses below 2^-126 is, times
-                        // the unit of at most 2^127, less than f16's least step. (Block-scaled rows: eight products
-                        // more a group than by a common factor, 0.5 to 2 % of a call.)
+                        // beside a weight of zero or near it. What the first product loses below 2^-126 (2^-150)
+                        // is, times a unit of at most 2^127, two of f16's least steps. (Block-scaled rows: eight
+                        // products more a group than by a common factor, 0.5 to 2 % of a call.)
                         w[i] = w[i] * vs[i / 4][i % 4] * cu;
                         most = fmaxf(most, w[i]);
                     }
@@ -1209,7 +1235,7 @@ Plan plan_of(size_t h, size_t hkv, size_t hd, size_t pos, size_t n, size_t windo
 template <int HDP, TreeElem E, int CW, int NSET, bool COPY>
 hipError_t launch(hipStream_t st, const Args &a) {
     using S = Shape<HDP, E, CW, NSET, COPY>;
-    constexpr size_t kTiles = (size_t)S::NBUF * S::TILE + S::QBYTES + (COPY ? S::T * 4 + 4 : 0);
+    constexpr size_t kTiles = (size_t)S::NBUF * S::TILE + S::QBYTES + S::STEEP + (COPY ? S::T * 4 + 4 : 0);
     const size_t nodes = std::min<size_t>(a.n, S::COLS);
     const size_t lds = kTiles + (nodes * a.words + (a.window > 0 ? a.n : 0)) * 4;
     constexpr size_t kMost = kTiles + (S::COLS * 8 + 256) * 4;

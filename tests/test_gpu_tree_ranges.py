@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 from tests._gpu import note
-from tests._tree import Cache, Nodes, attention, random_parents, visible
+from tests._tree import Cache, Nodes, attention, random_parents, rows, visible
 
 pytestmark = pytest.mark.gpu
 
@@ -42,3 +42,68 @@ def test_light_keys_with_large_values(dev, elem, gap, small, large, n):
             lost += (pos + n) * 2.0 ** -31 * 2 * max(tops) / (~light[:pos]).sum()
         assert np.isfinite(got).all()
         assert (np.abs(got - want) <= bound + lost).all(), (np.abs(got - want) / (bound + lost)).max()
+
+
+@pytest.mark.parametrize("power", [100, 116, 119, -100, -116, -119])
+@pytest.mark.parametrize("n", [3, 40])
+def test_keys_and_queries_of_unlike_size(dev, power, n):
+    """f32 K rows at one end of the range and queries at the other: ordinary scores."""
+    note(f"tree ranges, K 2^{power} n {n}")
+    rng = np.random.default_rng(2)
+    h, hkv, hd, pos = 8, 2, 64, 500
+    nodes = Nodes(dev, random_parents(n, rng))
+    # Multiples of 2^-6 up to 2^6: exact at either end.
+    k = np.clip(np.round(rows(rng, pos + n, hkv, hd) * 64), -4096, 4096) / 64 * 2.0 ** power
+    q = np.clip(np.round(rng.standard_normal((n, h, hd)) * 64), -256, 256) / 64 * 2.0 ** -power
+    k, q = k.astype(np.float32), q.astype(np.float32)
+    assert np.isfinite(k).all() and np.isfinite(q).all()
+    c = Cache(dev, "f32", pos + n, hkv, hd, k, rows(rng, pos + n, hkv, hd))
+    got = c.attend(dev, q, nodes, pos, 0.1)
+    want, bound = attention(q, k, c.v, visible(nodes.seen, nodes.depth, pos, 0), 0.1)
+    assert np.isfinite(got).all() and (np.abs(got - want) <= bound).all(), (np.abs(got - want) / bound).max()
+
+
+@pytest.mark.parametrize("size", [1e30, 1e35, 2e37])
+@pytest.mark.parametrize("side", ["k", "q"])
+def test_one_key_takes_all(dev, size, side):
+    """K rows (or queries) near the end of f32's range against ordinary ones: scores that f32 holds, the
+    largest of which takes a node's whole weight."""
+    note(f"tree ranges, {side} of {size}")
+    rng = np.random.default_rng(3)
+    h, hkv, hd, n, pos = 8, 2, 64, 9, 300
+    nodes = Nodes(dev, random_parents(n, rng))
+    k, v = (np.clip(rng.standard_normal((pos + n, hkv, hd)), -3, 3).astype(np.float32) for _ in range(2))
+    q = np.clip(rng.standard_normal((n, h, hd)), -3, 3).astype(np.float32)
+    if side == "k":
+        k = (k * np.float32(size)).astype(np.float32)
+    else:
+        q = (q * np.float32(size)).astype(np.float32)
+    c = Cache(dev, "f32", pos + n, hkv, hd, k, v)
+    got = c.attend(dev, q, nodes, pos, 0.1)
+    vis = visible(nodes.seen, nodes.depth, pos, 0)
+    for a in range(h):
+        x = np.where(vis, q[:, a].astype(np.float64) @ k[:, a // 4].astype(np.float64).T * 0.1, -np.inf)
+        order = np.sort(x, 1)
+        clear = order[:, -1] - order[:, -2] > 1e-4 * np.abs(x[np.isfinite(x)]).max()  # (beyond the scores' error)
+        assert clear.sum() > n // 2
+        want = v[x.argmax(1), a // 4]
+        assert np.isfinite(got[:, a]).all()
+        assert (np.abs(got[clear, a] - want[clear]) <= 2.0 ** -21 * np.abs(want[clear]) + 2.0 ** -38).all()
+
+
+def test_zero_rows_beside_large_ones_i8(dev):
+    """A row of zeros in a block of large K rows against large queries: its score is zero. The large rows are
+    drafted ones that the nodes here do not see."""
+    note("tree ranges, zero rows i8")
+    rng = np.random.default_rng(6)
+    h, hkv, hd, n, pos = 4, 2, 64, 12, 40
+    nodes = Nodes(dev, [-1] + [0] * (n - 1))
+    k, v = np.zeros((pos + n, hkv, hd), np.float32), rows(rng, pos + n, hkv, hd)
+    k[pos + 1] = 1e30 * rng.uniform(0.5, 1, (hkv, hd))
+    q = (rng.standard_normal((n, h, hd)) * 1e20).astype(np.float32)
+    c = Cache(dev, "i8", pos + n, hkv, hd, k, v, 16)
+    got = c.attend(dev, q, nodes, pos, 1.0)
+    free = ~nodes.seen[:, 1]
+    want, bound = attention(np.zeros_like(q), c.k, c.v, visible(nodes.seen, nodes.depth, pos, 0), 1.0)
+    assert free.sum() == n - 1 and np.isfinite(got[free]).all()
+    assert (np.abs(got - want) <= bound)[free].all()
