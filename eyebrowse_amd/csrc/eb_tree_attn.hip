@@ -36,8 +36,9 @@
 //
 // A key that a column does not see has weight exactly 0, and its V row is finite where any column
 // of the workgroup may not see it: in tiles with masked keys a row that is not finite becomes zeros
-// and its weight NaN, which reaches the columns that see it and no others. A column that sees nothing
-// gives zeros.
+// and its weight NaN, which reaches the columns that see it and no others. Where all see it, a half or
+// E4M3 row goes into the products as it is, and a column whose sums are not finite at the end is made
+// NaN whole (finite rows' sums cannot pass f32's range). A column that sees nothing gives zeros.
 //
 // What binds it, with 32 heads over 8 of 128 (whole calls in a graph): 4 nodes, the cache's bytes (behind
 // 30000 f32 keys 48 to 49 us, 5.1 TB/s, the rate of a large copy); 64 nodes, matrix instructions and the
@@ -1040,8 +1041,28 @@ void tree_attn_kernel(Args a) {
 #pragma unroll
     for (int s = 0; s < NSET; ++s) {
         const int c = col0 + (cw * NSET + s) * 16 + n;
+        if constexpr (!S::SCALED) {
+            average(s);
+            if (a.nsplit == 1) {  // (else the merge does so)
+                float top[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // largest magnitudes (maximum, unlike fmaxf, keeps NaN)
+#pragma unroll
+                for (int e = 0; e < S::ND; ++e)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)  // (stored rows: dims from hd on are the next head's)
+                        if (COPY || 64 * (e / 4) + 16 * g4 + 4 * r < hd)
+                            top[r] = __builtin_elementwise_maximum(top[r], fabsf(acc[s][e][r]));
+                float all = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top[0], top[1]),
+                                                          __builtin_elementwise_maximum(top[2], top[3]));
+                all = __builtin_elementwise_maximum(all, eb::lane_xor16(all));
+                all = __builtin_elementwise_maximum(all, eb::lane_xor32(all));
+                if (!(all < INFINITY)) {
+                    const float nan = __builtin_nanf("");
+#pragma unroll
+                    for (int e = 0; e < S::ND; ++e) acc[s][e] = f32x4{nan, nan, nan, nan};
+                }
+            }
+        }
         if (c >= a.ncols) continue;
-        if constexpr (!S::SCALED) average(s);
         const int node = node0 + my_node[s];
         const size_t row = (size_t)node * a.h + kvh * a.g + c - node * a.g;
         const size_t at = a.nsplit == 1 ? row : (size_t)split_id * a.n * a.h + row;
@@ -1068,13 +1089,15 @@ void tree_attn_kernel(Args a) {
     }
 }
 
-// o[row] = average of the splits' averages, each weighed by its sum of weights at one reference. Workgroup: one row (node and head); a group of
-// lanes holds the row's dims, four each, the groups share the splits, four at a time in flight. Bound
-// by latency and its launch: 480 rows of 9 splits 4.0 us in a trace, 2048 rows of 16 (17 MB) 6.1 to 6.8.
+// o[row] = average of the splits' averages, each weighed by its sum of weights at one reference. narrow: a
+// row with a dim that is not finite becomes NaN (the sums of half and E4M3 values are finite otherwise).
+// Workgroup: one row (node and head); a group of lanes holds the row's dims, four each, the groups share
+// the splits, four at a time in flight. Bound by latency and its launch: 480 rows of 9 splits 4.0 us in a trace, 2048 rows of 16 (17 MB) 6.1 to 6.8.
 constexpr int kMergeThreads = 256;
 __global__ __launch_bounds__(kMergeThreads) void tree_merge_kernel(const float *__restrict__ part_acc,
                                                               const float *__restrict__ part_ml, float *__restrict__ o,
-                                                              int rows, int hd, int nsplit, int lanes_log2) {
+                                                              int rows, int hd, int nsplit, int lanes_log2,
+                                                              bool narrow) {
     __shared__ float s_m[kMergeThreads], s_l[kMergeThreads];
     __shared__ f32x4 s_a[kMergeThreads];
     const int tid = threadIdx.x, row = blockIdx.x;
@@ -1132,6 +1155,13 @@ __global__ __launch_bounds__(kMergeThreads) void tree_merge_kernel(const float *
     for (int g = 0; g < groups; ++g) {
         const int i = (g << lanes_log2) + tid;
         At += (eb::fast_exp2(s_m[i] - mt) * s_l[i] * inv) * s_a[i];
+    }
+    if (narrow) {  // (the row's lanes are one wave's)
+        bool finite = true;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) finite = finite & (fabsf(At[r]) < INFINITY);
+        const float nan = __builtin_nanf("");
+        if (__builtin_amdgcn_ballot_w64(!finite) != 0) At = f32x4{nan, nan, nan, nan};
     }
     *reinterpret_cast<f32x4 *>(o + (size_t)row * hd + d) = At;
 }
@@ -1327,7 +1357,7 @@ eb_status launch_attn_tree(hipStream_t st, const TreeAttn &x, float *ws, size_t 
     int lanes_log2 = 0;
     while ((size_t)4 << lanes_log2 < x.hd) ++lanes_log2;
     tree_merge_kernel<<<(unsigned)rows, kMergeThreads, 0, st>>>(a.part_acc, a.part_ml, x.o, (int)rows, (int)x.hd, p.nsplit,
-                                                           lanes_log2);
+                                                           lanes_log2, x.elem == TreeElem::F16 || x.elem == TreeElem::E4M3);
     return check_launch("attn_tree (merge)");
 }
 

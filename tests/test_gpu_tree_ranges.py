@@ -4,6 +4,7 @@ import pytest
 
 from tests._gpu import note
 from tests._tree import Cache, Nodes, attention, random_parents, rows, visible
+from tests.test_gpu_tree_plans import launch
 
 pytestmark = pytest.mark.gpu
 
@@ -107,3 +108,29 @@ def test_zero_rows_beside_large_ones_i8(dev):
     want, bound = attention(np.zeros_like(q), c.k, c.v, visible(nodes.seen, nodes.depth, pos, 0), 1.0)
     assert free.sum() == n - 1 and np.isfinite(got[free]).all()
     assert (np.abs(got - want) <= bound)[free].all()
+
+
+@pytest.mark.parametrize("elem,what", [("f16", np.nan), ("f16", np.inf), ("f16", -np.inf), ("e4m3", np.nan),
+                                       ("f32", np.inf)])
+@pytest.mark.parametrize("hd,hkv,h,n", [(64, 2, 2, 9), (64, 2, 8, 12), (128, 2, 8, 40), (128, 1, 1, 5), (256, 2, 4, 30),
+                                        (256, 1, 2, 3), (24, 2, 4, 21), (120, 2, 6, 50)])
+@pytest.mark.parametrize("side", ["k", "v"])
+def test_bad_cached_row_that_all_see(dev, elem, what, hd, hkv, h, n, side):
+    """One value that is not finite, in a tile without masked keys, in the last one behind the drafted rows'
+    or in the first: every node's heads over its KV head are NaN, the other KV head's are untouched; one split and many."""
+    note(f"tree ranges, bad row {elem} {what} {side} {h}/{hkv}x{hd} n {n}")
+    rng = np.random.default_rng(5)
+    pos = 900
+    nodes = Nodes(dev, random_parents(n, rng))
+    q = rng.standard_normal((n, h, hd)).astype(np.float32)
+    k, v = rows(rng, pos + n, hkv, hd), rows(rng, pos + n, hkv, hd)
+    clean = {cus: launch(dev, Cache(dev, elem, pos + n, hkv, hd, k, v), elem, q, nodes, pos, 0.1, 0, cus)[0]
+             for cus in (1, 256)}
+    for at, dim in ((0, hd - 1), (413, 5), (pos - 1, 0)):
+        x = (k if side == "k" else v).copy()
+        x[at, 0, dim] = what
+        c = Cache(dev, elem, pos + n, hkv, hd, x if side == "k" else k, x if side == "v" else v)
+        for cus in (1, 256):
+            got = launch(dev, c, elem, q, nodes, pos, 0.1, 0, cus)[0]
+            assert np.isnan(got[:, :h // hkv]).all(), (at, cus, np.isnan(got[:, :h // hkv]).mean())
+            assert got[:, h // hkv:].tobytes() == clean[cus][:, h // hkv:].tobytes()
