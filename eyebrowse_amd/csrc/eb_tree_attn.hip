@@ -69,7 +69,7 @@ using eb::TreeElem;
 constexpr float kSlack = 8.0f;     // log2 units a score may exceed its reference by
 constexpr float kTop = 32768.0f;   // largest weight of a term (f16 holds 65504)
 constexpr float kUnit = 7.0f;      // log2 of a weight at its reference
-constexpr float kNoRef = -3.0e38f;  // a reference below all scores: no key yet
+constexpr float kNoRef = -3.4028235e38f;  // a reference below all scores (f32's lowest): no key yet
 constexpr unsigned kNone = 0x7FFFFFF0u;  // a byte offset past any tile
 // f32 K: a sum of up to 256 products of 2^14 times 2^14 times a row's power of two (2^-126 to 2^114) passes
 // f32's range although the column's power, which comes last, brings it back: the rows' powers are kept times

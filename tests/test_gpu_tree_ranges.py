@@ -134,3 +134,20 @@ def test_bad_cached_row_that_all_see(dev, elem, what, hd, hkv, h, n, side):
             got = launch(dev, c, elem, q, nodes, pos, 0.1, 0, cus)[0]
             assert np.isnan(got[:, :h // hkv]).all(), (at, cus, np.isnan(got[:, :h // hkv]).mean())
             assert got[:, h // hkv:].tobytes() == clean[cus][:, h // hkv:].tobytes()
+
+
+@pytest.mark.parametrize("elem", ["f32", "f16"])
+@pytest.mark.parametrize("size", [-2.2e38, 2.2e38, -2.3e38])
+def test_scores_at_the_ends(dev, elem, size):
+    """All keys alike, their scores' log2 units just inside f32's range: V's average."""
+    note(f"tree ranges, scores of {size} {elem}")
+    rng = np.random.default_rng(4)
+    h, hkv, hd, n, pos = 4, 2, 64, 5, 700
+    nodes = Nodes(dev, random_parents(n, rng))
+    k = np.broadcast_to(np.sign(rng.standard_normal((1, hkv, hd))), (pos + n, hkv, hd)).astype(np.float32) * np.float32(64)
+    v = rng.standard_normal((pos + n, hkv, hd)).astype(np.float32)
+    c = Cache(dev, elem, pos + n, hkv, hd, k, v)
+    q = np.repeat(k[:n], h // hkv, 1) * np.float32(size / 64 ** 3)
+    got = c.attend(dev, q, nodes, pos, 1.0)
+    want, bound = attention(np.zeros_like(q), c.k, c.v, visible(nodes.seen, nodes.depth, pos, 0), 1.0)
+    assert np.isfinite(got).all() and (np.abs(got - want) <= bound).all(), (np.abs(got - want) / bound).max()
