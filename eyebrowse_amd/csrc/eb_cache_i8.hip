@@ -16,6 +16,7 @@ struct Side {  // K or V
     const float *src;  // [count, hkv, hd]
     uint8_t *codes;
     uint8_t *exps;
+    uint32_t *tags;  // (eb::CacheI8)
 };
 
 // Workgroup (b, head, side): the new rows that fall into one block of one KV head, the block's
@@ -92,7 +93,10 @@ __global__ __launch_bounds__(kThreads) void kv_write_i8_kernel(Side k, Side v, i
             *p = eb::i8_recode(*p, old_e, e);
         }
     }
-    if (threadIdx.x == 0) s.exps[b * hkv + head] = (uint8_t)e;
+    if (threadIdx.x == 0) {
+        s.exps[b * hkv + head] = (uint8_t)e;
+        if (s.tags && blockIdx.x == 0) s.tags[eb::kTagWords * head] = 0;
+    }
 }
 
 struct ReadSide {
@@ -141,8 +145,9 @@ eb_status launch_kv_write_i8(hipStream_t st, const CacheI8 &c, const float *k, c
                              size_t count) {
     const size_t blocks = (dst + count - 1) / c.block - dst / c.block + 1;
     const dim3 grid((unsigned)blocks, (unsigned)c.hkv, 2);
-    kv_write_i8_kernel<<<grid, kThreads, 0, st>>>(Side{k, c.k, c.ks}, Side{v, c.v, c.vs}, (int)c.hkv, (int)c.hd,
-                                                  (int)c.block, dst, count);
+    kv_write_i8_kernel<<<grid, kThreads, 0, st>>>(Side{k, c.k, c.ks, c.tags},
+                                                  Side{v, c.v, c.vs, c.tags ? c.tags + eb::kTagWords * c.hkv : nullptr},
+                                                  (int)c.hkv, (int)c.hd, (int)c.block, dst, count);
     return check_launch("kv_write_i8");
 }
 

@@ -356,6 +356,7 @@ __global__ __launch_bounds__(kThreads, 2) void decode_i8_kernel(Args a, int hd) 
         }
         if (lane == 0) {
             exps[(size_t)b * hkv + kvh] = (uint8_t)e;
+            if (a.c.tags) a.c.tags[eb::kTagWords * (wave * hkv + kvh)] = 0;
             s_e[2 * wave] = lead ? old_e : e;
             s_e[2 * wave + 1] = e;
         }

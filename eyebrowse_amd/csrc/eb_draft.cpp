@@ -172,13 +172,14 @@ eb_status tree_checked(hipStream_t st, const Room &room, int cus, const TreeOper
     EB_TRY(eb::check_ptr(vc, "vcache"));
     EB_TRY(aligned({kc, vc}, 16, "attn_tree: the caches"));
     eb::TreeAttn a{t.q, kc, vc, nullptr, nullptr, 0, elem_of(dt), t.masks, window > 0 ? t.depths : nullptr, t.o,
-                   h, hkv, hd, pos, n, window, scale};
+                   h, hkv, hd, pos, n, window, scale, nullptr};
     return attend(st, room, a, cus);
 }
 
-// A block-scaled cache's layer, checked for its shape by the caller.
+// A block-scaled cache's layer, checked for its shape by the caller. tail: see TreeAttn.
 eb_status tree_i8_checked(hipStream_t st, const Room &room, int cus, const TreeOperands &t, const eb::CacheI8 &c,
-                          size_t h, size_t pos, size_t n, float scale, size_t window) {
+                          size_t h, size_t pos, size_t n, float scale, size_t window,
+                          const eb::DraftTail *tail = nullptr) {
     EB_TRY(shape_checked(h, c.hkv, c.hd, c.max_seq, EB_I8));
     EB_TRY(operands_checked(t, h, c.hd, pos, n, c.max_seq, window));
     if (n == 0) return eb::ok();
@@ -188,7 +189,7 @@ eb_status tree_i8_checked(hipStream_t st, const Room &room, int cus, const TreeO
     EB_TRY(eb::check_ptr(c.vs, "v exponents"));
     EB_TRY(aligned({c.k, c.v}, 16, "attn_tree: the codes"));
     eb::TreeAttn a{t.q, c.k, c.v, c.ks, c.vs, c.block, eb::TreeElem::I8, t.masks, window > 0 ? t.depths : nullptr, t.o,
-                   h, c.hkv, c.hd, pos, n, window, scale};
+                   h, c.hkv, c.hd, pos, n, window, scale, tail};
     return attend(st, room, a, cus);
 }
 
@@ -210,7 +211,35 @@ eb_status layer_i8(const eb_kv_cache *kv, size_t layer, eb_device *dev, eb::Cach
     EB_TRY(eb::check_tensor(kv->k[layer], EB_I8, "kv cache", dev));
     *out = eb::CacheI8{data<uint8_t>(kv->k[layer]), data<uint8_t>(kv->k_scale[layer]), data<uint8_t>(kv->v[layer]),
                        data<uint8_t>(kv->v_scale[layer]), kv->max_seq, kv->n_kv_heads,
-                       eb_tensor_dim(kv->k[layer], 2), kv->block};
+                       eb_tensor_dim(kv->k[layer], 2), kv->block, eb::draft_tags(kv, layer), kv->id};
+    return EB_OK;
+}
+
+// The layer's rows beside the cache. Room for the widest tree is taken once (whether it holds a draft is a tag on
+// the device), so that a captured pass and a captured compaction agree about it, whichever was captured first.
+eb_status draft_rows(eb_kv_cache *kv, size_t layer, eb_device *dev, eb::DraftRows *out) {
+    if (!kv->draft_v[layer]) {
+        const size_t shape[3] = {std::min(eb::kTreeMax, kv->max_seq), kv->n_kv_heads, eb_tensor_dim(kv->k[layer], 2)};
+        eb_tensor *k = nullptr, *v = nullptr;
+        EB_TRY(eb_tensor_empty(dev, shape, 3, EB_F32, &k));
+        Owned guard(k);
+        EB_TRY(eb_tensor_empty(dev, shape, 3, EB_F32, &v));
+        kv->draft_k[layer] = guard.release();
+        kv->draft_v[layer] = v;
+    }
+    *out = eb::DraftRows{data<float>(kv->draft_k[layer]), data<float>(kv->draft_v[layer])};
+    return EB_OK;
+}
+
+// Memory for a pass's tail (eb::DraftTail), of a size that does not depend on pos.
+eb_status tail_room(eb_device *dev, const eb::CacheI8 &c, size_t pos, size_t n, size_t window, Owned *hold,
+                    eb::DraftTail *out) {
+    const size_t codes = eb::tree_tail_rows(n, c.block) * c.hkv * c.hd;  // (a multiple of 16)
+    const size_t exps = eb::tree_tail_blocks(n, c.block) * c.hkv, shape[1] = {2 * codes + 2 * exps + 2 * c.hkv * n};
+    EB_TRY(eb_tensor_empty(dev, shape, 1, EB_U8, &hold->t));
+    uint8_t *p = data<uint8_t>(hold->t);
+    *out = eb::DraftTail{p, p + codes, p + 2 * codes, p + 2 * codes + exps, p + 2 * codes + 2 * exps,
+                         eb::tree_tail_row(pos, window, c.block)};
     return EB_OK;
 }
 
@@ -378,8 +407,12 @@ eb_status eb_kv_compact(eb_recorder *rec, eb_kv_cache *kv, const eb_tensor *path
         const size_t nl = std::min(layers - l0, eb::kMoveLayers);
         if (kv->block) {
             eb::CacheI8 c[eb::kMoveLayers];
-            for (size_t l = 0; l < nl; ++l) EB_TRY(layer_i8(kv, l0 + l, dev, &c[l]));
-            EB_TRY(eb::launch_kv_compact_i8(st, c, nl, data<uint32_t>(path), data<uint32_t>(count), n, pos));
+            eb::DraftRows drafts[eb::kMoveLayers];
+            for (size_t l = 0; l < nl; ++l) {
+                EB_TRY(layer_i8(kv, l0 + l, dev, &c[l]));
+                EB_TRY(draft_rows(kv, l0 + l, dev, &drafts[l]));
+            }
+            EB_TRY(eb::launch_kv_compact_i8(st, c, drafts, nl, data<uint32_t>(path), data<uint32_t>(count), n, pos));
         } else {
             eb::CacheRows c[eb::kMoveLayers];
             for (size_t l = 0; l < nl; ++l)
@@ -407,6 +440,8 @@ eb_status eb_kv_fork(eb_recorder *rec, eb_kv_cache *dst, const eb_kv_cache *src,
     if (count == 0) return eb::ok();
     // A launch's runs are of like length: a group of layers' rows, then their exponents.
     const hipStream_t st = stream_of(dev);
+    if (std::any_of(dst->draft_v.begin(), dst->draft_v.end(), [](const eb_tensor *t) { return t != nullptr; }))
+        EB_TRY(eb::drop_drafts(dst, st));
     eb::ByteRun runs[2 * eb::kMoveLayers];
     for (size_t l0 = 0; l0 < layers; l0 += eb::kMoveLayers) {
         const size_t nl = std::min(layers - l0, eb::kMoveLayers);
@@ -464,26 +499,31 @@ eb_status eb_attention_forward_tree_qkv(const eb_attention *attn, eb_recorder *r
     EB_TRY(holds(eb_tensor_numel(masks), rows * eb::tree_words(rows), "masks"));
     EB_TRY(holds(eb_tensor_numel(depths), rows, "depths"));
 
-    const size_t qshape[3] = {rows, H, hd}, kshape[3] = {rows, Hkv, hd}, oshape[2] = {rows, H * hd};
+    const size_t qshape[3] = {rows, H, hd}, oshape[2] = {rows, H * hd};
     eb_tensor *t = nullptr;
     EB_TRY(eb_tensor_empty(dev, qshape, 3, EB_F32, &t));
     Owned qr(t);
     EB_TRY(eb_tensor_empty(dev, oshape, 2, EB_F32, &t));
     Owned o(t);
     if (kv->block) {
-        // The row pass into f32 rows, their codes, then the attention.
-        EB_TRY(eb_tensor_empty(dev, kshape, 3, EB_F32, &t));
-        Owned kr(t);
-        EB_TRY(eb_tensor_empty(dev, kshape, 3, EB_F32, &t));
-        Owned vr(t);
+        // The row pass into f32 rows beside the cache, then the attention over the cache's rows and, from a
+        // copy of its end on, those rows' codes: written into the cache they would round the rows of pos's
+        // block for good, whatever becomes of the draft.
         eb::CacheI8 c;
         EB_TRY(layer_i8(kv, layer, dev, &c));
         EB_TRY(rows_checked(d, rope, base_pos + rows, dev));
+        TreeOperands operands;
+        EB_TRY(operands_of(qr.t, masks, depths, o.t, dev, &operands));
+        eb::DraftRows beside;
+        EB_TRY(draft_rows(kv, layer, dev, &beside));
+        Owned hold;
+        eb::DraftTail tail;
+        EB_TRY(tail_room(dev, c, base_pos, rows, d.window, &hold, &tail));
         eb::RowsArgs a{};
         a.nseg = 3;
         a.seg[0] = eb::RowSeg{data<float>(q), data<float>(qr.t), gain(d.q_norm), (int)H, 0, true, 4};
-        a.seg[1] = eb::RowSeg{data<float>(k), data<float>(kr.t), gain(d.k_norm), (int)Hkv, 0, true, 4};
-        a.seg[2] = eb::RowSeg{data<float>(v), data<float>(vr.t), gain(d.v_norm), (int)Hkv, 0, false, 4};
+        a.seg[1] = eb::RowSeg{data<float>(k), beside.k, gain(d.k_norm), (int)Hkv, 0, true, 4};
+        a.seg[2] = eb::RowSeg{data<float>(v), beside.v, gain(d.v_norm), (int)Hkv, 0, false, 4};
         a.rows = (int)rows;
         a.hd = (int)hd;
         a.eps = d.norm_eps;
@@ -492,8 +532,9 @@ eb_status eb_attention_forward_tree_qkv(const eb_attention *attn, eb_recorder *r
         a.rope_row0 = (int)base_pos;
         a.depths = data<uint32_t>(depths);
         EB_TRY(eb::launch_attn_rows(stream_of(dev), a));
-        EB_TRY(eb::launch_kv_write_i8(stream_of(dev), c, data<float>(kr.t), data<float>(vr.t), base_pos, rows));
-        EB_TRY(eb_attn_tree_i8(rec, qr.t, kv, layer, masks, depths, o.t, H, base_pos, rows, d.scale, d.window));
+        EB_TRY(eb::launch_kv_draft_i8(stream_of(dev), c, beside, tail, base_pos, rows));
+        EB_TRY(tree_i8_checked(stream_of(dev), Room{dev}, eb_device_cu_count(dev), operands, c, H, base_pos, rows,
+                               d.scale, d.window, &tail));
     } else {
         eb_tensor *kc = kv->k[layer], *vc = kv->v[layer];
         EB_TRY(eb::attn_rows_fused(rec, q, k, v, qr.t, kc, vc, rows, H, Hkv, hd, base_pos, kv->max_seq, d.q_norm,

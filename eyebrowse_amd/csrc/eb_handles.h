@@ -19,6 +19,12 @@ struct eb_kv_cache {
     size_t block = 0;
     size_t max_seq = 0;
     size_t n_kv_heads = 0;
+    // A block-scaled cache's drafted rows, which stay beside it until a compaction writes the accepted ones:
+    // f32 [up to 256, heads, head_dim] per layer (null before its first pass or compaction), and tags that
+    // tell whether they are a draft, and which (eb::CacheI8).
+    std::vector<eb_tensor *> draft_k, draft_v;
+    eb_tensor *draft_tags = nullptr;  // U32 [layers, K and V, heads, 4]
+    uint64_t id = 0;
 };
 
 struct eb_attention {
@@ -43,6 +49,10 @@ struct Owned {
         return x;
     }
 };
+
+// Block-scaled caches: a layer's tags (CacheI8), and no draft in any layer (any more).
+uint32_t *draft_tags(const eb_kv_cache *kv, size_t layer);
+eb_status drop_drafts(eb_kv_cache *kv, hipStream_t st);
 
 // Attention::forward between the projections over a block-scaled cache (eb_quant.cpp); the
 // arguments are checked as far as eb_attention_forward_qkv checks them for every cache.

@@ -51,7 +51,14 @@ constexpr size_t kMaxIndex = (size_t)1 << 31;
 struct CacheI8 {
     uint8_t *k, *ks, *v, *vs;  // codes [max_seq, hkv, hd], exponents [ceil(max_seq / block), hkv]
     size_t max_seq, hkv, hd, block;
+    // [K and V, hkv, 4], or null (a caller's memory): what draft lies beside the layer, as the two halves of
+    // the cache's own number, the position and how many rows. Memory that holds no such tag, whatever else it
+    // holds, lacks that number; whatever else writes rows takes it away.
+    uint32_t *tags = nullptr;
+    uint64_t id = 0;
 };
+// Tags of one head and side.
+constexpr size_t kTagWords = 4;
 
 // The caller's description of one, its shape and its buffers' sizes checked.
 eb_status cache_i8_of(const eb_cache_i8 *c, CacheI8 *out);

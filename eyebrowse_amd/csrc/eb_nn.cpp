@@ -128,6 +128,9 @@ void eb_kv_cache_release(eb_kv_cache *kv) {
     for (eb_tensor *t : kv->v) eb_tensor_release(t);
     for (eb_tensor *t : kv->k_scale) eb_tensor_release(t);
     for (eb_tensor *t : kv->v_scale) eb_tensor_release(t);
+    for (eb_tensor *t : kv->draft_k) eb_tensor_release(t);
+    for (eb_tensor *t : kv->draft_v) eb_tensor_release(t);
+    eb_tensor_release(kv->draft_tags);
     delete kv;
 }
 

@@ -3,6 +3,8 @@
 // translation unit (eb_linear_q4.hip, eb_cache_i8.hip, eb_decode_i8.hip, eb_prefill.hip,
 // eb_sample.hip).
 #include <algorithm>
+#include <atomic>
+#include <chrono>
 #include <climits>
 #include <cstdint>
 #include <memory>
@@ -48,6 +50,17 @@ eb_status not_captured(hipStream_t st, const char *what) {
 
 // ---- block-scaled caches --------------------------------------------------------------------
 
+// A cache's number (eb::CacheI8): of 64 bits that no other one has and no memory holds by chance, the lower half
+// not 0.
+uint64_t cache_number(const void *at) {
+    static std::atomic<uint64_t> count{0};
+    uint64_t x = ++count * 0x9E3779B97F4A7C15u + (uint64_t)std::chrono::steady_clock::now().time_since_epoch().count() +
+                 (uint64_t)reinterpret_cast<uintptr_t>(at);
+    x = (x ^ (x >> 30)) * 0xBF58476D1CE4E5B9u;
+    x = (x ^ (x >> 27)) * 0x94D049BB133111EBu;
+    return (x ^ (x >> 31)) | 1;
+}
+
 // Rows and elements of a row that the kernels index with 32 bits (a whole cache may pass 2^31).
 constexpr size_t kMaxRows = (size_t)1 << 27, kMaxRow = (size_t)1 << 20;
 
@@ -79,7 +92,7 @@ eb_status layer_of(const eb_kv_cache *kv, size_t layer, eb_device *dev, eb::Cach
     EB_TRY(eb::check_tensor(kv->k[layer], EB_I8, "kv cache", dev));
     *out = eb::CacheI8{data<uint8_t>(kv->k[layer]), data<uint8_t>(kv->k_scale[layer]), data<uint8_t>(kv->v[layer]),
                        data<uint8_t>(kv->v_scale[layer]), kv->max_seq, kv->n_kv_heads,
-                       eb_tensor_dim(kv->k[layer], 2), kv->block};
+                       eb_tensor_dim(kv->k[layer], 2), kv->block, eb::draft_tags(kv, layer), kv->id};
     return EB_OK;
 }
 
@@ -221,6 +234,15 @@ eb_status eb::cache_i8_of(const eb_cache_i8 *c, CacheI8 *out) {
     return EB_OK;
 }
 
+uint32_t *eb::draft_tags(const eb_kv_cache *kv, size_t layer) {
+    return data<uint32_t>(kv->draft_tags) + layer * 2 * kTagWords * kv->n_kv_heads;
+}
+
+eb_status eb::drop_drafts(eb_kv_cache *kv, hipStream_t st) {
+    const size_t bytes = eb_tensor_numel(kv->draft_tags) * sizeof(uint32_t);
+    return bytes == 0 ? EB_OK : launch_fill_u8(st, data<uint8_t>(kv->draft_tags), 0, bytes);
+}
+
 eb_status eb::attention_forward_i8(const eb_attention_desc &d, eb_recorder *rec, const eb_tensor *q,
                                    const eb_tensor *k, const eb_tensor *v, const eb_rope_tables *rope,
                                    eb_kv_cache *kv, size_t layer, size_t rows, size_t base_pos, eb_tensor **out) {
@@ -310,6 +332,11 @@ eb_status eb_kv_cache_new_i8(eb_device *dev, const size_t *head_dims, size_t n_l
                 EB_TRY(eb::launch_fill_u8(stream_of(dev), data<uint8_t>(t), 1, blocks * n_kv_heads));
         }
     }
+    kv->draft_k.resize(n_layers);
+    kv->draft_v.resize(n_layers);
+    const size_t tshape[4] = {n_layers, 2, n_kv_heads, eb::kTagWords};
+    EB_TRY(eb_tensor_empty(dev, tshape, 4, EB_U32, &kv->draft_tags));
+    kv->id = cache_number(kv.get());
     // Complete, as a tensor's write is: the next one to touch the exponents may be another stream,
     // which nothing orders behind this one.
     EB_HIP_TRY(hipStreamSynchronize(stream_of(dev)));

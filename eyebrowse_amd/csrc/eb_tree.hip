@@ -16,6 +16,7 @@
 
 namespace {
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kNodes = (int)eb::kTreeMax;
@@ -176,23 +177,137 @@ __global__ __launch_bounds__(kThreads) void kv_compact_kernel(CompactArgs a) {
     }
 }
 
+struct DraftSide {
+    const float *rows;     // [n, hkv, hd]
+    const uint8_t *codes, *exps;
+    uint8_t *tail_codes, *tail_exps, *bad;
+    unsigned *tags;
+};
+struct DraftArgs {
+    DraftSide k, v;
+    int row0, pos, n, hkv, hd, block_log2;
+    u32x4 tag;  // as written: the cache's number, pos, n
+};
+
+// Workgroup (b, head, side): one block of the tail, of one KV head: the cache's rows before pos, in the
+// exponent that a write of the block's drafted rows gives it, and those rows' codes. A row that is not finite
+// is zeros and a mark instead. The cache itself is not touched. Bound by latency: everything that a thread
+// keeps in registers (a block of 64 rows of 128) is on its way before the first wait.
+__global__ __launch_bounds__(kThreads) void kv_draft_i8_kernel(DraftArgs a) {
+    __shared__ unsigned s_max[2][kThreads / 64];
+    __shared__ unsigned s_bad[kNodes];
+    constexpr int kOld = 4, kNew = 8;
+    const DraftSide &s = blockIdx.z ? a.v : a.k;
+    const int head = blockIdx.y, tid = threadIdx.x;
+    const int b0 = a.row0 >> a.block_log2, b = b0 + (int)blockIdx.x;
+    const int first = b << a.block_log2, behind = first + (1 << a.block_log2);
+    const int lo = max(first, a.pos), hi = min(behind, a.pos + a.n);
+    const int from = max(first, a.row0), to = min(behind, a.pos);
+    const int per_row = a.hd / 4, per_old = a.hd / 16;
+    const int rows = max(hi - lo, 0), vecs = rows * per_row;  // drafted ones
+    const int kept = max(to - from, 0) * per_old;             // the cache's
+    const size_t stride = (size_t)a.hkv * a.hd, head0 = (size_t)head * a.hd;
+    const float *src = s.rows + (lo - a.pos) * stride + head0;
+    const uint8_t *old_src = s.codes + from * stride + head0;
+    uint8_t *new_dst = s.tail_codes + (lo - a.row0) * stride + head0, *old_dst = s.tail_codes + (from - a.row0) * stride + head0;
+    const bool lead = first < a.pos;
+    auto load = [&](int i) {
+        return *reinterpret_cast<const f32x4 *>(src + (size_t)(i / per_row) * stride + 4 * (i % per_row));
+    };
+    auto old_at = [&](int i) { return (size_t)(i / per_old) * stride + 16 * (i % per_old); };
+    auto magnitude = [](f32x4 x) {
+        unsigned top = 0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) top = max(top, eb::magnitude_bits(x[c]));
+        return top;
+    };
+    auto join = [&](unsigned top, unsigned (&to_all)[kThreads / 64]) {  // the workgroup's largest
+#pragma unroll
+        for (int m = 32; m > 0; m >>= 1) top = max(top, __shfl_xor(top, m));
+        if ((tid & 63) == 0) to_all[tid >> 6] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kThreads / 64; ++w) top = max(top, to_all[w]);
+        return top;
+    };
+    const unsigned old_e = lead ? s.exps[(size_t)b * a.hkv + head] : 0u;
+    f32x4 fresh[kNew];
+    u32x4 old[kOld];
+#pragma unroll
+    for (int j = 0; j < kNew; ++j)
+        fresh[j] = tid + j * kThreads < vecs ? load(tid + j * kThreads) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < kOld; ++j)
+        if (tid + j * kThreads < kept) old[j] = *reinterpret_cast<const u32x4 *>(old_src + old_at(tid + j * kThreads));
+    unsigned top = 0;
+#pragma unroll
+    for (int j = 0; j < kNew; ++j) top = max(top, magnitude(fresh[j]));
+    for (int i = tid + kNew * kThreads; i < vecs; i += kThreads) top = max(top, magnitude(load(i)));
+    if (tid < rows) s_bad[tid] = 0;
+    top = join(top, s_max[0]);
+    const bool some_bad = top >= 0x7F800000u;  // (uniform)
+    if (some_bad) {  // the rows that are not finite, and the others' largest
+        for (int i = tid; i < vecs; i += kThreads)
+            if (magnitude(load(i)) >= 0x7F800000u) s_bad[i / per_row] = 1;
+        __syncthreads();
+        top = 0;
+        for (int i = tid; i < vecs; i += kThreads)
+            if (!s_bad[i / per_row]) top = max(top, magnitude(load(i)));
+        top = join(top, s_max[1]);
+    }
+    unsigned e = eb::i8_exponent(top);
+    if (lead) e = rows > 0 ? eb::i8_join(old_e, e) : old_e;
+    auto store = [&](int i, f32x4 x) {
+        unsigned w = 0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) w |= eb::i8_code(x[c], e) << (8 * c);
+        if (some_bad && s_bad[i / per_row]) w = 0;
+        *reinterpret_cast<unsigned *>(new_dst + (size_t)(i / per_row) * stride + 4 * (i % per_row)) = w;
+    };
+    auto store_old = [&](int i, u32x4 w) {
+        if (e != old_e && e != eb::kNanExponent)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) w[c] = eb::i8_recode(w[c], old_e, e);
+        *reinterpret_cast<u32x4 *>(old_dst + old_at(i)) = w;
+    };
+#pragma unroll
+    for (int j = 0; j < kNew; ++j)
+        if (tid + j * kThreads < vecs) store(tid + j * kThreads, fresh[j]);
+    for (int i = tid + kNew * kThreads; i < vecs; i += kThreads) store(i, load(i));
+#pragma unroll
+    for (int j = 0; j < kOld; ++j)
+        if (tid + j * kThreads < kept) store_old(tid + j * kThreads, old[j]);
+    for (int i = tid + kOld * kThreads; i < kept; i += kThreads)
+        store_old(i, *reinterpret_cast<const u32x4 *>(old_src + old_at(i)));
+    if (tid < rows) s.bad[(size_t)head * a.n + (lo - a.pos) + tid] = (uint8_t)s_bad[tid];
+    if (tid == 0) {
+        s.tail_exps[blockIdx.x * a.hkv + head] = (uint8_t)e;
+        if (blockIdx.x == 0) reinterpret_cast<u32x4 *>(s.tags)[head] = a.tag;
+    }
+}
+
 struct CompactI8Args {
     struct Layer {
         uint8_t *codes[2], *exps[2];
+        const float *draft[2];
         int hd;
     } layer[kMaxLayers];
     const unsigned *path, *count;
+    unsigned *tags;  // of the first layer, and on
+    unsigned id_lo, id_hi;
     size_t pos;
     int n, hkv, block;
 };
 
 // Workgroup (head, layer and side): the branch's rows as the values they stand for, written at pos as
 // any rows are: block by block, with the least exponent that holds them and the block's earlier rows.
-// All codes and exponents are in LDS before the first is overwritten; no other workgroup touches them.
+// They are the draft's that lies beside the cache, where that is one of pos, which is then done with; else
+// the cache's own rows from pos on.
+// All of these' codes and exponents are in LDS before the first is overwritten; no other workgroup touches them.
 // Bound by latency (path, rows, then a block after another, with three barriers each): 8 heads of 128, 5 of
 // 21 rows in 28 layers 5.1 us, 8 of 64 in 32 layers 6.3, 64 of 256 12.2.
 __global__ __launch_bounds__(kThreads) void kv_compact_i8_kernel(CompactI8Args a) {
-    extern __shared__ unsigned s_code[];  // [n][hd / 4]
+    extern __shared__ unsigned s_code[];  // [n][hd / 4] (rows of the cache)
     __shared__ unsigned s_path[kNodes], s_exp[kNodes];
     __shared__ unsigned s_end, s_top;
     const CompactI8Args::Layer &layer = a.layer[blockIdx.y >> 1];
@@ -201,11 +316,29 @@ __global__ __launch_bounds__(kThreads) void kv_compact_i8_kernel(CompactI8Args a
     const size_t stride = (size_t)a.hkv * layer.hd;
     uint8_t *codes = layer.codes[side] + (size_t)head * layer.hd;
     uint8_t *exps = layer.exps[side] + head;
-    const int end = load_path(a.path, a.count, a.n, s_path, &s_end);
+    u32x4 *tags = reinterpret_cast<u32x4 *>(a.tags) + (size_t)blockIdx.y * a.hkv + head;
+    const u32x4 tag = *tags;
+    const float *draft = nullptr;
+    if (tag[0] == a.id_lo && tag[1] == a.id_hi && tag[2] == (unsigned)a.pos) draft = layer.draft[side];
+    const int end = load_path(a.path, a.count, draft ? min(a.n, (int)tag[3]) : a.n, s_path, &s_end);
+    if (draft) {
+        draft += (size_t)head * layer.hd;
+        if (tid == 0) *tags = u32x4{0u, 0u, 0u, 0u};  // (every thread has read it: load_path's barriers)
+    }
     auto word = [&](size_t row, int w) { return reinterpret_cast<unsigned *>(codes + row * stride + 4 * w); };
-    for (int i = tid; i < end * per_row; i += kThreads) s_code[i] = *word(a.pos + s_path[i / per_row], i % per_row);
-    if (tid < end) s_exp[tid] = exps[(a.pos + s_path[tid]) / a.block * a.hkv];
-    __syncthreads();
+    if (!draft) {
+        for (int i = tid; i < end * per_row; i += kThreads) s_code[i] = *word(a.pos + s_path[i / per_row], i % per_row);
+        if (tid < end) s_exp[tid] = exps[(a.pos + s_path[tid]) / a.block * a.hkv];
+        __syncthreads();
+    }
+    auto values = [&](int i) {  // four of the branch's row i / per_row
+        if (draft) return *reinterpret_cast<const f32x4 *>(draft + s_path[i / per_row] * stride + 4 * (i % per_row));
+        const float f = eb::i8_scale(s_exp[i / per_row], 0);
+        f32x4 x;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) x[c] = eb::i8_f32(s_code[i], c) * f;
+        return x;
+    };
     for (int lo = 0; lo < end;) {
         const size_t b = (a.pos + lo) / a.block, first = b * a.block;
         const int hi = (int)(first + a.block - a.pos) < end ? (int)(first + a.block - a.pos) : end;
@@ -213,10 +346,12 @@ __global__ __launch_bounds__(kThreads) void kv_compact_i8_kernel(CompactI8Args a
         if (tid == 0) s_top = 0;
         __syncthreads();
         unsigned top = 0;
-        for (int i = lo * per_row + tid; i < hi * per_row; i += kThreads) {
-            const float f = eb::i8_scale(s_exp[i / per_row], 0);
+        f32x4 kept = {0.0f, 0.0f, 0.0f, 0.0f};  // a thread's first
+        for (int i = lo * per_row + tid, i0 = i; i < hi * per_row; i += kThreads) {
+            const f32x4 x = values(i);
+            if (i == i0) kept = x;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) top = max(top, eb::magnitude_bits(eb::i8_f32(s_code[i], c) * f));
+            for (int c = 0; c < 4; ++c) top = max(top, eb::magnitude_bits(x[c]));
         }
 #pragma unroll
         for (int m = 32; m > 0; m >>= 1) top = max(top, __shfl_xor(top, m));
@@ -225,11 +360,11 @@ __global__ __launch_bounds__(kThreads) void kv_compact_i8_kernel(CompactI8Args a
         __syncthreads();
         unsigned e = eb::i8_exponent(s_top);
         if (lead) e = eb::i8_join(old_e, e);
-        for (int i = lo * per_row + tid; i < hi * per_row; i += kThreads) {
-            const float f = eb::i8_scale(s_exp[i / per_row], 0);
+        for (int i = lo * per_row + tid, i0 = i; i < hi * per_row; i += kThreads) {
+            const f32x4 x = i == i0 ? kept : values(i);
             unsigned w = 0;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) w |= eb::i8_code(eb::i8_f32(s_code[i], c) * f, e) << (8 * c);
+            for (int c = 0; c < 4; ++c) w |= eb::i8_code(x[c], e) << (8 * c);
             *word(a.pos + i / per_row, i % per_row) = w;
         }
         if (lead && e != old_e && e != eb::kNanExponent) {
@@ -309,9 +444,29 @@ eb_status launch_kv_compact(hipStream_t st, const CacheRows *layers, size_t n_la
     return check_launch("kv_compact");
 }
 
-eb_status launch_kv_compact_i8(hipStream_t st, const CacheI8 *layers, size_t n_layers, const uint32_t *path,
-                               const uint32_t *count, size_t n, size_t pos) {
+eb_status launch_kv_draft_i8(hipStream_t st, const CacheI8 &c, const DraftRows &d, const DraftTail &t, size_t pos,
+                             size_t n) {
+    DraftArgs a{};
+    a.k = DraftSide{d.k, c.k, c.ks, t.k, t.ks, t.bad, c.tags};
+    a.v = DraftSide{d.v, c.v, c.vs, t.v, t.vs, t.bad + c.hkv * n, c.tags + kTagWords * c.hkv};
+    a.row0 = (int)t.row0;
+    a.pos = (int)pos;
+    a.n = (int)n;
+    a.hkv = (int)c.hkv;
+    a.hd = (int)c.hd;
+    a.tag = u32x4{(unsigned)c.id, (unsigned)(c.id >> 32), (unsigned)pos, (unsigned)n};
+    while ((size_t)1 << a.block_log2 < c.block) ++a.block_log2;
+    const size_t blocks = (pos + n - 1) / c.block - t.row0 / c.block + 1;
+    if (blocks > tree_tail_blocks(n, c.block) || pos + n - t.row0 > tree_tail_rows(n, c.block))
+        return fail(EB_OTHER, "kv_draft_i8: rows %zu to %zu do not fit the tail", t.row0, pos + n);
+    kv_draft_i8_kernel<<<dim3((unsigned)blocks, (unsigned)c.hkv, 2), kThreads, 0, st>>>(a);
+    return check_launch("kv_draft_i8");
+}
+
+eb_status launch_kv_compact_i8(hipStream_t st, const CacheI8 *layers, const DraftRows *drafts, size_t n_layers,
+                               const uint32_t *path, const uint32_t *count, size_t n, size_t pos) {
     CompactI8Args a{};
+    static_assert(sizeof(a) <= 4096, "kernel arguments");
     a.path = path;
     a.count = count;
     a.pos = pos;
@@ -319,9 +474,12 @@ eb_status launch_kv_compact_i8(hipStream_t st, const CacheI8 *layers, size_t n_l
     size_t hd = 0;
     for (size_t l = 0; l < n_layers; ++l) {
         const CacheI8 &c = layers[l];
-        a.layer[l] = {{c.k, c.v}, {c.ks, c.vs}, (int)c.hd};
+        a.layer[l] = {{c.k, c.v}, {c.ks, c.vs}, {drafts[l].k, drafts[l].v}, (int)c.hd};
         hd = std::max(hd, c.hd);
     }
+    a.tags = layers[0].tags;
+    a.id_lo = (unsigned)layers[0].id;
+    a.id_hi = (unsigned)(layers[0].id >> 32);
     a.hkv = (int)layers[0].hkv;
     a.block = (int)layers[0].block;
     constexpr int kMost = kNodes * 256;  // (the widest tree and head: 64 KB, beside 2 KB of paths)

@@ -145,12 +145,15 @@ struct Args {
     const float *q;
     const char *k, *v;
     const uint8_t *ks, *vs;
+    const char *tk, *tv;  // (block-scaled) rows from tail0 on
+    const uint8_t *tks, *tvs, *bad;
     const unsigned *masks, *depths;
     float *o, *part_acc, *part_ml;
     int h, hkv, g, n, words, ncols, hd;
     unsigned g_inv;  // 2^32 / g, rounded up: exact for the at most 2^16 columns of a KV head
     int pos, window;
     int key0, tiles;  // the first key of tile 0; a tile at least
+    int tail0;        // the first key of some tile
     int nsplit, ncb, pairs, block_log2;
     float scale_log2;
 };
@@ -262,7 +265,8 @@ __device__ __forceinline__ int piece_xor(int r) {
     return RB >= 256 ? r & 15 : RB == 128 ? (r >> 1) & 7 : (r >> 2) & 3;
 }
 
-template <int HDP, TreeElem E, int CW, int NSET, bool COPY>
+// TAIL (block-scaled caches): keys from tail0 on are rows of the call's own, in place of the cache's.
+template <int HDP, TreeElem E, int CW, int NSET, bool COPY, bool TAIL>
 __global__ __launch_bounds__((Shape<HDP, E, CW, NSET, COPY>::THREADS),
                              (Shape<HDP, E, CW, NSET, COPY>::WGS * Shape<HDP, E, CW, NSET, COPY>::WAVES / 4))
 void tree_attn_kernel(Args a) {
@@ -292,12 +296,17 @@ void tree_attn_kernel(Args a) {
     int *s_any = reinterpret_cast<int *>(s_bad + T);  // (copied rows) a tile that has a row with NaN
     unsigned *s_mask = reinterpret_cast<unsigned *>(s_bad + (COPY ? T + 1 : 0));  // [nodes][words]
     int *s_depth = reinterpret_cast<int *>(s_mask + nodes * a.words);           // [n] (with a window)
+    unsigned *s_nan = reinterpret_cast<unsigned *>(s_depth + (a.window > 0 ? a.n : 0));  // [8] (with a tail)
 
     // ---- tiles: fetched into registers, then stored as operands -----------------------------------
     const bool vside = wave >= kWaves / 2;
     const int ht = tid % HT;
     const size_t row_bytes = (size_t)a.hkv * hd * ES;
     const char *base = (vside ? a.v : a.k) + (size_t)kvh * hd * ES;
+    const uint8_t *exps = vside ? a.vs : a.ks;
+    // (so that the tail's rows and exponents are found by the same key)
+    const char *tail_base = TAIL ? (vside ? a.tv : a.tk) + (size_t)kvh * hd - (size_t)a.tail0 * row_bytes : base;
+    const uint8_t *tail_exps = TAIL ? (vside ? a.tvs : a.tks) - (size_t)(a.tail0 >> a.block_log2) * a.hkv : exps;
     const unsigned lds0 = (unsigned)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)smem);
     unsigned piece[COPY ? S::CPW : 1];  // where this lane's pieces lie in a tile's rows
     if constexpr (COPY) {
@@ -314,7 +323,9 @@ void tree_attn_kernel(Args a) {
         const int r0 = a.key0 + t * T;
         const int left = min(end - r0, T);
         const int nbytes = left > 0 ? (int)((left - 1) * row_bytes) + hd * ES : 0;
-        const __amdgpu_buffer_rsrc_t res = eb::make_rsrc(base + (left > 0 ? (size_t)r0 * row_bytes : 0), nbytes);
+        const bool tail = TAIL && r0 >= a.tail0;
+        const __amdgpu_buffer_rsrc_t res =
+            eb::make_rsrc((tail ? tail_base : base) + (left > 0 ? (size_t)r0 * row_bytes : 0), nbytes);
         const unsigned dst = lds0 + b * S::TILE + (vside ? T * S::RB : 0) + (wave % (kWaves / 2)) * S::CPW * 1024;
 #pragma unroll
         for (int i = 0; i < S::CPW; ++i)  // (a copy may read m0 one wait state after its write at the soonest)
@@ -325,7 +336,7 @@ void tree_attn_kernel(Args a) {
             const size_t b0 = left > 0 ? (size_t)(r0 >> a.block_log2) : 0;
             const int last = left > 0 ? (r0 + left - 1) >> a.block_log2 : 0;
             const __amdgpu_buffer_rsrc_t eres = eb::make_rsrc(
-                (vside ? a.vs : a.ks) + b0 * a.hkv, left > 0 ? (last - (int)b0) * a.hkv + kvh + 1 : 0);
+                (tail ? tail_exps : exps) + b0 * a.hkv, left > 0 ? (last - (int)b0) * a.hkv + kvh + 1 : 0);
             const unsigned off = 16 * lane < left ? (((r0 + 16 * lane) >> a.block_log2) - (int)b0) * a.hkv + kvh : kNone;
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_ubyte %1, %2, 0 offen lds" ::"s"(
                              lds0 + b * S::TILE + 2 * T * S::RB + (vside ? 256 : 0)),
@@ -516,6 +527,9 @@ void tree_attn_kernel(Args a) {
     // ---- the columns' queries, masks and first keys -------------------------------------------------
     const unsigned first_mask = tid < nodes * a.words ? a.masks[(size_t)node0 * a.words + tid] : 0u;
     const unsigned first_depth = a.window > 0 && tid < a.n ? a.depths[tid] : 0u;
+    bool not_finite = false;  // (a node per thread) its row of K or V
+    if constexpr (TAIL)
+        if (tid < a.n) not_finite = (a.bad[(size_t)kvh * a.n + tid] | a.bad[(size_t)(a.hkv + kvh) * a.n + tid]) != 0;
     auto put_mask = [&](int i, unsigned w) {
         if (i % a.words == a.words - 1 && a.n % 32) w &= (1u << (a.n % 32)) - 1u;  // (no nodes past n)
         s_mask[i] = w;
@@ -581,7 +595,13 @@ void tree_attn_kernel(Args a) {
     if (COPY && tid == 0) *s_any = -1;
     if (a.window > 0)
         if (tid < a.n) s_depth[tid] = (int)min(first_depth, 1u << 27);  // (a node per thread at most)
+    if constexpr (TAIL) {
+        const unsigned long long some = __builtin_amdgcn_ballot_w64(not_finite);
+        if (lane < 2 && wave < 4) s_nan[2 * wave + lane] = (unsigned)(some >> (32 * lane));
+    }
     __syncthreads();
+    bool some_nan = false;  // (with a tail; uniform)
+    if constexpr (TAIL) some_nan = __builtin_amdgcn_ballot_w64(s_nan[lane & 7] != 0u) != 0;
     int safe_lo = 0;  // keys below it may be behind some column's window
     bool shallow = true;  // no drafted key is behind any node's window
     if (a.window > 0) {
@@ -1062,6 +1082,16 @@ void tree_attn_kernel(Args a) {
                 }
             }
         }
+        if (TAIL && some_nan) {  // drafted rows that are not finite: whom they reach
+            bool hit = false;
+            for (int w = 0; w < a.words; ++w)
+                for (unsigned m = s_mask[my_node[s] * a.words + w] & s_nan[w]; m != 0; m &= m - 1)
+                    hit = hit | (a.window == 0 || a.pos + s_depth[32 * w + __builtin_ctz(m)] >= my_first[s]);
+            const float nan = __builtin_nanf("");
+            if (hit)
+#pragma unroll
+                for (int e = 0; e < S::ND; ++e) acc[s][e] = f32x4{nan, nan, nan, nan};
+        }
         if (c >= a.ncols) continue;
         const int node = node0 + my_node[s];
         const size_t row = (size_t)node * a.h + kvh * a.g + c - node * a.g;
@@ -1225,11 +1255,10 @@ int widths_of(size_t cols, size_t hkv, size_t hd, TreeElem e, int cu_count, Widt
 
 Plan plan_of(size_t h, size_t hkv, size_t hd, size_t pos, size_t n, size_t window, TreeElem elem, int cu_count) {
     const size_t cols = n * (h / hkv);
-    const size_t first = window > 0 && pos + 1 > window ? pos + 1 - window : 0;
     Plan best{};
     best.hdp = hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
     best.copy = copies(elem, hd);
-    best.key0 = (int)(first & ~(size_t)15);
+    best.key0 = (int)eb::tree_first_key(pos, window);
     const size_t keys = pos + n - best.key0;
     float least = 0.0f;
     Width widths[3];
@@ -1262,15 +1291,16 @@ Plan plan_of(size_t h, size_t hkv, size_t hd, size_t pos, size_t n, size_t windo
     return best;
 }
 
-template <int HDP, TreeElem E, int CW, int NSET, bool COPY>
+template <int HDP, TreeElem E, int CW, int NSET, bool COPY, bool TAIL>
 hipError_t launch(hipStream_t st, const Args &a) {
     using S = Shape<HDP, E, CW, NSET, COPY>;
     constexpr size_t kTiles = (size_t)S::NBUF * S::TILE + S::QBYTES + S::STEEP + (COPY ? S::T * 4 + 4 : 0);
     const size_t nodes = std::min<size_t>(a.n, S::COLS);
-    const size_t lds = kTiles + (nodes * a.words + (a.window > 0 ? a.n : 0)) * 4;
-    constexpr size_t kMost = kTiles + (S::COLS * 8 + 256) * 4;
+    const size_t lds = kTiles + (nodes * a.words + (a.window > 0 ? a.n : 0) + (TAIL ? 8 : 0)) * 4;
+    constexpr size_t kMost = kTiles + (S::COLS * 8 + 256 + (TAIL ? 8 : 0)) * 4;
+    static_assert(!TAIL || eb::kTailStep % S::T == 0, "a tail starts with a tile");
     static_assert(kMost <= 160 * 1024 / S::WGS, "LDS of a CU");
-    const auto kernel = &tree_attn_kernel<HDP, E, CW, NSET, COPY>;
+    const auto kernel = &tree_attn_kernel<HDP, E, CW, NSET, COPY, TAIL>;
     if (lds > 64 * 1024) {
         static const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
                                                         hipFuncAttributeMaxDynamicSharedMemorySize, (int)kMost);
@@ -1281,20 +1311,20 @@ hipError_t launch(hipStream_t st, const Args &a) {
     return hipSuccess;
 }
 
-template <int HDP, TreeElem E, bool COPY>
+template <int HDP, TreeElem E, bool COPY, bool TAIL>
 hipError_t launch_cols(hipStream_t st, const Args &a, int cols) {
-    if (cols == 16) return launch<HDP, E, 1, 1, COPY>(st, a);
+    if (cols == 16) return launch<HDP, E, 1, 1, COPY, TAIL>(st, a);
     if constexpr (HDP < 256)
-        if (cols == 128) return launch<HDP, E, 4, 2, COPY>(st, a);
-    return launch<HDP, E, 4, 1, COPY>(st, a);
+        if (cols == 128) return launch<HDP, E, 4, 2, COPY, TAIL>(st, a);
+    return launch<HDP, E, 4, 1, COPY, TAIL>(st, a);
 }
 
-template <TreeElem E, bool COPY>
+template <TreeElem E, bool COPY, bool TAIL = false>
 hipError_t launch_elem(hipStream_t st, const Args &a, const Plan &p) {
-    if (p.hdp == 64) return launch_cols<64, E, COPY>(st, a, p.cols);
+    if (p.hdp == 64) return launch_cols<64, E, COPY, TAIL>(st, a, p.cols);
     if constexpr (COPY || E == TreeElem::F32)  // (E4M3 rows that end inside a piece: at most 120 dims)
-        if (p.hdp == 256) return launch_cols<256, E, COPY>(st, a, p.cols);
-    return launch_cols<128, E, COPY>(st, a, p.cols);
+        if (p.hdp == 256) return launch_cols<256, E, COPY, TAIL>(st, a, p.cols);
+    return launch_cols<128, E, COPY, TAIL>(st, a, p.cols);
 }
 
 }  // namespace
@@ -1324,6 +1354,14 @@ eb_status launch_attn_tree(hipStream_t st, const TreeAttn &x, float *ws, size_t 
     a.v = static_cast<const char *>(x.v);
     a.ks = x.ks;
     a.vs = x.vs;
+    if (x.tail) {
+        a.tk = reinterpret_cast<const char *>(x.tail->k);
+        a.tv = reinterpret_cast<const char *>(x.tail->v);
+        a.tks = x.tail->ks;
+        a.tvs = x.tail->vs;
+        a.bad = x.tail->bad;
+        a.tail0 = (int)x.tail->row0;
+    }
     a.masks = x.masks;
     a.depths = x.depths;
     a.o = x.o;
@@ -1348,7 +1386,8 @@ eb_status launch_attn_tree(hipStream_t st, const TreeAttn &x, float *ws, size_t 
     a.scale_log2 = x.scale * kLog2e;
     const hipError_t e = x.elem == TreeElem::F32   ? launch_elem<TreeElem::F32, false>(st, a, p)
                          : x.elem == TreeElem::F16 ? launch_elem<TreeElem::F16, true>(st, a, p)
-                         : x.elem == TreeElem::I8  ? launch_elem<TreeElem::I8, true>(st, a, p)
+                         : x.elem == TreeElem::I8  ? x.tail ? launch_elem<TreeElem::I8, true, true>(st, a, p)
+                                                            : launch_elem<TreeElem::I8, true>(st, a, p)
                          : p.copy                  ? launch_elem<TreeElem::E4M3, true>(st, a, p)
                                                    : launch_elem<TreeElem::E4M3, false>(st, a, p);
     if (e != hipSuccess) return hip_fail(e, "attn_tree launch set-up");

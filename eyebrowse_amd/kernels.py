@@ -568,7 +568,8 @@ def attn_tree(rec: Recorder, q: Tensor, kcache: Tensor, vcache: Tensor, masks: T
 
 def attn_tree_i8(rec: Recorder, q: Tensor, kv, layer: int, masks: Tensor, depths, o: Tensor, h: int,
                  pos: int, n: int, scale: float, window: int = 0) -> None:
-    """attn_tree over a block-scaled KvCache's layer."""
+    """attn_tree over a block-scaled KvCache's layer, the drafted rows written there by kv_write_i8
+    (Attention.forward_tree keeps them beside the cache instead)."""
     check(lib().eb_attn_tree_i8(rec.handle, q.handle, kv.handle, layer, masks.handle, _opt(depths),
                                 o.handle, h, pos, n, scale, window))
 
@@ -588,7 +589,8 @@ def tree_accept(rec: Recorder, tokens: Tensor, parents: Tensor, sampled: Tensor,
 
 
 def kv_compact(rec: Recorder, kv, path: Tensor, count: Tensor, n: int, pos: int) -> None:
-    """Rows pos + path[j] of every layer of a KvCache to rows pos + j, j < count, in place."""
+    """Rows pos + path[j] of every layer of a KvCache to rows pos + j, j < count, in place (a block-scaled
+    layer's with a draft at pos: the draft's rows path[j], written there)."""
     check(lib().eb_kv_compact(rec.handle, kv.handle, path.handle, count.handle, n, pos))
 
 

@@ -273,8 +273,9 @@ class Attention:
                          kv: KvCache, layer: int, masks: Tensor, depths: Tensor, rows: int,
                          base_pos: int) -> Tensor:
         """forward_qkv for the nodes of a drafted tree (no counterpart in the reference): node i at
-        position base_pos + depths[i], in cache row base_pos + i, seeing the cached keys and the
-        nodes of masks' row i (tree_plan gives both)."""
+        position base_pos + depths[i], in cache row base_pos + i (a block-scaled cache: beside it,
+        until kv_compact), seeing the cached keys and the nodes of masks' row i (tree_plan gives
+        both)."""
         out = c_vp()
         check(lib().eb_attention_forward_tree_qkv(self._h, rec.handle, q.handle, k.handle, v.handle,
                                                   rope.handle, kv.handle, layer, masks.handle,

@@ -724,11 +724,20 @@ eb_status eb_launch_sample(void *stream, const float *logits, size_t logits_nume
  * the cache does not hold yet. parents[i] (EB_I32) is an earlier node, or -1; anything else counts
  * as -1. Node i's K and V go to cache row pos + i, its position is pos + depth[i].
  *
+ * Over a block-scaled cache the layer (eb_attention_forward_tree[_qkv]) keeps the nodes' K and V beside
+ * the cache instead, in f32: written into it, a draft would round the certain rows of pos's block to its own
+ * exponent for good, accepted or not. The cache stays as it is until eb_kv_compact writes the accepted
+ * nodes' rows, or for good where none follows. Within the pass the nodes see the block's rows as one write of
+ * all n rows at pos would round them. Any other rows written to the layer, or a fork into the cache, drop
+ * its draft. A layer's first pass or compaction takes room for twice min(256, max_seq) f32 rows, which the
+ * cache keeps.
+ *
  * A step: eb_tree_plan; per layer eb_attention_forward_tree; logits of all nodes; a token for each
  * of them (eb_sample, one row per node; or the largest logit, at temperature 0); eb_tree_accept;
  * eb_kv_compact. The cache then holds rows up to pos + count, and the last emitted token is the next
  * root. The emitted tokens are the ones that decoding one by one would sample from the same numbers u
- * at those nodes: a node is accepted exactly if the token sampled at its parent is its own.
+ * at those nodes, up to the logits' rounding (a block-scaled cache's included): a node is accepted exactly
+ * if the token sampled at its parent is its own.
  * Trees, paths and counts are read from device memory when the work runs (a captured graph replays
  * with another tree of n nodes); n and pos are arguments.
  *
@@ -766,8 +775,9 @@ eb_status eb_launch_attn_prologue_tree(void *stream, const float *q, size_t q_nu
  * be NULL without a window. A node that sees nothing gives zeros. f32 accuracy over every cache
  * (f32, f16, E4M3; eb_attn_tree_i8: block-scaled): products on f16 matrix cores of f32 values in two
  * halves, 22 bits. Values of K or V that are not finite reach the nodes that see their row, whose
- * heads become NaN, and no others. At most 256 query heads per KV head. The same call gives the same
- * bits. */
+ * heads become NaN, and no others (a block-scaled cache's: those that see a row of their block).
+ * eb_attn_tree_i8 finds the drafted rows in the cache, where eb_kv_write_i8 put them. At most 256 query
+ * heads per KV head. The same call gives the same bits. */
 eb_status eb_attn_tree(eb_recorder *rec, const eb_tensor *q, const eb_tensor *kcache,
                        const eb_tensor *vcache, const eb_tensor *masks, const eb_tensor *depths,
                        eb_tensor *o, size_t h, size_t hkv, size_t pos, size_t n, size_t hd,
@@ -795,8 +805,9 @@ eb_status eb_launch_attn_tree_i8(void *stream, const float *q, size_t q_numel,
                                  float scale, size_t window, float *workspace,
                                  size_t workspace_floats, int cu_count);
 /* eb_attention_forward[_qkv] for a tree: norms, RoPE at the nodes' positions, their rows into the
- * cache at base_pos.., eb_attn_tree with the layer's window. x [rows, hidden], q [rows,
- * n_heads*hd], k / v [rows, n_kv_heads*hd]; any cache. */
+ * cache at base_pos.. (a block-scaled one's: beside it), eb_attn_tree with the layer's window. x [rows,
+ * hidden], q [rows, n_heads*hd], k / v [rows, n_kv_heads*hd]; any cache. Beside a block-scaled cache a
+ * node's row that is not finite reaches the nodes that see it, and no others. */
 eb_status eb_attention_forward_tree_qkv(const eb_attention *attn, eb_recorder *rec,
                                         const eb_tensor *q, const eb_tensor *k,
                                         const eb_tensor *v, const eb_rope_tables *rope,
@@ -822,9 +833,10 @@ eb_status eb_launch_tree_accept(void *stream, const uint32_t *tokens, size_t tok
                                 uint32_t *count, size_t n);
 /* Moves rows pos + path[j] of every layer's K and V to rows pos + j, j < min(count[0], n), in place.
  * The path counts up to its first entry that is not below n or not above the one before. The rows
- * behind keep what they hold. Any cache; a block-scaled one is read and written as eb_kv_read_i8 and
- * eb_kv_write_i8 do (the rows behind keep their codes; those in the last moved row's block take its
- * new exponent). */
+ * behind keep what they hold. Any cache. Of a block-scaled layer whose last tree pass was one at pos, the
+ * nodes' rows path[j] are written to pos + j, as by eb_kv_write_i8 of those rows alone, and the draft is done
+ * with; any other block-scaled layer's rows are read and written as eb_kv_read_i8 and eb_kv_write_i8 do
+ * (the rows behind keep their codes; those in the last moved row's block take its new exponent). */
 eb_status eb_kv_compact(eb_recorder *rec, eb_kv_cache *kv, const eb_tensor *path,
                         const eb_tensor *count, size_t n, size_t pos);
 /* Rows 0..count - 1 of every layer's K and V of src into dst: the same prompt continued twice. The
