@@ -234,12 +234,12 @@ eb_status draft_rows(eb_kv_cache *kv, size_t layer, eb_device *dev, eb::DraftRow
 // Memory for a pass's tail (eb::DraftTail), of a size that does not depend on pos.
 eb_status tail_room(eb_device *dev, const eb::CacheI8 &c, size_t pos, size_t n, size_t window, Owned *hold,
                     eb::DraftTail *out) {
-    const size_t codes = eb::tree_tail_rows(n, c.block) * c.hkv * c.hd;  // (a multiple of 16)
-    const size_t exps = eb::tree_tail_blocks(n, c.block) * c.hkv, shape[1] = {2 * codes + 2 * exps + 2 * c.hkv * n};
+    const size_t codes = eb::tree_tail_rows(n) * c.hkv * c.hd;  // (a multiple of 16)
+    const size_t exps = eb::tree_tail_blocks(n) * c.hkv, shape[1] = {2 * codes + 2 * exps + 2 * c.hkv * n};
     EB_TRY(eb_tensor_empty(dev, shape, 1, EB_U8, &hold->t));
     uint8_t *p = data<uint8_t>(hold->t);
     *out = eb::DraftTail{p, p + codes, p + 2 * codes, p + 2 * codes + exps, p + 2 * codes + 2 * exps,
-                         eb::tree_tail_row(pos, window, c.block)};
+                         eb::tree_tail_row(pos, window)};
     return EB_OK;
 }
 
@@ -508,7 +508,8 @@ eb_status eb_attention_forward_tree_qkv(const eb_attention *attn, eb_recorder *r
     if (kv->block) {
         // The row pass into f32 rows beside the cache, then the attention over the cache's rows and, from a
         // copy of its end on, those rows' codes: written into the cache they would round the rows of pos's
-        // block for good, whatever becomes of the draft.
+        // block for good, whatever becomes of the draft. (The copy has blocks of 16, the fewest that the
+        // attention tells apart, so that few rows are rounded to another's exponent even there.)
         eb::CacheI8 c;
         EB_TRY(layer_i8(kv, layer, dev, &c));
         EB_TRY(rows_checked(d, rope, base_pos + rows, dev));

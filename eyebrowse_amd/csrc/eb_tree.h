@@ -17,10 +17,10 @@ enum class TreeElem { F32, F16, E4M3, I8 };
 struct DraftRows {
     float *k, *v;  // [up to kTreeMax, hkv, hd]
 };
-// A pass's own copy of such a cache from row0 on, as a write of the drafted rows at pos would leave it, and
-// which of them are not finite: those take no part in their block's exponent.
+// A pass's own copy of such a cache from row0 on, in blocks of 16 rows, as a write of the drafted rows at pos
+// would leave it, and which of them are not finite: those take no part in their block's exponent.
 struct DraftTail {
-    uint8_t *k, *v, *ks, *vs;  // codes [rows from row0, hkv, hd], exponents [blocks from row0's, hkv]
+    uint8_t *k, *v, *ks, *vs;  // codes [rows from row0, hkv, hd], exponents [blocks, hkv]
     uint8_t *bad;              // [K and V, hkv, n]
     size_t row0;
 };
@@ -28,16 +28,16 @@ struct DraftTail {
 inline size_t tree_first_key(size_t pos, size_t window) {
     return (window > 0 && pos + 1 > window ? pos + 1 - window : 0) & ~(size_t)15;
 }
-// Where a tail starts: a tile of the attention (their sizes divide kTailStep) begins there, and pos's block
-// does not begin before it, or no earlier key is seen.
-constexpr size_t kTailStep = 128;
-inline size_t tree_tail_row(size_t pos, size_t window, size_t block) {
-    const size_t key0 = tree_first_key(pos, window), b0 = pos / block * block;
+// Where a tail starts: a tile of the attention (their sizes divide kTailStep) begins there, and pos's block of
+// 16 does not begin before it, or no earlier key is seen.
+constexpr size_t kTailStep = 128, kTailBlock = 16;
+inline size_t tree_tail_row(size_t pos, size_t window) {
+    const size_t key0 = tree_first_key(pos, window), b0 = pos & ~(kTailBlock - 1);
     return b0 > key0 ? key0 + (b0 - key0) / kTailStep * kTailStep : key0;
 }
 // Rows and blocks that a tail of n nodes has room for, wherever pos lies.
-inline size_t tree_tail_rows(size_t n, size_t block) { return kTailStep + block + n; }
-inline size_t tree_tail_blocks(size_t n, size_t block) { return tree_tail_rows(n, block) / block + 2; }
+inline size_t tree_tail_rows(size_t n) { return kTailStep + kTailBlock + n; }
+inline size_t tree_tail_blocks(size_t n) { return tree_tail_rows(n) / kTailBlock + 1; }
 eb_status launch_kv_draft_i8(hipStream_t st, const CacheI8 &c, const DraftRows &d, const DraftTail &t, size_t pos,
                              size_t n);
 

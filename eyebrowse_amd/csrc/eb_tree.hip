@@ -23,6 +23,7 @@ constexpr int kNodes = (int)eb::kTreeMax;
 constexpr int kWords = kNodes / 32;
 constexpr int kThreads = 256;
 constexpr unsigned kNobody = 0xFFFFFFFFu;
+constexpr int kBlock = (int)eb::kTailBlock;
 
 static_assert(kNodes == kThreads, "a node per thread");
 
@@ -189,32 +190,29 @@ struct DraftArgs {
     u32x4 tag;  // as written: the cache's number, pos, n
 };
 
-// Workgroup (b, head, side): one block of the tail, of one KV head: the cache's rows before pos, in the
-// exponent that a write of the block's drafted rows gives it, and those rows' codes. A row that is not finite
-// is zeros and a mark instead. The cache itself is not touched. Bound by latency: everything that a thread
-// keeps in registers (a block of 64 rows of 128) is on its way before the first wait.
+// Workgroup (b, head, side): 16 rows of the tail, of one KV head: the cache's rows before pos, in the exponent
+// that a write of the block's drafted rows gives it, and those rows' codes. A row that is not finite is zeros
+// and a mark instead. The cache itself is not touched. Bound by latency: every load is on its way before the
+// first wait.
 __global__ __launch_bounds__(kThreads) void kv_draft_i8_kernel(DraftArgs a) {
     __shared__ unsigned s_max[2][kThreads / 64];
-    __shared__ unsigned s_bad[kNodes];
-    constexpr int kOld = 4, kNew = 8;
+    __shared__ unsigned s_bad[kBlock];
+    constexpr int kNew = kBlock * 256 / 4 / kThreads;  // vectors of a thread, at the widest head
+    static_assert(kBlock * 256 / 16 <= kThreads, "a vector of old rows a thread");
     const DraftSide &s = blockIdx.z ? a.v : a.k;
     const int head = blockIdx.y, tid = threadIdx.x;
-    const int b0 = a.row0 >> a.block_log2, b = b0 + (int)blockIdx.x;
-    const int first = b << a.block_log2, behind = first + (1 << a.block_log2);
+    const int first = a.row0 + (int)blockIdx.x * kBlock, behind = first + kBlock;  // (row0 is a multiple of 16)
     const int lo = max(first, a.pos), hi = min(behind, a.pos + a.n);
-    const int from = max(first, a.row0), to = min(behind, a.pos);
     const int per_row = a.hd / 4, per_old = a.hd / 16;
     const int rows = max(hi - lo, 0), vecs = rows * per_row;  // drafted ones
-    const int kept = max(to - from, 0) * per_old;             // the cache's
+    const int kept = max(min(behind, a.pos) - first, 0) * per_old;  // the cache's
     const size_t stride = (size_t)a.hkv * a.hd, head0 = (size_t)head * a.hd;
     const float *src = s.rows + (lo - a.pos) * stride + head0;
-    const uint8_t *old_src = s.codes + from * stride + head0;
-    uint8_t *new_dst = s.tail_codes + (lo - a.row0) * stride + head0, *old_dst = s.tail_codes + (from - a.row0) * stride + head0;
+    uint8_t *new_dst = s.tail_codes + (lo - a.row0) * stride + head0;
     const bool lead = first < a.pos;
     auto load = [&](int i) {
         return *reinterpret_cast<const f32x4 *>(src + (size_t)(i / per_row) * stride + 4 * (i % per_row));
     };
-    auto old_at = [&](int i) { return (size_t)(i / per_old) * stride + 16 * (i % per_old); };
     auto magnitude = [](f32x4 x) {
         unsigned top = 0;
 #pragma unroll
@@ -230,55 +228,49 @@ __global__ __launch_bounds__(kThreads) void kv_draft_i8_kernel(DraftArgs a) {
         for (int w = 0; w < kThreads / 64; ++w) top = max(top, to_all[w]);
         return top;
     };
-    const unsigned old_e = lead ? s.exps[(size_t)b * a.hkv + head] : 0u;
+    const unsigned old_e = lead ? s.exps[(size_t)(first >> a.block_log2) * a.hkv + head] : 0u;
     f32x4 fresh[kNew];
-    u32x4 old[kOld];
+    u32x4 old = {0u, 0u, 0u, 0u};
+    const size_t old_at = (size_t)(tid / per_old) * stride + head0 + 16 * (tid % per_old);
 #pragma unroll
     for (int j = 0; j < kNew; ++j)
         fresh[j] = tid + j * kThreads < vecs ? load(tid + j * kThreads) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int j = 0; j < kOld; ++j)
-        if (tid + j * kThreads < kept) old[j] = *reinterpret_cast<const u32x4 *>(old_src + old_at(tid + j * kThreads));
+    if (tid < kept) old = *reinterpret_cast<const u32x4 *>(s.codes + first * stride + old_at);
     unsigned top = 0;
 #pragma unroll
     for (int j = 0; j < kNew; ++j) top = max(top, magnitude(fresh[j]));
-    for (int i = tid + kNew * kThreads; i < vecs; i += kThreads) top = max(top, magnitude(load(i)));
     if (tid < rows) s_bad[tid] = 0;
     top = join(top, s_max[0]);
     const bool some_bad = top >= 0x7F800000u;  // (uniform)
     if (some_bad) {  // the rows that are not finite, and the others' largest
-        for (int i = tid; i < vecs; i += kThreads)
-            if (magnitude(load(i)) >= 0x7F800000u) s_bad[i / per_row] = 1;
+#pragma unroll
+        for (int j = 0; j < kNew; ++j)
+            if (magnitude(fresh[j]) >= 0x7F800000u) s_bad[(tid + j * kThreads) / per_row] = 1;
         __syncthreads();
         top = 0;
-        for (int i = tid; i < vecs; i += kThreads)
-            if (!s_bad[i / per_row]) top = max(top, magnitude(load(i)));
+#pragma unroll
+        for (int j = 0; j < kNew; ++j)
+            if (tid + j * kThreads < vecs && !s_bad[(tid + j * kThreads) / per_row]) top = max(top, magnitude(fresh[j]));
         top = join(top, s_max[1]);
     }
     unsigned e = eb::i8_exponent(top);
     if (lead) e = rows > 0 ? eb::i8_join(old_e, e) : old_e;
-    auto store = [&](int i, f32x4 x) {
+#pragma unroll
+    for (int j = 0; j < kNew; ++j) {
+        const int i = tid + j * kThreads;
+        if (i >= vecs) continue;
         unsigned w = 0;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) w |= eb::i8_code(x[c], e) << (8 * c);
+        for (int c = 0; c < 4; ++c) w |= eb::i8_code(fresh[j][c], e) << (8 * c);
         if (some_bad && s_bad[i / per_row]) w = 0;
         *reinterpret_cast<unsigned *>(new_dst + (size_t)(i / per_row) * stride + 4 * (i % per_row)) = w;
-    };
-    auto store_old = [&](int i, u32x4 w) {
+    }
+    if (tid < kept) {
         if (e != old_e && e != eb::kNanExponent)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) w[c] = eb::i8_recode(w[c], old_e, e);
-        *reinterpret_cast<u32x4 *>(old_dst + old_at(i)) = w;
-    };
-#pragma unroll
-    for (int j = 0; j < kNew; ++j)
-        if (tid + j * kThreads < vecs) store(tid + j * kThreads, fresh[j]);
-    for (int i = tid + kNew * kThreads; i < vecs; i += kThreads) store(i, load(i));
-#pragma unroll
-    for (int j = 0; j < kOld; ++j)
-        if (tid + j * kThreads < kept) store_old(tid + j * kThreads, old[j]);
-    for (int i = tid + kOld * kThreads; i < kept; i += kThreads)
-        store_old(i, *reinterpret_cast<const u32x4 *>(old_src + old_at(i)));
+            for (int c = 0; c < 4; ++c) old[c] = eb::i8_recode(old[c], old_e, e);
+        *reinterpret_cast<u32x4 *>(s.tail_codes + (first - a.row0) * stride + old_at) = old;
+    }
     if (tid < rows) s.bad[(size_t)head * a.n + (lo - a.pos) + tid] = (uint8_t)s_bad[tid];
     if (tid == 0) {
         s.tail_exps[blockIdx.x * a.hkv + head] = (uint8_t)e;
@@ -456,8 +448,8 @@ eb_status launch_kv_draft_i8(hipStream_t st, const CacheI8 &c, const DraftRows &
     a.hd = (int)c.hd;
     a.tag = u32x4{(unsigned)c.id, (unsigned)(c.id >> 32), (unsigned)pos, (unsigned)n};
     while ((size_t)1 << a.block_log2 < c.block) ++a.block_log2;
-    const size_t blocks = (pos + n - 1) / c.block - t.row0 / c.block + 1;
-    if (blocks > tree_tail_blocks(n, c.block) || pos + n - t.row0 > tree_tail_rows(n, c.block))
+    const size_t blocks = (pos + n - 1 - t.row0) / kTailBlock + 1;
+    if (blocks > tree_tail_blocks(n) || pos + n - t.row0 > tree_tail_rows(n) || t.row0 % kTailBlock)
         return fail(EB_OTHER, "kv_draft_i8: rows %zu to %zu do not fit the tail", t.row0, pos + n);
     kv_draft_i8_kernel<<<dim3((unsigned)blocks, (unsigned)c.hkv, 2), kThreads, 0, st>>>(a);
     return check_launch("kv_draft_i8");

@@ -265,7 +265,8 @@ __device__ __forceinline__ int piece_xor(int r) {
     return RB >= 256 ? r & 15 : RB == 128 ? (r >> 1) & 7 : (r >> 2) & 3;
 }
 
-// TAIL (block-scaled caches): keys from tail0 on are rows of the call's own, in place of the cache's.
+// TAIL (block-scaled caches): keys from tail0 on are rows of the call's own, in place of the cache's, in blocks
+// of 16.
 template <int HDP, TreeElem E, int CW, int NSET, bool COPY, bool TAIL>
 __global__ __launch_bounds__((Shape<HDP, E, CW, NSET, COPY>::THREADS),
                              (Shape<HDP, E, CW, NSET, COPY>::WGS * Shape<HDP, E, CW, NSET, COPY>::WAVES / 4))
@@ -306,7 +307,7 @@ void tree_attn_kernel(Args a) {
     const uint8_t *exps = vside ? a.vs : a.ks;
     // (so that the tail's rows and exponents are found by the same key)
     const char *tail_base = TAIL ? (vside ? a.tv : a.tk) + (size_t)kvh * hd - (size_t)a.tail0 * row_bytes : base;
-    const uint8_t *tail_exps = TAIL ? (vside ? a.tvs : a.tks) - (size_t)(a.tail0 >> a.block_log2) * a.hkv : exps;
+    const uint8_t *tail_exps = TAIL ? (vside ? a.tvs : a.tks) - (size_t)(a.tail0 / 16) * a.hkv : exps;
     const unsigned lds0 = (unsigned)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)smem);
     unsigned piece[COPY ? S::CPW : 1];  // where this lane's pieces lie in a tile's rows
     if constexpr (COPY) {
@@ -333,11 +334,12 @@ void tree_attn_kernel(Args a) {
                          "v"(piece[i]), "s"(res)
                          : "memory", "m0");
         if constexpr (E == TreeElem::I8) {  // (every wave the same words: the counts stay alike)
-            const size_t b0 = left > 0 ? (size_t)(r0 >> a.block_log2) : 0;
-            const int last = left > 0 ? (r0 + left - 1) >> a.block_log2 : 0;
+            const int bl = tail ? 4 : a.block_log2;
+            const size_t b0 = left > 0 ? (size_t)(r0 >> bl) : 0;
+            const int last = left > 0 ? (r0 + left - 1) >> bl : 0;
             const __amdgpu_buffer_rsrc_t eres = eb::make_rsrc(
                 (tail ? tail_exps : exps) + b0 * a.hkv, left > 0 ? (last - (int)b0) * a.hkv + kvh + 1 : 0);
-            const unsigned off = 16 * lane < left ? (((r0 + 16 * lane) >> a.block_log2) - (int)b0) * a.hkv + kvh : kNone;
+            const unsigned off = 16 * lane < left ? (((r0 + 16 * lane) >> bl) - (int)b0) * a.hkv + kvh : kNone;
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_ubyte %1, %2, 0 offen lds" ::"s"(
                              lds0 + b * S::TILE + 2 * T * S::RB + (vside ? 256 : 0)),
                          "v"(off), "s"(eres)

@@ -727,8 +727,9 @@ eb_status eb_launch_sample(void *stream, const float *logits, size_t logits_nume
  * Over a block-scaled cache the layer (eb_attention_forward_tree[_qkv]) keeps the nodes' K and V beside
  * the cache instead, in f32: written into it, a draft would round the certain rows of pos's block to its own
  * exponent for good, accepted or not. The cache stays as it is until eb_kv_compact writes the accepted
- * nodes' rows, or for good where none follows. Within the pass the nodes see the block's rows as one write of
- * all n rows at pos would round them. Any other rows written to the layer, or a fork into the cache, drop
+ * nodes' rows, or for good where none follows. Within the pass the rows from pos on, and the up to 15 before
+ * them of the same aligned 16, have the codes that one write of all n rows at pos would give them in blocks
+ * of 16. Any other rows written to the layer, or a fork into the cache, drop
  * its draft. A layer's first pass or compaction takes room for twice min(256, max_seq) f32 rows, which the
  * cache keeps.
  *

@@ -300,3 +300,31 @@ def test_many_layers(dev):
         eb.kv_compact(rec, c, pt, ct, n, pos)
     rec.submit()
     same(seq)
+
+
+@pytest.mark.parametrize("block", [64, 256])
+@pytest.mark.parametrize("pos", [64, 69, 200])
+def test_pass_rounds_sixteen_rows_together(dev, block, pos):
+    """What the nodes see: the cache's rows as they are, but those of pos's aligned 16, and the nodes' own,
+    coded as by a cache whose blocks are 16 rows."""
+    note(f"i8 drafts, sixteen rows together, block {block} pos {pos}")
+    x = Layer(dev, block, 64, pos, 40)
+    x.v[20] *= 300  # (its neighbours only are rounded to its exponent)
+    got = x.forward(x.cache())
+    # The same codes, in a cache of blocks of 16.
+    kv, fine = x.cache(), eb.KvCache.new_i8(dev, 1, x.seq, x.hkv, x.hd, 16)
+    for a, b, e, f in ((kv.k, fine.k, kv.k_scale, fine.k_scale), (kv.v, fine.v, kv.v_scale, fine.v_scale)):
+        b[0].write(a[0].read_bytes())
+        exps = np.frombuffer(e[0].read_bytes(), np.uint8).reshape(-1, x.hkv)
+        f[0].write(np.repeat(exps, block // 16, 0)[:-(-x.seq // 16)].copy())
+    k_new, v_new = x.final_rows()
+    x.write(fine, k_new, v_new, pos)
+    f32 = eb.KvCache.new(dev, 1, x.seq, x.hkv, x.hd)
+    qo, o = (eb.Tensor.empty(dev, x.q.shape) for _ in range(2))
+    qt, kt, vt = (eb.Tensor.from_f32(dev, t.shape, t) for t in (x.q, x.k, x.v))
+    rec = eb.Recorder(dev)
+    eb.attn_prologue_tree(rec, qt, kt, vt, x.nodes.depths, qo, f32.k[0], f32.v[0], x.n, x.h, x.hkv, x.hd, pos, x.seq,
+                          *x.gains, EPS, x.rope.cos, x.rope.sin)
+    eb.attn_tree_i8(rec, qo, fine, 0, x.nodes.masks, None, o, x.h, pos, x.n, 0.2)
+    rec.submit()
+    assert got.tobytes() == o.read_bytes()
