@@ -402,17 +402,18 @@ eb_status eb_kv_compact(eb_recorder *rec, eb_kv_cache *kv, const eb_tensor *path
     for (size_t l = 0; l < layers; ++l)
         if (!kv->block && row_bytes(kv, l) % 4)
             return fail(EB_UNSUPPORTED_CONFIG, "kv_compact: rows of %zu bytes (a multiple of 4)", row_bytes(kv, l));
+    eb::CacheI8 caches[eb::kMoveLayers];
+    eb::DraftRows drafts[eb::kMoveLayers];
+    for (size_t l = 0; l < layers && kv->block; ++l) EB_TRY(draft_rows(kv, l, dev, &drafts[0]));  // (memory)
     const hipStream_t st = stream_of(dev);
     for (size_t l0 = 0; l0 < layers; l0 += eb::kMoveLayers) {
         const size_t nl = std::min(layers - l0, eb::kMoveLayers);
         if (kv->block) {
-            eb::CacheI8 c[eb::kMoveLayers];
-            eb::DraftRows drafts[eb::kMoveLayers];
             for (size_t l = 0; l < nl; ++l) {
-                EB_TRY(layer_i8(kv, l0 + l, dev, &c[l]));
+                EB_TRY(layer_i8(kv, l0 + l, dev, &caches[l]));
                 EB_TRY(draft_rows(kv, l0 + l, dev, &drafts[l]));
             }
-            EB_TRY(eb::launch_kv_compact_i8(st, c, drafts, nl, data<uint32_t>(path), data<uint32_t>(count), n, pos));
+            EB_TRY(eb::launch_kv_compact_i8(st, caches, drafts, nl, data<uint32_t>(path), data<uint32_t>(count), n, pos));
         } else {
             eb::CacheRows c[eb::kMoveLayers];
             for (size_t l = 0; l < nl; ++l)

@@ -313,10 +313,8 @@ __global__ __launch_bounds__(kThreads) void kv_compact_i8_kernel(CompactI8Args a
     const float *draft = nullptr;
     if (tag[0] == a.id_lo && tag[1] == a.id_hi && tag[2] == (unsigned)a.pos) draft = layer.draft[side];
     const int end = load_path(a.path, a.count, draft ? min(a.n, (int)tag[3]) : a.n, s_path, &s_end);
-    if (draft) {
-        draft += (size_t)head * layer.hd;
-        if (tid == 0) *tags = u32x4{0u, 0u, 0u, 0u};  // (every thread has read it: load_path's barriers)
-    }
+    if (tid == 0) *tags = u32x4{0u, 0u, 0u, 0u};  // (every thread has read it: load_path's barriers)
+    if (draft) draft += (size_t)head * layer.hd;
     auto word = [&](size_t row, int w) { return reinterpret_cast<unsigned *>(codes + row * stride + 4 * w); };
     if (!draft) {
         for (int i = tid; i < end * per_row; i += kThreads) s_code[i] = *word(a.pos + s_path[i / per_row], i % per_row);
