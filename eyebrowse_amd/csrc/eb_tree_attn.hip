@@ -41,12 +41,12 @@
 // NaN whole (finite rows' sums cannot pass f32's range). A column that sees nothing gives zeros.
 //
 // What binds it, with 32 heads over 8 of 128 (whole calls in a graph): 4 nodes, the cache's bytes (behind
-// 30000 f32 keys 48 to 49 us, 5.1 TB/s, the rate of a large copy); 64 nodes, matrix instructions and the
-// softmax and conversions beside them, which two waves to a SIMD overlap in part (behind 32000 half keys
-// 76 to 81 us, 416 to 440 TFLOP/s of the formula's products, twice that issued; 30000 E4M3 71 to 74,
-// block-scaled 87 to 89, f32 133 to 139 us); between, both, and the call's fixed parts: 3 to 5 us until
-// a workgroup's first tile is there, 4 to 6 us for the merge and its launch (21 nodes behind 8191
-// block-scaled keys 24 us).
+// 30000 f32 keys 48 to 49 us, 5.0 to 5.1 TB/s: 1.26 times what they take at the 6.35 TB/s that a copy of cache
+// rows reaches, the fixed parts below between); 64 nodes, matrix instructions and the softmax and conversions
+// beside them, which two waves to a SIMD overlap in part (behind 32000 half keys 76 to 83 us, 406 to 440
+// TFLOP/s of the formula's products, twice that issued; 30000 E4M3 71 to 76, block-scaled 90 to 91, f32 132 to
+// 140 us); between, both, and the call's fixed parts: 3 to 5 us until a workgroup's first tile is there, 4 to
+// 6 us for the merge and its launch (21 nodes behind 8191 block-scaled keys 24 us).
 #include "eb_cache_i8.h"
 #include "eb_tree.h"
 
@@ -1218,6 +1218,17 @@ struct Plan {
 //   16 nodes behind  8000 f32 keys:         41.7, 29.7       (41.3, 26.5)
 //   16 nodes of 16 heads behind 200 E4M3 keys: 8.3 with one split, 10.9 with 64 columns (7.1, 10.7)
 //   8 nodes of 16 heads behind 100 f32 keys: 10.5 with one split, 9.2 with four (16 columns)
+// 64 nodes behind 1000 half keys thus take 64 columns where 16 are the faster by 1.6 us. The products grow with
+// the dims and the softmax does not, hence the factor for other widths; 14 heads over 2 of 64, 16 over 8 of 256
+// (16, 64 and 128 columns, each with its best splits; the rule takes the fastest of each row):
+//   16 nodes of 64 behind 8000 half keys:   12.2, 12.8, 15.6 (12.4, 13.0, 15.0)
+//   64 nodes of 64 behind 8000 half keys:   19.3, 17.5, 20.8 (20.0, 18.3, 19.5)
+//   64 nodes of 64 behind 8000 f32 keys:    44.0, 25.7, 29.7 (45.4, 26.5, 26.8)
+//   16 nodes of 64 behind 1000 block-scaled: 9.5, 12.0, 15.8 (9.7, 11.9, 13.7)
+//   16 nodes of 256 behind 8000 f32 keys:   80.6, 51.2       (53.3, 35.0)
+//   64 nodes of 256 behind 8000 half keys:  55.1, 38.2       (82.0, 35.2)
+//   16 nodes of 256 behind 8000 block-scaled: 27.9, 29.8     (22.7, 23.7)
+//   32 nodes of 256 behind 2000 E4M3 keys:  18.2, 23.0       (17.0, 18.0)
 struct Cost {
     float set, chain;
 };
