@@ -52,6 +52,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <cmath>
 
 namespace {
 
@@ -75,7 +76,7 @@ constexpr unsigned kNone = 0x7FFFFFF0u;  // a byte offset past any tile
 // f32's range although the column's power, which comes last, brings it back: the rows' powers are kept times
 // this (2^-149 at least, which f32 holds), the columns' times its inverse.
 constexpr float kScoreShift = 0x1p-23f;
-constexpr unsigned kScoreShiftLog2 = 23;
+constexpr int kScoreShiftLog2 = 23;
 
 // How a call is run: COPY moves the cache's rows to LDS as they are (half rows, E4M3 rows of whole
 // 16-byte pieces, block-scaled codes); otherwise they pass through registers and become f16 there (f32
@@ -155,7 +156,8 @@ struct Args {
     int key0, tiles;  // the first key of tile 0; a tile at least
     int tail0;        // the first key of some tile
     int nsplit, ncb, pairs, block_log2;
-    float scale_log2;
+    float scale;  // scale log2(e) / 2^scale_power
+    int scale_power;
 };
 
 // 1 / l (to a step of f32: five of them meet in a result at most) for a sum of weights, which is at
@@ -570,21 +572,20 @@ void tree_attn_kernel(Args a) {
         }
         top = fmaxf(top, eb::lane_xor16(top));
         top = fmaxf(top, eb::lane_xor32(top));
-        // (q times scale log2(e), its largest in [2^13, 2^14) or, if the product rounds up, at 2^14)
-        const unsigned e = biased_exponent(fabsf(top * a.scale_log2));
+        // (q times scale log2(e), its largest in [2^13, 2^14) or, if the product rounds up, at 2^14; the scale as
+        // a fraction and a power of two, which joins q's, since the product may pass f32's range)
+        const unsigned e = biased_exponent(fabsf(top * a.scale));
+        const int power = (int)e - 140 + a.scale_power + (S::F32 ? kScoreShiftLog2 : 0), most = min(power, 127);
+        qs[s] = ldexpf(1.0f, most);
         if constexpr (S::F32) {
-            const unsigned shifted = e - 13u + kScoreShiftLog2, most = min(shifted, 254u);
-            qs[s] = pow2_biased(most);
-            steep = steep | (shifted > 254u);
-            if (g4 == 0 && kw == 0) s_steep[(cw * NSET + s) * 16 + n] = pow2_biased(127u + shifted - most);
-        } else {
-            qs[s] = pow2_biased(e - 13u);
+            steep = steep | (power > most);
+            if (g4 == 0 && kw == 0) s_steep[(cw * NSET + s) * 16 + n] = ldexpf(1.0f, power - most);
         }
-        const float f = pow2_biased(267u - e);  // (beside a scale of 4 and more it could pass f32's range)
+        const float f = pow2_biased(267u - e);
 #pragma unroll
         for (int i = 0; i < S::NC; ++i) {
             f16x8 lo;
-            split(x[i] * a.scale_log2 * f, qh[s][i], lo);
+            split(x[i] * f * a.scale, qh[s][i], lo);
             if constexpr (S::QLDS) {
                 if (kw == 0) *reinterpret_cast<f16x8 *>(s_ql + ((cw * NSET + s) * S::NC + i) * 1024 + lane * 16) = lo;
             } else {
@@ -1396,7 +1397,8 @@ eb_status launch_attn_tree(hipStream_t st, const TreeAttn &x, float *ws, size_t 
     a.ncb = p.ncb;
     a.pairs = (int)x.hkv * p.nsplit;
     while (x.block > 0 && (size_t)1 << a.block_log2 < x.block) ++a.block_log2;
-    a.scale_log2 = x.scale * kLog2e;
+    a.scale = std::frexp(x.scale * kLog2e, &a.scale_power);
+    if (!std::isfinite(a.scale)) a.scale_power = 0;
     const hipError_t e = x.elem == TreeElem::F32   ? launch_elem<TreeElem::F32, false>(st, a, p)
                          : x.elem == TreeElem::F16 ? launch_elem<TreeElem::F16, true>(st, a, p)
                          : x.elem == TreeElem::I8  ? x.tail ? launch_elem<TreeElem::I8, true, true>(st, a, p)

@@ -151,3 +151,24 @@ def test_scores_at_the_ends(dev, elem, size):
     got = c.attend(dev, q, nodes, pos, 1.0)
     want, bound = attention(np.zeros_like(q), c.k, c.v, visible(nodes.seen, nodes.depth, pos, 0), 1.0)
     assert np.isfinite(got).all() and (np.abs(got - want) <= bound).all(), (np.abs(got - want) / bound).max()
+
+
+@pytest.mark.parametrize("elem,k_power,q_power,scale_power", [
+    ("f32", -130, 120, 10), ("f32", -120, 100, 20), ("f32", 120, -130, 10), ("f32", 0, -100, 100), ("f32", 0, 100, -100),
+    ("f32", 100, 15, -115), ("f16", 0, 100, -100), ("f16", -10, -100, 110), ("f16", 0, -126, 126), ("f16", -10, 120, -110)])
+@pytest.mark.parametrize("n", [3, 40])
+def test_scales_of_any_size(dev, elem, k_power, q_power, scale_power, n):
+    """Ordinary scores of queries whose product with the scale f32 does not hold, or only in part."""
+    note(f"tree ranges, {elem} K 2^{k_power} q 2^{q_power} scale 2^{scale_power} n {n}")
+    rng = np.random.default_rng(7)
+    h, hkv, hd, pos = 8, 2, 64, 400
+    nodes = Nodes(dev, random_parents(n, rng))
+    # Multiples of 2^-4 and 2^-6 below 2^6 and 2^2: exact at either end, down to 2^-149 (half: 2^-24).
+    k = np.clip(np.round(rows(rng, pos + n, hkv, hd) * 16), -1024, 1024) / 16 * 2.0 ** k_power
+    q = np.clip(np.round(rng.standard_normal((n, h, hd)) * 64), -256, 256) / 64 * 2.0 ** q_power
+    k, q, scale = k.astype(np.float32), q.astype(np.float32), np.float32(0.1 * 2.0 ** scale_power)
+    c = Cache(dev, elem, pos + n, hkv, hd, k, rows(rng, pos + n, hkv, hd))
+    assert np.array_equal(c.k, k)
+    got = c.attend(dev, q, nodes, pos, float(scale))
+    want, bound = attention(q, c.k, c.v, visible(nodes.seen, nodes.depth, pos, 0), np.float64(scale))
+    assert np.isfinite(got).all() and (np.abs(got - want) <= bound).all(), (np.abs(got - want) / bound).max()
