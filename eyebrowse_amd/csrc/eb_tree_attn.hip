@@ -1125,7 +1125,8 @@ void tree_attn_kernel(Args a) {
 // o[row] = average of the splits' averages, each weighed by its sum of weights at one reference. narrow: a
 // row with a dim that is not finite becomes NaN (the sums of half and E4M3 values are finite otherwise).
 // Workgroup: one row (node and head); a group of lanes holds the row's dims, four each, the groups share
-// the splits, four at a time in flight. Bound by latency and its launch: 480 rows of 9 splits 4.0 us in a trace, 2048 rows of 16 (17 MB) 6.1 to 6.8.
+// the splits, four at a time in flight. Bound by latency and its launch: 480 rows of 9 splits 4.0 us in a
+// trace, 2048 rows of 16 (17 MB) 6.1 to 6.8.
 constexpr int kMergeThreads = 256;
 __global__ __launch_bounds__(kMergeThreads) void tree_merge_kernel(const float *__restrict__ part_acc,
                                                               const float *__restrict__ part_ml, float *__restrict__ o,
